@@ -125,6 +125,55 @@ PB200_API int pb200_flash_attn_ext(const float * q, const void * k_f16, const vo
                                    int n_head, int n_head_kv, int n_kv, const int64_t * q_nb, const int64_t * k_nb, const int64_t * v_nb, int64_t mask_nb1,
                                    float scale, float max_bias, float logit_softcap, void * stream);
 
+/* ---- a cache of 4-bit keys and values in pages ----
+ * A page holds 64 cells of every layer and kv head; sequences have lists of pages (tables), in any order, and may share them.  Page i lies at pages + i *
+ * pb200_kv4_page_bytes: chunks [n_layer][n_head_kv], each 64 key rows and 64 value rows of head_dim numbers in 4 bits, with a scale (f16 of 8 significant bits) for
+ * every 32 of them: 144 bytes for a cell's key and value of 128 (f16: 512).  A number is (n - 8) * scale; scale = the block's number of largest magnitude / -8
+ * (of several, the first), rounded to 8 bits, n = round(x / scale) + 8 in 0 .. 15.  NaN counts as 0, magnitudes beyond 21760 as 21760: a cache holds numbers only.
+ * csrc/kv4.cuh says where the bits lie.  head_dim 64 or 128 (others: PB200_ENOTSUP).  pages: device memory at a 16-byte boundary, which the caller owns.
+ * Numbers in device memory (cells, tables, lengths) are checked by the kernels: what names no cell of the cache is not stored, read as a cell that nobody sees.
+ * Calls are ordered by their streams alone; nothing is kept from one to the next but in the cache. */
+enum { PB200_KV4_CELLS = 64 };
+typedef struct pb200_kv4_cache {
+    void *  pages;
+    int64_t n_pages;
+    int32_t n_layer, n_head_kv, head_dim, _pad;
+} pb200_kv4_cache;
+/* rotation as in pb200_rope, the angles in 64 bits; n_dims a multiple of 8 (others: PB200_ENOTSUP), 0: none; mode 0: neighbouring pairs, 2: halves */
+typedef struct pb200_rope_args {
+    int32_t n_dims, mode, n_ctx_orig;
+    float   freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow;
+    const float * freq_factors;   /* device [n_dims / 2], or NULL */
+} pb200_rope_args;
+PB200_API size_t pb200_kv4_page_bytes(int n_layer, int n_head_kv, int head_dim);   /* 0: not supported */
+/* The rows of n_tokens tokens, one launch: queries and keys normed per head (x / sqrt(mean(x^2) + eps) * weight, weights f32 [head_dim] at 16 bytes, either may be NULL),
+ * rotated by the token's position, queries to q_out (which may be q), keys and values into cell cells[t] = page * 64 + cell of the layer (negative: not stored; no two tokens
+ * have the same).  type: PB200_TYPE_F32, F16 or BF16 of q, q_out, k and v; rows of ld* numbers (a multiple of 4), heads next to each other, at 4 numbers' boundaries.
+ * n_head 0: keys and values alone. */
+PB200_API int pb200_kv4_append(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * q_out, int64_t ldq_out, const void * k, int64_t ldk,
+                               const void * v, int64_t ldv, int64_t n_tokens, int n_head, const int64_t * cells, const int32_t * pos, const float * q_norm, const float * k_norm,
+                               float eps, const pb200_rope_args * rope, void * stream);
+/* the numbers that n cells hold, rows [n_head_kv][head_dim] of a type (F32 and F16 hold them exactly); k or v may be NULL; a cell outside of the cache leaves its rows as they were */
+PB200_API int pb200_kv4_load(const pb200_kv4_cache * cache, int layer, int type, const int64_t * cells, int64_t n, void * k, int64_t ldk, void * v, int64_t ldv, void * stream);
+/* Attention of a ragged batch.  The queries of sequence s are the rows q_start[s] .. q_start[s+1]-1 of q (device [n_seq + 1], rising), the last kv_len[s] cells' own: query i of n
+ * stands at position p = kv_len[s] - n + i and sees the cells 0 .. p; with window > 0 those of the last `window` positions and the first keep_first.  Cell j is cell j % 64 of
+ * page table[s * table_ld + j / 64].  out[t][head] = sum of softmax(scale q k) v over what it sees, zeros if that is nothing; rows outside q_start[0] .. q_start[n_seq]-1, and
+ * queries beyond the first max_q of a sequence, stay as they were.  n_tokens: rows of q and out; max_q: the most queries of one sequence.  q, out: rows of [n_head][head_dim] of the
+ * type as in pb200_kv4_append, not overlapping.  q, softmax weights and sums have 22 bits and more with F32; with F16 and BF16 prompts' weights are rounded to f16.
+ * ws: pb200_kv4_attn_workspace_bytes, zeroed once by the caller, for calls that follow one another (one per stream, also of graphs that may run at the same time). */
+PB200_API size_t pb200_kv4_attn_workspace_bytes(int n_head, int n_head_kv, int head_dim);
+PB200_API int pb200_kv4_attn(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
+                             const int32_t * kv_len, const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, void * ws,
+                             size_t ws_bytes, void * stream);
+/* Copies of whole pages, all layers: page src[i] to page dst[i] (HOST arrays, not needed after the call).  A sequence that forks shares its full pages with the new one, and
+ * copies the last, which both go on writing.  PB200_EINVAL where a page is written twice, or written and read. */
+PB200_API int pb200_kv4_copy_pages(const pb200_kv4_cache * cache, const int32_t * src, const int32_t * dst, int n, void * stream);
+/* Cells that a sequence keeps, to pages of their own, all layers: cell index[s * index_ld + i] of table row s becomes cell i of row s of `to`, i < count[s] <= max_count
+ * (device arrays).  Bits are moved as they are: keys stay rotated for the positions that they had.  Pages of `to` are none of the pages that are read, and of one sequence each;
+ * their other cells stay as they were.  Behind it the old pages are free. */
+PB200_API int pb200_kv4_compact(const pb200_kv4_cache * cache, int n_seq, const int32_t * table, int64_t table_ld, const int32_t * to, int64_t to_ld, const int32_t * index,
+                                int64_t index_ld, const int32_t * count, int max_count, void * stream);
+
 /* ---- fused decode launches (what the engine is made of), for graph-level fusion in a host such as the ggml-backend plugin ---- */
 typedef struct pb200_gemv_mat {
     int32_t type;          /* k-quant type of W (Q4_K / Q5_K / Q6_K) */

@@ -12,6 +12,6 @@ and Ruvuvik (chunked attention, latent attention with learned sinks, the WKV mix
 This Python package is only the thin ctypes binding plus the schedulers; it never falls back to a CPU path: importing
 :mod:`host` raises if the CUDA library is missing.
 """
-from .host import Lib, Model, HParams, lib_path, build, TYPES  # noqa: F401
+from .host import Lib, Model, HParams, Kv4Cache, RopeArgs, lib_path, build, TYPES  # noqa: F401
 from .scheduler import BatchScheduler, Request  # noqa: F401
 from .pipeline import PipelineRunner, RingRunner, PrefillPipeline, layer_windows  # noqa: F401

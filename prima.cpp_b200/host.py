@@ -37,6 +37,16 @@ class BatchEntry(C.Structure):
     _fields_ = [("seq", C.c_int32), ("n_tokens", C.c_int32), ("tokens", C.POINTER(C.c_int32)), ("n_want", C.c_int32), ("want", C.POINTER(C.c_int32))]
 
 
+class Kv4Cache(C.Structure):
+    """pb200_kv4_cache: 4-bit keys and values in pages; `pages` is device memory of n_pages * pb200_kv4_page_bytes."""
+    _fields_ = [("pages", C.c_void_p), ("n_pages", C.c_int64), ("n_layer", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("_pad", C.c_int32)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_dims", "mode", "n_ctx_orig")] + \
+               [(n, C.c_float) for n in ("freq_base", "freq_scale", "ext_factor", "attn_factor", "beta_fast", "beta_slow")] + [("freq_factors", C.c_void_p)]
+
+
 class Pb200Error(RuntimeError):
     pass
 
@@ -131,6 +141,16 @@ class Lib:
         c.pb200_batch_step.argtypes = [vp, C.c_int, C.POINTER(BatchEntry), vp, vp]
         c.pb200_debug_tap_layers.argtypes = [vp, C.c_int]
         c.pb200_debug_profile.argtypes = [vp, C.c_int]
+        cache, st = C.POINTER(Kv4Cache), C.c_size_t
+        c.pb200_kv4_page_bytes.restype = st
+        c.pb200_kv4_page_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
+        c.pb200_kv4_append.argtypes = [cache, C.c_int, C.c_int, vp, i64, vp, i64, vp, i64, vp, i64, i64, C.c_int, vp, vp, vp, vp, f32, C.POINTER(RopeArgs), vp]
+        c.pb200_kv4_load.argtypes = [cache, C.c_int, C.c_int, vp, i64, vp, i64, vp, i64, vp]
+        c.pb200_kv4_attn_workspace_bytes.restype = st
+        c.pb200_kv4_attn_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
+        c.pb200_kv4_attn.argtypes = [cache, C.c_int, C.c_int, vp, i64, vp, i64, C.c_int, C.c_int, vp, vp, vp, i64, i64, C.c_int, f32, C.c_int, C.c_int, vp, st, vp]
+        c.pb200_kv4_copy_pages.argtypes = [cache, vp, vp, C.c_int, vp]
+        c.pb200_kv4_compact.argtypes = [cache, C.c_int, vp, i64, vp, i64, vp, i64, vp, C.c_int, vp]
         c.pb200_dense.argtypes = [C.c_int, vp, i64, vp, i64, vp, i64, C.c_int, C.c_int, C.c_int, vp, vp, i64, f32, vp]
 
     @classmethod
