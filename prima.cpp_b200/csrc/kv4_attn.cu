@@ -3,7 +3,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/prima_b200.h"
-#include "kv4.cuh"
+#include "kv4_attn.cuh"
 
 namespace pb {
 namespace {
@@ -88,11 +88,10 @@ int attn(const Kv4Attn & a, int D, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv4_attn_workspace(int, int, int) { return 16; }
+size_t kv4_attn_workspace(int D, int, int) { return KV4_MAX_CTAS * sizeof(int) + kv4_rows_workspace(D); }
 
 int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t st) {
-    (void) ws;
-    return type == PB200_TYPE_F32 ? attn<float>(a, D, st) : type == PB200_TYPE_F16 ? attn<__half>(a, D, st) : attn<__nv_bfloat16>(a, D, st);
+    return launch_kv4_attn_rows(a, D, type, 1 << 30, (int *) ws, (char *) ws + KV4_MAX_CTAS * sizeof(int), st);
 }
 
 }  // namespace pb

@@ -1,0 +1,62 @@
+// prima.cpp_b200/csrc/kv4_attn.cuh — what the attention kernels over the 4-bit cache share: which pages a sequence's queries see, and in what order.
+#pragma once
+#include "kv4.cuh"
+#include "tc.cuh"
+
+namespace pb {
+
+constexpr int KV4_MAX_CTAS = 256;      // of a launch: parts and counters of the workspace are by CTA
+
+// A sequence: its queries' rows, and the pages that any of them sees: the first `keep`, then those from page `from` on.  At least one page, so that rows which see
+// nothing are written.  All numbers come from device memory and are taken for what they may be: rows beyond the arrays, negative lengths, short tables.
+struct Kv4Seq {
+    int64_t q0;                // first row
+    int n_q, p0;               // queries; position of the first
+    int pages, keep, from;
+    __device__ __forceinline__ long long items(int n_head_kv, int tile) const { return n_q > 0 ? (long long) n_head_kv * ((n_rows + tile - 1) / tile) : 0; }
+    __device__ __forceinline__ long long units(int n_head_kv, int tile) const { return items(n_head_kv, tile) * pages; }
+    int n_rows;                // queries x heads of a group
+};
+// many: sequences with more than most_rows rows, otherwise the others
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_rows, bool many) {
+    Kv4Seq q{};
+    if (s >= A.n_seq) return q;
+    const long long a = A.q_start[s], b = A.q_start[s + 1];
+    if (a < 0 || b <= a || b > A.n_tokens) return q;
+    const int all = (int) (b - a), n = min(all, A.max_q);
+    if (((long long) n * A.group > most_rows) != many) return q;
+    q.q0 = a;
+    q.n_q = n;
+    q.n_rows = n * A.group;
+    const int len = max(A.kv_len[s], 0);
+    q.p0 = len - all;
+    const int last_p = q.p0 + n - 1;
+    q.pages = 1;
+    if (last_p >= 0) {
+        const int ld = (int) (A.table_ld < 0x1ffffff ? A.table_ld : 0x1ffffff);   // cells have 31 bits
+        const int last = min(last_p / KV4_CELLS, ld - 1);
+        int from = 0, keep = 0;
+        if (A.window > 0 && q.p0 - A.window + 1 > 0) {
+            from = (q.p0 - A.window + 1) / KV4_CELLS;
+            keep = min(A.first / KV4_CELLS + (A.first % KV4_CELLS != 0), from);
+        }
+        q.keep = min(keep, last + 1);
+        q.from = from;
+        q.pages = max(1, q.keep + max(0, last + 1 - from));
+    }
+    return q;
+}
+// the i-th of its pages: which one of the sequence, and its number in the pool (-1: none)
+__device__ __forceinline__ int kv4_page_index(const Kv4Seq & q, int i) { return i < q.keep ? i : i - q.keep + q.from; }
+__device__ __forceinline__ int kv4_page(const Kv4Attn & A, const Kv4Seq & q, int s, int i) {
+    const int at = kv4_page_index(q, i);
+    if (q.p0 + q.n_q <= 0 || at >= A.table_ld) return -1;
+    const int id = A.table[s * A.table_ld + at];
+    return id >= 0 && id < A.cache.n_pages ? id : -1;
+}
+
+struct KrWork { int most_rows; int * counters; void * parts; int * abort_flag; };
+size_t kv4_rows_workspace(int D);
+int launch_kv4_attn_rows(const Kv4Attn & a, int D, int type, int most_rows, int * counters, void * parts, cudaStream_t st);
+
+}  // namespace pb

@@ -75,13 +75,13 @@ def unpack(raw, dim):
 
 
 def attend(q, pages, table, q_start, kv_len, n_head_kv, dim, scale, window=0, first=0):
-    """q float64 [tokens, heads, dim], pages uint8 [pages, heads, bytes] of a layer -> (out, bound of the error of a kernel with 32-bit sums in units of the largest
-    value), rows without a sequence NaN.
+    """q float64 [tokens, heads, dim], pages uint8 [pages, heads, bytes] of a layer -> (out, bound of the error of a kernel with 32-bit sums, largest sum of a
+    score's magnitudes); rows without a sequence NaN.
 
     The bound: a score is a sum of dim products, each rounded and added with 2^-23 of the sum of magnitudes at most, twice that for operands of 22 bits; a weight is
     off by its score's error, 2^-22 of the exponential and 2^-23 of its argument, |score| times that; the sums run over steps of 16 cells and 64 parts."""
     out = np.full(q.shape, np.nan)
-    bound = np.zeros(q.shape)
+    bound, reach = np.zeros(q.shape), 0.0
     group = q.shape[1] // n_head_kv
     for s in range(len(kv_len)):
         n = q_start[s + 1] - q_start[s]
@@ -109,9 +109,10 @@ def attend(q, pages, table, q_start, kv_len, n_head_kv, dim, scale, window=0, fi
                 w /= w.sum(-1, keepdims=True)
                 out[row, h * group:(h + 1) * group] = w @ vv
                 mag = (np.abs(qq) @ np.abs(kk).T).max(-1) * abs(scale)
+                reach = max(reach, float(mag.max()))
                 rel = 2 * (dim + 8) * 2.0 ** -23 * mag + np.abs(z).max(-1) * 2.0 ** -22 + 2.0 ** -20 + (see.sum() / 16 + 64) * 2.0 ** -23
                 bound[row, h * group:(h + 1) * group] = (rel * np.abs(vv).max())[:, None]
-    return out, bound
+    return out, bound, reach
 
 
 def append(x, weight, eps, pos, w, mode, n_dims, mscale=1.0):

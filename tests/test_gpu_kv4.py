@@ -74,7 +74,7 @@ class Attn:
         got = (self.out if out is None else out).double().cpu().numpy()
         assert np.all(got[:, self.heads * self.dim:] == 7.0), "behind a row"
         got = got[:, :self.heads * self.dim].reshape(self.tokens, self.heads, self.dim)
-        want, bound = self.want()
+        want, bound, reach = self.want()
         mine = np.zeros(self.tokens, bool)
         for s in range(len(self.kv_np)):
             n = self.q_start_np[s + 1] - self.q_start_np[s]
@@ -89,7 +89,9 @@ class Attn:
         worst = np.max(np.abs(got - want) - tol) if got.size else 0.0
         assert worst <= 0.0, f"{worst} beyond the bound; largest difference {np.max(np.abs(got - want))}"
         if self.type == "f32" and got.size and np.linalg.norm(want) > 0:
-            assert np.linalg.norm(got - want) <= 1e-5 * np.linalg.norm(want)
+            # on the whole much nearer, but for large scores: the last four roundings of one (a block's sum onto the others, the factor, the difference to the maximum) are 2^-24 of up to
+            # the sum of its magnitudes each, and change its weight by as much
+            assert np.linalg.norm(got - want) <= (1e-5 + 2.0 ** -22 * reach) * np.linalg.norm(want)
         return got
 
 
@@ -527,7 +529,7 @@ def test_a_request_from_prompt_to_fork_and_eviction(pkg, lib, cuda):
         lib.check(lib.c.pb200_kv4_attn(C.byref(cache), 0, 0, at[0], W, ptr(out), H * D, H, n, ptr(dev[3]), ptr(dev[4]), ptr(dev[2]), P, T, new, D ** -0.5, 0, 0, ptr(ws), ws.numel(), None))
         torch.cuda.synchronize()
         q = x[:, :H * D].double().cpu().numpy().reshape(T, H, D)
-        want, bound = R.attend(q, pages.cpu().numpy(), table, np.arange(0, T + 1, new), np.array(lens), HK, D, D ** -0.5)
+        want, bound, _ = R.attend(q, pages.cpu().numpy(), table, np.arange(0, T + 1, new), np.array(lens), HK, D, D ** -0.5)
         got = out.double().cpu().numpy().reshape(T, H, D)
         assert np.all(np.abs(got - want) <= bound + 2.0 ** -24 * np.abs(want))
         k, v = (torch.zeros(T, HK * D, device="cuda") for _ in range(2))
