@@ -110,6 +110,9 @@ int pb200_kv4_attn(const pb200_kv4_cache * c, int layer, int type, const void * 
     if (!rows_ok(q, ldq, n_head * D, eb) || !rows_ok(out, ldo, n_head * D, eb)) return PB200_EINVAL;
     if (!ws || ((uintptr_t) ws & 15) || ws_bytes < pb200_kv4_attn_workspace_bytes(n_head, c->n_head_kv, c->head_dim)) return PB200_EINVAL;
     if (n_seq == 0 || n_tokens == 0 || max_q == 0) return 0;
+    // pages of all sequences, heads and tiles of eight rows are counted in 31 bits
+    const double rows = (double) std::min<int64_t>(max_q, n_tokens) * (n_head / c->n_head_kv);
+    if ((double) n_seq * (double) std::min<int64_t>(table_ld, (INT32_MAX / PB200_KV4_CELLS) + 1) * c->n_head_kv * std::ceil(rows / 8) >= 2147483648.0 || rows >= 2147483648.0) return PB200_ENOTSUP;
     if (overlap(q, ((n_tokens - 1) * ldq + n_head * D) * eb, out, ((n_tokens - 1) * ldo + n_head * D) * eb)) return PB200_EINVAL;
     const Kv4Attn a{layer_of(c, layer), q, ldq, out, ldo, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};
     g_launches++;

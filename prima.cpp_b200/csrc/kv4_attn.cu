@@ -88,10 +88,10 @@ int attn(const Kv4Attn & a, int D, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv4_attn_workspace(int D, int, int) { return KV4_MAX_CTAS * sizeof(int) + kv4_rows_workspace(D); }
+size_t kv4_attn_workspace(int D, int, int) { return KV4_COUNTERS * sizeof(int) + kv4_rows_workspace(D); }
 
 int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t st) {
-    return launch_kv4_attn_rows(a, D, type, 1 << 30, (int *) ws, (char *) ws + KV4_MAX_CTAS * sizeof(int), st);
+    return launch_kv4_attn_rows(a, D, type, 1 << 30, (int *) ws, (char *) ws + KV4_COUNTERS * sizeof(int), st);
 }
 
 }  // namespace pb

@@ -5,7 +5,8 @@
 
 namespace pb {
 
-constexpr int KV4_MAX_CTAS = 256;      // of a launch: parts and counters of the workspace are by CTA
+constexpr int KV4_MAX_CTAS = 160;      // of a launch: the workspace has parts by CTA and warp
+constexpr int KV4_COUNTERS = 16384;    // in front of them
 
 // A sequence: its queries' rows, and the pages that any of them sees: the first `keep`, then those from page `from` on.  At least one page, so that rows which see
 // nothing are written.  All numbers come from device memory and are taken for what they may be: rows beyond the arrays, negative lengths, short tables.
@@ -13,9 +14,9 @@ struct Kv4Seq {
     int64_t q0;                // first row
     int n_q, p0;               // queries; position of the first
     int pages, keep, from;
-    __device__ __forceinline__ long long items(int n_head_kv, int tile) const { return n_q > 0 ? (long long) n_head_kv * ((n_rows + tile - 1) / tile) : 0; }
-    __device__ __forceinline__ long long units(int n_head_kv, int tile) const { return items(n_head_kv, tile) * pages; }
     int n_rows;                // queries x heads of a group
+    __device__ __forceinline__ int items(int n_head_kv, int tile) const { return n_q > 0 ? n_head_kv * ((n_rows + tile - 1) / tile) : 0; }
+    __device__ __forceinline__ int units(int n_head_kv, int tile) const { return items(n_head_kv, tile) * pages; }
 };
 // many: sequences with more than most_rows rows, otherwise the others
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_rows, bool many) {

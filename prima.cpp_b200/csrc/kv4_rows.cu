@@ -11,10 +11,11 @@
 // the tensor core's alignment of its 16 terms.  16-bit queries are one f16 number, exactly: a row is scaled by a power of two.
 // Softmax by running maximum and sum, per page of 64 cells.
 //
-// Work.  The pages that a (sequence, tile, kv head) sees, all of them in a row, are dealt out to the CTAs in equal shares, so that lengths do not matter; a CTA's warps take the
-// pages of its share in turns, each through a ring of its own (one bulk copy per page: a head's chunk is contiguous), and add up an item in shared memory.  An item that
-// is cut goes through the workspace: the CTA that comes last adds the parts in their order (no atomics on numbers, equal calls give equal bits).  Where items have fewer pages than a
-// CTA has warps, a warp takes whole items.
+// Work.  The pages that a (sequence, tile, kv head) sees, all of them in a row, are dealt out to the warps in equal shares, so that lengths do not matter.  A warp walks its
+// share by itself, pages on their way through a ring of its own (one bulk copy per page: a head's chunk is contiguous), and writes items that it has whole.  Of one that is cut it leaves
+// its part in the workspace; once a CTA's warps are through, those that share an item add up its parts, and where it reaches beyond the CTA, the last warp of all adds
+// what the CTAs have: always in their order (no atomics on numbers, equal calls give equal bits).  One barrier a CTA: with one per item, warps waited for each other for a
+// page's time at every item (83 us for 32 sequences of up to 8192 cells).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -27,21 +28,31 @@
 namespace pb {
 namespace {
 
-constexpr int KR_WARPS = 12, KR_THREADS = 32 * KR_WARPS, KR_ROWS = 8;
+constexpr int KR_ROWS = 8;
+// Warps of a CTA, one CTA to an SM: 168 registers (16 warps of 128: 94 us for two sequences of 131071 and 65001 cells, these 65).  Stages of a warp's ring: a page each.
+constexpr int KR_WARPS = 12, KR_THREADS = 32 * KR_WARPS;
 template <int D> constexpr int kr_stages() { return D == 128 ? 2 : 4; }
 constexpr int KR_UP = 12;   // F32: weights are 2^12 larger than exp(score - maximum): those of 2^-26 are normal f16 numbers
 
-// what a warp hands to its CTA, a CTA to the last one: sums of 2^(score - m) v, and of the weights
-template <int D> struct KrPart { float o[KR_ROWS][D + 4]; float m[KR_ROWS], l[KR_ROWS]; };
-static_assert(sizeof(KrPart<128>) <= kv4_chunk_bytes(128) && sizeof(KrPart<64>) <= kv4_chunk_bytes(64), "a warp's part goes through its ring");
+// a part of an item: sums of 2^(score - m) v, and of the weights
+template <int D> struct KrPart { float o[KR_ROWS][D]; float m[KR_ROWS], l[KR_ROWS]; };
+// workspace: parts of the warps (0: of an item that began before the warp's share, 1: of one that begins in it and goes on), parts of the CTAs in the same way
+template <int D> struct KrParts { KrPart<D> warp[KV4_MAX_CTAS * KR_WARPS][2], cta[KV4_MAX_CTAS][2]; };
 
+// A segment: pages [pa, pb) (of those that it sees) of an item, which are the units k0 .. u - 1.
+struct KrSegment {
+    Kv4Seq q;
+    int s, before;             // the sequence, units in front of it
+    int u;                     // the unit behind the segment
+    int tile, hk, pa, pb, k0;
+};
 template <int D> struct __align__(128) KrSmem {
     __align__(128) uint8_t ring[KR_WARPS][kr_stages<D>()][kv4_chunk_bytes(D)];
     uint64_t full[KR_WARPS][kr_stages<D>()];
-    long long scan[KR_WARPS], items[KR_WARPS], before[KR_WARPS];
-    KrPart<D> * part[KR_WARPS];
-    int seq[KR_WARPS];
-    int last, abort;
+    KrSegment get[KR_WARPS];   // where each warp's fetching is
+    KrSegment begin[KR_WARPS];
+    int scan[KR_WARPS];
+    int abort;
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -54,16 +65,63 @@ __device__ __forceinline__ void mma16816_from(float (&d)[4], float c0, float c1,
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
-__device__ __forceinline__ void fma2(float & x, float & y, float a, float b, float d) {   // x += a d, y += b d
-    asm("{\n.reg .b64 p, q, r;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %3};\nmov.b64 r, {%4, %4};\nfma.rn.f32x2 p, q, r, p;\nmov.b64 {%0, %1}, p;\n}" : "+f"(x), "+f"(y) : "f"(a), "f"(b), "f"(d));
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+template <typename T> __device__ __forceinline__ float2 to_f32x2(uint32_t w) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+
+// four numbers of a row of an item: parts added up in their order
+struct KrSum {
+    float top = -INFINITY, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    // of a part with maximum mi where all parts' is t (a row that is no number has no maximum)
+    static __device__ __forceinline__ float factor(float mi, float li, float t) { return mi == -INFINITY ? (li == li ? 0.f : 1.f) : ex2(mi - t); }
+    template <typename At>
+    __device__ __forceinline__ void add(int n, int r, int d4, At && at) {
+        constexpr int ONCE = 8;                          // on their way from L2 together
+        for (int i0 = 0; i0 < n; i0 += ONCE) {
+            float mi[ONCE], li[ONCE], t = top;
+            float4 y[ONCE];
+#pragma unroll
+            for (int k = 0; k < ONCE; k++) {
+                const auto * p = at(min(i0 + k, n - 1));
+                mi[k] = __ldcg(&p->m[r]);
+                li[k] = __ldcg(&p->l[r]);
+                y[k] = __ldcg(reinterpret_cast<const float4 *>(&p->o[r][d4]));
+            }
+#pragma unroll
+            for (int k = 0; k < ONCE; k++) t = fmaxf(t, mi[k]);
+            const float f = factor(top, l, t);
+            top = t;
+            l *= f;
+            x.x *= f; x.y *= f; x.z *= f; x.w *= f;
+#pragma unroll
+            for (int k = 0; k < ONCE; k++)
+                if (i0 + k < n) {
+                    const float h = factor(mi[k], li[k], t);
+                    l = fmaf(li[k], h, l);
+                    x.x = fmaf(y[k].x, h, x.x); x.y = fmaf(y[k].y, h, x.y); x.z = fmaf(y[k].z, h, x.z); x.w = fmaf(y[k].w, h, x.w);
+                }
+        }
+    }
+    template <typename T> __device__ __forceinline__ void write(T * to) const {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        store4(to, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    }
+};
+// row r of a segment's tile in the output
+template <typename T, int D>
+__device__ __forceinline__ T * kr_row(const Kv4Attn & A, const KrSegment & at, int r) {
+    const int row = at.tile * KR_ROWS + r, t = row / A.group;
+    return (T *) A.out + (at.q.q0 + t) * A.ldo + (int64_t) (at.hk * A.group + row - t * A.group) * D;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_constant__ Kv4Attn A, const __grid_constant__ KrWork W) {
@@ -74,60 +132,62 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
     KrSmem<D> & S = *reinterpret_cast<KrSmem<D> *>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31, g = lane >> 2, c = lane & 3;
     volatile int * cta_abort = &S.abort;
-    if (tid < KR_WARPS * STAGES) mbar_init(&S.full[tid / STAGES][tid % STAGES], 1);
-    if (tid == 0) { mbar_fence_init(); S.abort = 0; }
-
-    // ---- shares: units (pages of items) in the order of sequences, tiles, heads, pages ----
     const int hks = A.cache.n_head_kv;
-    long long units = 0, items = 0, n = 0;     // n: of this thread's last sequence
-    for (int s = tid; s < A.n_seq; s += KR_THREADS) {
-        const Kv4Seq q = kv4_seq(A, s, W.most_rows, false);
-        n = q.units(hks, KR_ROWS);
-        units += n;
-        items += q.items(hks, KR_ROWS);
+
+    // ---- shares: units (pages of items) in the order of sequences, tiles, heads, pages; a thread has a sequence ----
+    Kv4Seq mine = kv4_seq(A, tid, W.most_rows, false);
+    int n = mine.units(hks, KR_ROWS), units = n;
+    if (lane < STAGES) {
+        mbar_init(&S.full[warp][lane], 1);
+        mbar_fence_init();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    long long x = units;                       // sums over the lanes up to this one
+    if (tid == 0) S.abort = 0;
+    for (int s = tid + KR_THREADS; s < A.n_seq; s += KR_THREADS) units += kv4_seq(A, s, W.most_rows, false).units(hks, KR_ROWS);
+    auto upto = [&](int x) {                   // sum over the lanes up to this one
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-        items += __shfl_xor_sync(0xffffffffu, items, o);
-    }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        return x;
+    };
+    int x = upto(units);
     if (lane == 31) S.scan[warp] = x;
-    if (lane == 0) S.items[warp] = items;
     __syncthreads();
-    long long total = 0, n_items = 0, front = 0;
+    int total = 0, front = 0;
 #pragma unroll
     for (int w = 0; w < KR_WARPS; w++) {
-        if (w < warp) front += S.scan[w];
-        total += S.scan[w];
-        n_items += S.items[w];
+        const int k = S.scan[w];
+        if (w < warp) front += k;
+        total += k;
     }
     if (total == 0) return;
-    const bool by_warp = total < n_items * KR_WARPS;    // fewer pages an item than a CTA has warps
-    const long long among = by_warp ? (long long) gridDim.x * KR_WARPS : (long long) gridDim.x;
-    long long share = (total + among - 1) / among;
-    if (!by_warp && share < KR_WARPS) share = KR_WARPS;
-    // the sequences in which the shares begin
-    const long long cta0 = (long long) blockIdx.x * (by_warp ? KR_WARPS : 1) * share;
-    auto begins = [&](int s, long long before, long long n) {
+    // warps at work in a CTA: few pages go to one warp of each of an SM's four schedulers, on as many SMs as that takes
+    const int at_work = total >= (int) gridDim.x * KR_WARPS ? KR_WARPS : max(4, (total + (int) gridDim.x - 1) / (int) gridDim.x);
+    const int share = (int) (((unsigned) total + gridDim.x * at_work - 1) / (gridDim.x * at_work));
+    const int me = blockIdx.x * at_work + warp;
+    // the sequences in which the warps' shares begin
+    const long long cta0 = (long long) blockIdx.x * at_work * share;
+    auto begins = [&](const Kv4Seq & q, int s, int before, int n) {
+        if (before >= cta0 + (long long) at_work * share || before + n <= cta0) return;
 #pragma unroll 1
-        for (int w = 0; w < (by_warp ? KR_WARPS : 1); w++) {
+        for (int w = 0; w < at_work; w++) {
             const long long u = cta0 + w * share;
-            if (u >= before && u < before + n) { S.seq[w] = s; S.before[w] = before; }
+            if (u >= before && u < before + n) {
+                S.begin[w].q = q;
+                S.begin[w].s = s;
+                S.begin[w].before = before;
+            }
         }
     };
-    if (A.n_seq <= KR_THREADS) begins(tid, front + x - units, units);
+    if (A.n_seq <= KR_THREADS) begins(mine, tid, front + x - n, n);
     else {
-        long long before = 0;
+        int before = 0;
         for (int s0 = 0; s0 < A.n_seq; s0 += KR_THREADS) {
-            n = kv4_seq(A, s0 + tid, W.most_rows, false).units(hks, KR_ROWS);
-            x = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
+            mine = kv4_seq(A, s0 + tid, W.most_rows, false);
+            n = mine.units(hks, KR_ROWS);
+            x = upto(n);
             __syncthreads();
             if (lane == 31) S.scan[warp] = x;
             __syncthreads();
@@ -136,113 +196,126 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                 if (w < warp) front += S.scan[w];
                 before += S.scan[w];
             }
-            begins(s0 + tid, front + x - n, n);
+            begins(mine, s0 + tid, front + x - n, n);
         }
     }
     __syncthreads();
-    const long long u0 = cta0 + (by_warp ? warp * share : 0), u1 = u0 + share < total ? u0 + share : total;
+    const long long u0_ = cta0 + (long long) warp * share;
+    const int u0 = warp < at_work && u0_ < total ? (int) u0_ : total, u1 = total - u0 < share ? total : u0 + share;
 
-    // a place in the row of units: sequence, its first unit, the unit
-    struct Place { long long u, before; int s; Kv4Seq q; };
-    auto settle = [&](Place & p) {   // onto a sequence that has unit p.u
-        while (p.u < u1 && p.u >= p.before + p.q.units(hks, KR_ROWS)) {
+    // the segment that begins at p.u: false if there is none in the share
+    auto next = [&](KrSegment & p) {
+        if (p.u >= u1) return false;
+        while (p.u - p.before >= p.q.units(hks, KR_ROWS)) {
             p.before += p.q.units(hks, KR_ROWS);
-            p.s++;
+            if (++p.s >= A.n_seq) return false;
             p.q = kv4_seq(A, p.s, W.most_rows, false);
         }
-    };
-    Place get{u0, 0, 0, {}};
-    if (u0 < u1) {
-        get.s = S.seq[by_warp ? warp : 0];
-        get.before = S.before[by_warp ? warp : 0];
-        get.q = kv4_seq(A, get.s, W.most_rows, false);
-    }
-    if (by_warp && u0 < u1) {   // whole items: those that begin in the share
-        const long long in = get.u - get.before;
-        const long long r = in % get.q.pages;
-        if (r) get.u += get.q.pages - r;
-        settle(get);
-    }
-    Place put = get;
-
-    // ---- pages on their way: the share's pages go to the warps in turns, of a segment [pa, pb) of an item every step-th from pa + first on ----
-    const int step = by_warp ? 1 : KR_WARPS;
-    auto first_of = [&](long long u) { return by_warp ? 0 : (warp + KR_WARPS - (int) ((u - u0) % KR_WARPS)) % KR_WARPS; };   // u: the segment's first unit
-    uint64_t policy;
-    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    int f_pb = 0, f_page = 0, f_hk = 0;       // the segment that is fetched, the next page of it
-    bool f_more = false;
-    auto segment = [&](Place & p, int & pa, int & pb, int & tile, int & hk, int & first) {   // false: no more
-        if (p.u >= u1) return false;
-        settle(p);
-        const long long in = p.u - p.before;
-        const int item = (int) (in / p.q.pages);
-        pa = (int) (in - (long long) item * p.q.pages);
-        const long long rest = by_warp ? p.q.pages : u1 - p.u;
-        pb = (int) (pa + rest < p.q.pages ? pa + rest : p.q.pages);
-        tile = item / hks;
-        hk = item % hks;
-        first = pa + first_of(p.u);
-        p.u += pb - pa;
+        const int in = p.u - p.before, item = in / p.q.pages;
+        p.pa = in - item * p.q.pages;
+        p.pb = min(p.q.pages, p.pa + u1 - p.u);
+        p.tile = item / hks;
+        p.hk = item - p.tile * hks;
+        p.k0 = p.u;
+        p.u += p.pb - p.pa;
         return true;
     };
-    auto next_page = [&]() {   // page number of the next page of this warp, or -1 (nothing to fetch); moves on
-        while (true) {
-            if (f_more && f_page < f_pb) {
-                const int i = f_page;
-                f_page += step;
-                return kv4_page(A, get.q, get.s, i);
-            }
-            int pa, tile;
-            f_more = segment(get, pa, f_pb, tile, f_hk, f_page);
-            if (!f_more) return -2;
-        }
-    };
-    uint32_t issued = 0, used = 0;                      // pages asked for and taken, of this warp
-    int ids[STAGES];                                    // their numbers (-1: none), by stage
-    auto fetch = [&]() {
-        const int id = next_page();
-        const int st = (int) (issued % STAGES);
+    KrSegment put;
+    bool more = false;
+    if (u0 < u1) {
+        put = S.begin[warp];
+        put.u = u0;
+        more = next(put);
+    }
+    // queries of a segment: lane (g, c) has of row g the numbers 32 b + 8 c + e
+    constexpr int RAW = F32 ? 4 : 2;
+    uint32_t raw[NB][2][RAW];
+    auto ask = [&](const KrSegment & p) {
+        const int row = p.tile * KR_ROWS + g;
+        const bool have = row < p.q.n_rows;
+        const int t = row / A.group;
+        const T * src = (const T *) A.q + (p.q.q0 + t) * A.ldq + (int64_t) (p.hk * A.group + row - t * A.group) * D + 8 * c;
 #pragma unroll
-        for (int i = 0; i < STAGES; i++)
-            if (i == st) ids[i] = id;
-        if (id >= 0 && elect_one()) {
-            mbar_arrive_expect_tx(&S.full[warp][st], CHUNK);
-            bulk_g2s(S.ring[warp][st], kv4_chunk<D>(A.cache, id, f_hk), CHUNK, &S.full[warp][st], policy);
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if constexpr (F32) {
+                    const uint4 w = have ? *reinterpret_cast<const uint4 *>(src + 32 * b + 4 * h) : make_uint4(0u, 0u, 0u, 0u);
+                    raw[b][h][0] = w.x; raw[b][h][1] = w.y; raw[b][h][2] = w.z; raw[b][h][3] = w.w;
+                } else {
+                    const uint2 w = have ? *reinterpret_cast<const uint2 *>(src + 32 * b + 4 * h) : make_uint2(0u, 0u);
+                    raw[b][h][0] = w.x; raw[b][h][1] = w.y;
+                }
+            }
+    };
+    if (more) ask(put);                                 // ahead of the pages, which fill the memory's queues
+
+    // ---- pages on their way: unit u goes through stage (u - u0) % STAGES ----
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    if (more && lane == 0) S.get[warp] = put;
+    __syncwarp();
+    uint32_t none = 0;                                  // stages whose page is none: nothing is on its way
+    auto fetch = [&](int u) {                           // by ascending u
+        if (u >= u1) return;
+        if (u >= S.get[warp].u) {
+            KrSegment p = S.get[warp];
+            next(p);
+            __syncwarp();
+            if (lane == 0) S.get[warp] = p;
+            __syncwarp();
+        }
+        const KrSegment & p = S.get[warp];
+        const int id = kv4_page(A, p.q, p.s, p.pa + u - p.k0), st = (u - u0) % STAGES;
+        none = id >= 0 ? none & ~(1u << st) : none | 1u << st;
+        if (elect_one()) {
+            if (id >= 0) {
+                mbar_arrive_expect_tx(&S.full[warp][st], CHUNK);
+                bulk_g2s(S.ring[warp][st], kv4_chunk<D>(A.cache, id, p.hk), CHUNK, &S.full[warp][st], policy);
+            } else mbar_arrive(&S.full[warp][st]);
         }
         __syncwarp();
-        issued++;
     };
-    uint32_t phases = 0;
-    for (int i = 0; i < STAGES; i++) fetch();
+    for (int k = 0; k < STAGES; k++) fetch(u0 + k);
 
     // ---- segments ----
-    int pa, pb, tile, hk, first;
-    while (segment(put, pa, pb, tile, hk, first)) {
-        const Kv4Seq q = put.q;
-        const int row0 = tile * KR_ROWS, rows = min(KR_ROWS, q.n_q * A.group - row0);
-        // queries: lane (g, c) has of row g the numbers 32 b + 8 c + e, as pairs; F32: two f16 numbers each (high, low), otherwise pairs 1 and 3 a 16th
+    KrParts<D> & parts = *reinterpret_cast<KrParts<D> *>(W.parts);
+    KrSegment cut[2];                                   // items of which this warp has a part: one that began before, one that goes on
+    cut[0].q.n_q = cut[1].q.n_q = 0;
+    while (more) {
+        const KrSegment at = put;
+        const Kv4Seq & q = at.q;
+        const int row0 = at.tile * KR_ROWS, rows = min(KR_ROWS, q.n_rows - row0);
+        // queries as pairs; F32: two f16 numbers each (high, low), otherwise pairs 1 and 3 a 16th
         uint32_t qf[LO][NB][4];
         float start[NB][2], mult[2];
         int pos[2];
         {
-            float x[NB][8];
+            float x[NB][8], top = 0.f;
             const int row = row0 + g;
             const bool have = g < rows;
-            const T * src = (const T *) A.q + (q.q0 + row / A.group) * A.ldq + (int64_t) (hk * A.group + row % A.group) * D + 8 * c;
-            float top = 0.f;
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const float4 lo4 = have ? load4(src + 32 * b) : make_float4(0.f, 0.f, 0.f, 0.f), hi4 = have ? load4(src + 32 * b + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-                x[b][0] = lo4.x; x[b][1] = lo4.y; x[b][2] = lo4.z; x[b][3] = lo4.w;
-                x[b][4] = hi4.x; x[b][5] = hi4.y; x[b][6] = hi4.z; x[b][7] = hi4.w;
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[b][e]));
-            }
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[b][4 * h + e] = __uint_as_float(raw[b][h][e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float2 v = to_f32x2<T>(raw[b][h][e]);
+                            x[b][4 * h + 2 * e] = v.x;
+                            x[b][4 * h + 2 * e + 1] = v.y;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[b][4 * h + e]));
+                }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // the row's power of two: its largest number comes to 2^13 .. 2^14
-            const int ex = top > 0.f && top < INFINITY ? max(-126, min(126, 13 - ilogbf(top))) : 0;
+            const int ex = top > 0.f && top < INFINITY ? min(126, 140 - (int) (__float_as_uint(top) >> 23)) : 0;
             const float up = __int_as_float((ex + 127) << 23) * (A.scale < 0.f ? -1.f : 1.f);
             float sums[NB];
 #pragma unroll
@@ -265,45 +338,34 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             }
             // of a row's sums: the power of two, n * 2^-24, and scores in units of log2; never 0: a masked score stays -inf
             const float down = fmaxf(fabsf(A.scale) * (F32 ? 1.4426950408889634f : 1.4426950408889634f * 16777216.f) * __int_as_float((127 - ex) << 23), FLT_MIN);
-            const int at = q.p0 + row / A.group;
+            const int p = q.p0 + row / A.group;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int from = 4 * (2 * c + i);                               // a lane of row 2 c + i
                 mult[i] = __shfl_sync(0xffffffffu, down, from);
-                pos[i] = __shfl_sync(0xffffffffu, have ? at : -1, from);
+                pos[i] = __shfl_sync(0xffffffffu, have ? p : -1, from);
 #pragma unroll
                 for (int b = 0; b < NB; b++) start[b][i] = F32 ? 0.f : __shfl_sync(0xffffffffu, sums[b], from);
             }
         }
         const int p_lo = q.p0 + row0 / A.group, p_hi = q.p0 + (row0 + rows - 1) / A.group;   // of the tile's rows
 
-        // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1; 16 bits: odd numbers 16 times as large, and o8: 8 times the sum of scaled weights (odd: 128 times)
-        float o[NB][2][4], o8[F32 ? 1 : NB][4];
+        // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1 (16 bits: times 2^-24, and 2^-20 the odd ones)
+        float o[NB][2][4];
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
         int up = F32 ? KR_UP : 15;                      // weights are exp(score - maximum) * 2^up
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                o[b][0][i] = o[b][1][i] = 0.f;
-                if constexpr (!F32) o8[b][i] = 0.f;
-            }
-        bool any = false;
-        uint8_t * held = nullptr;                       // the stage of the segment's last page: handed back behind the merge
-        for (int i = first; i < pb; i += step) {
-            const int st = (int) (used % STAGES);
-            int id = -1;
-#pragma unroll
-            for (int k = 0; k < STAGES; k++)
-                if (k == st) id = ids[k];
-            used++;
-            const bool keep = !by_warp && i + step >= pb;
-            if (id >= 0) {
-                mbar_wait(&S.full[warp][st], phases >> st & 1, cta_abort, W.abort_flag);
-                phases ^= 1u << st;
+            for (int i = 0; i < 4; i++) o[b][0][i] = o[b][1][i] = 0.f;
+        for (int u = at.k0; u < at.u; u++) {
+            const int st = (u - u0) % STAGES;
+            const bool have = !(none >> st & 1);
+            mbar_wait(&S.full[warp][st], (uint32_t) ((u - u0) / STAGES) & 1, cta_abort, W.abort_flag);
+            if (have) {
                 uint8_t * chunk = S.ring[warp][st];
                 uint8_t * const vs = chunk + 2 * kv4_rows_bytes(D) + kv4_scales_bytes(D);
-                const int base = kv4_page_index(q, i) * KV4_CELLS;
+                const int base = kv4_page_index(q, at.pa + u - at.k0) * KV4_CELLS;
                 const bool whole = base + 63 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + 63 < A.first);
                 if (!whole) {   // a weight of zero does not silence a scale that is no number: cells nobody sees may hold anything
 #pragma unroll
@@ -331,8 +393,6 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                     }
                     const uint8_t * ks = chunk + 2 * kv4_rows_bytes(D) + kv4_scale(D, 16 * j + g, 0);
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; i4++) sc[j][i4] = 0.f;
-#pragma unroll
                     for (int b = 0; b < NB; b++) {
                         float acc[4];
                         const uint32_t a1 = wa[b] >> 8, b1 = wb[b] >> 8;
@@ -348,8 +408,11 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                             mma16816_from(acc, start[b][0], start[b][1], wa[b] & 0x000f000fu, wb[b] & 0x000f000fu, wa[b] & 0x00f000f0u, wb[b] & 0x00f000f0u, qf[0][b][0], qf[0][b][1]);
                             mma16816(acc, a1 & 0x000f000fu, b1 & 0x000f000fu, a1 & 0x00f000f0u, b1 & 0x00f000f0u, qf[0][b][2], qf[0][b][3]);
                         }
-                        fma2(sc[j][0], sc[j][1], acc[0], acc[1], __half2float(*reinterpret_cast<const __half *>(ks + 4 * b)));
-                        fma2(sc[j][2], sc[j][3], acc[2], acc[3], __half2float(*reinterpret_cast<const __half *>(ks + 4 * b + 16 * NB)));
+                        const float da = __half2float(*reinterpret_cast<const __half *>(ks + 4 * b)), db = __half2float(*reinterpret_cast<const __half *>(ks + 4 * b + 16 * NB));
+                        sc[j][0] = b == 0 ? acc[0] * da : fmaf(acc[0], da, sc[j][0]);
+                        sc[j][1] = b == 0 ? acc[1] * da : fmaf(acc[1], da, sc[j][1]);
+                        sc[j][2] = b == 0 ? acc[2] * db : fmaf(acc[2], db, sc[j][2]);
+                        sc[j][3] = b == 0 ? acc[3] * db : fmaf(acc[3], db, sc[j][3]);
                     }
                 }
                 if (!whole) {
@@ -399,10 +462,6 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                             o[b][h][0] *= f[0]; o[b][h][1] *= f[1];
                             o[b][h][2] *= f[0]; o[b][h][3] *= f[1];
                         }
-                        if constexpr (!F32) {
-                            o8[b][0] *= f[0]; o8[b][1] *= f[1];
-                            o8[b][2] *= f[0]; o8[b][3] *= f[1];
-                        }
                     }
                 }
                 const float off[2] = {m[0] == -INFINITY ? 0.f : (float) up - m[0], m[1] == -INFINITY ? 0.f : (float) up - m[1]};
@@ -411,7 +470,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
 #pragma unroll
                 for (int x8 = 0; x8 < 8; x8++) {
                     const float e0 = ex2(fmaf(sc[x8 >> 1][2 * (x8 & 1)], mult[0], off[0])), e1 = ex2(fmaf(sc[x8 >> 1][2 * (x8 & 1) + 1], mult[1], off[1]));
-                    fma2(l[0], l[1], e0, e1, 1.f);
+                    l[0] += e0;
+                    l[1] += e1;
                     const __half2 h = __floats2half2_rn(e0, e1);
                     pf[0][x8] = transposed(h2u(h));
                     if constexpr (F32) {
@@ -461,17 +521,17 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                             const uint32_t s0 = u[0] >> 8, s1 = u[1] >> 8;
                             mma16816(o[b][0], u[0] & 0x000f000fu, u[0] & 0x00f000f0u, u[1] & 0x000f000fu, u[1] & 0x00f000f0u, p0, p1);
                             mma16816(o[b][1], s0 & 0x000f000fu, s0 & 0x00f000f0u, s1 & 0x000f000fu, s1 & 0x00f000f0u, p0, p1);
-                            mma16816(o8[b], 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, p0, p1);
+#pragma unroll
+                            for (int h = 0; h < 2; h++) mma16816(o[b][h], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, p0, p1);   // - 8
                         }
                     }
                 }
-                any = true;
             }
-            if (!keep) {
-                __syncwarp();
-                fetch();
-            } else held = S.ring[warp][st];
+            __syncwarp();
+            fetch(u + STAGES);
         }
+        more = next(put);
+        if (more) ask(put);                             // the next item's queries, on their way meanwhile
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             l[k] += __shfl_xor_sync(0xffffffffu, l[k], 4);
@@ -484,98 +544,75 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) o[b][h][i] = (o[b][h][i] - o8[b][i]) * (i < 2 ? 16777216.f : 1048576.f);
-        T * out = (T *) A.out + (int64_t) hk * A.group * D;
-        auto row_of = [&](int r) { return out + (q.q0 + (row0 + r) / A.group) * A.ldo + (int64_t) ((row0 + r) % A.group) * D; };
-        if (by_warp) {
+                    for (int i = 0; i < 4; i++) o[b][h][i] *= i < 2 ? 16777216.f : 1048576.f;
+        if (at.pa == 0 && at.pb == q.pages) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const int r = 2 * c + k;
                 const float inv = l[k] == 0.f ? 0.f : 1.f / l[k];
-                if (r < rows)
+                if (r < rows) {
+                    T * to = kr_row<T, D>(A, at, r) + 4 * g;
 #pragma unroll
-                    for (int b = 0; b < NB; b++)
-                        store4(row_of(r) + 32 * b + 4 * g, make_float4(o[b][0][k] * inv, o[b][0][2 + k] * inv, o[b][1][k] * inv, o[b][1][2 + k] * inv));
+                    for (int b = 0; b < NB; b++) store4(to + 32 * b, make_float4(o[b][0][k] * inv, o[b][0][2 + k] * inv, o[b][1][k] * inv, o[b][1][2 + k] * inv));
+                }
             }
-            continue;
-        }
-        // ---- the CTA's sum ----
-        KrPart<D> * part = reinterpret_cast<KrPart<D> *>(held);
-        if (any) {
-            __syncwarp();
+        } else {
+            const int which = at.pa > 0 ? 0 : 1;
+            if (which) cut[1] = at; else cut[0] = at;
+            KrPart<D> & to = parts.warp[me][which];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const int r = 2 * c + k;
 #pragma unroll
-                for (int b = 0; b < NB; b++) *reinterpret_cast<float4 *>(&part->o[r][32 * b + 4 * g]) = make_float4(o[b][0][k], o[b][0][2 + k], o[b][1][k], o[b][1][2 + k]);
-                if (g == 0) { part->m[r] = m[k] - (float) up; part->l[r] = l[k]; }
+                for (int b = 0; b < NB; b++) *reinterpret_cast<float4 *>(&to.o[r][32 * b + 4 * g]) = make_float4(o[b][0][k], o[b][0][2 + k], o[b][1][k], o[b][1][2 + k]);
+                if (g == 0) { to.m[r] = m[k] - (float) up; to.l[r] = l[k]; }
             }
         }
-        if (lane == 0) S.part[warp] = any ? part : nullptr;
-        __syncthreads();
-        const bool full = pa == 0 && pb == q.pages;
-        KrPart<D> * ws = reinterpret_cast<KrPart<D> *>(W.parts);
-        KrPart<D> * to = &ws[2 * blockIdx.x + (pa > 0 ? 0 : 1)];
-        const int r = tid / (D / 4), d4 = 4 * (tid % (D / 4));
-        auto write = [&](float4 x, float sum) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (r < rows) store4(row_of(r) + d4, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-        };
-        // parts in their order: at(i) is one, or none
-        float top = -INFINITY, sum = 0.f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](float mi, float li, float4 y) {
-            const float tn = fmaxf(top, mi);
-            const float f = top == -INFINITY ? (sum == sum ? 0.f : 1.f) : ex2(top - tn), h = mi == -INFINITY ? (li == li ? 0.f : 1.f) : ex2(mi - tn);
-            top = tn;
-            sum = sum * f + li * h;
-            x.x = x.x * f + y.x * h; x.y = x.y * f + y.y * h; x.z = x.z * f + y.z * h; x.w = x.w * f + y.w * h;
-        };
-        if (r < KR_ROWS) {
-#pragma unroll 2
-            for (int i = 0; i < KR_WARPS; i++)
-                if (const KrPart<D> * p = S.part[i]) add(p->m[r], p->l[r], *reinterpret_cast<const float4 *>(&p->o[r][d4]));
-            if (full) write(x, sum);
-            else {
-                *reinterpret_cast<float4 *>(&to->o[r][d4]) = x;
-                if (d4 == 0) { to->m[r] = top; to->l[r] = sum; }
+    }
+
+    // ---- items that were cut ----
+    __syncthreads();                                    // the CTA's parts are there
+#pragma unroll 1
+    for (int i = 0; i < 2; i++) {
+        const KrSegment & at = cut[i];
+        if (at.q.n_q == 0) continue;
+        const int a0 = at.before + (at.tile * hks + at.hk) * at.q.pages;             // the item's first unit
+        const int w0 = a0 / share, w1 = (a0 + at.q.pages - 1) / share;               // the warps that share it
+        const int f0 = max(w0, (int) blockIdx.x * at_work), f1 = min(w1, (int) blockIdx.x * at_work + at_work - 1);   // of this CTA
+        const bool here = f0 == w0 && f1 == w1;
+        const int rows = min(KR_ROWS, at.q.n_rows - at.tile * KR_ROWS);
+        KrPart<D> & mid = parts.cta[blockIdx.x][f0 == w0 ? 1 : 0];
+        // slices of 32 x 4 numbers: a warp of the CTA each, and where the item reaches beyond the CTA, the last of them among the CTAs adds theirs
+        constexpr int SLICES = KR_ROWS * D / 128;
+        const int b0 = me - f0, many = f1 - f0 + 1;
+        for (int b = b0; b < SLICES; b += many) {
+            const int e = b * 32 + lane, r = e / (D / 4), d4 = 4 * (e % (D / 4));
+            KrSum sum;
+            sum.add(many, r, d4, [&](int k) { return &parts.warp[f0 + k][f0 + k == w0 ? 1 : 0]; });
+            if (here) {
+                if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
+            } else {
+                *reinterpret_cast<float4 *>(&mid.o[r][d4]) = sum.x;
+                if (d4 == 0) { mid.m[r] = sum.top; mid.l[r] = sum.l; }
             }
         }
-        if (!full) {
-            const long long a0 = put.before + (long long) (tile * hks + hk) * q.pages;                     // the item's first unit
-            const int c0 = (int) (a0 / share), n_parts = (int) ((a0 + q.pages - 1) / share) - c0 + 1;       // the CTAs that share it
+        if (here || b0 >= SLICES) continue;
+        __syncwarp();
+        const int c0 = w0 / at_work, c1 = w1 / at_work;
+        bool last = false;
+        if (lane < SLICES && lane % many == b0) {
+            __threadfence();                            // behind the warp's barrier: all its lanes' numbers
+            int * counter = &W.counters[w0 * SLICES + lane];
+            last = atomicAdd(counter, 1) == c1 - c0;
+            if (last) *counter = 0;
             __threadfence();
-            __syncthreads();
-            if (tid == 0) S.last = atomicAdd(&W.counters[c0], 1) == n_parts - 1;
-            __syncthreads();
-            if (S.last) {
-                __threadfence();
-                if (r < KR_ROWS) {
-                    top = -INFINITY; sum = 0.f; x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    constexpr int AT_ONCE = 8;                       // on their way from L2 together
-                    for (int i0 = 0; i0 < n_parts; i0 += AT_ONCE) {
-                        float mi[AT_ONCE], li[AT_ONCE];
-                        float4 y[AT_ONCE];
-#pragma unroll
-                        for (int k = 0; k < AT_ONCE; k++) {
-                            const int i = min(i0 + k, n_parts - 1);
-                            const KrPart<D> * p = &ws[2 * (c0 + i) + (i == 0 ? 1 : 0)];
-                            mi[k] = __ldcg(&p->m[r]);
-                            li[k] = __ldcg(&p->l[r]);
-                            y[k] = __ldcg(reinterpret_cast<const float4 *>(&p->o[r][d4]));
-                        }
-#pragma unroll
-                        for (int k = 0; k < AT_ONCE; k++)
-                            if (i0 + k < n_parts) add(mi[k], li[k], y[k]);
-                    }
-                    write(x, sum);
-                }
-                if (tid == 0) W.counters[c0] = 0;
-            }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // what was read and written of a stage, the next copy overwrites
-        __syncthreads();
-        if (held) fetch();
+        for (uint32_t left = __ballot_sync(0xffffffffu, last); left; left &= left - 1) {
+            const int e = (__ffs((int) left) - 1) * 32 + lane, r = e / (D / 4), d4 = 4 * (e % (D / 4));
+            KrSum sum;
+            sum.add(c1 - c0 + 1, r, d4, [&](int k) { return &parts.cta[c0 + k][k == 0 ? 1 : 0]; });
+            if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
+        }
     }
 }
 
@@ -592,7 +629,8 @@ int rows_launch(const Kv4Attn & a, const KrWork & w, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv4_rows_workspace(int D) { return 2 * (size_t) KV4_MAX_CTAS * (D == 128 ? sizeof(KrPart<128>) : sizeof(KrPart<64>)); }
+size_t kv4_rows_workspace(int D) { return D == 128 ? sizeof(KrParts<128>) : sizeof(KrParts<64>); }
+static_assert(KV4_COUNTERS >= KV4_MAX_CTAS * KR_WARPS * KR_ROWS, "a counter for each slice of a warp's item");
 
 int launch_kv4_attn_rows(const Kv4Attn & a, int D, int type, int most_rows, int * counters, void * parts, cudaStream_t st) {
     const KrWork w{most_rows, counters, parts, abort_flag()};

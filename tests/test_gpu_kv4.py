@@ -100,6 +100,7 @@ TOKEN_CASES = [
     ([1], [1], 4, 4, 0, 0), ([1], [63], 8, 2, 0, 0), ([1], [64], 8, 1, 0, 0), ([1], [65], 6, 2, 0, 0), ([1], [0], 8, 2, 0, 0), ([1], [700], 7, 1, 0, 0), ([1], [2500], 32, 8, 0, 0),
     ([1] * 5, [1, 130, 0, 64, 511], 16, 2, 0, 0), ([2, 1, 0, 5], [2, 300, 90, 77], 4, 1, 0, 0), ([3], [1], 8, 2, 0, 0), ([4, 2], [2, 0], 4, 2, 0, 0),
     ([1] * 3, [500, 64, 3], 8, 2, 100, 0), ([1] * 3, [500, 300, 3], 8, 2, 1, 0), ([1, 2], [900, 400], 8, 2, 64, 4), ([1] * 2, [900, 700], 16, 1, 130, 65), ([5], [400], 10, 2, 30, 1),
+    ([1] * 12, [500 + 321 * i for i in range(12)], 16, 8, 0, 0), ([1] * 3, [20000, 9, 6400], 8, 8, 0, 0),   # shares of many pages, which hold the ends of several items
     ([1] * 40, list(range(0, 400, 10)), 8, 4, 0, 0), ([1], [700], 40, 2, 0, 0), ([1] * 2, [300, 20], 3, 3, 0, 0), ([1] * 300, [3 * i for i in range(300)], 4, 1, 0, 0),
 ]
 
