@@ -5,7 +5,8 @@
 
 namespace pb {
 
-constexpr int KV4_MAX_CTAS = 160;      // of a launch: the workspace has parts by CTA and warp
+constexpr int KV4_MAX_CTAS = 152;      // of a launch: the workspace has parts by CTA and warp
+constexpr int KV4_SLOTS = 256;         // and by piece of a cut item: these are 5 / 3 of the CTAs at most
 constexpr int KV4_COUNTERS = 16384;    // in front of them
 
 // A sequence: its queries' rows, and the pages that any of them sees: the first `keep`, then those from page `from` on.  At least one page, so that rows which see
@@ -18,6 +19,19 @@ struct Kv4Seq {
     __device__ __forceinline__ int items(int n_head_kv, int tile) const { return n_q > 0 ? n_head_kv * ((n_rows + tile - 1) / tile) : 0; }
     __device__ __forceinline__ int units(int n_head_kv, int tile) const { return items(n_head_kv, tile) * pages; }
 };
+// the pages that queries at the positions lo .. hi see
+__device__ __forceinline__ void kv4_pages(const Kv4Attn & A, int lo, int hi, Kv4Seq & q) {
+    q.pages = 1;
+    q.keep = q.from = 0;
+    if (hi < 0) return;
+    const int ld = (int) (A.table_ld < 0x1ffffff ? A.table_ld : 0x1ffffff);   // cells have 31 bits
+    const int last = min(hi / KV4_CELLS, ld - 1);
+    if (A.window > 0 && lo - A.window + 1 > 0) {
+        q.from = (lo - A.window + 1) / KV4_CELLS;
+        q.keep = min(min(A.first / KV4_CELLS + (A.first % KV4_CELLS != 0), q.from), last + 1);
+    }
+    q.pages = max(1, q.keep + max(0, last + 1 - q.from));
+}
 // many: sequences with more than most_rows rows, otherwise the others
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_rows, bool many) {
     Kv4Seq q{};
@@ -31,20 +45,7 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_row
     q.n_rows = n * A.group;
     const int len = max(A.kv_len[s], 0);
     q.p0 = len - all;
-    const int last_p = q.p0 + n - 1;
-    q.pages = 1;
-    if (last_p >= 0) {
-        const int ld = (int) (A.table_ld < 0x1ffffff ? A.table_ld : 0x1ffffff);   // cells have 31 bits
-        const int last = min(last_p / KV4_CELLS, ld - 1);
-        int from = 0, keep = 0;
-        if (A.window > 0 && q.p0 - A.window + 1 > 0) {
-            from = (q.p0 - A.window + 1) / KV4_CELLS;
-            keep = min(A.first / KV4_CELLS + (A.first % KV4_CELLS != 0), from);
-        }
-        q.keep = min(keep, last + 1);
-        q.from = from;
-        q.pages = max(1, q.keep + max(0, last + 1 - from));
-    }
+    kv4_pages(A, q.p0, q.p0 + n - 1, q);
     return q;
 }
 // the i-th of its pages: which one of the sequence, and its number in the pool (-1: none)
@@ -56,8 +57,16 @@ __device__ __forceinline__ int kv4_page(const Kv4Attn & A, const Kv4Seq & q, int
     return id >= 0 && id < A.cache.n_pages ? id : -1;
 }
 
+__device__ __forceinline__ void tmem_alloc(uint32_t * at, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) { asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory"); }
+
 struct KrWork { int most_rows; int * counters; void * parts; int * abort_flag; };
 size_t kv4_rows_workspace(int D);
 int launch_kv4_attn_rows(const Kv4Attn & a, int D, int type, int most_rows, int * counters, void * parts, cudaStream_t st);
+size_t kv4_prompt_workspace(int D);
+int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st);
 
 }  // namespace pb

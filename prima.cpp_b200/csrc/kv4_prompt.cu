@@ -1,0 +1,584 @@
+// prima.cpp_b200/csrc/kv4_prompt.cu — attention over the 4-bit cache (kv4.cuh) for sequences with many query rows, on the 5th-generation tensor cores.
+//
+// Mathematics.  S = Q K^T, P = 2^(S c - reference), O += P V, divided by the row's sum at the end.  Keys and values are f16 numbers exactly; queries become f16 (a row by a power of two:
+// 16-bit ones exactly, F32 as two numbers, 22 bits), weights f16 (F32: two numbers).  A row's reference is the largest score of its first tile; it moves only where a
+// score lies beyond it by more than 2^8, and then its sum and O are scaled.
+//
+// Work.  An item is a (sequence, kv head, tile of query rows: tokens x heads of the group); 16 bits have two row tiles of 128 that share each expanded key tile, F32 one.  Key tiles are
+// two pages.  CTAs (one to an SM) take items by tickets, long ones of a sequence first; where there are fewer items than SMs, long items are cut into pieces, which a second
+// kernel adds up in their order.
+//   warps 0 - 3    expand: a thread has a cell's row of keys, then one of values: raw words in registers a tile ahead, f16 into the swizzle-128B images, two stages each
+//   warps 4 - 11   softmax: a thread has a row of S (4 - 7: first row tile, 8 - 11: second), which is also a lane of tensor memory
+//   warp 12        MMA issuer, owner of the tensor memory, and of the tickets
+// Tensor memory: S / P of either row tile at 0 and 256, O at 128 and 384.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cfloat>
+#include <type_traits>
+
+#include "../../include/prima_b200.h"
+#include "kv4_attn.cuh"
+
+namespace pb {
+namespace {
+
+constexpr int KP_THREADS = 13 * 32, KP_TILE = 128, KP_BLOCK = 16384;   // a block: 128 rows of 64 entries
+constexpr float KP_UP = 6.f;            // weights are up to 2^(8 + 6)
+template <typename T> constexpr int kp_groups() { return std::is_same<T, float>::value ? 1 : 2; }
+template <typename T> constexpr int kp_rows() { return KP_TILE * kp_groups<T>(); }
+
+struct KpPiece {               // what a ticket stands for
+    int s, hk, row0, rows;     // sequence, kv head, first row (of the sequence's) and rows of the tile
+    int a, b, tiles;           // key tiles [a, b) of the item's
+    int slot, part, parts;     // of its part in the workspace (-1: the whole item), which of how many
+    Kv4Seq q;                  // pages that the tile's rows see
+    int p_lo, p_hi;            // positions of the tile's first and last row
+};
+template <int D> struct KpPart { float o[2 * KP_TILE][D]; float m[2 * KP_TILE], l[2 * KP_TILE]; };
+template <int D> struct KpSmem {
+    uint8_t q[2][D / 64][KP_BLOCK];            // 16 bits: either row tile; F32: high and low
+    uint8_t k[2][D / 64][KP_BLOCK], v[2][D / 64][KP_BLOCK];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+    float mult[2 * KP_TILE];
+    KpPiece piece;
+    uint32_t tmem_base;
+    int abort, more, total, items;
+};
+// tickets: two words, and for each slot whether a cut item's parts begin there (cleared in front of the kernel); cut: long items may be
+struct KpWork { int most_rows; int * tickets; void * parts; int * abort_flag; int cut; };
+template <int D> struct KpParts { KpPart<D> part[KV4_SLOTS]; KpPiece first[KV4_SLOTS]; };
+constexpr int KP_FLAGS = 2;
+
+// the tile's rows [row0, row0 + rows) of a sequence: positions and pages
+__device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpPiece & p) {
+    p.p_lo = q.p0 + p.row0 / A.group;
+    p.p_hi = q.p0 + (p.row0 + p.rows - 1) / A.group;
+    p.q = q;
+    kv4_pages(A, p.p_lo, p.p_hi, p.q);
+    p.tiles = (p.q.pages + 1) / 2;
+}
+// Items, their pieces and slots, in the order of tickets: sequences, tiles from the last on, heads, pieces.  Every CTA and the joining kernel count them in the same way.
+struct KpCount { int pieces, cut; };
+template <int ROWS>
+__device__ __forceinline__ KpCount kp_count(const Kv4Attn & A, const Kv4Seq & q, int limit) {   // of a sequence; limit: pieces are no longer (0: items are whole)
+    if (q.n_q == 0) return {0, 0};
+    const int n = (q.n_rows + ROWS - 1) / ROWS;
+    if (limit == 0) return {n * A.cache.n_head_kv, 0};
+    KpCount c{0, 0};
+    for (int i = 0; i < n; i++) {
+        KpPiece p;
+        p.row0 = i * ROWS;
+        p.rows = min(ROWS, q.n_rows - p.row0);
+        kp_span(A, q, p);
+        const int k = 2 * p.tiles > 3 * limit ? (p.tiles + limit - 1) / limit : 1;
+        c.pieces += k;
+        c.cut += k > 1 ? k : 0;
+    }
+    c.pieces *= A.cache.n_head_kv;
+    c.cut *= A.cache.n_head_kv;
+    return c;
+}
+template <int ROWS>
+__device__ __forceinline__ int kp_tiles(const Kv4Attn & A, const Kv4Seq & q) {   // key tiles of a sequence's items of one head
+    int sum = 0;
+    for (int r = 0; r < q.n_rows; r += ROWS) {
+        KpPiece p;
+        p.row0 = r;
+        p.rows = min(ROWS, q.n_rows - r);
+        kp_span(A, q, p);
+        sum += p.tiles;
+    }
+    return sum;
+}
+// by a warp: the longest piece that is not cut again, 0 where items stay whole
+template <int ROWS>
+__device__ __forceinline__ int kp_limit(const Kv4Attn & A, const KpWork & W, int ctas) {
+    if (!W.cut) return 0;
+    int sum = 0;
+    for (int s = threadIdx.x & 31; s < A.n_seq; s += 32) sum += kp_tiles<ROWS>(A, kv4_seq(A, s, W.most_rows, true));
+    sum = __reduce_add_sync(0xffffffffu, sum) * A.cache.n_head_kv;
+    return max(4, (sum + ctas - 1) / ctas);
+}
+// by a warp: what ticket t stands for; false: there is none
+template <int ROWS>
+__device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, int limit, int t, KpPiece & p) {
+    const int lane = threadIdx.x & 31;
+    int before = 0, cut = 0;
+    for (int s0 = 0; s0 < A.n_seq; s0 += 32) {
+        const Kv4Seq q = kv4_seq(A, s0 + lane, W.most_rows, true);
+        const KpCount n = kp_count<ROWS>(A, q, limit);
+        int x = n.pieces, y = n.cut;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) { x += u; y += v; }
+        }
+        const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
+        if (!in) {
+            before += __shfl_sync(0xffffffffu, x, 31);
+            cut += __shfl_sync(0xffffffffu, y, 31);
+            continue;
+        }
+        const int at = __ffs((int) in) - 1;
+        int i = t - before - __shfl_sync(0xffffffffu, x - n.pieces, at);     // piece of the sequence
+        cut += __shfl_sync(0xffffffffu, y - n.cut, at);
+        p.s = s0 + at;
+        const Kv4Seq mine = kv4_seq(A, p.s, W.most_rows, true);
+        for (int tile = (mine.n_rows + ROWS - 1) / ROWS - 1; tile >= 0; tile--) {
+            p.row0 = tile * ROWS;
+            p.rows = min(ROWS, mine.n_rows - p.row0);
+            kp_span(A, mine, p);
+            const int k = limit > 0 && 2 * p.tiles > 3 * limit ? (p.tiles + limit - 1) / limit : 1;
+            if (i < k * A.cache.n_head_kv) {
+                p.hk = i / k;
+                p.part = i - p.hk * k;
+                p.parts = k;
+                p.a = (int) ((long long) p.tiles * p.part / k);
+                p.b = (int) ((long long) p.tiles * (p.part + 1) / k);
+                p.slot = k > 1 ? cut + i : -1;
+                return true;
+            }
+            i -= k * A.cache.n_head_kv;
+            cut += k > 1 ? k * A.cache.n_head_kv : 0;
+        }
+        return false;
+    }
+    return false;
+}
+
+template <typename T> __device__ __forceinline__ float4 q_load(const T * p) { return load4(p); }
+__device__ __forceinline__ uint32_t hu(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 uh(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+__device__ __forceinline__ void group_barrier(int grp) { asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory"); }
+// eight numbers (four to a half-word, the halves' i-th next to each other) times their scale, as f16
+__device__ __forceinline__ uint4 expand(uint32_t w, __half2 d) {
+    const uint32_t s = w >> 8;
+    const __half2 e = __float2half2_rn(1032.f), o = __float2half2_rn(72.f);
+    return make_uint4(hu(__hmul2(__hsub2(uh((w & 0x000f000fu) | 0x64006400u), e), d)), hu(__hmul2(__hsub2(uh((w & 0x00f000f0u) | 0x54005400u), o), d)),
+                      hu(__hmul2(__hsub2(uh((s & 0x000f000fu) | 0x64006400u), e), d)), hu(__hmul2(__hsub2(uh((s & 0x00f000f0u) | 0x54005400u), o), d)));
+}
+template <typename T, int D>
+__global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
+    constexpr bool F32 = std::is_same<T, float>::value;
+    constexpr int GROUPS = kp_groups<T>(), ROWS = kp_rows<T>(), NB = D / 32;
+    extern __shared__ uint8_t smem_raw[];
+    KpSmem<D> & S = *reinterpret_cast<KpSmem<D> *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    volatile int * cta_abort = &S.abort;
+    if (warp == 12) {
+        if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                mbar_init(&S.k_full[i], 4);
+                mbar_init(&S.v_full[i], 4);
+                mbar_init(&S.k_empty[i], 1);
+                mbar_init(&S.v_empty[i], 1);
+                mbar_init(&S.s_full[i], 1);
+                mbar_init(&S.p_full[i], 4);
+                mbar_init(&S.o_full[i], 1);
+            }
+            S.abort = 0;
+            mbar_fence_init();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        tmem_alloc(&S.tmem_base, 512);
+    }
+    int limit = 0, ticket = blockIdx.x;
+    if (warp == 12) {
+        limit = kp_limit<ROWS>(A, W, gridDim.x);
+        const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece);
+        if (lane == 0) S.more = more;
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *(volatile uint32_t *) &S.tmem_base;
+    uint32_t tiles[2] = {0, 0}, pieces[2] = {0, 0};   // key tiles and pieces in front, of either row tile (all roles count them)
+    while (*(volatile int *) &S.more) {
+        const KpPiece & P = S.piece;
+        const int n = P.b - P.a, groups = P.rows > KP_TILE ? 2 : 1;
+        if (warp < 4) {
+            // ---- expand ----
+            const int x = threadIdx.x, half = x >> 6, t6 = x & 63, r = t6, tv = (r & ~7) | ((r & 3) << 1) | ((r >> 2) & 1);
+            constexpr int WORDS = NB == 4 ? 4 : 2;                 // of a quarter of a row
+            uint32_t kw[4][WORDS], vw[4][WORDS], ks[NB], vs[NB];
+            auto chunk_of = [&](int j) {                          // this half's page of tile j, none: null
+                const int i = 2 * (P.a + j) + half;
+                const int id = j < n && i < P.q.pages ? kv4_page(A, P.q, P.s, i) : -1;
+                return id >= 0 ? kv4_chunk<D>(A.cache, id, P.hk) : nullptr;
+            };
+            auto rows_of = [&](const uint8_t * row, const uint8_t * scales, uint32_t (&w)[4][WORDS], uint32_t (&d)[NB]) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if constexpr (NB == 4) *reinterpret_cast<uint4 *>(w[c]) = row ? *reinterpret_cast<const uint4 *>(row + 16 * c) : make_uint4(0u, 0u, 0u, 0u);
+                    else *reinterpret_cast<uint2 *>(w[c]) = row ? *reinterpret_cast<const uint2 *>(row + 8 * c) : make_uint2(0u, 0u);
+                }
+                if constexpr (NB == 4) *reinterpret_cast<uint4 *>(d) = row ? *reinterpret_cast<const uint4 *>(scales) : make_uint4(0u, 0u, 0u, 0u);
+                else *reinterpret_cast<uint2 *>(d) = row ? *reinterpret_cast<const uint2 *>(scales) : make_uint2(0u, 0u);
+            };
+            const uint8_t * now = chunk_of(0), * later = chunk_of(1);
+            auto ask_k = [&](const uint8_t * p) { rows_of(p ? p + t6 * (D / 2) : nullptr, p + 2 * kv4_rows_bytes(D) + kv4_scale(D, t6 & ~1, 0), kw, ks); };
+            auto ask_v = [&](const uint8_t * p) {
+                rows_of(p ? p + kv4_rows_bytes(D) + r * (D / 2) : nullptr, p + 2 * kv4_rows_bytes(D) + kv4_scales_bytes(D) + kv4_scale(D, tv & ~1, 0), vw, vs);
+            };
+            ask_k(now);
+            ask_v(now);
+            for (int j = 0; j < n; j++) {
+                const uint32_t u = tiles[0] + (uint32_t) j;
+                const int st = (int) (u & 1);
+                const uint8_t * third = chunk_of(j + 2);
+                if (u >= 2) mbar_wait(&S.k_empty[st], (u / 2 - 1) & 1, cta_abort, W.abort_flag);
+                {
+                    const uint32_t odd = t6 & 1 ? 0x3232u : 0x1010u;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const __half2 d = uh(__byte_perm(ks[b], 0u, odd));
+#pragma unroll
+                        for (int c = 0; c < 4; c++) *reinterpret_cast<uint4 *>(S.k[st][b >> 1] + x * 128 + ((((b & 1) * 4 + c) ^ (x & 7)) << 4)) = expand(kw[c][b], d);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.k_full[st]);
+                ask_k(later);
+                if (u >= 2) mbar_wait(&S.v_empty[st], (u / 2 - 1) & 1, cta_abort, W.abort_flag);
+                {
+                    const int i = 2 * (P.a + j) + half, cell = kv4_page_index(P.q, i) * KV4_CELLS + tv, t = half * 64 + tv;
+                    // a weight of zero does not silence a scale that is no number: cells nobody sees may hold anything
+                    const bool seen = cell <= P.p_hi && (A.window <= 0 || P.p_lo - cell < A.window || cell < A.first);
+                    const uint32_t odd = tv & 1 ? 0x3232u : 0x1010u;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const __half2 d = uh(seen ? __byte_perm(vs[b], 0u, odd) : 0u);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            // words 2c, 2c+1 of the row: half-word b of either
+                            const uint32_t w = __byte_perm(vw[c][b / 2], vw[c][WORDS / 2 + b / 2], b & 1 ? 0x7632 : 0x5410);
+                            const int q = c ^ (2 * ((r >> 1) & 1));
+                            *reinterpret_cast<uint4 *>(S.v[st][b >> 1] + t * 128 + ((((b & 1) * 4 + q) ^ (t & 7)) << 4)) = expand(w, d);
+                        }
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.v_full[st]);
+                ask_v(later);
+                later = third;
+            }
+        } else if (warp == 12) {
+            // ---- MMA ----
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t) (128 >> 3) << 17) | ((uint32_t) (128 >> 4) << 24);
+            constexpr uint32_t idesc_v = (1u << 4) | ((uint32_t) (D >> 3) << 17) | ((uint32_t) (128 >> 4) << 24) | (1u << 16);
+            asm volatile("bar.sync 4, %0;" ::"n"(32 * (1 + 4 * GROUPS)) : "memory");      // the queries are there
+            auto scores = [&](int grp, int st) {
+                if (elect_one()) {
+#pragma unroll
+                    for (int part = 0; part < (F32 ? 2 : 1); part++) {
+                        const uint64_t dq = desc_sw128(smem_u32(S.q[F32 ? part : grp])), dk = desc_sw128(smem_u32(S.k[st]));
+#pragma unroll
+                        for (int k = 0; k < D / 16; k++)
+                            mma_f16<1>(tmem + 256 * grp, dq + (k >> 2) * (KP_BLOCK >> 4) + 2 * (k & 3), dk + (k >> 2) * (KP_BLOCK >> 4) + 2 * (k & 3), idesc, (uint32_t) ((part | k) != 0));
+                    }
+                    mma_commit(&S.s_full[grp]);
+                    if (grp == groups - 1) mma_commit(&S.k_empty[st]);
+                }
+                __syncwarp();
+            };
+            for (int j = -1; j < n; j++) {
+                const uint32_t u = tiles[0] + (uint32_t) j;
+                const int st = (int) (u & 1), st1 = (int) ((u + 1) & 1);
+                for (int grp = 0; grp < groups; grp++) {
+                    if (j >= 0) {
+                        if (grp == 0) mbar_wait(&S.v_full[st], (u / 2) & 1, cta_abort, W.abort_flag);
+                        mbar_wait(&S.p_full[grp], (tiles[grp] + (uint32_t) j) & 1, cta_abort, W.abort_flag);
+                        __syncwarp();
+                        fence_after();
+                        if (elect_one()) {
+                            const uint64_t dv = desc_sw128_mn(smem_u32(S.v[st]), KP_BLOCK);
+#pragma unroll
+                            for (int part = 0; part < (F32 ? 2 : 1); part++)
+#pragma unroll
+                                for (int k = 0; k < 8; k++)
+                                    mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * grp + 64 * part + 8 * k, dv + k * (2048 >> 4), idesc_v, (uint32_t) ((j | part | k) != 0));
+                            if (j == n - 1) mma_commit(&S.o_full[grp]);
+                            if (grp == groups - 1) mma_commit(&S.v_empty[st]);
+                        }
+                        __syncwarp();
+                    }
+                    if (j + 1 < n) {                              // behind the P V that reads this tensor memory: MMAs run in order
+                        if (grp == 0) mbar_wait(&S.k_full[st1], ((u + 1) / 2) & 1, cta_abort, W.abort_flag);
+                        __syncwarp();
+                        fence_after();
+                        scores(grp, st1);
+                    }
+                }
+            }
+        } else if ((warp - 4) >> 2 < GROUPS) {
+            // ---- softmax ----
+            const int grp = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane, w = warp - 4 - 4 * grp;
+            // queries -> f16 in the swizzle-128B image: a warp has whole rows, 8 of them on their way; a row's largest number comes to 2^13 .. 2^14
+            constexpr int LPR = D / 4, RPW = 32 / LPR;            // lanes to a row, rows to a pass
+            const int sub = lane / LPR, l4 = lane % LPR;
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32; i0 += 8 * RPW) {
+                float4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int rr = grp * KP_TILE + w * 32 + i0 + i * RPW + sub, at = P.row0 + rr, t = at / A.group;
+                    v[i] = rr < P.rows ? q_load((const T *) A.q + (P.q.q0 + t) * A.ldq + (int64_t) (P.hk * A.group + at - t * A.group) * D + 4 * l4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int rr = w * 32 + i0 + i * RPW + sub;
+                    float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const int ex = top > 0.f && top < INFINITY ? min(126, 140 - (int) (__float_as_uint(top) >> 23)) : 0;
+                    const float up = __int_as_float((ex + 127) << 23) * (A.scale < 0.f ? -1.f : 1.f);
+                    if (l4 == 0) S.mult[grp * KP_TILE + rr] = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23), FLT_MIN);
+                    const float x0 = v[i].x * up, x1 = v[i].y * up, x2 = v[i].z * up, x3 = v[i].w * up;
+                    const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
+                    const int at = (l4 >> 4) * KP_BLOCK + rr * 128 + ((((l4 & 15) >> 1) ^ (rr & 7)) << 4) + (l4 & 1) * 8;
+                    *reinterpret_cast<uint2 *>(&S.q[F32 ? 0 : grp][0][0] + at) = make_uint2(hu(h0), hu(h1));
+                    if constexpr (F32) {
+                        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+                        *reinterpret_cast<uint2 *>(&S.q[1][0][0] + at) = make_uint2(hu(__floats2half2_rn(x0 - b0.x, x1 - b0.y)), hu(__floats2half2_rn(x2 - b1.x, x3 - b1.y)));
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("bar.sync 4, %0;" ::"n"(32 * (1 + 4 * GROUPS)) : "memory");
+            if (grp < groups) {
+                const int at = P.row0 + grp * KP_TILE + row;
+                const int pos = grp * KP_TILE + row < P.rows ? P.q.p0 + at / A.group : -1;
+                const float c = S.mult[grp * KP_TILE + row];
+                const uint32_t mine = tmem + ((uint32_t) (quad * 32) << 16) + 256 * grp;
+                const int g_lo = P.q.p0 + (P.row0 + grp * KP_TILE) / A.group;      // of this row tile: the first row's position
+                float m = -INFINITY, l = 0.f;
+                float t[32];
+                uint32_t * tv = reinterpret_cast<uint32_t *>(t);
+                for (int j = 0; j < n; j++) {
+                    const int i0 = 2 * (P.a + j), i1 = i0 + 1;
+                    // first cells of the two pages; of none: beyond everything
+                    const int c0 = kv4_page(A, P.q, P.s, i0) >= 0 ? kv4_page_index(P.q, i0) * KV4_CELLS : 0x7fffff00;
+                    const int c1 = i1 < P.q.pages && kv4_page(A, P.q, P.s, i1) >= 0 ? kv4_page_index(P.q, i1) * KV4_CELLS : 0x7fffff00;
+                    const bool whole = c1 <= g_lo - 63 && c0 <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
+                    auto take = [&](int h) {                       // 32 scores; a masked one is -inf
+                        TMEM_LD32(mine + 32 * h, tv);
+                        tmem_wait_ld();
+                        if (!whole) {
+                            const int base = (h < 2 ? c0 : c1) + 32 * (h & 1);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) {
+                                const int cell = base + i;
+                                t[i] = cell <= pos && (A.window <= 0 || pos - cell < A.window || cell < A.first) ? t[i] : -INFINITY;
+                            }
+                        }
+                    };
+                    mbar_wait(&S.s_full[grp], (tiles[grp] + (uint32_t) j) & 1, cta_abort, W.abort_flag);
+                    __syncwarp();
+                    fence_after();
+                    float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        take(h);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) tm[i & 3] = fmaxf(tm[i & 3], t[i]);
+                    }
+                    const float top = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * c;
+                    const bool move = top > m + 8.f;               // (the first: m is -inf)
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2(m - top);
+                        if (move) m = top;
+                        l *= f;
+                        if (j > 0) {
+#pragma unroll
+                            for (int h = 0; h < D; h += 32) {
+                                TMEM_LD32(mine + 128 + h, tv);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; i++) t[i] *= f;
+                                TMEM_ST16(mine + 128 + h, tv);
+                                TMEM_ST16(mine + 128 + h + 16, tv + 16);
+                            }
+                        }
+                    }
+                    const float off = m == -INFINITY ? 0.f : KP_UP - m;
+                    float e4[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t lo[F32 ? 64 : 1];
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        take(h);
+                        uint32_t p[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float a = ex2(fmaf(t[2 * i], c, off)), b = ex2(fmaf(t[2 * i + 1], c, off));
+                            e4[i & 1] += a;
+                            e4[2 + (i & 1)] += b;
+                            const __half2 hi = __floats2half2_rn(a, b);
+                            p[i] = hu(hi);
+                            if constexpr (F32) {
+                                const float2 back = __half22float2(hi);
+                                lo[16 * h + i] = hu(__floats2half2_rn(a - back.x, b - back.y));
+                            }
+                        }
+                        TMEM_ST16(mine + 16 * h, p);               // over scores that have been read
+                    }
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int h = 0; h < 4; h++) TMEM_ST16(mine + 64 + 16 * h, lo + 16 * h);
+                    }
+                    l += (e4[0] + e4[1]) + (e4[2] + e4[3]);
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&S.p_full[grp]);
+                }
+                mbar_wait(&S.o_full[grp], pieces[grp] & 1, cta_abort, W.abort_flag);
+                __syncwarp();
+                fence_after();
+                if (P.slot < 0) {
+                    // through the queries' memory (all scores are made), rows of 128-byte pieces rotated by the row, so that a warp stores whole rows
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    T * os = reinterpret_cast<T *>(&S.q[F32 ? 0 : grp][0][0]);
+                    constexpr int PIECE = 4, PIECES = D / PIECE;   // numbers to a piece
+#pragma unroll
+                    for (int h = 0; h < D; h += 32) {
+                        TMEM_LD32(mine + 128 + h, tv);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) t[i] *= inv;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {           // columns 0 2 4 6 | 1 3 5 7 of an eight are numbers 0 1 2 3 | 4 5 6 7
+                            store4(os + row * D + ((h + i) / 4 + row) % PIECES * 4, make_float4(t[i], t[i + 2], t[i + 4], t[i + 6]));
+                            store4(os + row * D + ((h + i) / 4 + 1 + row) % PIECES * 4, make_float4(t[i + 1], t[i + 3], t[i + 5], t[i + 7]));
+                        }
+                    }
+                    group_barrier(grp);
+#pragma unroll 4
+                    for (int i = 0; i < 32 / RPW; i++) {
+                        const int rr = w * 32 + i * RPW + sub, ar = P.row0 + grp * KP_TILE + rr, tt = ar / A.group;
+                        const float4 v = load4(os + rr * D + (l4 + rr) % PIECES * 4);
+                        if (grp * KP_TILE + rr < P.rows) store4((T *) A.out + (P.q.q0 + tt) * A.ldo + (int64_t) (P.hk * A.group + ar - tt * A.group) * D + 4 * l4, v);
+                    }
+                } else {
+                    KpPart<D> & part = reinterpret_cast<KpParts<D> *>(W.parts)->part[P.slot];
+                    if (threadIdx.x == 128 && P.part == 0) {
+                        reinterpret_cast<KpParts<D> *>(W.parts)->first[P.slot] = P;
+                        W.tickets[KP_FLAGS + P.slot] = 1;
+                    }
+                    const int pr = grp * KP_TILE + row;
+#pragma unroll
+                    for (int h = 0; h < D; h += 32) {
+                        TMEM_LD32(mine + 128 + h, tv);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            *reinterpret_cast<float4 *>(&part.o[pr][h + i]) = make_float4(t[i], t[i + 2], t[i + 4], t[i + 6]);
+                            *reinterpret_cast<float4 *>(&part.o[pr][h + i + 4]) = make_float4(t[i + 1], t[i + 3], t[i + 5], t[i + 7]);
+                        }
+                    }
+                    part.m[pr] = m;
+                    part.l[pr] = l;
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fence_before();
+        __syncthreads();
+        tiles[0] += (uint32_t) n;
+        pieces[0]++;
+        if (groups == 2) {
+            tiles[1] += (uint32_t) n;
+            pieces[1]++;
+        }
+        if (warp == 12) {
+            if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[0], 1);
+            ticket = __shfl_sync(0xffffffffu, ticket, 0);
+            const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece);
+            if (lane == 0) S.more = more;
+        }
+        __syncthreads();
+        fence_after();
+    }
+    if (warp == 12) {
+        tmem_free(tmem, 512);
+        if (lane == 0 && atomicAdd(&W.tickets[1], 1) == (int) gridDim.x - 1) W.tickets[0] = W.tickets[1] = 0;   // the last CTA: every ticket has been drawn
+    }
+}
+
+// Items that were cut: parts in their order, a warp to a row.  blockIdx.x: where an item's parts may begin
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
+    constexpr int PER = D / 32, ONCE = 4;
+    if (W.tickets[KP_FLAGS + blockIdx.x] == 0) return;
+    const KpParts<D> & all = *reinterpret_cast<const KpParts<D> *>(W.parts);
+    const KpPiece & p = all.first[blockIdx.x];
+    const KpPart<D> * parts = &all.part[blockIdx.x];
+    const int lane = threadIdx.x & 31, n = p.parts;
+    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < p.rows; r += gridDim.y * 8) {
+        float top = -INFINITY, l = 0.f, x[PER];
+        for (int i = 0; i < n; i++) top = fmaxf(top, parts[i].m[r]);
+#pragma unroll
+        for (int e = 0; e < PER; e++) x[e] = 0.f;
+        for (int i0 = 0; i0 < n; i0 += ONCE) {
+            float mi[ONCE], li[ONCE], y[ONCE][PER];
+#pragma unroll
+            for (int k = 0; k < ONCE; k++) {
+                const int i = min(i0 + k, n - 1);
+                mi[k] = parts[i].m[r];
+                li[k] = parts[i].l[r];
+#pragma unroll
+                for (int e = 0; e < PER; e++) y[k][e] = parts[i].o[r][e * 32 + lane];
+            }
+#pragma unroll
+            for (int k = 0; k < ONCE; k++)
+                if (i0 + k < n) {
+                    const float f = mi[k] == -INFINITY ? (li[k] == li[k] ? 0.f : 1.f) : ex2(mi[k] - top);     // a row that is no number has no maximum
+                    l = fmaf(li[k], f, l);
+#pragma unroll
+                    for (int e = 0; e < PER; e++) x[e] = fmaf(y[k][e], f, x[e]);
+                }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int at = p.row0 + r, tt = at / A.group;
+        T * out = (T *) A.out + (p.q.q0 + tt) * A.ldo + (int64_t) (p.hk * A.group + at - tt * A.group) * D;
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            if constexpr (std::is_same<T, float>::value) out[e * 32 + lane] = x[e] * inv;
+            else if constexpr (std::is_same<T, __half>::value) out[e * 32 + lane] = __float2half_rn(x[e] * inv);
+            else out[e * 32 + lane] = __float2bfloat16_rn(x[e] * inv);
+        }
+    }
+}
+
+template <typename T, int D>
+int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st) {
+    constexpr size_t smem = sizeof(KpSmem<D>) + 1024;
+    static_assert(smem <= 232448, "shared memory of an SM");
+    static FuncAttrCache cache;
+    cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_prompt<T, D>, smem, true);
+    if (e != cudaSuccess) return (int) e;
+    const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
+    w.cut = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv < ctas;
+    if (w.cut && (e = cudaMemsetAsync(w.tickets + KP_FLAGS, 0, KV4_SLOTS * sizeof(int), st)) != cudaSuccess) return (int) e;
+    k_kv4_attn_prompt<T, D><<<ctas, KP_THREADS, smem, st>>>(a, w);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !w.cut) return (int) e;
+    k_kv4_join<T, D><<<dim3(KV4_SLOTS, 4), 256, 0, st>>>(a, w);
+    return (int) cudaGetLastError();
+}
+
+}  // namespace
+
+size_t kv4_prompt_workspace(int D) { return D == 128 ? sizeof(KpParts<128>) : sizeof(KpParts<64>); }
+
+int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st) {
+    const KpWork w{most_rows, tickets, parts, abort_flag(), 0};
+    if (D == 128) return type == PB200_TYPE_F32 ? prompt_launch<float, 128>(a, w, st) : type == PB200_TYPE_F16 ? prompt_launch<__half, 128>(a, w, st) : prompt_launch<__nv_bfloat16, 128>(a, w, st);
+    return type == PB200_TYPE_F32 ? prompt_launch<float, 64>(a, w, st) : type == PB200_TYPE_F16 ? prompt_launch<__half, 64>(a, w, st) : prompt_launch<__nv_bfloat16, 64>(a, w, st);
+}
+
+}  // namespace pb
