@@ -10,7 +10,7 @@
 //   warps 0 - 3    expand: a thread has a cell's row of keys, then one of values: raw words in registers a tile ahead, f16 into the swizzle-128B images, two stages each
 //   warps 4 - 11   softmax: a thread has a row of S (4 - 7: first row tile, 8 - 11: second), which is also a lane of tensor memory
 //   warp 12        MMA issuer, owner of the tensor memory, and of the tickets
-// Tensor memory: S / P of either row tile at 0 and 256, O at 128 and 384.
+// Tensor memory: S / P of either row tile at 0 and 256 (F32: the weights' low parts there), O at 128 and 384.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -147,10 +147,15 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, int
     return false;
 }
 
-template <typename T> __device__ __forceinline__ float4 q_load(const T * p) { return load4(p); }
 __device__ __forceinline__ uint32_t hu(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 uh(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-__device__ __forceinline__ void group_barrier(int grp) { asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory"); }
+// waits for loads from tensor memory; what v holds may be used behind it only
+#define TMEM_ARRIVED(v) \
+    asm volatile("tcgen05.wait::ld.sync.aligned;" \
+                 : "+r"((v)[0]), "+r"((v)[1]), "+r"((v)[2]), "+r"((v)[3]), "+r"((v)[4]), "+r"((v)[5]), "+r"((v)[6]), "+r"((v)[7]), "+r"((v)[8]), "+r"((v)[9]), "+r"((v)[10]), "+r"((v)[11]), "+r"((v)[12]), "+r"((v)[13]), "+r"((v)[14]), "+r"((v)[15]), \
+                   "+r"((v)[16]), "+r"((v)[17]), "+r"((v)[18]), "+r"((v)[19]), "+r"((v)[20]), "+r"((v)[21]), "+r"((v)[22]), "+r"((v)[23]), "+r"((v)[24]), "+r"((v)[25]), "+r"((v)[26]), "+r"((v)[27]), "+r"((v)[28]), "+r"((v)[29]), "+r"((v)[30]), "+r"((v)[31]) \
+                 : \
+                 : "memory")
 // eight numbers (four to a half-word, the halves' i-th next to each other) times their scale, as f16
 __device__ __forceinline__ uint4 expand(uint32_t w, __half2 d) {
     const uint32_t s = w >> 8;
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             for (int part = 0; part < (F32 ? 2 : 1); part++)
 #pragma unroll
                                 for (int k = 0; k < 8; k++)
-                                    mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * grp + 64 * part + 8 * k, dv + k * (2048 >> 4), idesc_v, (uint32_t) ((j | part | k) != 0));
+                                    mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * (grp + part) + 8 * k, dv + k * (2048 >> 4), idesc_v, (uint32_t) ((j | part | k) != 0));
                             if (j == n - 1) mma_commit(&S.o_full[grp]);
                             if (grp == groups - 1) mma_commit(&S.v_empty[st]);
                         }
@@ -319,19 +324,25 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             // ---- softmax ----
             const int grp = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane, w = warp - 4 - 4 * grp;
             // queries -> f16 in the swizzle-128B image: a warp has whole rows, 8 of them on their way; a row's largest number comes to 2^13 .. 2^14
-            constexpr int LPR = D / 4, RPW = 32 / LPR;            // lanes to a row, rows to a pass
+            constexpr int LPR = D / 4, RPW = 32 / LPR, ONCE = 16; // lanes to a row, rows to a pass, passes on their way
             const int sub = lane / LPR, l4 = lane % LPR;
+            // this lane's row of the tile: its token and head, and where they lie (others' by shuffles: a division costs more than a row)
+            const int at = P.row0 + grp * KP_TILE + row, tok = at / A.group, head = P.hk * A.group + at - tok * A.group;
+            const bool mine_is = grp * KP_TILE + row < P.rows;
+            const uint32_t valid = __ballot_sync(0xffffffffu, mine_is);
+            const int64_t q_at = (P.q.q0 + tok) * A.ldq + (int64_t) head * D;
 #pragma unroll 1
-            for (int i0 = 0; i0 < 32; i0 += 8 * RPW) {
-                float4 v[8];
+            for (int i0 = 0; i0 < 32 / RPW; i0 += ONCE) {
+                float4 v[ONCE];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int rr = grp * KP_TILE + w * 32 + i0 + i * RPW + sub, at = P.row0 + rr, t = at / A.group;
-                    v[i] = rr < P.rows ? q_load((const T *) A.q + (P.q.q0 + t) * A.ldq + (int64_t) (P.hk * A.group + at - t * A.group) * D + 4 * l4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < ONCE; i++) {
+                    const int rr = (i0 + i) * RPW + sub;
+                    const int64_t from = __shfl_sync(0xffffffffu, q_at, rr);
+                    v[i] = valid >> rr & 1 ? load4((const T *) A.q + from + 4 * l4) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int rr = w * 32 + i0 + i * RPW + sub;
+                for (int i = 0; i < ONCE; i++) {
+                    const int rr = w * 32 + (i0 + i) * RPW + sub;
                     float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
 #pragma unroll
                     for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -340,52 +351,54 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     if (l4 == 0) S.mult[grp * KP_TILE + rr] = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23), FLT_MIN);
                     const float x0 = v[i].x * up, x1 = v[i].y * up, x2 = v[i].z * up, x3 = v[i].w * up;
                     const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
-                    const int at = (l4 >> 4) * KP_BLOCK + rr * 128 + ((((l4 & 15) >> 1) ^ (rr & 7)) << 4) + (l4 & 1) * 8;
-                    *reinterpret_cast<uint2 *>(&S.q[F32 ? 0 : grp][0][0] + at) = make_uint2(hu(h0), hu(h1));
+                    const int to = (l4 >> 4) * KP_BLOCK + rr * 128 + ((((l4 & 15) >> 1) ^ (rr & 7)) << 4) + (l4 & 1) * 8;
+                    *reinterpret_cast<uint2 *>(&S.q[F32 ? 0 : grp][0][0] + to) = make_uint2(hu(h0), hu(h1));
                     if constexpr (F32) {
                         const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-                        *reinterpret_cast<uint2 *>(&S.q[1][0][0] + at) = make_uint2(hu(__floats2half2_rn(x0 - b0.x, x1 - b0.y)), hu(__floats2half2_rn(x2 - b1.x, x3 - b1.y)));
+                        *reinterpret_cast<uint2 *>(&S.q[1][0][0] + to) = make_uint2(hu(__floats2half2_rn(x0 - b0.x, x1 - b0.y)), hu(__floats2half2_rn(x2 - b1.x, x3 - b1.y)));
                     }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("bar.sync 4, %0;" ::"n"(32 * (1 + 4 * GROUPS)) : "memory");
             if (grp < groups) {
-                const int at = P.row0 + grp * KP_TILE + row;
-                const int pos = grp * KP_TILE + row < P.rows ? P.q.p0 + at / A.group : -1;
+                const int pos = mine_is ? P.q.p0 + tok : -1;
                 const float c = S.mult[grp * KP_TILE + row];
                 const uint32_t mine = tmem + ((uint32_t) (quad * 32) << 16) + 256 * grp;
                 const int g_lo = P.q.p0 + (P.row0 + grp * KP_TILE) / A.group;      // of this row tile: the first row's position
                 float m = -INFINITY, l = 0.f;
-                float t[32];
-                uint32_t * tv = reinterpret_cast<uint32_t *>(t);
+                float t[2][32];                                    // scores, 32 being worked on and 32 on their way
+                uint32_t * const t0 = reinterpret_cast<uint32_t *>(t[0]), * const t1 = reinterpret_cast<uint32_t *>(t[1]);
                 for (int j = 0; j < n; j++) {
                     const int i0 = 2 * (P.a + j), i1 = i0 + 1;
                     // first cells of the two pages; of none: beyond everything
                     const int c0 = kv4_page(A, P.q, P.s, i0) >= 0 ? kv4_page_index(P.q, i0) * KV4_CELLS : 0x7fffff00;
                     const int c1 = i1 < P.q.pages && kv4_page(A, P.q, P.s, i1) >= 0 ? kv4_page_index(P.q, i1) * KV4_CELLS : 0x7fffff00;
                     const bool whole = c1 <= g_lo - 63 && c0 <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
-                    auto take = [&](int h) {                       // 32 scores; a masked one is -inf
-                        TMEM_LD32(mine + 32 * h, tv);
-                        tmem_wait_ld();
-                        if (!whole) {
-                            const int base = (h < 2 ? c0 : c1) + 32 * (h & 1);
+                    auto mask = [&](float (&x)[32], int h) {       // a score that is not seen is -inf
+                        if (whole) return;
+                        const int base = (h < 2 ? c0 : c1) + 32 * (h & 1);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                const int cell = base + i;
-                                t[i] = cell <= pos && (A.window <= 0 || pos - cell < A.window || cell < A.first) ? t[i] : -INFINITY;
-                            }
+                        for (int i = 0; i < 32; i++) {
+                            const int cell = base + i;
+                            x[i] = cell <= pos && (A.window <= 0 || pos - cell < A.window || cell < A.first) ? x[i] : -INFINITY;
                         }
                     };
                     mbar_wait(&S.s_full[grp], (tiles[grp] + (uint32_t) j) & 1, cta_abort, W.abort_flag);
                     __syncwarp();
                     fence_after();
                     float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    TMEM_LD32(mine, t0);
 #pragma unroll
                     for (int h = 0; h < 4; h++) {
-                        take(h);
+                        if (h & 1) TMEM_ARRIVED(t1);
+                        else TMEM_ARRIVED(t0);
+                        if (h & 1) TMEM_LD32(mine + 32 * ((h + 1) & 3), t0);      // (behind the last: the first again)
+                        else TMEM_LD32(mine + 32 * ((h + 1) & 3), t1);
+                        float(&x)[32] = t[h & 1];
+                        mask(x, h);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) tm[i & 3] = fmaxf(tm[i & 3], t[i]);
+                        for (int i = 0; i < 32; i++) tm[i & 3] = fmaxf(tm[i & 3], x[i]);
                     }
                     const float top = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * c;
                     const bool move = top > m + 8.f;               // (the first: m is -inf)
@@ -396,39 +409,42 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         if (j > 0) {
 #pragma unroll
                             for (int h = 0; h < D; h += 32) {
-                                TMEM_LD32(mine + 128 + h, tv);
-                                tmem_wait_ld();
+                                TMEM_LD32(mine + 128 + h, t1);
+                                TMEM_ARRIVED(t1);
 #pragma unroll
-                                for (int i = 0; i < 32; i++) t[i] *= f;
-                                TMEM_ST16(mine + 128 + h, tv);
-                                TMEM_ST16(mine + 128 + h + 16, tv + 16);
+                                for (int i = 0; i < 32; i++) t[1][i] *= f;
+                                TMEM_ST16(mine + 128 + h, t1);
+                                TMEM_ST16(mine + 128 + h + 16, t1 + 16);
                             }
                         }
                     }
                     const float off = m == -INFINITY ? 0.f : KP_UP - m;
                     float e4[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t lo[F32 ? 64 : 1];
 #pragma unroll
                     for (int h = 0; h < 4; h++) {
-                        take(h);
-                        uint32_t p[16];
+                        if (h & 1) TMEM_ARRIVED(t1);
+                        else TMEM_ARRIVED(t0);
+                        if (h < 3) {
+                            if (h & 1) TMEM_LD32(mine + 32 * (h + 1), t0);
+                            else TMEM_LD32(mine + 32 * (h + 1), t1);
+                        }
+                        float(&x)[32] = t[h & 1];
+                        mask(x, h);
+                        uint32_t p[16], lo[F32 ? 16 : 1];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float a = ex2(fmaf(t[2 * i], c, off)), b = ex2(fmaf(t[2 * i + 1], c, off));
+                            const float a = ex2(fmaf(x[2 * i], c, off)), b = ex2(fmaf(x[2 * i + 1], c, off));
                             e4[i & 1] += a;
                             e4[2 + (i & 1)] += b;
                             const __half2 hi = __floats2half2_rn(a, b);
                             p[i] = hu(hi);
                             if constexpr (F32) {
                                 const float2 back = __half22float2(hi);
-                                lo[16 * h + i] = hu(__floats2half2_rn(a - back.x, b - back.y));
+                                lo[i] = hu(__floats2half2_rn(a - back.x, b - back.y));
                             }
                         }
-                        TMEM_ST16(mine + 16 * h, p);               // over scores that have been read
-                    }
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int h = 0; h < 4; h++) TMEM_ST16(mine + 64 + 16 * h, lo + 16 * h);
+                        TMEM_ST16(mine + 16 * h, p);               // over scores that have been read (what is on its way lies behind)
+                        if constexpr (F32) TMEM_ST16(mine + 256 + 16 * h, lo);
                     }
                     l += (e4[0] + e4[1]) + (e4[2] + e4[3]);
                     tmem_wait_st();
@@ -446,22 +462,24 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     constexpr int PIECE = 4, PIECES = D / PIECE;   // numbers to a piece
 #pragma unroll
                     for (int h = 0; h < D; h += 32) {
-                        TMEM_LD32(mine + 128 + h, tv);
-                        tmem_wait_ld();
+                        TMEM_LD32(mine + 128 + h, t0);
+                        TMEM_ARRIVED(t0);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) t[i] *= inv;
+                        for (int i = 0; i < 32; i++) t[0][i] *= inv;
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {           // columns 0 2 4 6 | 1 3 5 7 of an eight are numbers 0 1 2 3 | 4 5 6 7
-                            store4(os + row * D + ((h + i) / 4 + row) % PIECES * 4, make_float4(t[i], t[i + 2], t[i + 4], t[i + 6]));
-                            store4(os + row * D + ((h + i) / 4 + 1 + row) % PIECES * 4, make_float4(t[i + 1], t[i + 3], t[i + 5], t[i + 7]));
+                            store4(os + row * D + ((h + i) / 4 + row) % PIECES * 4, make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]));
+                            store4(os + row * D + ((h + i) / 4 + 1 + row) % PIECES * 4, make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]));
                         }
                     }
-                    group_barrier(grp);
-#pragma unroll 4
+                    __syncwarp();                                  // a warp reads its own rows
+                    const int64_t o_at = (P.q.q0 + tok) * A.ldo + (int64_t) head * D;
+#pragma unroll 8
                     for (int i = 0; i < 32 / RPW; i++) {
-                        const int rr = w * 32 + i * RPW + sub, ar = P.row0 + grp * KP_TILE + rr, tt = ar / A.group;
-                        const float4 v = load4(os + rr * D + (l4 + rr) % PIECES * 4);
-                        if (grp * KP_TILE + rr < P.rows) store4((T *) A.out + (P.q.q0 + tt) * A.ldo + (int64_t) (P.hk * A.group + ar - tt * A.group) * D + 4 * l4, v);
+                        const int rr = i * RPW + sub;
+                        const float4 v = load4(os + (w * 32 + rr) * D + (l4 + rr) % PIECES * 4);
+                        const int64_t to = __shfl_sync(0xffffffffu, o_at, rr);
+                        if (valid >> rr & 1) store4((T *) A.out + to + 4 * l4, v);
                     }
                 } else {
                     KpPart<D> & part = reinterpret_cast<KpParts<D> *>(W.parts)->part[P.slot];
@@ -472,12 +490,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     const int pr = grp * KP_TILE + row;
 #pragma unroll
                     for (int h = 0; h < D; h += 32) {
-                        TMEM_LD32(mine + 128 + h, tv);
-                        tmem_wait_ld();
+                        TMEM_LD32(mine + 128 + h, t0);
+                        TMEM_ARRIVED(t0);
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
-                            *reinterpret_cast<float4 *>(&part.o[pr][h + i]) = make_float4(t[i], t[i + 2], t[i + 4], t[i + 6]);
-                            *reinterpret_cast<float4 *>(&part.o[pr][h + i + 4]) = make_float4(t[i + 1], t[i + 3], t[i + 5], t[i + 7]);
+                            *reinterpret_cast<float4 *>(&part.o[pr][h + i]) = make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]);
+                            *reinterpret_cast<float4 *>(&part.o[pr][h + i + 4]) = make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]);
                         }
                     }
                     part.m[pr] = m;
