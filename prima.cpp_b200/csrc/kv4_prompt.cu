@@ -40,10 +40,11 @@ template <int D> struct KpSmem {
     uint8_t q[2][D / 64][KP_BLOCK];            // 16 bits: either row tile; F32: high and low
     uint8_t k[2][D / 64][KP_BLOCK], v[2][D / 64][KP_BLOCK];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+    KpPiece piece[2];          // the one at hand and the next
     float mult[2 * KP_TILE];
-    KpPiece piece;
+    int cell[4][2];            // first cells of a key tile's pages (of none: beyond everything)
     uint32_t tmem_base;
-    int abort, more, total, items;
+    int abort, more[2];
 };
 // tickets: two words, and for each slot whether a cut item's parts begin there (cleared in front of the kernel); cut: long items may be
 struct KpWork { int most_rows; int * tickets; void * parts; int * abort_flag; int cut; };
@@ -125,6 +126,18 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, int
         cut += __shfl_sync(0xffffffffu, y - n.cut, at);
         p.s = s0 + at;
         const Kv4Seq mine = kv4_seq(A, p.s, W.most_rows, true);
+        if (limit == 0) {
+            const int tile = i / A.cache.n_head_kv;
+            p.row0 = ((mine.n_rows + ROWS - 1) / ROWS - 1 - tile) * ROWS;
+            p.rows = min(ROWS, mine.n_rows - p.row0);
+            kp_span(A, mine, p);
+            p.hk = i - tile * A.cache.n_head_kv;
+            p.part = p.a = 0;
+            p.b = p.tiles;
+            p.parts = 1;
+            p.slot = -1;
+            return true;
+        }
         for (int tile = (mine.n_rows + ROWS - 1) / ROWS - 1; tile >= 0; tile--) {
             p.row0 = tile * ROWS;
             p.rows = min(ROWS, mine.n_rows - p.row0);
@@ -193,16 +206,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     int limit = 0, ticket = blockIdx.x;
     if (warp == 12) {
         limit = kp_limit<ROWS>(A, W, gridDim.x);
-        const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece);
-        if (lane == 0) S.more = more;
+        const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece[0]);
+        if (lane == 0) S.more[0] = more;
     }
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = *(volatile uint32_t *) &S.tmem_base;
     uint32_t tiles[2] = {0, 0}, pieces[2] = {0, 0};   // key tiles and pieces in front, of either row tile (all roles count them)
-    while (*(volatile int *) &S.more) {
-        const KpPiece & P = S.piece;
+    while (*(volatile int *) &S.more[pieces[0] & 1]) {
+        const KpPiece & P = S.piece[pieces[0] & 1];
         const int n = P.b - P.a, groups = P.rows > KP_TILE ? 2 : 1;
         if (warp < 4) {
             // ---- expand ----
@@ -234,6 +247,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 const uint32_t u = tiles[0] + (uint32_t) j;
                 const int st = (int) (u & 1);
                 const uint8_t * third = chunk_of(j + 2);
+                if (t6 == 0) S.cell[u & 3][half] = now ? kv4_page_index(P.q, 2 * (P.a + j) + half) * KV4_CELLS : 0x7fffff00;
                 if (u >= 2) mbar_wait(&S.k_empty[st], (u / 2 - 1) & 1, cta_abort, W.abort_flag);
                 {
                     const uint32_t odd = t6 & 1 ? 0x3232u : 0x1010u;
@@ -270,6 +284,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.v_full[st]);
                 ask_v(later);
+                now = later;
                 later = third;
             }
         } else if (warp == 12) {
@@ -320,6 +335,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     }
                 }
             }
+            if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[0], 1);
+            ticket = __shfl_sync(0xffffffffu, ticket, 0);
+            const int later = (pieces[0] + 1) & 1;
+            const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
+            if (lane == 0) S.more[later] = more;
         } else if ((warp - 4) >> 2 < GROUPS) {
             // ---- softmax ----
             const int grp = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane, w = warp - 4 - 4 * grp;
@@ -370,23 +390,28 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 float t[2][32];                                    // scores, 32 being worked on and 32 on their way
                 uint32_t * const t0 = reinterpret_cast<uint32_t *>(t[0]), * const t1 = reinterpret_cast<uint32_t *>(t[1]);
                 for (int j = 0; j < n; j++) {
-                    const int i0 = 2 * (P.a + j), i1 = i0 + 1;
-                    // first cells of the two pages; of none: beyond everything
-                    const int c0 = kv4_page(A, P.q, P.s, i0) >= 0 ? kv4_page_index(P.q, i0) * KV4_CELLS : 0x7fffff00;
-                    const int c1 = i1 < P.q.pages && kv4_page(A, P.q, P.s, i1) >= 0 ? kv4_page_index(P.q, i1) * KV4_CELLS : 0x7fffff00;
-                    const bool whole = c1 <= g_lo - 63 && c0 <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
-                    auto mask = [&](float (&x)[32], int h) {       // a score that is not seen is -inf
-                        if (whole) return;
-                        const int base = (h < 2 ? c0 : c1) + 32 * (h & 1);
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const int cell = base + i;
-                            x[i] = cell <= pos && (A.window <= 0 || pos - cell < A.window || cell < A.first) ? x[i] : -INFINITY;
-                        }
-                    };
                     mbar_wait(&S.s_full[grp], (tiles[grp] + (uint32_t) j) & 1, cta_abort, W.abort_flag);
                     __syncwarp();
                     fence_after();
+                    // (four of them: written for tile j + 4 behind the scores of j + 2, which come behind the weights of j)
+                    const int c0 = *(volatile int *) &S.cell[(tiles[0] + (uint32_t) j) & 3][0], c1 = *(volatile int *) &S.cell[(tiles[0] + (uint32_t) j) & 3][1];
+                    const bool whole = c1 <= g_lo - 63 && c0 <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
+                    if (!whole) {   // a score that is not seen is -inf: in its place, ahead of the passes over the tile
+                        const int from = A.window > 0 ? max(0, pos - A.window + 1) : 0;
+#pragma unroll 1
+                        for (int h = 0; h < 4; h++) {
+                            const int base = (h < 2 ? c0 : c1) + 32 * (h & 1);
+                            auto below = [&](int cell) { const int k = cell - base; return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };     // cells in front of it
+                            const uint32_t seen = pos < 0 || base > pos ? 0u : below(pos + 1) & (~below(from) | below(A.first));
+                            TMEM_LD32(mine + 32 * h, t0);
+                            TMEM_ARRIVED(t0);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) t[0][i] = seen >> i & 1 ? t[0][i] : -INFINITY;
+                            TMEM_ST16(mine + 32 * h, t0);
+                            TMEM_ST16(mine + 32 * h + 16, t0 + 16);
+                        }
+                        tmem_wait_st();
+                    }
                     float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     TMEM_LD32(mine, t0);
 #pragma unroll
@@ -396,7 +421,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         if (h & 1) TMEM_LD32(mine + 32 * ((h + 1) & 3), t0);      // (behind the last: the first again)
                         else TMEM_LD32(mine + 32 * ((h + 1) & 3), t1);
                         float(&x)[32] = t[h & 1];
-                        mask(x, h);
 #pragma unroll
                         for (int i = 0; i < 32; i++) tm[i & 3] = fmaxf(tm[i & 3], x[i]);
                     }
@@ -429,7 +453,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             else TMEM_LD32(mine + 32 * (h + 1), t1);
                         }
                         float(&x)[32] = t[h & 1];
-                        mask(x, h);
                         uint32_t p[16], lo[F32 ? 16 : 1];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
@@ -512,13 +535,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             tiles[1] += (uint32_t) n;
             pieces[1]++;
         }
-        if (warp == 12) {
-            if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[0], 1);
-            ticket = __shfl_sync(0xffffffffu, ticket, 0);
-            const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece);
-            if (lane == 0) S.more = more;
-        }
-        __syncthreads();
         fence_after();
     }
     if (warp == 12) {
