@@ -4,13 +4,13 @@
 // 16-bit ones exactly, F32 as two numbers, 22 bits), weights f16 (F32: two numbers).  A row's reference is the largest score of its first tile; it moves only where a
 // score lies beyond it by more than 2^8, and then its sum and O are scaled.
 //
-// Work.  An item is a (sequence, kv head, tile of query rows: tokens x heads of the group); 16 bits have two row tiles of 128 that share each expanded key tile, F32 one.  Key tiles are
-// two pages.  CTAs (one to an SM) take items by tickets, long ones of a sequence first; where there are fewer items than SMs, long items are cut into pieces, which a second
+// Work.  An item is a (sequence, kv head, tile of query rows: tokens x heads of the group).  Two softmax groups keep the tensor cores busy in turns: with 16 bits each has 128 rows, which
+// share each expanded key tile; with F32 both have the same 128 rows and every other key tile, and their sums are joined at the end.  Key tiles are two pages.  CTAs (one to an SM) take items by tickets, long ones of a sequence first; where there are fewer items than SMs, long items are cut into pieces, which a second
 // kernel adds up in their order.
 //   warps 0 - 3    expand: a thread has a cell's row of keys, then one of values: raw words in registers a tile ahead, f16 into the swizzle-128B images, two stages each
-//   warps 4 - 11   softmax: a thread has a row of S (4 - 7: first row tile, 8 - 11: second), which is also a lane of tensor memory
+//   warps 4 - 11   softmax, groups of four: a thread has a row of S, which is also a lane of tensor memory
 //   warp 12        MMA issuer, owner of the tensor memory, and of the tickets
-// Tensor memory: S / P of either row tile at 0 and 256 (F32: the weights' low parts there), O at 128 and 384.
+// Tensor memory: S / P of either group at 0 and 256, O at 128 and 384.  Weights lie over their scores: 16 columns for 32, F32's low parts in the other 16.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -25,8 +25,7 @@ namespace {
 
 constexpr int KP_THREADS = 13 * 32, KP_TILE = 128, KP_BLOCK = 16384;   // a block: 128 rows of 64 entries
 constexpr float KP_UP = 6.f;            // weights are up to 2^(8 + 6)
-template <typename T> constexpr int kp_groups() { return std::is_same<T, float>::value ? 1 : 2; }
-template <typename T> constexpr int kp_rows() { return KP_TILE * kp_groups<T>(); }
+template <typename T> constexpr int kp_rows() { return std::is_same<T, float>::value ? KP_TILE : 2 * KP_TILE; }   // of an item
 
 struct KpPiece {               // what a ticket stands for
     int s, hk, row0, rows;     // sequence, kv head, first row (of the sequence's) and rows of the tile
@@ -41,7 +40,7 @@ template <int D> struct KpSmem {
     uint8_t k[2][D / 64][KP_BLOCK], v[2][D / 64][KP_BLOCK];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
     KpPiece piece[2];          // the one at hand and the next
-    float mult[2 * KP_TILE];
+    float mult[2 * KP_TILE], other[2][KP_TILE];
     int cell[4][2];            // first cells of a key tile's pages (of none: beyond everything)
     uint32_t tmem_base;
     int abort, more[2];
@@ -179,7 +178,7 @@ __device__ __forceinline__ uint4 expand(uint32_t w, __half2 d) {
 template <typename T, int D>
 __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
     constexpr bool F32 = std::is_same<T, float>::value;
-    constexpr int GROUPS = kp_groups<T>(), ROWS = kp_rows<T>(), NB = D / 32;
+    constexpr int ROWS = kp_rows<T>(), NB = D / 32;
     extern __shared__ uint8_t smem_raw[];
     KpSmem<D> & S = *reinterpret_cast<KpSmem<D> *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
@@ -213,10 +212,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     __syncthreads();
     fence_after();
     const uint32_t tmem = *(volatile uint32_t *) &S.tmem_base;
-    uint32_t tiles[2] = {0, 0}, pieces[2] = {0, 0};   // key tiles and pieces in front, of either row tile (all roles count them)
-    while (*(volatile int *) &S.more[pieces[0] & 1]) {
-        const KpPiece & P = S.piece[pieces[0] & 1];
-        const int n = P.b - P.a, groups = P.rows > KP_TILE ? 2 : 1;
+    uint32_t tiles = 0, pieces = 0, of_group[2] = {0, 0}, ends[2] = {0, 0};   // key tiles and pieces in front; key tiles and pieces of either group (all roles count them)
+    while (*(volatile int *) &S.more[pieces & 1]) {
+        const KpPiece & P = S.piece[pieces & 1];
+        const int n = P.b - P.a, groups = (F32 ? n > 1 : P.rows > KP_TILE) ? 2 : 1;      // groups at work
         if (warp < 4) {
             // ---- expand ----
             const int x = threadIdx.x, half = x >> 6, t6 = x & 63, r = t6, tv = (r & ~7) | ((r & 3) << 1) | ((r >> 2) & 1);
@@ -244,7 +243,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             ask_k(now);
             ask_v(now);
             for (int j = 0; j < n; j++) {
-                const uint32_t u = tiles[0] + (uint32_t) j;
+                const uint32_t u = tiles + (uint32_t) j;
                 const int st = (int) (u & 1);
                 const uint8_t * third = chunk_of(j + 2);
                 if (t6 == 0) S.cell[u & 3][half] = now ? kv4_page_index(P.q, 2 * (P.a + j) + half) * KV4_CELLS : 0x7fffff00;
@@ -291,8 +290,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             // ---- MMA ----
             constexpr uint32_t idesc = (1u << 4) | ((uint32_t) (128 >> 3) << 17) | ((uint32_t) (128 >> 4) << 24);
             constexpr uint32_t idesc_v = (1u << 4) | ((uint32_t) (D >> 3) << 17) | ((uint32_t) (128 >> 4) << 24) | (1u << 16);
-            asm volatile("bar.sync 4, %0;" ::"n"(32 * (1 + 4 * GROUPS)) : "memory");      // the queries are there
-            auto scores = [&](int grp, int st) {
+            asm volatile("bar.sync 4, 288;" ::: "memory");        // the queries are there
+            // S of a tile behind the P V that reads this tensor memory (MMAs run in order)
+            auto scores = [&](int grp, uint32_t u) {
+                const int st = (int) (u & 1);
+                if (F32 || grp == 0) mbar_wait(&S.k_full[st], (u / 2) & 1, cta_abort, W.abort_flag);
+                __syncwarp();
+                fence_after();
                 if (elect_one()) {
 #pragma unroll
                     for (int part = 0; part < (F32 ? 2 : 1); part++) {
@@ -302,99 +306,108 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             mma_f16<1>(tmem + 256 * grp, dq + (k >> 2) * (KP_BLOCK >> 4) + 2 * (k & 3), dk + (k >> 2) * (KP_BLOCK >> 4) + 2 * (k & 3), idesc, (uint32_t) ((part | k) != 0));
                     }
                     mma_commit(&S.s_full[grp]);
-                    if (grp == groups - 1) mma_commit(&S.k_empty[st]);
+                    if (F32 || grp == groups - 1) mma_commit(&S.k_empty[st]);
                 }
                 __syncwarp();
             };
-            for (int j = -1; j < n; j++) {
-                const uint32_t u = tiles[0] + (uint32_t) j;
-                const int st = (int) (u & 1), st1 = (int) ((u + 1) & 1);
-                for (int grp = 0; grp < groups; grp++) {
-                    if (j >= 0) {
-                        if (grp == 0) mbar_wait(&S.v_full[st], (u / 2) & 1, cta_abort, W.abort_flag);
-                        mbar_wait(&S.p_full[grp], (tiles[grp] + (uint32_t) j) & 1, cta_abort, W.abort_flag);
-                        __syncwarp();
-                        fence_after();
-                        if (elect_one()) {
-                            const uint64_t dv = desc_sw128_mn(smem_u32(S.v[st]), KP_BLOCK);
+            auto values = [&](int grp, uint32_t u, int i, bool last) {       // i: which of the group's tiles
+                const int st = (int) (u & 1);
+                if (F32 || grp == 0) mbar_wait(&S.v_full[st], (u / 2) & 1, cta_abort, W.abort_flag);
+                mbar_wait(&S.p_full[grp], (of_group[grp] + (uint32_t) i) & 1, cta_abort, W.abort_flag);
+                __syncwarp();
+                fence_after();
+                if (elect_one()) {
+                    const uint64_t dv = desc_sw128_mn(smem_u32(S.v[st]), KP_BLOCK);
 #pragma unroll
-                            for (int part = 0; part < (F32 ? 2 : 1); part++)
+                    for (int part = 0; part < (F32 ? 2 : 1); part++)
 #pragma unroll
-                                for (int k = 0; k < 8; k++)
-                                    mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * (grp + part) + 8 * k, dv + k * (2048 >> 4), idesc_v, (uint32_t) ((j | part | k) != 0));
-                            if (j == n - 1) mma_commit(&S.o_full[grp]);
-                            if (grp == groups - 1) mma_commit(&S.v_empty[st]);
-                        }
-                        __syncwarp();
-                    }
-                    if (j + 1 < n) {                              // behind the P V that reads this tensor memory: MMAs run in order
-                        if (grp == 0) mbar_wait(&S.k_full[st1], ((u + 1) / 2) & 1, cta_abort, W.abort_flag);
-                        __syncwarp();
-                        fence_after();
-                        scores(grp, st1);
-                    }
+                        for (int k = 0; k < 8; k++)
+                            mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * grp + 32 * (k >> 1) + 8 * (k & 1) + 16 * part, dv + k * (2048 >> 4), idesc_v, (uint32_t) ((i | part | k) != 0));
+                    if (last) mma_commit(&S.o_full[grp]);
+                    if (F32 || grp == groups - 1) mma_commit(&S.v_empty[st]);
                 }
+                __syncwarp();
+            };
+            if constexpr (F32) {
+                for (int j = -2; j < n; j++) {
+                    if (j >= 0) values(j & 1, tiles + (uint32_t) j, j >> 1, j + 2 >= n);
+                    if (j + 2 < n) scores(j & 1, tiles + (uint32_t) (j + 2));
+                }
+            } else {
+                for (int j = -1; j < n; j++)
+                    for (int grp = 0; grp < groups; grp++) {
+                        if (j >= 0) values(grp, tiles + (uint32_t) j, j, j == n - 1);
+                        if (j + 1 < n) scores(grp, tiles + (uint32_t) (j + 1));
+                    }
             }
             if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[0], 1);
             ticket = __shfl_sync(0xffffffffu, ticket, 0);
-            const int later = (pieces[0] + 1) & 1;
+            const int later = (pieces + 1) & 1;
             const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
             if (lane == 0) S.more[later] = more;
-        } else if ((warp - 4) >> 2 < GROUPS) {
+        } else {
             // ---- softmax ----
-            const int grp = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane, w = warp - 4 - 4 * grp;
-            // queries -> f16 in the swizzle-128B image: a warp has whole rows, 8 of them on their way; a row's largest number comes to 2^13 .. 2^14
-            constexpr int LPR = D / 4, RPW = 32 / LPR, ONCE = 16; // lanes to a row, rows to a pass, passes on their way
-            const int sub = lane / LPR, l4 = lane % LPR;
-            // this lane's row of the tile: its token and head, and where they lie (others' by shuffles: a division costs more than a row)
-            const int at = P.row0 + grp * KP_TILE + row, tok = at / A.group, head = P.hk * A.group + at - tok * A.group;
-            const bool mine_is = grp * KP_TILE + row < P.rows;
+            const int grp = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;       // (the quarter of tensor memory that a warp reaches is its number's last two bits)
+            const int rows0 = F32 ? 0 : grp * KP_TILE;                                        // the group's first row of the item
+            // this lane's row: its token and head, and where they lie (others' by shuffles: a division costs more than a row)
+            const int at = P.row0 + rows0 + row, tok = at / A.group, head = P.hk * A.group + at - tok * A.group;
+            const bool mine_is = rows0 + row < P.rows;
             const uint32_t valid = __ballot_sync(0xffffffffu, mine_is);
             const int64_t q_at = (P.q.q0 + tok) * A.ldq + (int64_t) head * D;
+            // queries -> f16 in the swizzle-128B image: 8 numbers to a lane; a row's largest comes to 2^13 .. 2^14.  F32: half of a warp's rows are its sister's
+            {
+                constexpr int LPR = D / 8, RPW = 32 / LPR, PASSES = 32 / RPW / (F32 ? 2 : 1), ONCE = PASSES < 8 ? PASSES : 8;    // lanes to a row, rows at once
+                const int sub = lane / LPR, l8 = lane % LPR;
 #pragma unroll 1
-            for (int i0 = 0; i0 < 32 / RPW; i0 += ONCE) {
-                float4 v[ONCE];
+                for (int i0 = 0; i0 < PASSES; i0 += ONCE) {
+                    float4 v[ONCE][2];
 #pragma unroll
-                for (int i = 0; i < ONCE; i++) {
-                    const int rr = (i0 + i) * RPW + sub;
-                    const int64_t from = __shfl_sync(0xffffffffu, q_at, rr);
-                    v[i] = valid >> rr & 1 ? load4((const T *) A.q + from + 4 * l4) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
+                    for (int i = 0; i < ONCE; i++) {
+                        const int rr = (i0 + i + (F32 ? grp * PASSES : 0)) * RPW + sub;
+                        const T * from = (const T *) A.q + __shfl_sync(0xffffffffu, q_at, rr) + 8 * l8;
+                        v[i][0] = valid >> rr & 1 ? load4(from) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        v[i][1] = valid >> rr & 1 ? load4(from + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
 #pragma unroll
-                for (int i = 0; i < ONCE; i++) {
-                    const int rr = w * 32 + (i0 + i) * RPW + sub;
-                    float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+                    for (int i = 0; i < ONCE; i++) {
+                        const int rr = quad * 32 + (i0 + i + (F32 ? grp * PASSES : 0)) * RPW + sub;
+                        float4 x = v[i][0], y = v[i][1];
+                        float top = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
 #pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int ex = top > 0.f && top < INFINITY ? min(126, 140 - (int) (__float_as_uint(top) >> 23)) : 0;
-                    const float up = __int_as_float((ex + 127) << 23) * (A.scale < 0.f ? -1.f : 1.f);
-                    if (l4 == 0) S.mult[grp * KP_TILE + rr] = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23), FLT_MIN);
-                    const float x0 = v[i].x * up, x1 = v[i].y * up, x2 = v[i].z * up, x3 = v[i].w * up;
-                    const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
-                    const int to = (l4 >> 4) * KP_BLOCK + rr * 128 + ((((l4 & 15) >> 1) ^ (rr & 7)) << 4) + (l4 & 1) * 8;
-                    *reinterpret_cast<uint2 *>(&S.q[F32 ? 0 : grp][0][0] + to) = make_uint2(hu(h0), hu(h1));
-                    if constexpr (F32) {
-                        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-                        *reinterpret_cast<uint2 *>(&S.q[1][0][0] + to) = make_uint2(hu(__floats2half2_rn(x0 - b0.x, x1 - b0.y)), hu(__floats2half2_rn(x2 - b1.x, x3 - b1.y)));
+                        for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const int ex = top > 0.f && top < INFINITY ? min(126, 140 - (int) (__float_as_uint(top) >> 23)) : 0;
+                        const float up = __int_as_float((ex + 127) << 23) * (A.scale < 0.f ? -1.f : 1.f);
+                        // scores in units of log2; never 0: a masked score stays -inf
+                        if (l8 == 0) S.mult[rows0 + rr] = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23), FLT_MIN);
+                        x.x *= up; x.y *= up; x.z *= up; x.w *= up; y.x *= up; y.y *= up; y.z *= up; y.w *= up;
+                        const __half2 h[4] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w), __floats2half2_rn(y.x, y.y), __floats2half2_rn(y.z, y.w)};
+                        const int to = (l8 >> 3) * KP_BLOCK + rr * 128 + (((l8 & 7) ^ (rr & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(&S.q[F32 ? 0 : grp][0][0] + to) = make_uint4(hu(h[0]), hu(h[1]), hu(h[2]), hu(h[3]));
+                        if constexpr (F32) {
+                            const float2 b[4] = {__half22float2(h[0]), __half22float2(h[1]), __half22float2(h[2]), __half22float2(h[3])};
+                            *reinterpret_cast<uint4 *>(&S.q[1][0][0] + to) =
+                                make_uint4(hu(__floats2half2_rn(x.x - b[0].x, x.y - b[0].y)), hu(__floats2half2_rn(x.z - b[1].x, x.w - b[1].y)),
+                                           hu(__floats2half2_rn(y.x - b[2].x, y.y - b[2].y)), hu(__floats2half2_rn(y.z - b[3].x, y.w - b[3].y)));
+                        }
                     }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("bar.sync 4, %0;" ::"n"(32 * (1 + 4 * GROUPS)) : "memory");
+            asm volatile("bar.sync 4, 288;" ::: "memory");
             if (grp < groups) {
                 const int pos = mine_is ? P.q.p0 + tok : -1;
-                const float c = S.mult[grp * KP_TILE + row];
+                const float c = S.mult[rows0 + row];
                 const uint32_t mine = tmem + ((uint32_t) (quad * 32) << 16) + 256 * grp;
-                const int g_lo = P.q.p0 + (P.row0 + grp * KP_TILE) / A.group;      // of this row tile: the first row's position
+                const int g_lo = P.q.p0 + (P.row0 + rows0) / A.group;              // of the group's first row
                 float m = -INFINITY, l = 0.f;
                 float t[2][32];                                    // scores, 32 being worked on and 32 on their way
                 uint32_t * const t0 = reinterpret_cast<uint32_t *>(t[0]), * const t1 = reinterpret_cast<uint32_t *>(t[1]);
-                for (int j = 0; j < n; j++) {
-                    mbar_wait(&S.s_full[grp], (tiles[grp] + (uint32_t) j) & 1, cta_abort, W.abort_flag);
+                for (int j = F32 ? grp : 0, i = 0; j < n; j += F32 ? 2 : 1, i++) {
+                    mbar_wait(&S.s_full[grp], (of_group[grp] + (uint32_t) i) & 1, cta_abort, W.abort_flag);
                     __syncwarp();
                     fence_after();
                     // (four of them: written for tile j + 4 behind the scores of j + 2, which come behind the weights of j)
-                    const int c0 = *(volatile int *) &S.cell[(tiles[0] + (uint32_t) j) & 3][0], c1 = *(volatile int *) &S.cell[(tiles[0] + (uint32_t) j) & 3][1];
+                    const int c0 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][0], c1 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][1];
                     const bool whole = c1 <= g_lo - 63 && c0 <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
                     if (!whole) {   // a score that is not seen is -inf: in its place, ahead of the passes over the tile
                         const int from = A.window > 0 ? max(0, pos - A.window + 1) : 0;
@@ -430,7 +443,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2(m - top);
                         if (move) m = top;
                         l *= f;
-                        if (j > 0) {
+                        if (i > 0) {
 #pragma unroll
                             for (int h = 0; h < D; h += 32) {
                                 TMEM_LD32(mine + 128 + h, t1);
@@ -466,8 +479,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                                 lo[i] = hu(__floats2half2_rn(a - back.x, b - back.y));
                             }
                         }
-                        TMEM_ST16(mine + 16 * h, p);               // over scores that have been read (what is on its way lies behind)
-                        if constexpr (F32) TMEM_ST16(mine + 256 + 16 * h, lo);
+                        TMEM_ST16(mine + 32 * h, p);               // over the scores
+                        if constexpr (F32) TMEM_ST16(mine + 32 * h + 16, lo);
                     }
                     l += (e4[0] + e4[1]) + (e4[2] + e4[3]);
                     tmem_wait_st();
@@ -475,65 +488,104 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&S.p_full[grp]);
                 }
-                mbar_wait(&S.o_full[grp], pieces[grp] & 1, cta_abort, W.abort_flag);
+                // F32: all scores are made before the queries' memory is used again
+                for (int k = 0; k < 2; k++)
+                    if (F32 ? k < groups : k == grp) mbar_wait(&S.o_full[k], ends[k] & 1, cta_abort, W.abort_flag);
                 __syncwarp();
                 fence_after();
-                if (P.slot < 0) {
-                    // through the queries' memory (all scores are made), rows of 128-byte pieces rotated by the row, so that a warp stores whole rows
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    T * os = reinterpret_cast<T *>(&S.q[F32 ? 0 : grp][0][0]);
-                    constexpr int PIECE = 4, PIECES = D / PIECE;   // numbers to a piece
+                constexpr int PIECE = 4, PIECES = D / PIECE;       // numbers to a piece; row r's pieces are rotated by r
+                float mine_f = 1.f, other = 0.f;                    // F32: factors of the groups' sums
+                float * const os32 = reinterpret_cast<float *>(&S.q[0][0][0]) + row * D;
+                if (F32 && groups == 2) {                           // the second group's sums go to the first through the queries' memory
+                    if (grp == 1) {
+#pragma unroll
+                        for (int h = 0; h < D; h += 32) {
+                            TMEM_LD32(mine + 128 + h, t0);
+                            TMEM_ARRIVED(t0);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) store4(os32 + ((h + i) / 4 + row) % PIECES * 4, make_float4(t[0][i], t[0][i + 1], t[0][i + 2], t[0][i + 3]));
+                        }
+                        S.other[0][row] = m;
+                        S.other[1][row] = l;
+                    }
+                    asm volatile("bar.sync 5, 256;" ::: "memory");
+                    if (grp == 0) {
+                        const float m2 = S.other[0][row], l2 = S.other[1][row], top = fmaxf(m, m2);
+                        // a row that is no number has no maximum
+                        const float f = m == -INFINITY ? (l == l ? 0.f : 1.f) : ex2(m - top);
+                        other = m2 == -INFINITY ? (l2 == l2 ? 0.f : 1.f) : ex2(m2 - top);
+                        l = l * f + l2 * other;
+                        m = top;
+                        mine_f = f;
+                    }
+                }
+                if (!F32 || grp == 0) {
+                    const float inv = P.slot >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                    KpPart<D> * part = nullptr;
+                    if (P.slot >= 0) {
+                        part = &reinterpret_cast<KpParts<D> *>(W.parts)->part[P.slot];
+                        part->m[rows0 + row] = m;
+                        part->l[rows0 + row] = l;
+                        if (threadIdx.x == 128 && P.part == 0) {
+                            reinterpret_cast<KpParts<D> *>(W.parts)->first[P.slot] = P;
+                            W.tickets[KP_FLAGS + P.slot] = 1;
+                        }
+                    }
+                    // through the queries' memory, so that a warp stores whole rows
+                    T * os = reinterpret_cast<T *>(&S.q[F32 ? 0 : grp][0][0]) + row * D;
 #pragma unroll
                     for (int h = 0; h < D; h += 32) {
                         TMEM_LD32(mine + 128 + h, t0);
                         TMEM_ARRIVED(t0);
+                        if (F32 && groups == 2) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 y = *reinterpret_cast<const float4 *>(os32 + ((h + i) / 4 + row) % PIECES * 4);
+                                t[0][i] = t[0][i] * mine_f + y.x * other;
+                                t[0][i + 1] = t[0][i + 1] * mine_f + y.y * other;
+                                t[0][i + 2] = t[0][i + 2] * mine_f + y.z * other;
+                                t[0][i + 3] = t[0][i + 3] * mine_f + y.w * other;
+                            }
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; i++) t[0][i] *= inv;
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {           // columns 0 2 4 6 | 1 3 5 7 of an eight are numbers 0 1 2 3 | 4 5 6 7
-                            store4(os + row * D + ((h + i) / 4 + row) % PIECES * 4, make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]));
-                            store4(os + row * D + ((h + i) / 4 + 1 + row) % PIECES * 4, make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]));
+                            const float4 a = make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]), b = make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]);
+                            if (part) {
+                                *reinterpret_cast<float4 *>(&part->o[rows0 + row][h + i]) = a;
+                                *reinterpret_cast<float4 *>(&part->o[rows0 + row][h + i + 4]) = b;
+                            } else {
+                                store4(os + ((h + i) / 4 + row) % PIECES * 4, a);
+                                store4(os + ((h + i) / 4 + 1 + row) % PIECES * 4, b);
+                            }
                         }
                     }
-                    __syncwarp();                                  // a warp reads its own rows
-                    const int64_t o_at = (P.q.q0 + tok) * A.ldo + (int64_t) head * D;
+                    if (!part) {
+                        constexpr int LPR = D / 4, RPW = 32 / LPR;
+                        const int sub = lane / LPR, l4 = lane % LPR;
+                        __syncwarp();                               // a warp reads its own rows
+                        const int64_t o_at = (P.q.q0 + tok) * A.ldo + (int64_t) head * D;
+                        const T * rows = reinterpret_cast<const T *>(&S.q[F32 ? 0 : grp][0][0]) + quad * 32 * D;
 #pragma unroll 8
-                    for (int i = 0; i < 32 / RPW; i++) {
-                        const int rr = i * RPW + sub;
-                        const float4 v = load4(os + (w * 32 + rr) * D + (l4 + rr) % PIECES * 4);
-                        const int64_t to = __shfl_sync(0xffffffffu, o_at, rr);
-                        if (valid >> rr & 1) store4((T *) A.out + to + 4 * l4, v);
-                    }
-                } else {
-                    KpPart<D> & part = reinterpret_cast<KpParts<D> *>(W.parts)->part[P.slot];
-                    if (threadIdx.x == 128 && P.part == 0) {
-                        reinterpret_cast<KpParts<D> *>(W.parts)->first[P.slot] = P;
-                        W.tickets[KP_FLAGS + P.slot] = 1;
-                    }
-                    const int pr = grp * KP_TILE + row;
-#pragma unroll
-                    for (int h = 0; h < D; h += 32) {
-                        TMEM_LD32(mine + 128 + h, t0);
-                        TMEM_ARRIVED(t0);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            *reinterpret_cast<float4 *>(&part.o[pr][h + i]) = make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]);
-                            *reinterpret_cast<float4 *>(&part.o[pr][h + i + 4]) = make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]);
+                        for (int i = 0; i < 32 / RPW; i++) {
+                            const int rr = i * RPW + sub;
+                            const float4 v = load4(rows + rr * D + (l4 + quad * 32 + rr) % PIECES * 4);
+                            const int64_t to = __shfl_sync(0xffffffffu, o_at, rr);
+                            if (valid >> rr & 1) store4((T *) A.out + to + 4 * l4, v);
                         }
                     }
-                    part.m[pr] = m;
-                    part.l[pr] = l;
                 }
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fence_before();
         __syncthreads();
-        tiles[0] += (uint32_t) n;
-        pieces[0]++;
-        if (groups == 2) {
-            tiles[1] += (uint32_t) n;
-            pieces[1]++;
+        tiles += (uint32_t) n;
+        pieces++;
+        for (int grp = 0; grp < groups; grp++) {
+            of_group[grp] += (uint32_t) (F32 ? (n - grp + 1) / 2 : n);
+            ends[grp]++;
         }
         fence_after();
     }
