@@ -31,6 +31,9 @@ namespace {
 constexpr int KR_ROWS = 8;
 // Warps of a CTA, one CTA to an SM: 168 registers (16 warps of 128: 94 us for two sequences of 131071 and 65001 cells, these 65).  Stages of a warp's ring: a page each.
 constexpr int KR_WARPS = 12, KR_THREADS = 32 * KR_WARPS;
+// Few pages go to as many warps of a CTA at least: one for each of an SM's schedulers.  us, with 4 / 8 / 12: a token of 32 heads over 8 behind 100 cells 11.6 / 15.4 / 19.1, behind
+// 1000 13.6 / 15.2 / 20.1, behind 4000 17.1 / 17.9 / 19.5
+constexpr int KR_LEAST = 4;
 template <int D> constexpr int kr_stages() { return D == 128 ? 2 : 4; }
 constexpr int KR_UP = 12;   // F32: weights are 2^12 larger than exp(score - maximum): those of 2^-26 are normal f16 numbers
 
@@ -51,6 +54,8 @@ template <int D> struct __align__(128) KrSmem {
     uint64_t full[KR_WARPS][kr_stages<D>()];
     KrSegment get[KR_WARPS];   // where each warp's fetching is
     KrSegment begin[KR_WARPS];
+    KrSegment cut[KR_WARPS][2];       // items of which a warp has a part: one that began before its share, one that goes on
+    const KrPart<D> * part[KR_WARPS][2];
     int scan[KR_WARPS];
     int abort;
 };
@@ -83,18 +88,19 @@ struct KrSum {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     // of a part with maximum mi where all parts' is t (a row that is no number has no maximum)
     static __device__ __forceinline__ float factor(float mi, float li, float t) { return mi == -INFINITY ? (li == li ? 0.f : 1.f) : ex2(mi - t); }
-    template <typename At>
+    // ONCE parts on their way together; far: of other CTAs, from L2
+    template <int ONCE, bool FAR, typename At>
     __device__ __forceinline__ void add(int n, int r, int d4, At && at) {
-        constexpr int ONCE = 8;                          // on their way from L2 together
         for (int i0 = 0; i0 < n; i0 += ONCE) {
             float mi[ONCE], li[ONCE], t = top;
             float4 y[ONCE];
 #pragma unroll
             for (int k = 0; k < ONCE; k++) {
                 const auto * p = at(min(i0 + k, n - 1));
-                mi[k] = __ldcg(&p->m[r]);
-                li[k] = __ldcg(&p->l[r]);
-                y[k] = __ldcg(reinterpret_cast<const float4 *>(&p->o[r][d4]));
+                const float4 * o = reinterpret_cast<const float4 *>(&p->o[r][d4]);
+                mi[k] = FAR ? __ldcg(&p->m[r]) : p->m[r];
+                li[k] = FAR ? __ldcg(&p->l[r]) : p->l[r];
+                y[k] = FAR ? __ldcg(o) : *o;
             }
 #pragma unroll
             for (int k = 0; k < ONCE; k++) t = fmaxf(t, mi[k]);
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
     }
     if (total == 0) return;
     // warps at work in a CTA: few pages go to one warp of each of an SM's four schedulers, on as many SMs as that takes
-    const int at_work = total >= (int) gridDim.x * KR_WARPS ? KR_WARPS : max(4, (total + (int) gridDim.x - 1) / (int) gridDim.x);
+    const int at_work = total >= (int) gridDim.x * KR_WARPS ? KR_WARPS : max(KR_LEAST, (total + (int) gridDim.x - 1) / (int) gridDim.x);
     const int share = (int) (((unsigned) total + gridDim.x * at_work - 1) / (gridDim.x * at_work));
     const int me = blockIdx.x * at_work + warp;
     // the sequences in which the warps' shares begin
@@ -256,22 +262,28 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
     if (more && lane == 0) S.get[warp] = put;
     __syncwarp();
     uint32_t none = 0;                                  // stages whose page is none: nothing is on its way
+    int ids = -1, ids0 = 0, ids1 = 0, f_hk = 0;         // page numbers of the units ids0 .. ids1 - 1 of a segment, one to a lane; its kv head
     auto fetch = [&](int u) {                           // by ascending u
         if (u >= u1) return;
-        if (u >= S.get[warp].u) {
+        if (u >= ids1) {
             KrSegment p = S.get[warp];
-            next(p);
-            __syncwarp();
-            if (lane == 0) S.get[warp] = p;
-            __syncwarp();
+            if (u >= p.u) {
+                next(p);
+                __syncwarp();
+                if (lane == 0) S.get[warp] = p;
+                __syncwarp();
+            }
+            ids0 = u;
+            ids1 = min(u + 32, p.u);
+            f_hk = p.hk;
+            ids = u + lane < ids1 ? kv4_page(A, p.q, p.s, p.pa + u + lane - p.k0) : -1;
         }
-        const KrSegment & p = S.get[warp];
-        const int id = kv4_page(A, p.q, p.s, p.pa + u - p.k0), st = (u - u0) % STAGES;
+        const int id = __shfl_sync(0xffffffffu, ids, u - ids0), st = (u - u0) % STAGES;
         none = id >= 0 ? none & ~(1u << st) : none | 1u << st;
         if (elect_one()) {
             if (id >= 0) {
                 mbar_arrive_expect_tx(&S.full[warp][st], CHUNK);
-                bulk_g2s(S.ring[warp][st], kv4_chunk<D>(A.cache, id, p.hk), CHUNK, &S.full[warp][st], policy);
+                bulk_g2s(S.ring[warp][st], kv4_chunk<D>(A.cache, id, f_hk), CHUNK, &S.full[warp][st], policy);
             } else mbar_arrive(&S.full[warp][st]);
         }
         __syncwarp();
@@ -280,8 +292,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
 
     // ---- segments ----
     KrParts<D> & parts = *reinterpret_cast<KrParts<D> *>(W.parts);
-    KrSegment cut[2];                                   // items of which this warp has a part: one that began before, one that goes on
-    cut[0].q.n_q = cut[1].q.n_q = 0;
+    if (lane < 2) S.cut[warp][lane].q.n_q = 0;
+    __syncwarp();
     while (more) {
         const KrSegment at = put;
         const Kv4Seq & q = at.q;
@@ -557,9 +569,13 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                 }
             }
         } else {
+            // a part: where the share ends, through the warp's ring, which is empty then
             const int which = at.pa > 0 ? 0 : 1;
-            if (which) cut[1] = at; else cut[0] = at;
-            KrPart<D> & to = parts.warp[me][which];
+            KrPart<D> & to = more ? parts.warp[me][which] : *reinterpret_cast<KrPart<D> *>(S.ring[warp][0]);
+            if (lane == 0) {
+                S.cut[warp][which] = at;
+                S.part[warp][which] = &to;
+            }
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const int r = 2 * c + k;
@@ -572,45 +588,41 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
 
     // ---- items that were cut ----
     __syncthreads();                                    // the CTA's parts are there
+    // of each, slices of 32 x 4 numbers, which go to the CTA's warps in turns; where the item reaches beyond the CTA, the last of the CTAs to come adds theirs
+    constexpr int SLICES = KR_ROWS * D / 128;
+    const int first = blockIdx.x * at_work;
+    int turn = 0;
 #pragma unroll 1
-    for (int i = 0; i < 2; i++) {
-        const KrSegment & at = cut[i];
+    for (int k = 0; k < 2 * at_work; k++) {
+        const KrSegment & at = S.cut[k >> 1][k & 1];
         if (at.q.n_q == 0) continue;
         const int a0 = at.before + (at.tile * hks + at.hk) * at.q.pages;             // the item's first unit
         const int w0 = a0 / share, w1 = (a0 + at.q.pages - 1) / share;               // the warps that share it
-        const int f0 = max(w0, (int) blockIdx.x * at_work), f1 = min(w1, (int) blockIdx.x * at_work + at_work - 1);   // of this CTA
-        const bool here = f0 == w0 && f1 == w1;
-        const int rows = min(KR_ROWS, at.q.n_rows - at.tile * KR_ROWS);
-        KrPart<D> & mid = parts.cta[blockIdx.x][f0 == w0 ? 1 : 0];
-        // slices of 32 x 4 numbers: a warp of the CTA each, and where the item reaches beyond the CTA, the last of them among the CTAs adds theirs
-        constexpr int SLICES = KR_ROWS * D / 128;
-        const int b0 = me - f0, many = f1 - f0 + 1;
-        for (int b = b0; b < SLICES; b += many) {
+        const int f0 = max(w0, first), f1 = min(w1, first + at_work - 1);            // of this CTA
+        if (f0 != first + (k >> 1)) continue;                                        // (each item once: where its first warp stands)
+        const int c0 = w0 / at_work, c1 = w1 / at_work, rows = min(KR_ROWS, at.q.n_rows - at.tile * KR_ROWS);
+        for (int b = 0; b < SLICES; b++) {
+            if (turn++ % KR_WARPS != warp) continue;
             const int e = b * 32 + lane, r = e / (D / 4), d4 = 4 * (e % (D / 4));
             KrSum sum;
-            sum.add(many, r, d4, [&](int k) { return &parts.warp[f0 + k][f0 + k == w0 ? 1 : 0]; });
-            if (here) {
-                if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
-            } else {
+            sum.add<KR_WARPS, false>(f1 - f0 + 1, r, d4, [&](int i) { return S.part[f0 - first + i][f0 + i == w0 ? 1 : 0]; });
+            if (c0 != c1) {
+                KrPart<D> & mid = parts.cta[blockIdx.x][f0 == w0 ? 1 : 0];
                 *reinterpret_cast<float4 *>(&mid.o[r][d4]) = sum.x;
                 if (d4 == 0) { mid.m[r] = sum.top; mid.l[r] = sum.l; }
+                __syncwarp();
+                int last = 0;
+                if (lane == 0) {
+                    __threadfence();                        // behind the warp's barrier: all its lanes' numbers
+                    int * counter = &W.counters[w0 * SLICES + b];
+                    last = atomicAdd(counter, 1) == c1 - c0;
+                    if (last) *counter = 0;
+                    __threadfence();
+                }
+                if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+                sum = KrSum();
+                sum.add<16, true>(c1 - c0 + 1, r, d4, [&](int i) { return &parts.cta[c0 + i][i == 0 ? 1 : 0]; });
             }
-        }
-        if (here || b0 >= SLICES) continue;
-        __syncwarp();
-        const int c0 = w0 / at_work, c1 = w1 / at_work;
-        bool last = false;
-        if (lane < SLICES && lane % many == b0) {
-            __threadfence();                            // behind the warp's barrier: all its lanes' numbers
-            int * counter = &W.counters[w0 * SLICES + lane];
-            last = atomicAdd(counter, 1) == c1 - c0;
-            if (last) *counter = 0;
-            __threadfence();
-        }
-        for (uint32_t left = __ballot_sync(0xffffffffu, last); left; left &= left - 1) {
-            const int e = (__ffs((int) left) - 1) * 32 + lane, r = e / (D / 4), d4 = 4 * (e % (D / 4));
-            KrSum sum;
-            sum.add(c1 - c0 + 1, r, d4, [&](int k) { return &parts.cta[c0 + k][k == 0 ? 1 : 0]; });
             if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
         }
     }
@@ -630,6 +642,7 @@ int rows_launch(const Kv4Attn & a, const KrWork & w, cudaStream_t st) {
 }  // namespace
 
 size_t kv4_rows_workspace(int D) { return D == 128 ? sizeof(KrParts<128>) : sizeof(KrParts<64>); }
+static_assert(sizeof(KrPart<128>) <= kv4_chunk_bytes(128) && sizeof(KrPart<64>) <= kv4_chunk_bytes(64), "a part goes through a stage");
 static_assert(KV4_COUNTERS >= KV4_MAX_CTAS * KR_WARPS * KR_ROWS, "a counter for each slice of a warp's item");
 
 int launch_kv4_attn_rows(const Kv4Attn & a, int D, int type, int most_rows, int * counters, void * parts, cudaStream_t st) {
