@@ -9,7 +9,7 @@
 namespace pb {
 namespace {
 
-constexpr int KA_THREADS = 256;
+constexpr int KA_THREADS = 256, KA_WARPS = KA_THREADS / 32;
 
 template <typename T>
 struct AppendParams {
@@ -21,103 +21,145 @@ struct AppendParams {
     const float * q_norm; const float * k_norm;
     float eps;
 };
+__device__ __forceinline__ void raw4(const float * p, uint32_t (&w)[4]) { *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(p); }
+template <typename T> __device__ __forceinline__ void raw4(const T * p, uint32_t (&w)[2]) { *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p); }
 
-// A CTA takes a token and a part of its rows (heads of q, k, v), a quarter of a head's numbers at a time to a thread: D / 4 lanes hold a row, four neighbouring
-// numbers each.  What decides which of 16 steps a number falls to is computed so that it does not depend on an order: the mean of squares and the angles in
-// 64 bits, rounded once, products and sums of the rotation in 32 bits without contraction.
-template <typename T, int D>
-__global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant__ AppendParams<T> P, const __grid_constant__ Kv4Rope R) {
-    constexpr int LPR = D / 4, NB = D / 32;       // lanes to a row
-    __shared__ float2 cs[D / 2];
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    const int pairs = R.n_dims / 2;
-    if (threadIdx.x < pairs) {
-        const double a = (double) P.pos[t] * R.w[threadIdx.x] / (R.freq_factors ? (double) R.freq_factors[threadIdx.x] : 1.0);
+// A CTA takes TOKENS tokens and a part of their heads, a warp R heads of q, of k or of v at a time (R rows on their way together): D / 4 lanes hold a row, four neighbouring numbers
+// each.  What decides which of 16 steps a number falls to is computed so that it does not depend on an order: the mean of squares and the angles in 64 bits, rounded
+// once, products and sums of the rotation in 32 bits without contraction.
+template <typename T, int D, int TOKENS, int R>
+__global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant__ AppendParams<T> P, const __grid_constant__ Kv4Rope RP) {
+    constexpr int LPR = D / 4, RPW = 32 / LPR, HEADS = R * RPW;      // lanes to a row, rows to a warp's instruction, heads to an item
+    __shared__ float2 cs[TOKENS][D / 2];
+    const int t0 = blockIdx.x * TOKENS, tokens = min(TOKENS, P.n_tokens - t0), lane = threadIdx.x & 31;
+    const int pairs = RP.n_dims / 2, hk = P.cache.n_head_kv;
+    const int sub = lane / LPR, l = lane % LPR, d = 4 * l, b = d / 32;
+    const int of_q = (P.n_head + HEADS - 1) / HEADS, of_kv = (hk + HEADS - 1) / HEADS, of_token = of_q + 2 * of_kv, items = tokens * of_token;
+    const int step = KA_WARPS * gridDim.y;
+    uint32_t raw[R][sizeof(T) == 4 ? 4 : 2];
+    int t = 0, kind = 0, head0 = 0, heads = 0;                       // of the item at hand: token, 0 q 1 k 2 v, its first head, heads there are
+    auto ask = [&](int item) {
+        t = item / of_token;
+        const int i = item - t * of_token;
+        kind = i < of_q ? 0 : i < of_q + of_kv ? 1 : 2;
+        head0 = (kind == 0 ? i : kind == 1 ? i - of_q : i - of_q - of_kv) * HEADS;
+        heads = kind == 0 ? P.n_head : hk;
+        const int64_t row = t0 + t;
+        const T * src = (kind == 0 ? P.q + row * P.ldq : kind == 1 ? P.k + row * P.ldk : P.v + row * P.ldv) + d;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int head = head0 + r * RPW + sub;
+            if (head < heads) raw4(src + (int64_t) head * D, raw[r]);
+            else
+                for (uint32_t & w : raw[r]) w = 0u;
+        }
+    };
+    int item = blockIdx.y * KA_WARPS + (threadIdx.x >> 5);
+    if (item < items) ask(item);                                     // on its way beside the angles
+    for (int i = threadIdx.x; i < tokens * pairs; i += KA_THREADS) {
+        const int at = i / pairs, pair = i - at * pairs;
+        const double a = (double) P.pos[t0 + at] * RP.w[pair] / (RP.freq_factors ? (double) RP.freq_factors[pair] : 1.0);
         double s, c;
         sincos(a, &s, &c);
-        cs[threadIdx.x] = make_float2(__fmul_rn((float) c, R.mscale), __fmul_rn((float) s, R.mscale));
+        cs[at][pair] = make_float2(__fmul_rn((float) c, RP.mscale), __fmul_rn((float) s, RP.mscale));
     }
     __syncthreads();
-    const int64_t cell = P.cells[t];
-    const bool stored = cell >= 0 && cell < P.cache.n_pages * KV4_CELLS;
-    const int hk = P.cache.n_head_kv, rows = P.n_head + 2 * hk;
-    const int sub = lane / LPR, l = lane % LPR, d = 4 * l;
-    const int per = 32 / LPR * (KA_THREADS / 32);
-    for (int r0 = blockIdx.y * per; r0 < rows; r0 += gridDim.y * per) {
-        const int row = r0 + (threadIdx.x >> 5) * (32 / LPR) + sub;
-        const bool mine = row < rows;
-        const int kind = !mine ? 3 : row < P.n_head ? 0 : row < P.n_head + hk ? 1 : 2;
-        const int head = kind == 0 ? row : kind == 1 ? row - P.n_head : row - P.n_head - hk;
-        const T * src = kind == 0 ? P.q + t * P.ldq : kind == 1 ? P.k + t * P.ldk : P.v + t * P.ldv;
-        float4 x4 = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (mine) x4 = load4(src + (int64_t) head * D + d);
-        float x[4] = {x4.x, x4.y, x4.z, x4.w};
-        const float * w = kind == 0 ? P.q_norm : kind == 1 ? P.k_norm : nullptr;
-        if (P.q_norm || P.k_norm) {
-            double sum = 0.0;
+    for (; item < items; item += step) {
+        float x[R][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) sum += (double) x[i] * (double) x[i];
+        for (int r = 0; r < R; r++) {
+            const float4 v = load4(reinterpret_cast<const T *>(raw[r]));
+            x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
+        }
+        const int at = t, is = kind, first = head0, n = heads;
+        if (item + step < items) ask(item + step);
+        const float * w = is == 0 ? P.q_norm : is == 1 ? P.k_norm : nullptr;
+        if (w) {
+            const float4 w4 = load4(w + d);
 #pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (w) {
-                const float r = (float) (1.0 / sqrt(sum / D + (double) P.eps));
-                const float4 w4 = load4(w + d);
-                x[0] = __fmul_rn(__fmul_rn(x[0], r), w4.x);
-                x[1] = __fmul_rn(__fmul_rn(x[1], r), w4.y);
-                x[2] = __fmul_rn(__fmul_rn(x[2], r), w4.z);
-                x[3] = __fmul_rn(__fmul_rn(x[3], r), w4.w);
+            for (int r = 0; r < R; r++) {
+                double sum = 0.0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum += (double) x[r][i] * (double) x[r][i];
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float f = (float) (1.0 / sqrt(sum / D + (double) P.eps));
+                x[r][0] = __fmul_rn(__fmul_rn(x[r][0], f), w4.x);
+                x[r][1] = __fmul_rn(__fmul_rn(x[r][1], f), w4.y);
+                x[r][2] = __fmul_rn(__fmul_rn(x[r][2], f), w4.z);
+                x[r][3] = __fmul_rn(__fmul_rn(x[r][3], f), w4.w);
             }
         }
-        if (pairs > 0) {
-            const int half = pairs / 4;            // lanes between the two of a pair (mode 2)
-            float y[4];
+        if (is < 2 && pairs > 0) {
+            const bool turns = d < 2 * pairs;
+            if (RP.mode == 0) {                                      // neighbours: both in this lane
+                const float2 a0 = turns ? cs[at][d / 2] : make_float2(1.f, 0.f), a1 = turns ? cs[at][d / 2 + 1] : make_float2(1.f, 0.f);
+                if (turns) {
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const float y0 = x[r][0], y1 = x[r][1], y2 = x[r][2], y3 = x[r][3];
+                        x[r][0] = __fsub_rn(__fmul_rn(y0, a0.x), __fmul_rn(y1, a0.y));
+                        x[r][1] = __fadd_rn(__fmul_rn(y0, a0.y), __fmul_rn(y1, a0.x));
+                        x[r][2] = __fsub_rn(__fmul_rn(y2, a1.x), __fmul_rn(y3, a1.y));
+                        x[r][3] = __fadd_rn(__fmul_rn(y2, a1.y), __fmul_rn(y3, a1.x));
+                    }
+                }
+            } else {                                                 // halves: the other one pairs / 4 lanes away
+                const bool lower = d < pairs;
+                const int other = lower ? lane + pairs / 4 : lane - pairs / 4;
+                float2 a[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) a[i] = turns ? cs[at][lower ? d + i : d + i - pairs] : make_float2(1.f, 0.f);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float y = __shfl_sync(0xffffffffu, x[r][i], other);
+                        if (turns) x[r][i] = lower ? __fsub_rn(__fmul_rn(x[r][i], a[i].x), __fmul_rn(y, a[i].y)) : __fadd_rn(__fmul_rn(y, a[i].y), __fmul_rn(x[r][i], a[i].x));
+                    }
+            }
+        }
+        if (is == 0) {
+            T * to = P.q_out + (t0 + at) * P.ldqo + d;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const int head = first + r * RPW + sub;
+                if (head < n) store4(to + (int64_t) head * D, make_float4(x[r][0], x[r][1], x[r][2], x[r][3]));
+            }
+            continue;
+        }
+        const int64_t cell = P.cells[t0 + at];
+        if (cell < 0 || cell >= P.cache.n_pages * KV4_CELLS) continue;
+        const int c = (int) (cell % KV4_CELLS);
+        uint8_t * page = kv4_chunk<D>(P.cache, cell / KV4_CELLS, 0);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            // the block's number of largest magnitude (of several, the first), scale, bits
+            float most = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float o = __shfl_sync(0xffffffffu, x[i], R.mode == 0 ? lane ^ 0 : d < pairs ? lane + half : lane - half);
-                y[i] = R.mode == 0 ? x[i ^ 1] : o;
+                x[r][i] = kv4_finite(x[r][i]);
+                if (i == 0 || fabsf(x[r][i]) > fabsf(most)) most = x[r][i];
             }
-            if (kind < 2 && d < 2 * pairs) {
+            float top = fabsf(most);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const bool first = R.mode == 0 ? (i & 1) == 0 : d < pairs;
-                    const float2 a = cs[R.mode == 0 ? (d + i) / 2 : first ? d + i : d + i - pairs];
-                    x[i] = first ? __fsub_rn(__fmul_rn(x[i], a.x), __fmul_rn(y[i], a.y)) : __fadd_rn(__fmul_rn(y[i], a.y), __fmul_rn(x[i], a.x));
-                }
-            }
+            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const uint32_t who = __ballot_sync(0xffffffffu, fabsf(most) == top) & (0xffu << (lane & 24));
+            const float scale = kv4_scale_of(__shfl_sync(0xffffffffu, most, __ffs((int) who) - 1));
+            uint32_t m[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) m[i] = kv4_bits_of(x[r][i], scale);
+            const int head = first + r * RPW + sub;
+            uint8_t * chunk = page + (int64_t) head * kv4_chunk_bytes(D);
+            if (is == 1) {
+                uint32_t word = (m[0] | m[1] << 16 | m[2] << 4 | m[3] << 20) << (8 * (l & 1));
+                word |= __shfl_xor_sync(0xffffffffu, word, 1);
+                if (head < n && (l & 1) == 0) *reinterpret_cast<uint32_t *>(chunk + kv4_k_word(D, c, (d / 8) % 4, b)) = word;
+            } else if (head < n)
+                *reinterpret_cast<uint16_t *>(chunk + kv4_rows_bytes(D) + kv4_v_word(D, c, (d / 4) % 8, b)) = (uint16_t) (m[0] | m[1] << 4 | m[2] << 8 | m[3] << 12);
+            if (head < n && (l & 7) == 0)
+                *reinterpret_cast<__half *>(chunk + 2 * kv4_rows_bytes(D) + (is == 2 ? kv4_scales_bytes(D) : 0) + kv4_scale(D, c, b)) = __float2half_rn(scale);
         }
-        if (kind == 0) store4(P.q_out + t * P.ldqo + (int64_t) head * D + d, make_float4(x[0], x[1], x[2], x[3]));
-        // keys and values: the block's number of largest magnitude (of several, the first), scale, bits
-        float most = 0.f;
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[i] = kv4_finite(x[i]);
-            if (fabsf(x[i]) > fabsf(most) || i == 0) most = x[i];
-        }
-        float top = fabsf(most);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        any = fabsf(most) == top;
-        const uint32_t who = __ballot_sync(0xffffffffu, any) & (0xffu << (lane & 24));
-        const float scale = kv4_scale_of(__shfl_sync(0xffffffffu, most, __ffs((int) who) - 1));
-        uint32_t n[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) n[i] = kv4_bits_of(x[i], scale);
-        const int b = d / 32;
-        uint32_t word = (n[0] | n[1] << 16 | n[2] << 4 | n[3] << 20) << (8 * (l & 1));
-        word |= __shfl_xor_sync(0xffffffffu, word, 1);
-        if ((kind == 1 || kind == 2) && stored) {
-            const int at = (int) (cell % KV4_CELLS);
-            uint8_t * chunk = kv4_chunk<D>(P.cache, cell / KV4_CELLS, head);
-            if (kind == 1) {
-                if ((l & 1) == 0) *reinterpret_cast<uint32_t *>(chunk + kv4_k_word(D, at, (d / 8) % 4, b)) = word;
-            } else {
-                *reinterpret_cast<uint16_t *>(chunk + kv4_rows_bytes(D) + kv4_v_word(D, at, (d / 4) % 8, b)) = (uint16_t) (n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12);
-            }
-            if ((l & 7) == 0)
-                *reinterpret_cast<__half *>(chunk + 2 * kv4_rows_bytes(D) + (kind == 2 ? kv4_scales_bytes(D) : 0) + kv4_scale(D, at, b)) = __float2half_rn(scale);
-        }
-        (void) NB;
     }
 }
 
@@ -147,39 +189,72 @@ __global__ void __launch_bounds__(256) k_kv4_load(const Kv4 cache, const int64_t
     }
 }
 
-constexpr int KC_PAIRS = 256;
+constexpr int KC_PAIRS = 256, KC_ONCE = 4;
 struct CopyPairs { int32_t src[KC_PAIRS], dst[KC_PAIRS]; };
 __global__ void __launch_bounds__(256) k_kv4_copy_pages(uint8_t * pages, int64_t page_bytes, const __grid_constant__ CopyPairs p) {
     const uint4 * s = reinterpret_cast<const uint4 *>(pages + p.src[blockIdx.y] * page_bytes);
     uint4 * d = reinterpret_cast<uint4 *>(pages + p.dst[blockIdx.y] * page_bytes);
     const int64_t n = page_bytes / 16;
-    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) d[i] = s[i];
+    for (int64_t i0 = (int64_t) blockIdx.x * (KC_ONCE * 256) + threadIdx.x; i0 < n; i0 += (int64_t) gridDim.x * (KC_ONCE * 256)) {
+        uint4 v[KC_ONCE];
+#pragma unroll
+        for (int i = 0; i < KC_ONCE; i++)
+            if (i0 + i * 256 < n) v[i] = s[i0 + i * 256];
+#pragma unroll
+        for (int i = 0; i < KC_ONCE; i++)
+            if (i0 + i * 256 < n) d[i0 + i * 256] = v[i];
+    }
 }
 
+// Eight threads to a cell: each an eighth of its key row, one of the eight words of its value row (which lie in another order there and here) and a scale or two.  What the tables
+// say serves KM_CHUNKS chunks (heads and layers), which are on their way together.
+constexpr int KM_CHUNKS = 8;
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_compact(uint8_t * pages, int64_t n_pages, int rows, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to,
+__global__ void __launch_bounds__(256) k_kv4_compact(uint8_t * pages, int64_t n_pages, int chunks, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to,
                                                      const int32_t * index, int64_t ld_index, const int32_t * count) {
-    constexpr int NB = D / 32;
-    const int s = blockIdx.z, row = blockIdx.y;
-    const int i = blockIdx.x * 16 + (threadIdx.x >> 4), l = threadIdx.x & 15;     // 16 threads to a cell
+    constexpr int NB = D / 32, WORDS = D / 64;                           // 32-bit words of an eighth of a row
+    const int s = blockIdx.z, i = blockIdx.x * 32 + (threadIdx.x >> 3), l = threadIdx.x & 7;
     if (i >= count[s]) return;
     const int32_t c = index[s * ld_index + i];
     if (c < 0 || c / KV4_CELLS >= ld_from || i / KV4_CELLS >= ld_to) return;
     const int64_t a = from[s * ld_from + c / KV4_CELLS], b = to[s * ld_to + i / KV4_CELLS];
     if (a < 0 || a >= n_pages || b < 0 || b >= n_pages) return;
-    const int64_t page_bytes = (int64_t) rows * kv4_chunk_bytes(D);
-    const uint8_t * src = pages + a * page_bytes + (int64_t) row * kv4_chunk_bytes(D);
-    uint8_t * dst = pages + b * page_bytes + (int64_t) row * kv4_chunk_bytes(D);
+    const int64_t page_bytes = (int64_t) chunks * kv4_chunk_bytes(D);
+    const uint8_t * src = pages + a * page_bytes;
+    uint8_t * dst = pages + b * page_bytes;
     const int ct = c % KV4_CELLS, it = i % KV4_CELLS;
-    for (int w = l; w < D / 8; w += 16) {
-        *reinterpret_cast<uint32_t *>(dst + kv4_k_word(D, it, 0, w)) = *reinterpret_cast<const uint32_t *>(src + kv4_k_word(D, ct, 0, w));
-        for (int h = 2 * w; h < 2 * w + 2; h++)
-            *reinterpret_cast<uint16_t *>(dst + kv4_rows_bytes(D) + kv4_v_word(D, it, h / NB, h % NB)) =
-                *reinterpret_cast<const uint16_t *>(src + kv4_rows_bytes(D) + kv4_v_word(D, ct, h / NB, h % NB));
-    }
-    if (l < 2 * NB) {
-        const int part = 2 * kv4_rows_bytes(D) + (l / NB) * kv4_scales_bytes(D);
-        *reinterpret_cast<uint16_t *>(dst + part + kv4_scale(D, it, l % NB)) = *reinterpret_cast<const uint16_t *>(src + part + kv4_scale(D, ct, l % NB));
+    const int k_src = kv4_k_word(D, ct, 0, l * WORDS), k_dst = kv4_k_word(D, it, 0, l * WORDS);
+    const int v_src = kv4_rows_bytes(D) + kv4_v_word(D, ct, l, 0), v_dst = kv4_rows_bytes(D) + kv4_v_word(D, it, l, 0);
+    const int part = 2 * kv4_rows_bytes(D) + (l / NB) * kv4_scales_bytes(D), s_src = part + kv4_scale(D, ct, l % NB), s_dst = part + kv4_scale(D, it, l % NB);
+    for (int r0 = blockIdx.y * KM_CHUNKS; r0 < chunks; r0 += gridDim.y * KM_CHUNKS) {
+        uint32_t k[KM_CHUNKS][WORDS], v[KM_CHUNKS][WORDS];
+        uint16_t sc[KM_CHUNKS];
+#pragma unroll
+        for (int r = 0; r < KM_CHUNKS; r++) {
+            if (r0 + r >= chunks) continue;
+            const uint8_t * p = src + (int64_t) (r0 + r) * kv4_chunk_bytes(D);
+            if constexpr (WORDS == 2) {
+                *reinterpret_cast<uint2 *>(k[r]) = *reinterpret_cast<const uint2 *>(p + k_src);
+                *reinterpret_cast<uint2 *>(v[r]) = *reinterpret_cast<const uint2 *>(p + v_src);
+            } else {
+                k[r][0] = *reinterpret_cast<const uint32_t *>(p + k_src);
+                v[r][0] = *reinterpret_cast<const uint32_t *>(p + v_src);
+            }
+            if (l < 2 * NB) sc[r] = *reinterpret_cast<const uint16_t *>(p + s_src);
+        }
+#pragma unroll
+        for (int r = 0; r < KM_CHUNKS; r++) {
+            if (r0 + r >= chunks) continue;
+            uint8_t * p = dst + (int64_t) (r0 + r) * kv4_chunk_bytes(D);
+            if constexpr (WORDS == 2) {
+                *reinterpret_cast<uint2 *>(p + k_dst) = make_uint2(k[r][0], k[r][1]);
+                *reinterpret_cast<uint2 *>(p + v_dst) = make_uint2(v[r][0], v[r][1]);
+            } else {
+                *reinterpret_cast<uint32_t *>(p + k_dst) = k[r][0];
+                *reinterpret_cast<uint32_t *>(p + v_dst) = v[r][0];
+            }
+            if (l < 2 * NB) *reinterpret_cast<uint16_t *>(p + s_dst) = sc[r];
+        }
     }
 }
 
@@ -187,10 +262,17 @@ template <typename T>
 int append(const Kv4 & cache, int D, const void * q, int64_t ldq, void * q_out, int64_t ldqo, const void * k, int64_t ldk, const void * v, int64_t ldv, int64_t n, int n_head,
            const int64_t * cells, const int32_t * pos, const float * q_norm, const float * k_norm, float eps, const Kv4Rope & rope, cudaStream_t st) {
     const AppendParams<T> p{cache, (const T *) q, (const T *) k, (const T *) v, (T *) q_out, ldq, ldqo, ldk, ldv, n_head, (int) n, cells, pos, q_norm, k_norm, eps};
-    const int per = 32 / (D / 4) * (KA_THREADS / 32), rows = n_head + 2 * cache.n_head_kv;
-    const dim3 grid((unsigned) n, (unsigned) ((rows + per - 1) / per < 1024 ? (rows + per - 1) / per : 1024));
-    if (D == 128) k_kv4_append<T, 128><<<grid, KA_THREADS, 0, st>>>(p, rope);
-    else k_kv4_append<T, 64><<<grid, KA_THREADS, 0, st>>>(p, rope);
+    // Many tokens: four to a CTA, so that angles are made once, and four heads to a warp.  Few: a CTA has a token's heads in part, which makes the angles again for each
+    if (n >= 4 * sm_count()) {
+        const unsigned grid = (unsigned) ((n + 3) / 4);
+        if (D == 128) k_kv4_append<T, 128, 4, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
+        else k_kv4_append<T, 64, 4, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
+    } else {
+        const int64_t items = (n_head + 2 * (int64_t) cache.n_head_kv + 32 / (D / 4) - 1) / (32 / (D / 4)), parts = (items + KA_WARPS - 1) / KA_WARPS, most = (4 * sm_count() + n - 1) / n;
+        const dim3 grid((unsigned) n, (unsigned) (parts < most ? parts : most));
+        if (D == 128) k_kv4_append<T, 128, 1, 1><<<grid, KA_THREADS, 0, st>>>(p, rope);
+        else k_kv4_append<T, 64, 1, 1><<<grid, KA_THREADS, 0, st>>>(p, rope);
+    }
     return (int) cudaGetLastError();
 }
 template <typename T>
@@ -220,8 +302,8 @@ int launch_kv4_copy_pages(uint8_t * pages, int64_t page_bytes, const int32_t * s
         CopyPairs p{};
         const int m = n - at < KC_PAIRS ? n - at : KC_PAIRS;
         for (int i = 0; i < m; i++) { p.src[i] = src[at + i]; p.dst[i] = dst[at + i]; }
-        const int64_t want = (page_bytes / 16 + 255) / 256;
-        k_kv4_copy_pages<<<dim3((unsigned) (want < 64 ? want : 64), (unsigned) m), 256, 0, st>>>(pages, page_bytes, p);
+        const int64_t want = (page_bytes / 16 + KC_ONCE * 256 - 1) / (KC_ONCE * 256), most = (16 * sm_count() + m - 1) / m;
+        k_kv4_copy_pages<<<dim3((unsigned) (want < most ? want : most), (unsigned) m), 256, 0, st>>>(pages, page_bytes, p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return (int) e;
     }
@@ -230,7 +312,7 @@ int launch_kv4_copy_pages(uint8_t * pages, int64_t page_bytes, const int32_t * s
 
 int launch_kv4_compact(uint8_t * pages, int64_t n_pages, int rows, int D, int n_seq, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to, const int32_t * index,
                        int64_t ld_index, const int32_t * count, int most, cudaStream_t st) {
-    const dim3 grid((unsigned) ((most + 15) / 16), (unsigned) rows, (unsigned) n_seq);
+    const dim3 grid((unsigned) ((most + 31) / 32), (unsigned) ((rows + KM_CHUNKS - 1) / KM_CHUNKS), (unsigned) n_seq);
     if (D == 128) k_kv4_compact<128><<<grid, 256, 0, st>>>(pages, n_pages, rows, from, ld_from, to, ld_to, index, ld_index, count);
     else k_kv4_compact<64><<<grid, 256, 0, st>>>(pages, n_pages, rows, from, ld_from, to, ld_to, index, ld_index, count);
     return (int) cudaGetLastError();
