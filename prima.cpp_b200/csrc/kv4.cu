@@ -3,13 +3,15 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/prima_b200.h"
 #include "kv4.cuh"
 
 namespace pb {
 namespace {
 
-constexpr int KA_THREADS = 256, KA_WARPS = KA_THREADS / 32;
+constexpr int KA_THREADS = 256, KA_WARPS = KA_THREADS / 32, KA_CTAS = 4;
 
 template <typename T>
 struct AppendParams {
@@ -24,20 +26,45 @@ struct AppendParams {
 __device__ __forceinline__ void raw4(const float * p, uint32_t (&w)[4]) { *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(p); }
 template <typename T> __device__ __forceinline__ void raw4(const T * p, uint32_t (&w)[2]) { *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p); }
 
-// A CTA takes TOKENS tokens and a part of their heads, a warp R heads of q, of k or of v at a time (R rows on their way together): D / 4 lanes hold a row, four neighbouring numbers
+// the sum of four squares to 47 bits: products and sums of 32 bits with what their roundings left (two conversions to 64 bits where four numbers are eight operations)
+__device__ __forceinline__ double squares(const float (&x)[4]) {
+    float hi = 0.f, lo = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float p = __fmul_rn(x[i], x[i]), s = __fadd_rn(hi, p), t = __fsub_rn(s, hi);
+        lo += __fadd_rn(__fsub_rn(hi, __fsub_rn(s, t)), __fsub_rn(p, t)) + fmaf(x[i], x[i], -p);
+        hi = s;
+    }
+    if (!(hi > 1e-30f && hi < 1e38f)) {   // squares that leave the range of 32 bits
+        double sum = 0.0;
+        for (float v : x) sum += (double) v * (double) v;
+        return sum;
+    }
+    return (double) hi + (double) lo;
+}
+// 1 / sqrt(v) rounded to 32 bits: two steps of Newton's method in 64 bits from the 32-bit function (a square root and a division of 64 bits take five times as long)
+__device__ __forceinline__ float inverse_root(double v) {
+    if (!(v > 1e-30 && v < 1e38)) return (float) (1.0 / sqrt(v));
+    double y = (double) rsqrtf((float) v);
+    y = y * (1.5 - 0.5 * v * y * y);
+    y = y * (1.5 - 0.5 * v * y * y);
+    return (float) y;
+}
+
+// A CTA takes TOKENS tokens at a time and a part of their heads, a warp R heads of q, of k or of v at a time (R rows on their way together): D / 4 lanes hold a row, four neighbouring numbers
 // each.  What decides which of 16 steps a number falls to is computed so that it does not depend on an order: the mean of squares and the angles in 64 bits, rounded
 // once, products and sums of the rotation in 32 bits without contraction.
 template <typename T, int D, int TOKENS, int R>
-__global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant__ AppendParams<T> P, const __grid_constant__ Kv4Rope RP) {
+__global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid_constant__ AppendParams<T> P, const __grid_constant__ Kv4Rope RP) {
     constexpr int LPR = D / 4, RPW = 32 / LPR, HEADS = R * RPW;      // lanes to a row, rows to a warp's instruction, heads to an item
     __shared__ float2 cs[TOKENS][D / 2];
-    const int t0 = blockIdx.x * TOKENS, tokens = min(TOKENS, P.n_tokens - t0), lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
     const int pairs = RP.n_dims / 2, hk = P.cache.n_head_kv;
     const int sub = lane / LPR, l = lane % LPR, d = 4 * l, b = d / 32;
-    const int of_q = (P.n_head + HEADS - 1) / HEADS, of_kv = (hk + HEADS - 1) / HEADS, of_token = of_q + 2 * of_kv, items = tokens * of_token;
+    const int of_q = (P.n_head + HEADS - 1) / HEADS, of_kv = (hk + HEADS - 1) / HEADS, of_token = of_q + 2 * of_kv;
     const int step = KA_WARPS * gridDim.y;
     uint32_t raw[R][sizeof(T) == 4 ? 4 : 2];
-    int t = 0, kind = 0, head0 = 0, heads = 0;                       // of the item at hand: token, 0 q 1 k 2 v, its first head, heads there are
+    int t0 = blockIdx.x * TOKENS, t = 0, kind = 0, head0 = 0, heads = 0;   // of the item at hand: token, 0 q 1 k 2 v, its first head, heads there are
     auto ask = [&](int item) {
         t = item / of_token;
         const int i = item - t * of_token;
@@ -54,8 +81,11 @@ __global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant
                 for (uint32_t & w : raw[r]) w = 0u;
         }
     };
+    for (; t0 < P.n_tokens; t0 += gridDim.x * TOKENS) {
+    const int tokens = min(TOKENS, P.n_tokens - t0), items = tokens * of_token;
     int item = blockIdx.y * KA_WARPS + (threadIdx.x >> 5);
     if (item < items) ask(item);                                     // on its way beside the angles
+    __syncthreads();                                                 // those of the tokens in front have been used
     for (int i = threadIdx.x; i < tokens * pairs; i += KA_THREADS) {
         const int at = i / pairs, pair = i - at * pairs;
         const double a = (double) P.pos[t0 + at] * RP.w[pair] / (RP.freq_factors ? (double) RP.freq_factors[pair] : 1.0);
@@ -76,18 +106,36 @@ __global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant
         const float * w = is == 0 ? P.q_norm : is == 1 ? P.k_norm : nullptr;
         if (w) {
             const float4 w4 = load4(w + d);
+            float f[R];
+            if constexpr (R == 4) {   // four rows at once: each step of the sum halves the rows that a lane adds up for, until a quarter of a row's lanes has one
+                constexpr int H = LPR / 2, Q = LPR / 4;
+                double v[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[r] = squares(x[r]);
+                const bool h = lane & H, q = lane & Q;
+#pragma unroll
+                for (int r = 0; r < 2; r++) v[r] = (h ? v[r + 2] : v[r]) + __shfl_xor_sync(0xffffffffu, h ? v[r] : v[r + 2], H);
+                double sum = (q ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, q ? v[0] : v[1], Q);
+#pragma unroll
+                for (int o = Q / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float mine = inverse_root(sum * (1.0 / D) + (double) P.eps);
+#pragma unroll
+                for (int r = 0; r < 4; r++) f[r] = __shfl_sync(0xffffffffu, mine, sub * LPR + (r >> 1) * H + (r & 1) * Q);
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    double sum = squares(x[r]);
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    f[r] = inverse_root(sum * (1.0 / D) + (double) P.eps);
+                }
+            }
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                double sum = 0.0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) sum += (double) x[r][i] * (double) x[r][i];
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const float f = (float) (1.0 / sqrt(sum / D + (double) P.eps));
-                x[r][0] = __fmul_rn(__fmul_rn(x[r][0], f), w4.x);
-                x[r][1] = __fmul_rn(__fmul_rn(x[r][1], f), w4.y);
-                x[r][2] = __fmul_rn(__fmul_rn(x[r][2], f), w4.z);
-                x[r][3] = __fmul_rn(__fmul_rn(x[r][3], f), w4.w);
+                x[r][0] = __fmul_rn(__fmul_rn(x[r][0], f[r]), w4.x);
+                x[r][1] = __fmul_rn(__fmul_rn(x[r][1], f[r]), w4.y);
+                x[r][2] = __fmul_rn(__fmul_rn(x[r][2], f[r]), w4.z);
+                x[r][3] = __fmul_rn(__fmul_rn(x[r][3], f[r]), w4.w);
             }
         }
         if (is < 2 && pairs > 0) {
@@ -109,13 +157,16 @@ __global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant
                 const int other = lower ? lane + pairs / 4 : lane - pairs / 4;
                 float2 a[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) a[i] = turns ? cs[at][lower ? d + i : d + i - pairs] : make_float2(1.f, 0.f);
+                for (int i = 0; i < 4; i++) {
+                    a[i] = turns ? cs[at][lower ? d + i : d + i - pairs] : make_float2(1.f, 0.f);
+                    if (lower) a[i].y = -a[i].y;
+                }
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float y = __shfl_sync(0xffffffffu, x[r][i], other);
-                        if (turns) x[r][i] = lower ? __fsub_rn(__fmul_rn(x[r][i], a[i].x), __fmul_rn(y, a[i].y)) : __fadd_rn(__fmul_rn(y, a[i].y), __fmul_rn(x[r][i], a[i].x));
+                        if (turns) x[r][i] = __fadd_rn(__fmul_rn(x[r][i], a[i].x), __fmul_rn(y, a[i].y));
                     }
             }
         }
@@ -146,9 +197,10 @@ __global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant
             for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const uint32_t who = __ballot_sync(0xffffffffu, fabsf(most) == top) & (0xffu << (lane & 24));
             const float scale = kv4_scale_of(__shfl_sync(0xffffffffu, most, __ffs((int) who) - 1));
+            const float inv = __frcp_rn(scale);
             uint32_t m[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) m[i] = kv4_bits_of(x[r][i], scale);
+            for (int i = 0; i < 4; i++) m[i] = kv4_bits_of(x[r][i], scale, inv);
             const int head = first + r * RPW + sub;
             uint8_t * chunk = page + (int64_t) head * kv4_chunk_bytes(D);
             if (is == 1) {
@@ -160,6 +212,7 @@ __global__ void __launch_bounds__(KA_THREADS) k_kv4_append(const __grid_constant
             if (head < n && (l & 7) == 0)
                 *reinterpret_cast<__half *>(chunk + 2 * kv4_rows_bytes(D) + (is == 2 ? kv4_scales_bytes(D) : 0) + kv4_scale(D, c, b)) = __float2half_rn(scale);
         }
+    }
     }
 }
 
@@ -264,7 +317,7 @@ int append(const Kv4 & cache, int D, const void * q, int64_t ldq, void * q_out, 
     const AppendParams<T> p{cache, (const T *) q, (const T *) k, (const T *) v, (T *) q_out, ldq, ldqo, ldk, ldv, n_head, (int) n, cells, pos, q_norm, k_norm, eps};
     // Many tokens: four to a CTA, so that angles are made once, and four heads to a warp.  Few: a CTA has a token's heads in part, which makes the angles again for each
     if (n >= 4 * sm_count()) {
-        const unsigned grid = (unsigned) ((n + 3) / 4);
+        const unsigned grid = (unsigned) std::min<int64_t>((n + 3) / 4, KA_CTAS * sm_count());       // as many as are at work together
         if (D == 128) k_kv4_append<T, 128, 4, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
         else k_kv4_append<T, 64, 4, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
     } else {

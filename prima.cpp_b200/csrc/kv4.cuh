@@ -48,8 +48,13 @@ __device__ __forceinline__ uint8_t * kv4_chunk(const Kv4 & c, int64_t page, int 
 
 // A block's scale from its number of largest magnitude: bf16 rounds to the 8 significant bits
 __device__ __forceinline__ float kv4_scale_of(float most) { return __half2float(__float2half_rn(__bfloat162float(__float2bfloat16_rn(most * -0.125f)))); }
-__device__ __forceinline__ uint32_t kv4_bits_of(float x, float scale) {
-    return scale == 0.f ? 8u : (uint32_t) fminf(fmaxf(rintf(__fdiv_rn(x, scale)) + 8.f, 0.f), 15.f);
+// rint(x / scale) + 8, by the reciprocal of the scale: that product is within 2^-22 of the quotient (of up to 8.03), and only next to a half is the quotient itself needed
+__device__ __forceinline__ uint32_t kv4_bits_of(float x, float scale, float inv) {
+    if (scale == 0.f) return 8u;
+    const float y = x * inv;
+    float n = rintf(y);
+    if (fabsf(fabsf(y - n) - 0.5f) < 4e-6f) n = rintf(__fdiv_rn(x, scale));
+    return (uint32_t) fminf(fmaxf(n + 8.f, 0.f), 15.f);
 }
 // the cache holds numbers only: a value that is none would reach rows that do not see its cell (0 * NaN)
 __device__ __forceinline__ float kv4_finite(float x) { return x != x ? 0.f : fminf(fmaxf(x, -KV4_MOST), KV4_MOST); }

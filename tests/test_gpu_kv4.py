@@ -386,6 +386,32 @@ def test_append_shapes(pkg, lib, cuda, tokens, heads, kv_heads):
     check_append(r, "f32", heads, kv_heads, 128, cells, pos, 128, 2, n_pages)
 
 
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [40, 700])
+def test_append_norms_of_any_magnitude(pkg, lib, cuda, type_, tokens):
+    """Squares that leave the range of 32 bits, upwards and downwards."""
+    rng = np.random.default_rng(29)
+    n_pages, heads, kv_heads, dim = -(-tokens // 64), 4, 2, 128
+    x = rng.standard_normal((tokens, heads + 2 * kv_heads, dim)) * (10.0 ** np.linspace(-30, 30, tokens))[:, None, None]
+    x_d = torch.from_numpy(x).to(TORCH[type_]).cuda().reshape(tokens, -1)
+    x = x_d.double().cpu().numpy().reshape(tokens, heads + 2 * kv_heads, dim)
+    pages = torch.zeros(n_pages, kv_heads, R.chunk_bytes(dim), dtype=torch.uint8, device="cuda")
+    cache, width, size = pkg.Kv4Cache(pages.data_ptr(), n_pages, 1, kv_heads, dim), x_d.shape[1], x_d.element_size()
+    w = torch.ones(dim, device="cuda")
+    cells, q = torch.arange(tokens, device="cuda"), torch.zeros(tokens, heads * dim, dtype=TORCH[type_], device="cuda")
+    at = [C.c_void_p(x_d.data_ptr() + i * dim * size) for i in (0, heads, heads + kv_heads)]
+    lib.check(lib.c.pb200_kv4_append(C.byref(cache), 0, R.CODE[type_], at[0], width, ptr(q), heads * dim, at[1], width, at[2], width, tokens, heads, ptr(cells), None, ptr(w), ptr(w), 1e-12,
+                                     None, None))
+    torch.cuda.synchronize()
+    zero = np.zeros(tokens, np.int64)
+    want_q, want_k = (R.append(y, np.ones(dim), 1e-12, zero, None, 0, 0) for y in (x[:, :heads], x[:, heads:heads + kv_heads]))
+    assert np.all(np.abs(q.double().cpu().numpy().reshape(want_q.shape) - want_q) <= (4 * 2.0 ** -24 + R.HALF_STEP[type_] * 1.01) * np.abs(want_q) + 1e-38)
+    k = R.unpack(pages.cpu().numpy(), dim)[0].transpose(0, 2, 1, 3).reshape(-1, kv_heads, dim)[:tokens]
+    # tiny rows: a scale below f16's normal range is off by 2^-25 at most, and a number eight times as much
+    step = np.abs(np.repeat(R.quantize(want_k)[1], 32, -1))
+    assert np.all(np.abs(k - want_k) <= step * (1.0 + 2.0 ** -4) + 2.0 ** -22)
+
+
 def test_append_in_place_and_in_a_layer(pkg, lib, cuda):
     rng = np.random.default_rng(23)
     cells, pos = np.arange(20) * 3, np.arange(20)
