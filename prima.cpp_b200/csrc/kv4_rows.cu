@@ -288,8 +288,6 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
         }
         __syncwarp();
     };
-    for (int k = 0; k < STAGES; k++) fetch(u0 + k);
-
     // ---- segments ----
     KrParts<D> & parts = *reinterpret_cast<KrParts<D> *>(W.parts);
     if (lane < 2) S.cut[warp][lane].q.n_q = 0;
@@ -360,10 +358,12 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                 for (int b = 0; b < NB; b++) start[b][i] = F32 ? 0.f : __shfl_sync(0xffffffffu, sums[b], from);
             }
         }
+        if (at.k0 == u0)                                // the first pages, behind the queries: these would wait for all that is on its way to this SM
+            for (int k = 0; k < STAGES; k++) fetch(u0 + k);
         const int p_lo = q.p0 + row0 / A.group, p_hi = q.p0 + (row0 + rows - 1) / A.group;   // of the tile's rows
 
         // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1 (16 bits: times 2^-24, and 2^-20 the odd ones)
-        float o[NB][2][4];
+        float o[NB][2][4], less[4] = {0.f, 0.f, 0.f, 0.f};     // less: 16 bits: row b: - 8 * 2^-24 times the sum of block b's scaled weights
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
         int up = F32 ? KR_UP : 15;                      // weights are exp(score - maximum) * 2^up
 #pragma unroll
@@ -474,6 +474,9 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                             o[b][h][0] *= f[0]; o[b][h][1] *= f[1];
                             o[b][h][2] *= f[0]; o[b][h][3] *= f[1];
                         }
+                        if (!F32 && b == 0) {
+                            less[0] *= f[0]; less[1] *= f[1];
+                        }
                     }
                 }
                 const float off[2] = {m[0] == -INFINITY ? 0.f : (float) up - m[0], m[1] == -INFINITY ? 0.f : (float) up - m[1]};
@@ -533,8 +536,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                             const uint32_t s0 = u[0] >> 8, s1 = u[1] >> 8;
                             mma16816(o[b][0], u[0] & 0x000f000fu, u[0] & 0x00f000f0u, u[1] & 0x000f000fu, u[1] & 0x00f000f0u, p0, p1);
                             mma16816(o[b][1], s0 & 0x000f000fu, s0 & 0x00f000f0u, s1 & 0x000f000fu, s1 & 0x00f000f0u, p0, p1);
-#pragma unroll
-                            for (int h = 0; h < 2; h++) mma16816(o[b][h], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, p0, p1);   // - 8
+                            const uint32_t eights = g == b ? 0x80088008u : 0u;
+                            mma16816(less, eights, 0u, eights, 0u, p0, p1);
                         }
                     }
                 }
@@ -554,9 +557,14 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int k = 0; k < 2; k++) {
+                    const float n8 = __shfl_sync(0xffffffffu, less[k], 4 * b + c);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) o[b][h][i] *= i < 2 ? 16777216.f : 1048576.f;
+                    for (int h = 0; h < 2; h++) {
+                        o[b][h][k] = (o[b][h][k] + n8) * 16777216.f;
+                        o[b][h][2 + k] = fmaf(n8, 16.f, o[b][h][2 + k]) * 1048576.f;
+                    }
+                }
         if (at.pa == 0 && at.pb == q.pages) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -590,41 +598,67 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
     __syncthreads();                                    // the CTA's parts are there
     // of each, slices of 32 x 4 numbers, which go to the CTA's warps in turns; where the item reaches beyond the CTA, the last of the CTAs to come adds theirs
     constexpr int SLICES = KR_ROWS * D / 128;
+    static_assert(SLICES <= KR_WARPS && 2 * KR_WARPS <= 32, "a warp has a slice of an item at most, a lane of it an item");
     const int first = blockIdx.x * at_work;
-    int turn = 0;
-#pragma unroll 1
-    for (int k = 0; k < 2 * at_work; k++) {
-        const KrSegment & at = S.cut[k >> 1][k & 1];
-        if (at.q.n_q == 0) continue;
+    int w0 = 0, w1 = 0, f1 = 0;                          // lane: the warps that share item `lane`, the last of them in this CTA
+    bool here = false;                                   // (each item once: where its first warp in this CTA stands)
+    if (lane < 2 * at_work && S.cut[lane >> 1][lane & 1].q.n_q > 0) {
+        const KrSegment & at = S.cut[lane >> 1][lane & 1];
         const int a0 = at.before + (at.tile * hks + at.hk) * at.q.pages;             // the item's first unit
-        const int w0 = a0 / share, w1 = (a0 + at.q.pages - 1) / share;               // the warps that share it
-        const int f0 = max(w0, first), f1 = min(w1, first + at_work - 1);            // of this CTA
-        if (f0 != first + (k >> 1)) continue;                                        // (each item once: where its first warp stands)
-        const int c0 = w0 / at_work, c1 = w1 / at_work, rows = min(KR_ROWS, at.q.n_rows - at.tile * KR_ROWS);
-        for (int b = 0; b < SLICES; b++) {
-            if (turn++ % KR_WARPS != warp) continue;
-            const int e = b * 32 + lane, r = e / (D / 4), d4 = 4 * (e % (D / 4));
+        w0 = a0 / share;
+        w1 = (a0 + at.q.pages - 1) / share;
+        f1 = min(w1, first + at_work - 1);
+        here = max(w0, first) == first + (lane >> 1);
+    }
+    uint32_t tasks = 0;                                  // items of which this warp has a slice that is to be joined with other CTAs'; lane: its counter
+    int counter = 0, others = 0, turn = warp;
+    auto item = [&](int k, auto && f) {                  // f(segment, slice, its warps)
+        const int b = turn % KR_WARPS;
+        if (b >= SLICES) return;
+        const KrSegment & at = S.cut[k >> 1][k & 1];
+        const int v0 = __shfl_sync(0xffffffffu, w0, k), v1 = __shfl_sync(0xffffffffu, w1, k), e = b * 32 + lane;
+        f(at, b, v0, v1, e / (D / 4), 4 * (e % (D / 4)), min(KR_ROWS, at.q.n_rows - at.tile * KR_ROWS));
+    };
+    for (uint32_t left = __ballot_sync(0xffffffffu, here); left; left &= left - 1, turn += KR_WARPS - SLICES) {
+        const int k = __ffs((int) left) - 1, to = __shfl_sync(0xffffffffu, f1, k);
+        item(k, [&](const KrSegment & at, int b, int v0, int v1, int r, int d4, int rows) {
+            const int f0 = max(v0, first);
             KrSum sum;
-            sum.add<KR_WARPS, false>(f1 - f0 + 1, r, d4, [&](int i) { return S.part[f0 - first + i][f0 + i == w0 ? 1 : 0]; });
-            if (c0 != c1) {
-                KrPart<D> & mid = parts.cta[blockIdx.x][f0 == w0 ? 1 : 0];
-                *reinterpret_cast<float4 *>(&mid.o[r][d4]) = sum.x;
-                if (d4 == 0) { mid.m[r] = sum.top; mid.l[r] = sum.l; }
-                __syncwarp();
-                int last = 0;
-                if (lane == 0) {
-                    __threadfence();                        // behind the warp's barrier: all its lanes' numbers
-                    int * counter = &W.counters[w0 * SLICES + b];
-                    last = atomicAdd(counter, 1) == c1 - c0;
-                    if (last) *counter = 0;
-                    __threadfence();
-                }
-                if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-                sum = KrSum();
-                sum.add<16, true>(c1 - c0 + 1, r, d4, [&](int i) { return &parts.cta[c0 + i][i == 0 ? 1 : 0]; });
+            sum.add<KR_WARPS, false>(to - f0 + 1, r, d4, [&](int i) { return S.part[f0 - first + i][f0 + i == v0 ? 1 : 0]; });
+            if (v0 >= first && v1 < first + at_work) {
+                if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
+                return;
             }
+            KrPart<D> & mid = parts.cta[blockIdx.x][f0 == v0 ? 1 : 0];
+            *reinterpret_cast<float4 *>(&mid.o[r][d4]) = sum.x;
+            if (d4 == 0) { mid.m[r] = sum.top; mid.l[r] = sum.l; }
+            tasks |= 1u << k;
+            if (lane == k) {
+                counter = v0 * SLICES + b;
+                others = v1 / at_work - v0 / at_work;
+            }
+        });
+    }
+    if (!tasks) return;
+    __syncwarp();
+    bool last = false;
+    if (tasks >> lane & 1) {
+        __threadfence();                                 // behind the warp's barrier: all its lanes' numbers
+        last = atomicAdd(&W.counters[counter], 1) == others;
+        if (last) W.counters[counter] = 0;
+        __threadfence();
+    }
+    const uint32_t mine_last = __ballot_sync(0xffffffffu, last);
+    turn = warp;
+    for (uint32_t left = __ballot_sync(0xffffffffu, here); left; left &= left - 1, turn += KR_WARPS - SLICES) {
+        const int k = __ffs((int) left) - 1;
+        if (!(mine_last >> k & 1)) continue;
+        item(k, [&](const KrSegment & at, int, int v0, int v1, int r, int d4, int rows) {
+            const int c0 = v0 / at_work, c1 = v1 / at_work;
+            KrSum sum;
+            sum.add<16, true>(c1 - c0 + 1, r, d4, [&](int i) { return &parts.cta[c0 + i][i == 0 ? 1 : 0]; });
             if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
-        }
+        });
     }
 }
 
