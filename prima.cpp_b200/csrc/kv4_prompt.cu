@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 fence_after();
                 if (elect_one()) {
 #pragma unroll
-                    for (int part = 0; part < (F32 ? 2 : 1); part++) {
-                        const uint64_t dq = desc_sw128(smem_u32(S.q[F32 ? part : grp])), dk = desc_sw128(smem_u32(S.k[st]));
+                    for (int part = 0; part < (F32 ? 2 : 1); part++) {   // F32: the low parts first: every product is aligned to the sum so far and cut off (1.4e-6 -> 1.1e-6)
+                        const uint64_t dq = desc_sw128(smem_u32(S.q[F32 ? 1 - part : grp])), dk = desc_sw128(smem_u32(S.k[st]));
 #pragma unroll
                         for (int k = 0; k < D / 16; k++)
                             mma_f16<1>(tmem + 256 * grp, dq + (k >> 2) * (KP_BLOCK >> 4) + 2 * (k & 3), dk + (k >> 2) * (KP_BLOCK >> 4) + 2 * (k & 3), idesc, (uint32_t) ((part | k) != 0));
