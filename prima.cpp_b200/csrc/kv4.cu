@@ -51,6 +51,8 @@ __device__ __forceinline__ float inverse_root(double v) {
     return (float) y;
 }
 
+// Bound: instructions: a row's norm and rotation, and a stored row's scale and steps, about as much again each as reading and writing a row of queries.  us, 2048 tokens of 32 heads over 8
+// of 128, bf16: 28 (and 6 for k_kv4_load; floor 8.4 of both); 64 tokens in F32 3.  With roots and quotients of 64 and 32 bits 42, a head to a warp and angles once for 8 rows 57.
 // A CTA takes TOKENS tokens at a time and a part of their heads, a warp R heads of q, of k or of v at a time (R rows on their way together): D / 4 lanes hold a row, four neighbouring numbers
 // each.  What decides which of 16 steps a number falls to is computed so that it does not depend on an order: the mean of squares and the angles in 64 bits, rounded
 // once, products and sums of the rotation in 32 bits without contraction.
@@ -242,6 +244,7 @@ __global__ void __launch_bounds__(256) k_kv4_load(const Kv4 cache, const int64_t
     }
 }
 
+// Bound: memory.  48 pages of 2.4 MB, three copies of each source: 27 us (151 MB read once and written; floor 23).  One 16-byte piece a thread on its way: 34.
 constexpr int KC_PAIRS = 256, KC_ONCE = 4;
 struct CopyPairs { int32_t src[KC_PAIRS], dst[KC_PAIRS]; };
 __global__ void __launch_bounds__(256) k_kv4_copy_pages(uint8_t * pages, int64_t page_bytes, const __grid_constant__ CopyPairs p) {
@@ -260,7 +263,8 @@ __global__ void __launch_bounds__(256) k_kv4_copy_pages(uint8_t * pages, int64_t
 }
 
 // Eight threads to a cell: each an eighth of its key row, one of the eight words of its value row (which lie in another order there and here) and a scale or two.  What the tables
-// say serves KM_CHUNKS chunks (heads and layers), which are on their way together.
+// say serves KM_CHUNKS chunks (heads and layers), which are on their way together.  Bound: memory, by pieces of 64 bytes: 4000 of 8000 cells, 64 chunks, 20.5 us (floor 11.3); two bytes of
+// values at a time and a chunk to a thread 38.
 constexpr int KM_CHUNKS = 8;
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_compact(uint8_t * pages, int64_t n_pages, int chunks, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to,

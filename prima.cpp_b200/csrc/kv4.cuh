@@ -104,7 +104,11 @@ struct Kv4Attn {
     int max_q, window, first;
     float scale;
 };
-size_t kv4_attn_workspace(int D, int n_head, int n_head_kv);
-int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t st);
+// A sequence with up to so many rows (queries x heads of a group) goes to the kernel of few rows, which walks its pages once for every eight of them; the other one has tiles of 128 and
+// 256 rows whatever there are.  us, 8 sequences of 4096 cells, 32 heads over 8, few rows / prompt: bf16, 20 rows 38.7 / 77.5, 32 48.3 / 78.0, 48 59.8 / 80.7; F32, 32 65.8 / 78.0,
+// 48 85.6 / 80.3.  64 sequences of 1000 cells, bf16: 32 rows 84 / 120, 48 109 / 120.
+constexpr int KV4_FEW_ROWS = 48, KV4_FEW_ROWS_F32 = 32;
+size_t kv4_attn_workspace(int D);
+int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t st, int & launches);   // launches: kernels, added up
 
 }  // namespace pb

@@ -48,7 +48,7 @@ int pb200_kv4_append(const pb200_kv4_cache * c, int layer, int type, const void 
     if (e) return e;
     const int eb = elem_bytes(type);
     const int64_t D = c->head_dim, kd = c->n_head_kv * D;
-    if (!eb || layer < 0 || layer >= c->n_layer || n_tokens < 0 || n_tokens > INT32_MAX || n_head < 0 || !cells) return PB200_EINVAL;
+    if (!eb || layer < 0 || layer >= c->n_layer || n_tokens < 0 || n_tokens > 1 << 30 || n_head < 0 || !cells) return PB200_EINVAL;
     if (!rows_ok(k, ldk, kd, eb) || !rows_ok(v, ldv, kd, eb)) return PB200_EINVAL;
     if (n_head > 0 && (!rows_ok(q, ldq, n_head * D, eb) || !rows_ok(q_out, ldq_out, n_head * D, eb))) return PB200_EINVAL;
     if ((((uintptr_t) q_norm | (uintptr_t) k_norm) & 15) || ((q_norm || k_norm) && !(eps >= 0.f))) return PB200_EINVAL;
@@ -95,7 +95,7 @@ int pb200_kv4_load(const pb200_kv4_cache * c, int layer, int type, const int64_t
 }
 
 size_t pb200_kv4_attn_workspace_bytes(int n_head, int n_head_kv, int head_dim) {
-    return n_head > 0 && n_head_kv > 0 && n_head % n_head_kv == 0 && kv4_dim_ok(head_dim) ? kv4_attn_workspace(head_dim, n_head, n_head_kv) : 0;
+    return n_head > 0 && n_head_kv > 0 && n_head % n_head_kv == 0 && kv4_dim_ok(head_dim) ? kv4_attn_workspace(head_dim) : 0;
 }
 
 int pb200_kv4_attn(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
@@ -110,13 +110,17 @@ int pb200_kv4_attn(const pb200_kv4_cache * c, int layer, int type, const void * 
     if (!rows_ok(q, ldq, n_head * D, eb) || !rows_ok(out, ldo, n_head * D, eb)) return PB200_EINVAL;
     if (!ws || ((uintptr_t) ws & 15) || ws_bytes < pb200_kv4_attn_workspace_bytes(n_head, c->n_head_kv, c->head_dim)) return PB200_EINVAL;
     if (n_seq == 0 || n_tokens == 0 || max_q == 0) return 0;
-    // pages of all sequences, heads and tiles of eight rows are counted in 31 bits
-    const double rows = (double) std::min<int64_t>(max_q, n_tokens) * (n_head / c->n_head_kv);
-    if ((double) n_seq * (double) std::min<int64_t>(table_ld, (INT32_MAX / PB200_KV4_CELLS) + 1) * c->n_head_kv * std::ceil(rows / 8) >= 2147483648.0 || rows >= 2147483648.0) return PB200_ENOTSUP;
+    // what the kernels count in 31 bits: pages of all sequences, heads and tiles of eight rows where rows are few, tiles of all prompts otherwise
+    const double group = n_head / c->n_head_kv, rows = std::min(std::min<double>(max_q, (double) n_tokens) * group, (double) KV4_FEW_ROWS);
+    const double pages = (double) n_seq * (double) std::min<int64_t>(table_ld, INT32_MAX / PB200_KV4_CELLS) * c->n_head_kv * std::ceil(rows / 8);
+    const double tiles = ((double) n_tokens * group / 128 + n_seq) * c->n_head_kv;
+    if (pages >= 2147483648.0 || tiles >= 2147483648.0 || n_tokens * group >= 2147483648.0) return PB200_ENOTSUP;
     if (overlap(q, ((n_tokens - 1) * ldq + n_head * D) * eb, out, ((n_tokens - 1) * ldo + n_head * D) * eb)) return PB200_EINVAL;
     const Kv4Attn a{layer_of(c, layer), q, ldq, out, ldo, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};
-    g_launches++;
-    return launch_kv4_attn(a, c->head_dim, type, ws, (cudaStream_t) stream);
+    int launches = 0;
+    const int rc = launch_kv4_attn(a, c->head_dim, type, ws, (cudaStream_t) stream, launches);
+    g_launches += launches;
+    return rc;
 }
 
 int pb200_kv4_copy_pages(const pb200_kv4_cache * c, const int32_t * src, const int32_t * dst, int n, void * stream) {

@@ -67,6 +67,6 @@ struct KrWork { int most_rows; int * counters; void * parts; int * abort_flag; }
 size_t kv4_rows_workspace(int D);
 int launch_kv4_attn_rows(const Kv4Attn & a, int D, int type, int most_rows, int * counters, void * parts, cudaStream_t st);
 size_t kv4_prompt_workspace(int D);
-int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st);
+int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st, int & launches);
 
 }  // namespace pb

@@ -5,12 +5,19 @@
 // score lies beyond it by more than 2^8, and then its sum and O are scaled.
 //
 // Work.  An item is a (sequence, kv head, tile of query rows: tokens x heads of the group).  Two softmax groups keep the tensor cores busy in turns: with 16 bits each has 128 rows, which
-// share each expanded key tile; with F32 both have the same 128 rows and every other key tile, and their sums are joined at the end.  Key tiles are two pages.  CTAs (one to an SM) take items by tickets, long ones of a sequence first; where there are fewer items than SMs, long items are cut into pieces, which a second
-// kernel adds up in their order.
+// share each expanded key tile; with F32 both have the same 128 rows and every other key tile, and their sums are joined at the end.  Key tiles are two pages.  CTAs (one to an SM) take
+// items by tickets, long ones of a sequence first; where there are fewer items than SMs, long items are cut into pieces, which a second kernel adds up in their order.
 //   warps 0 - 3    expand: a thread has a cell's row of keys, then one of values: raw words in registers a tile ahead, f16 into the swizzle-128B images, two stages each
 //   warps 4 - 11   softmax, groups of four: a thread has a row of S, which is also a lane of tensor memory
 //   warp 12        MMA issuer, owner of the tensor memory, and of the tickets
 // Tensor memory: S / P of either group at 0 and 256, O at 128 and 384.  Weights lie over their scores: 16 columns for 32, F32's low parts in the other 16.
+//
+// Bound: with 16 bits a key tile takes 3700 clocks for 256 rows: MMAs 2100 (S with both operands in shared memory, which also takes the expanded tiles), exponentials 2050 a scheduler, two
+// softmax groups and expansion side by side; an item adds 10000 for queries, first tile, output.  us: 2048 tokens of 32 heads over 8 57 (602 TFLOP/s of visible pairs; over an f16 cache
+// k_attn_prefill_tc takes 58), a plain form of elementary operations 3066; F32, 1077 queries behind up to 5077 cells 92 (with 13 for the sequence of one query), 5200.
+// On the way, us at 2048 tokens: scores 32 at a time, waited for, masks within the passes 124; the next 32 on their way 102; masks in a pass of their own over edge tiles (their code was a
+// third of what was fetched and not run) 64; eight numbers of a query to a lane 57.  A row to a thread for the queries is no faster (its loads are 256 bytes apart).
+// Error against 64 bits with F32: 4e-7 at 128 cells, 1.1e-6 at 5000: MMAs cut off what they add to O, and O is the sum of all tiles.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -641,7 +648,7 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
 }
 
 template <typename T, int D>
-int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st) {
+int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) {
     constexpr size_t smem = sizeof(KpSmem<D>) + 1024;
     static_assert(smem <= 232448, "shared memory of an SM");
     static FuncAttrCache cache;
@@ -650,6 +657,7 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st) {
     const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
     w.cut = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv < ctas;
     if (w.cut && (e = cudaMemsetAsync(w.tickets + KP_FLAGS, 0, KV4_SLOTS * sizeof(int), st)) != cudaSuccess) return (int) e;
+    launches += w.cut ? 2 : 1;
     k_kv4_attn_prompt<T, D><<<ctas, KP_THREADS, smem, st>>>(a, w);
     e = cudaGetLastError();
     if (e != cudaSuccess || !w.cut) return (int) e;
@@ -661,10 +669,10 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st) {
 
 size_t kv4_prompt_workspace(int D) { return D == 128 ? sizeof(KpParts<128>) : sizeof(KpParts<64>); }
 
-int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st) {
+int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st, int & launches) {
     const KpWork w{most_rows, tickets, parts, abort_flag(), 0};
-    if (D == 128) return type == PB200_TYPE_F32 ? prompt_launch<float, 128>(a, w, st) : type == PB200_TYPE_F16 ? prompt_launch<__half, 128>(a, w, st) : prompt_launch<__nv_bfloat16, 128>(a, w, st);
-    return type == PB200_TYPE_F32 ? prompt_launch<float, 64>(a, w, st) : type == PB200_TYPE_F16 ? prompt_launch<__half, 64>(a, w, st) : prompt_launch<__nv_bfloat16, 64>(a, w, st);
+    if (D == 128) return type == PB200_TYPE_F32 ? prompt_launch<float, 128>(a, w, st, launches) : type == PB200_TYPE_F16 ? prompt_launch<__half, 128>(a, w, st, launches) : prompt_launch<__nv_bfloat16, 128>(a, w, st, launches);
+    return type == PB200_TYPE_F32 ? prompt_launch<float, 64>(a, w, st, launches) : type == PB200_TYPE_F16 ? prompt_launch<__half, 64>(a, w, st, launches) : prompt_launch<__nv_bfloat16, 64>(a, w, st, launches);
 }
 
 }  // namespace pb

@@ -15,7 +15,13 @@
 // share by itself, pages on their way through a ring of its own (one bulk copy per page: a head's chunk is contiguous), and writes items that it has whole.  Of one that is cut it leaves
 // its part in the workspace; once a CTA's warps are through, those that share an item add up its parts, and where it reaches beyond the CTA, the last warp of all adds
 // what the CTAs have: always in their order (no atomics on numbers, equal calls give equal bits).  One barrier a CTA: with one per item, warps waited for each other for a
-// page's time at every item (83 us for 32 sequences of up to 8192 cells).
+// page's time at every item (83 us for 32 sequences of up to 8192 cells; this 53).
+//
+// Bound: where there is much to read, half of the time is the memory's and half the start and the joins: of 57 us for two sequences of 131071 and 65001 cells (226 MB, 34.5 at the rate of a
+// copy) 2 are the shares, 4 the wait for queries and first pages, 40 the pages (5300 clocks each for 12 warps of an SM, 19 bytes a clock and SM; with the values left out 5000: the copies
+// set the pace), 6 the joins.  Where there is little, the chain of launch, lengths, page numbers, page, join: 14 us for a token behind 1000 cells.
+// us: 32 sequences of 17 .. 8192 cells, 32 heads over 8, 53 (floor 24); 256 of 1000 .. 3000 132 (91); 16 in windows of 1024, heads of 64, 14.  Products on scaled values, a CTA's warps joining
+// at every item, parts loaded one by one: 107, 79 and 22 for the first, the long two and the windows.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -29,7 +35,7 @@ namespace pb {
 namespace {
 
 constexpr int KR_ROWS = 8;
-// Warps of a CTA, one CTA to an SM: 168 registers (16 warps of 128: 94 us for two sequences of 131071 and 65001 cells, these 65).  Stages of a warp's ring: a page each.
+// Warps of a CTA, one CTA to an SM: 168 registers (16 warps of 128: 94 us where these took 65, 8 warps of 234 the same).  Stages of a warp's ring: a page each.
 constexpr int KR_WARPS = 12, KR_THREADS = 32 * KR_WARPS;
 // Few pages go to as many warps of a CTA at least: one for each of an SM's schedulers.  us, with 4 / 8 / 12: a token of 32 heads over 8 behind 100 cells 11.6 / 15.4 / 19.1, behind
 // 1000 13.6 / 15.2 / 20.1, behind 4000 17.1 / 17.9 / 19.5

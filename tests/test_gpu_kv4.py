@@ -219,9 +219,10 @@ def test_large_and_small_queries(pkg, lib, cuda, type_):
         a.check()
 
 
+@pytest.mark.parametrize("type_", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("q,kv", MIXED, ids=["tokens", "prompts"])
-def test_a_query_that_is_no_number_stays_alone(pkg, lib, cuda, q, kv):
-    a = Attn(pkg, lib, 10, "f32", 8, 2, 128, q, kv)
+def test_a_query_that_is_no_number_stays_alone(pkg, lib, cuda, type_, q, kv):
+    a = Attn(pkg, lib, 10, type_, 8, 2, 128, q, kv)
     a.call()
     torch.cuda.synchronize()
     clean = a.out.clone()
@@ -277,6 +278,19 @@ def test_calls_on_two_streams(pkg, lib, cuda):
     torch.cuda.synchronize()
     a.check()
     b.check()
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("n,prompts", [(385, 0), (1000, 0), (500, 3)])
+def test_more_sequences_than_threads(pkg, lib, cuda, type_, n, prompts):
+    """Single tokens of many short sequences, a few prompts among them."""
+    rng = np.random.default_rng(30)
+    q, kv = [1] * n, list(rng.integers(0, 140, n))
+    for i in range(prompts):
+        q[100 + 150 * i], kv[100 + 150 * i] = 90 + i, 300 * i + 90
+    a = Attn(pkg, lib, 17, type_, 4, 2, 64, q, [int(k) for k in kv])
+    a.call()
+    a.check()
 
 
 def test_shared_pages(pkg, lib, cuda):

@@ -84,6 +84,17 @@ def test_attention_refuses(lib, cache, kw):
     assert lib.c.pb200_kv4_attn(*attn_args(cache, **kw)) == -1
 
 
+def test_counts_beyond_31_bits(lib, pkg):
+    """What the kernels count in 31 bits: refused where it would not fit, and only there (an address that no call gets to use: what is not refused ends in a launch without a GPU)."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("would run on the GPU")
+    many = pkg.Kv4Cache(BASE, 1 << 30, 1, 8, 128)
+    big = dict(ldq=1024, ldo=1024, n_head=8, out=1 << 50, n_tokens=1 << 20, max_q=1)
+    assert lib.c.pb200_kv4_attn(*attn_args(many, n_seq=1 << 16, table_ld=4096, **big)) == -3
+    assert lib.c.pb200_kv4_attn(*attn_args(many, n_seq=64, table_ld=4096, **dict(big, max_q=2048))) not in (0, -1, -3)
+
+
 def test_nothing_to_do_is_no_error(lib, cache):
     for kw in (dict(n_seq=0), dict(n_tokens=0), dict(max_q=0)):
         assert lib.c.pb200_kv4_attn(*attn_args(cache, **kw)) == 0
