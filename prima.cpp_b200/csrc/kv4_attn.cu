@@ -9,9 +9,9 @@
 
 namespace pb {
 
-// counters (rows: one per warp and slice, zero between calls), tickets and a word for each slot, then the parts of either kernel, which run one after the other
+// counters (rows: one per warp and slice), tickets and a word for each slot, all zero between calls; then the parts of either kernel, which may run at the same time
 static size_t counters() { return (KV4_COUNTERS + 64 + KV4_SLOTS) * sizeof(int); }
-size_t kv4_attn_workspace(int D) { return counters() + std::max(kv4_rows_workspace(D), kv4_prompt_workspace(D)); }
+size_t kv4_attn_workspace(int D) { return counters() + kv4_rows_workspace(D) + kv4_prompt_workspace(D); }
 
 int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t st, int & launches) {
     int * words = (int *) ws;
@@ -24,7 +24,7 @@ int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t 
         if (e || most <= few) return e;
     }
     // a single sequence is a prompt, as far as the host can tell: whatever rows it has
-    return launch_kv4_attn_prompt(a, D, type, a.n_seq > 1 ? few : 0, words + KV4_COUNTERS, parts, st, launches);
+    return launch_kv4_attn_prompt(a, D, type, a.n_seq > 1 ? few : 0, words + KV4_COUNTERS, (char *) parts + kv4_rows_workspace(D), st, launches);
 }
 
 }  // namespace pb

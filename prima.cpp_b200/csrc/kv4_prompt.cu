@@ -52,10 +52,10 @@ template <int D> struct KpSmem {
     uint32_t tmem_base;
     int abort, more[2];
 };
-// tickets: two words, and for each slot whether a cut item's parts begin there (cleared in front of the kernel); cut: long items may be
+// tickets: two words, and for each slot how many of the joining kernel's CTAs have yet to come for the item whose parts begin there; all zero between calls.  cut: long items may be
 struct KpWork { int most_rows; int * tickets; void * parts; int * abort_flag; int cut; };
 template <int D> struct KpParts { KpPart<D> part[KV4_SLOTS]; KpPiece first[KV4_SLOTS]; };
-constexpr int KP_FLAGS = 2;
+constexpr int KP_FLAGS = 2, KP_JOIN = 4;   // KP_JOIN: CTAs for a cut item
 
 // the tile's rows [row0, row0 + rows) of a sequence: positions and pages
 __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpPiece & p) {
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         part->l[rows0 + row] = l;
                         if (threadIdx.x == 128 && P.part == 0) {
                             reinterpret_cast<KpParts<D> *>(W.parts)->first[P.slot] = P;
-                            W.tickets[KP_FLAGS + P.slot] = 1;
+                            W.tickets[KP_FLAGS + P.slot] = KP_JOIN;
                         }
                     }
                     // through the queries' memory, so that a warp stores whole rows
@@ -596,6 +596,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
         }
         fence_after();
     }
+    pdl_wait();                                    // the end of this kernel is the end of the one in front
     if (warp == 12) {
         tmem_free(tmem, 512);
         if (lane == 0 && atomicAdd(&W.tickets[1], 1) == (int) gridDim.x - 1) W.tickets[0] = W.tickets[1] = 0;   // the last CTA: every ticket has been drawn
@@ -606,7 +607,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
     constexpr int PER = D / 32, ONCE = 4;
-    if (W.tickets[KP_FLAGS + blockIdx.x] == 0) return;
+    int * const left = &W.tickets[KP_FLAGS + blockIdx.x];
+    if (*(volatile int *) left == 0) return;      // (not 0 until this CTA has taken itself off)
     const KpParts<D> & all = *reinterpret_cast<const KpParts<D> *>(W.parts);
     const KpPiece & p = all.first[blockIdx.x];
     const KpPart<D> * parts = &all.part[blockIdx.x];
@@ -645,6 +647,8 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
             else out[e * 32 + lane] = __float2bfloat16_rn(x[e] * inv);
         }
     }
+    __syncthreads();
+    if (threadIdx.x == 0) atomicSub(left, 1);
 }
 
 template <typename T, int D>
@@ -656,12 +660,18 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     if (e != cudaSuccess) return (int) e;
     const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
     w.cut = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv < ctas;
-    if (w.cut && (e = cudaMemsetAsync(w.tickets + KP_FLAGS, 0, KV4_SLOTS * sizeof(int), st)) != cudaSuccess) return (int) e;
     launches += w.cut ? 2 : 1;
-    k_kv4_attn_prompt<T, D><<<ctas, KP_THREADS, smem, st>>>(a, w);
-    e = cudaGetLastError();
+    // Behind the kernel of few rows (most_rows > 0), CTAs start where that has none at work: it has nothing that they read, and all in front of it has ended when it starts
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(KP_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = w.most_rows > 0 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, k_kv4_attn_prompt<T, D>, a, w);
     if (e != cudaSuccess || !w.cut) return (int) e;
-    k_kv4_join<T, D><<<dim3(KV4_SLOTS, 4), 256, 0, st>>>(a, w);
+    k_kv4_join<T, D><<<dim3(KV4_SLOTS, KP_JOIN), 256, 0, st>>>(a, w);
     return (int) cudaGetLastError();
 }
 

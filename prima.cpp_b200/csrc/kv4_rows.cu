@@ -146,6 +146,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
     volatile int * cta_abort = &S.abort;
     const int hks = A.cache.n_head_kv;
 
+    pdl_trigger();                                      // the prompts' kernel may start where this one has no work
+
     // ---- shares: units (pages of items) in the order of sequences, tiles, heads, pages; a thread has a sequence ----
     Kv4Seq mine = kv4_seq(A, tid, W.most_rows, false);
     int n = mine.units(hks, KR_ROWS), units = n;
