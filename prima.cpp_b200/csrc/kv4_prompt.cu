@@ -22,6 +22,7 @@
 #include <cuda_runtime.h>
 
 #include <cfloat>
+#include <climits>
 #include <type_traits>
 
 #include "../../include/prima_b200.h"
@@ -52,10 +53,10 @@ template <int D> struct KpSmem {
     uint32_t tmem_base;
     int abort, more[2];
 };
-// tickets: two words, and for each slot how many of the joining kernel's CTAs have yet to come for the item whose parts begin there; all zero between calls.  cut: long items may be
+// tickets: words that are zero between calls.  cut: long items may be
 struct KpWork { int most_rows; int * tickets; void * parts; int * abort_flag; int cut; };
-template <int D> struct KpParts { KpPart<D> part[KV4_SLOTS]; KpPiece first[KV4_SLOTS]; };
-constexpr int KP_FLAGS = 2, KP_JOIN = 4;   // KP_JOIN: CTAs for a cut item
+enum { KP_DRAWN, KP_DONE, KP_CUT, KP_JOINED };             // tickets drawn, CTAs that are through; items that were cut, joining CTAs that are through
+template <int D> struct KpParts { KpPart<D> part[KV4_SLOTS]; KpPiece item[KV4_SLOTS]; };   // item: those that were cut, their first pieces
 
 // the tile's rows [row0, row0 + rows) of a sequence: positions and pages
 __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpPiece & p) {
@@ -65,103 +66,150 @@ __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpP
     kv4_pages(A, p.p_lo, p.p_hi, p.q);
     p.tiles = (p.q.pages + 1) / 2;
 }
-// Items, their pieces and slots, in the order of tickets: sequences, tiles from the last on, heads, pieces.  Every CTA and the joining kernel count them in the same way.
-struct KpCount { int pieces, cut; };
-template <int ROWS>
-__device__ __forceinline__ KpCount kp_count(const Kv4Attn & A, const Kv4Seq & q, int limit) {   // of a sequence; limit: pieces are no longer (0: items are whole)
-    if (q.n_q == 0) return {0, 0};
-    const int n = (q.n_rows + ROWS - 1) / ROWS;
-    if (limit == 0) return {n * A.cache.n_head_kv, 0};
-    KpCount c{0, 0};
-    for (int i = 0; i < n; i++) {
-        KpPiece p;
-        p.row0 = i * ROWS;
-        p.rows = min(ROWS, q.n_rows - p.row0);
-        kp_span(A, q, p);
-        const int k = 2 * p.tiles > 3 * limit ? (p.tiles + limit - 1) / limit : 1;
-        c.pieces += k;
-        c.cut += k > 1 ? k : 0;
+// Items, their pieces and slots, in the order of tickets: sequences, tiles from the last on, heads, pieces; every CTA counts them in the same way.  Where long items may be cut there are
+// 32 sequences at most, of which those with the longest items come first.
+constexpr int KP_CUT_SEQ = 32;
+__device__ __forceinline__ int kp_pieces(int tiles, int limit) { return 2 * tiles > 3 * limit ? (tiles + limit - 1) / limit : 1; }
+// by a warp: row tiles of the sequences in that order, of each from the last on, 32 at a time, one to a lane; f(whether there is one, it) returns whether to go on
+template <int ROWS, typename F>
+__device__ __forceinline__ void kp_walk(const Kv4Attn & A, const KpWork & W, F && f) {
+    const int lane = threadIdx.x & 31;
+    const Kv4Seq own = kv4_seq(A, lane, W.most_rows, true);
+    const int len = own.n_q > 0 ? own.p0 + own.n_q : INT_MIN;
+    int rank = 0, from = 0;
+    for (int i = 0; i < 32; i++) {
+        const int other = __shfl_sync(0xffffffffu, len, i);
+        rank += other > len || (other == len && i < lane);
     }
-    c.pieces *= A.cache.n_head_kv;
-    c.cut *= A.cache.n_head_kv;
-    return c;
-}
-template <int ROWS>
-__device__ __forceinline__ int kp_tiles(const Kv4Attn & A, const Kv4Seq & q) {   // key tiles of a sequence's items of one head
-    int sum = 0;
-    for (int r = 0; r < q.n_rows; r += ROWS) {
-        KpPiece p;
-        p.row0 = r;
-        p.rows = min(ROWS, q.n_rows - r);
-        kp_span(A, q, p);
-        sum += p.tiles;
+    for (int i = 0; i < 32; i++)
+        if (__shfl_sync(0xffffffffu, rank, i) == lane) from = i;
+    const int n = __shfl_sync(0xffffffffu, own.n_q > 0 ? (own.n_rows + ROWS - 1) / ROWS : 0, from);      // tiles of the lane-th of the order
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
     }
-    return sum;
+    const int all = __shfl_sync(0xffffffffu, x, 31);
+    for (int m0 = 0; m0 < all; m0 += 32) {
+        const int m = m0 + lane;
+        int r = 0;                                    // how many sequences end in front of tile m
+#pragma unroll
+        for (int step = 16; step > 0; step >>= 1)
+            if (__shfl_sync(0xffffffffu, x, r + step - 1) <= m) r += step;
+        r = min(r, 31);
+        const int tile = __shfl_sync(0xffffffffu, x, r) - 1 - m, src = __shfl_sync(0xffffffffu, from, r);
+        KpPiece p{};
+        Kv4Seq q{};
+        q.q0 = __shfl_sync(0xffffffffu, own.q0, src);
+        q.n_q = __shfl_sync(0xffffffffu, own.n_q, src);
+        q.p0 = __shfl_sync(0xffffffffu, own.p0, src);
+        q.n_rows = __shfl_sync(0xffffffffu, own.n_rows, src);
+        const bool is = m < all;
+        if (is) {
+            p.s = src;
+            p.row0 = tile * ROWS;
+            p.rows = min(ROWS, q.n_rows - p.row0);
+            kp_span(A, q, p);
+        }
+        if (!f(is, p)) return;
+    }
 }
-// by a warp: the longest piece that is not cut again, 0 where items stay whole
+// by a warp: how long pieces may be, 0 where items stay whole.  Of the even share, 4 / 3 and 2 of it that which ends first
 template <int ROWS>
 __device__ __forceinline__ int kp_limit(const Kv4Attn & A, const KpWork & W, int ctas) {
     if (!W.cut) return 0;
     int sum = 0;
-    for (int s = threadIdx.x & 31; s < A.n_seq; s += 32) sum += kp_tiles<ROWS>(A, kv4_seq(A, s, W.most_rows, true));
+    kp_walk<ROWS>(A, W, [&](bool, const KpPiece & p) { sum += p.tiles; return true; });
     sum = __reduce_add_sync(0xffffffffu, sum) * A.cache.n_head_kv;
-    return max(4, (sum + ctas - 1) / ctas);
+    const int share = max(4, (sum + ctas - 1) / ctas), limits[3] = {share, share + (share + 2) / 3, 2 * share};
+    int pieces[3] = {0, 0, 0}, longest[3] = {0, 0, 0};
+    kp_walk<ROWS>(A, W, [&](bool is, const KpPiece & p) {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (is) {
+                const int k = kp_pieces(p.tiles, limits[i]);
+                pieces[i] += k;
+                longest[i] = max(longest[i], (p.tiles + k - 1) / k);
+            }
+        return true;
+    });
+    int best = share, best_cost = INT_MAX;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        const int n = __reduce_add_sync(0xffffffffu, pieces[i]) * A.cache.n_head_kv, most = __reduce_max_sync(0xffffffffu, longest[i]);
+        // a piece's start and end are about three tiles; rounds of the longest, or, where lengths differ, long ones first: 4 / 3 of the mean at most
+        const int mean4 = (int) ((4ll * (sum + 3ll * n) / 3 + ctas - 1) / ctas), cost = min((n + ctas - 1) / ctas * (most + 3), max(most + 3, mean4));
+        if (cost < best_cost) { best = limits[i]; best_cost = cost; }
+    }
+    return best;
 }
 // by a warp: what ticket t stands for; false: there is none
 template <int ROWS>
-__device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, int limit, int t, KpPiece & p) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, int limit, int t, KpPiece & out) {
+    const int lane = threadIdx.x & 31, hks = A.cache.n_head_kv;
     int before = 0, cut = 0;
-    for (int s0 = 0; s0 < A.n_seq; s0 += 32) {
-        const Kv4Seq q = kv4_seq(A, s0 + lane, W.most_rows, true);
-        const KpCount n = kp_count<ROWS>(A, q, limit);
-        int x = n.pieces, y = n.cut;
+    bool found = false;
+    if (limit > 0) {
+        kp_walk<ROWS>(A, W, [&](bool is, KpPiece & p) {
+            const int k = is ? kp_pieces(p.tiles, limit) : 0, c = k > 1 ? k : 0;
+            int x = k * hks, y = c * hks;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
-            if (lane >= o) { x += u; y += v; }
-        }
-        const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
-        if (!in) {
-            before += __shfl_sync(0xffffffffu, x, 31);
-            cut += __shfl_sync(0xffffffffu, y, 31);
-            continue;
-        }
-        const int at = __ffs((int) in) - 1;
-        int i = t - before - __shfl_sync(0xffffffffu, x - n.pieces, at);     // piece of the sequence
-        cut += __shfl_sync(0xffffffffu, y - n.cut, at);
-        p.s = s0 + at;
-        const Kv4Seq mine = kv4_seq(A, p.s, W.most_rows, true);
-        if (limit == 0) {
-            const int tile = i / A.cache.n_head_kv;
-            p.row0 = ((mine.n_rows + ROWS - 1) / ROWS - 1 - tile) * ROWS;
-            p.rows = min(ROWS, mine.n_rows - p.row0);
-            kp_span(A, mine, p);
-            p.hk = i - tile * A.cache.n_head_kv;
-            p.part = p.a = 0;
-            p.b = p.tiles;
-            p.parts = 1;
-            p.slot = -1;
-            return true;
-        }
-        for (int tile = (mine.n_rows + ROWS - 1) / ROWS - 1; tile >= 0; tile--) {
-            p.row0 = tile * ROWS;
-            p.rows = min(ROWS, mine.n_rows - p.row0);
-            kp_span(A, mine, p);
-            const int k = limit > 0 && 2 * p.tiles > 3 * limit ? (p.tiles + limit - 1) / limit : 1;
-            if (i < k * A.cache.n_head_kv) {
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= o) { x += u; y += v; }
+            }
+            const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
+            if (!in) {
+                before += __shfl_sync(0xffffffffu, x, 31);
+                cut += __shfl_sync(0xffffffffu, y, 31);
+                return true;
+            }
+            if (lane == __ffs((int) in) - 1) {
+                const int i = t - before - (x - k * hks);
                 p.hk = i / k;
                 p.part = i - p.hk * k;
                 p.parts = k;
                 p.a = (int) ((long long) p.tiles * p.part / k);
                 p.b = (int) ((long long) p.tiles * (p.part + 1) / k);
-                p.slot = k > 1 ? cut + i : -1;
-                return true;
+                p.slot = k > 1 ? cut + (y - c * hks) + i : -1;
+                out = p;
             }
-            i -= k * A.cache.n_head_kv;
-            cut += k > 1 ? k * A.cache.n_head_kv : 0;
+            found = true;
+            return false;
+        });
+        __syncwarp();
+        return found;
+    }
+    for (int s0 = 0; s0 < A.n_seq; s0 += 32) {
+        const Kv4Seq q = kv4_seq(A, s0 + lane, W.most_rows, true);
+        const int n = q.n_q > 0 ? (q.n_rows + ROWS - 1) / ROWS * hks : 0;
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += u;
         }
-        return false;
+        const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
+        if (!in) {
+            before += __shfl_sync(0xffffffffu, x, 31);
+            continue;
+        }
+        if (lane == __ffs((int) in) - 1) {
+            const int i = t - before - (x - n), tile = i / hks;
+            KpPiece p{};
+            p.s = s0 + lane;
+            p.row0 = ((q.n_rows + ROWS - 1) / ROWS - 1 - tile) * ROWS;
+            p.rows = min(ROWS, q.n_rows - p.row0);
+            kp_span(A, q, p);
+            p.hk = i - tile * hks;
+            p.b = p.tiles;
+            p.parts = 1;
+            p.slot = -1;
+            out = p;
+        }
+        __syncwarp();
+        return true;
     }
     return false;
 }
@@ -347,7 +395,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         if (j + 1 < n) scores(grp, tiles + (uint32_t) (j + 1));
                     }
             }
-            if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[0], 1);
+            if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[KP_DRAWN], 1);
             ticket = __shfl_sync(0xffffffffu, ticket, 0);
             const int later = (pieces + 1) & 1;
             const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
@@ -533,10 +581,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         part = &reinterpret_cast<KpParts<D> *>(W.parts)->part[P.slot];
                         part->m[rows0 + row] = m;
                         part->l[rows0 + row] = l;
-                        if (threadIdx.x == 128 && P.part == 0) {
-                            reinterpret_cast<KpParts<D> *>(W.parts)->first[P.slot] = P;
-                            W.tickets[KP_FLAGS + P.slot] = KP_JOIN;
-                        }
+                        if (threadIdx.x == 128 && P.part == 0) reinterpret_cast<KpParts<D> *>(W.parts)->item[atomicAdd(&W.tickets[KP_CUT], 1)] = P;
                     }
                     // through the queries' memory, so that a warp stores whole rows
                     T * os = reinterpret_cast<T *>(&S.q[F32 ? 0 : grp][0][0]) + row * D;
@@ -599,56 +644,65 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     pdl_wait();                                    // the end of this kernel is the end of the one in front
     if (warp == 12) {
         tmem_free(tmem, 512);
-        if (lane == 0 && atomicAdd(&W.tickets[1], 1) == (int) gridDim.x - 1) W.tickets[0] = W.tickets[1] = 0;   // the last CTA: every ticket has been drawn
+        if (lane == 0 && atomicAdd(&W.tickets[KP_DONE], 1) == (int) gridDim.x - 1) W.tickets[KP_DRAWN] = W.tickets[KP_DONE] = 0;   // the last CTA: every ticket has been drawn
     }
 }
 
-// Items that were cut: parts in their order, a warp to a row.  blockIdx.x: where an item's parts may begin
+// Items that were cut, eight rows to a CTA at a time: a warp adds a row's parts in their order, a lane D / 32 numbers.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
-    constexpr int PER = D / 32, ONCE = 4;
-    int * const left = &W.tickets[KP_FLAGS + blockIdx.x];
-    if (*(volatile int *) left == 0) return;      // (not 0 until this CTA has taken itself off)
+    constexpr int PER = D / 32, ONCE = 8, EIGHTS = kp_rows<T>() / 8;
+    const int lane = threadIdx.x & 31, items = *(volatile int *) &W.tickets[KP_CUT];
     const KpParts<D> & all = *reinterpret_cast<const KpParts<D> *>(W.parts);
-    const KpPiece & p = all.first[blockIdx.x];
-    const KpPart<D> * parts = &all.part[blockIdx.x];
-    const int lane = threadIdx.x & 31, n = p.parts;
-    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < p.rows; r += gridDim.y * 8) {
+    for (int task = blockIdx.x; task < items * EIGHTS; task += gridDim.x) {
+        const KpPiece & p = all.item[task / EIGHTS];
+        const int r = task % EIGHTS * 8 + (threadIdx.x >> 5), n = p.parts;
+        if (r >= p.rows) continue;
+        const KpPart<D> * parts = &all.part[p.slot];
         float top = -INFINITY, l = 0.f, x[PER];
-        for (int i = 0; i < n; i++) top = fmaxf(top, parts[i].m[r]);
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, parts[i].m[r]);
+        top = warp_max(top);
 #pragma unroll
         for (int e = 0; e < PER; e++) x[e] = 0.f;
-        for (int i0 = 0; i0 < n; i0 += ONCE) {
-            float mi[ONCE], li[ONCE], y[ONCE][PER];
-#pragma unroll
-            for (int k = 0; k < ONCE; k++) {
-                const int i = min(i0 + k, n - 1);
-                mi[k] = parts[i].m[r];
-                li[k] = parts[i].l[r];
-#pragma unroll
-                for (int e = 0; e < PER; e++) y[k][e] = parts[i].o[r][e * 32 + lane];
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            float f = 0.f, fl = 0.f;
+            if (i0 + lane < n) {
+                const float mi = parts[i0 + lane].m[r], li = parts[i0 + lane].l[r];
+                f = mi == -INFINITY ? (li == li ? 0.f : 1.f) : ex2(mi - top);     // a row that is no number has no maximum
+                fl = li * f;
             }
+            l += warp_sum(fl);
+            for (int i1 = 0; i1 < min(32, n - i0); i1 += ONCE) {
+                float y[ONCE][PER];
 #pragma unroll
-            for (int k = 0; k < ONCE; k++)
-                if (i0 + k < n) {
-                    const float f = mi[k] == -INFINITY ? (li[k] == li[k] ? 0.f : 1.f) : ex2(mi[k] - top);     // a row that is no number has no maximum
-                    l = fmaf(li[k], f, l);
-#pragma unroll
-                    for (int e = 0; e < PER; e++) x[e] = fmaf(y[k][e], f, x[e]);
+                for (int k = 0; k < ONCE; k++) {
+                    const float * o = &parts[min(i0 + i1 + k, n - 1)].o[r][lane * PER];
+                    if constexpr (PER == 4) *reinterpret_cast<float4 *>(y[k]) = *reinterpret_cast<const float4 *>(o);
+                    else *reinterpret_cast<float2 *>(y[k]) = *reinterpret_cast<const float2 *>(o);
                 }
+#pragma unroll
+                for (int k = 0; k < ONCE; k++) {
+                    const float h = __shfl_sync(0xffffffffu, f, i1 + k);          // (behind the last: 0)
+                    if (i0 + i1 + k < n)
+#pragma unroll
+                        for (int e = 0; e < PER; e++) x[e] = fmaf(y[k][e], h, x[e]);
+                }
+            }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int at = p.row0 + r, tt = at / A.group;
-        T * out = (T *) A.out + (p.q.q0 + tt) * A.ldo + (int64_t) (p.hk * A.group + at - tt * A.group) * D;
+        T * out = (T *) A.out + (p.q.q0 + tt) * A.ldo + (int64_t) (p.hk * A.group + at - tt * A.group) * D + lane * PER;
+        if constexpr (PER == 4) store4(out, make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv));
+        else
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
-            if constexpr (std::is_same<T, float>::value) out[e * 32 + lane] = x[e] * inv;
-            else if constexpr (std::is_same<T, __half>::value) out[e * 32 + lane] = __float2half_rn(x[e] * inv);
-            else out[e * 32 + lane] = __float2bfloat16_rn(x[e] * inv);
-        }
+            for (int e = 0; e < PER; e++) {
+                if constexpr (std::is_same<T, float>::value) out[e] = x[e] * inv;
+                else if constexpr (std::is_same<T, __half>::value) out[e] = __float2half_rn(x[e] * inv);
+                else out[e] = __float2bfloat16_rn(x[e] * inv);
+            }
     }
     __syncthreads();
-    if (threadIdx.x == 0) atomicSub(left, 1);
+    if (threadIdx.x == 0 && atomicAdd(&W.tickets[KP_JOINED], 1) == (int) gridDim.x - 1) W.tickets[KP_CUT] = W.tickets[KP_JOINED] = 0;
 }
 
 template <typename T, int D>
@@ -659,7 +713,7 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_prompt<T, D>, smem, true);
     if (e != cudaSuccess) return (int) e;
     const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
-    w.cut = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv < ctas;
+    w.cut = a.n_seq <= KP_CUT_SEQ && (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv < ctas;
     launches += w.cut ? 2 : 1;
     // Behind the kernel of few rows (most_rows > 0), CTAs start where that has none at work: it has nothing that they read, and all in front of it has ended when it starts
     cudaLaunchConfig_t cfg{};
@@ -671,7 +725,7 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     cfg.numAttrs = w.most_rows > 0 ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, k_kv4_attn_prompt<T, D>, a, w);
     if (e != cudaSuccess || !w.cut) return (int) e;
-    k_kv4_join<T, D><<<dim3(KV4_SLOTS, KP_JOIN), 256, 0, st>>>(a, w);
+    k_kv4_join<T, D><<<4 * sm_count(), 256, 0, st>>>(a, w);
     return (int) cudaGetLastError();
 }
 
