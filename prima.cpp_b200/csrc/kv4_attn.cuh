@@ -26,7 +26,7 @@ __device__ __forceinline__ void kv4_pages(const Kv4Attn & A, int lo, int hi, Kv4
     if (hi < 0) return;
     const int ld = (int) (A.table_ld < 0x1ffffff ? A.table_ld : 0x1ffffff);   // cells have 31 bits
     const int last = min(hi / KV4_CELLS, ld - 1);
-    if (A.window > 0 && lo - A.window + 1 > 0) {
+    if (A.window > 0 && lo >= A.window) {
         q.from = (lo - A.window + 1) / KV4_CELLS;
         q.keep = min(min(A.first / KV4_CELLS + (A.first % KV4_CELLS != 0), q.from), last + 1);
     }

@@ -182,6 +182,14 @@ def test_windows_walk_over_anything(pkg, lib, cuda, q, kv):
     a.check()
 
 
+@pytest.mark.parametrize("window,first", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (5, 2 ** 31 - 1)])
+@pytest.mark.parametrize("q,kv", [([1, 3, 1], [300, 1, 0]), ([200, 60, 1], [400, 20, 70])], ids=["tokens", "prompts"])
+def test_windows_as_wide_as_can_be(pkg, lib, cuda, q, kv, window, first):
+    a = Attn(pkg, lib, 18, "f32", 8, 2, 64, q, kv, window=window, first=first)
+    a.call()
+    a.check()
+
+
 @pytest.mark.parametrize("q,kv", MIXED, ids=["tokens", "prompts"])
 def test_queries_beyond_the_most_stay(pkg, lib, cuda, q, kv):
     a = Attn(pkg, lib, 6, "f32", 8, 2, 128, [n + 2 for n in q], kv)
