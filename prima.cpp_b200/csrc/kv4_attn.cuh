@@ -36,14 +36,14 @@ __device__ __forceinline__ void kv4_pages(const Kv4Attn & A, int lo, int hi, Kv4
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_rows, bool many) {
     Kv4Seq q{};
     if (s >= A.n_seq) return q;
-    const long long a = A.q_start[s], b = A.q_start[s + 1];
+    const long long a = A.q_start[s], b = A.q_start[s + 1], cells = A.kv_len[s];     // (all on their way)
     if (a < 0 || b <= a || b > A.n_tokens) return q;
     const int all = (int) (b - a), n = min(all, A.max_q);
     if (((long long) n * A.group > most_rows) != many) return q;
     q.q0 = a;
     q.n_q = n;
     q.n_rows = n * A.group;
-    const int len = max(A.kv_len[s], 0);
+    const int len = max((int) cells, 0);
     q.p0 = len - all;
     kv4_pages(A, q.p0, q.p0 + n - 1, q);
     return q;

@@ -32,6 +32,7 @@ namespace pb {
 namespace {
 
 constexpr int KP_THREADS = 13 * 32, KP_TILE = 128, KP_BLOCK = 16384;   // a block: 128 rows of 64 entries
+constexpr int KP_CUT_SEQ = 32, KP_CUT_TILES = KV4_MAX_CTAS + KP_CUT_SEQ;     // where long items may be cut: sequences, row tiles
 constexpr float KP_UP = 6.f;            // weights are up to 2^(8 + 6)
 template <typename T> constexpr int kp_rows() { return std::is_same<T, float>::value ? KP_TILE : 2 * KP_TILE; }   // of an item
 
@@ -52,6 +53,7 @@ template <int D> struct KpSmem {
     int cell[4][2];            // first cells of a key tile's pages (of none: beyond everything)
     uint32_t tmem_base;
     int abort, more[2];
+    int order[KP_CUT_SEQ], lens[KP_CUT_TILES];
 };
 // tickets: words that are zero between calls.  cut: long items may be
 struct KpWork { int most_rows; int * tickets; void * parts; int * abort_flag; int cut; };
@@ -67,129 +69,125 @@ __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpP
     p.tiles = (p.q.pages + 1) / 2;
 }
 // Items, their pieces and slots, in the order of tickets: sequences, tiles from the last on, heads, pieces; every CTA counts them in the same way.  Where long items may be cut there are
-// 32 sequences at most, of which those with the longest items come first.
-constexpr int KP_CUT_SEQ = 32;
+// 32 sequences at most, of which those with the longest items come first, and a plan of a warp's: in a lane the lane-th sequence, the one that is lane-th in that order, and how many row
+// tiles that and those in front have; in shared memory the row tiles' key tiles.
+struct KpPlan { Kv4Seq own; int from, ends, limit; };      // limit: how long pieces may be, 0 where items stay whole
 __device__ __forceinline__ int kp_pieces(int tiles, int limit) { return 2 * tiles > 3 * limit ? (tiles + limit - 1) / limit : 1; }
-// by a warp: row tiles of the sequences in that order, of each from the last on, 32 at a time, one to a lane; f(whether there is one, it) returns whether to go on
-template <int ROWS, typename F>
-__device__ __forceinline__ void kp_walk(const Kv4Attn & A, const KpWork & W, F && f) {
-    const int lane = threadIdx.x & 31;
-    const Kv4Seq own = kv4_seq(A, lane, W.most_rows, true);
-    const int len = own.n_q > 0 ? own.p0 + own.n_q : INT_MIN;
-    int rank = 0, from = 0;
-    for (int i = 0; i < 32; i++) {
-        const int other = __shfl_sync(0xffffffffu, len, i);
-        rank += other > len || (other == len && i < lane);
-    }
-    for (int i = 0; i < 32; i++)
-        if (__shfl_sync(0xffffffffu, rank, i) == lane) from = i;
-    const int n = __shfl_sync(0xffffffffu, own.n_q > 0 ? (own.n_rows + ROWS - 1) / ROWS : 0, from);      // tiles of the lane-th of the order
-    int x = n;
+__device__ __forceinline__ int warp_running_sum(int x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += u;
+        if ((int) (threadIdx.x & 31) >= o) x += u;
     }
-    const int all = __shfl_sync(0xffffffffu, x, 31);
+    return x;
+}
+__device__ __forceinline__ Kv4Seq warp_seq(const Kv4Seq & own, int src) {       // the lane src's, without its pages
+    Kv4Seq q{};
+    q.q0 = __shfl_sync(0xffffffffu, own.q0, src);
+    q.n_q = __shfl_sync(0xffffffffu, own.n_q, src);
+    q.p0 = __shfl_sync(0xffffffffu, own.p0, src);
+    q.n_rows = __shfl_sync(0xffffffffu, own.n_rows, src);
+    return q;
+}
+template <int ROWS>
+__device__ __forceinline__ KpPlan kp_plan(const Kv4Attn & A, const KpWork & W, int ctas, int * order, int * lens) {
+    KpPlan plan{};
+    if (!W.cut) return plan;
+    const int lane = threadIdx.x & 31;
+    plan.own = kv4_seq(A, lane, W.most_rows, true);
+    const int len = plan.own.n_q > 0 ? plan.own.p0 + plan.own.n_q : INT_MIN;
+    int rank = lane < A.n_seq ? 0 : lane;
+    for (int i = 0; i < A.n_seq; i++) {
+        const int other = __shfl_sync(0xffffffffu, len, i);
+        if (lane < A.n_seq) rank += other > len || (other == len && i < lane);
+    }
+    order[rank] = lane;
+    __syncwarp();
+    plan.from = order[lane];
+    plan.ends = warp_running_sum(__shfl_sync(0xffffffffu, plan.own.n_q > 0 ? (plan.own.n_rows + ROWS - 1) / ROWS : 0, plan.from));
+    const int all = __shfl_sync(0xffffffffu, plan.ends, 31);
+    if (all > KP_CUT_TILES) return plan;              // (starts that are in no order)
+    int sum = 0;
     for (int m0 = 0; m0 < all; m0 += 32) {
         const int m = m0 + lane;
         int r = 0;                                    // how many sequences end in front of tile m
 #pragma unroll
         for (int step = 16; step > 0; step >>= 1)
-            if (__shfl_sync(0xffffffffu, x, r + step - 1) <= m) r += step;
+            if (__shfl_sync(0xffffffffu, plan.ends, r + step - 1) <= m) r += step;
         r = min(r, 31);
-        const int tile = __shfl_sync(0xffffffffu, x, r) - 1 - m, src = __shfl_sync(0xffffffffu, from, r);
         KpPiece p{};
-        Kv4Seq q{};
-        q.q0 = __shfl_sync(0xffffffffu, own.q0, src);
-        q.n_q = __shfl_sync(0xffffffffu, own.n_q, src);
-        q.p0 = __shfl_sync(0xffffffffu, own.p0, src);
-        q.n_rows = __shfl_sync(0xffffffffu, own.n_rows, src);
-        const bool is = m < all;
-        if (is) {
-            p.s = src;
-            p.row0 = tile * ROWS;
+        p.row0 = (__shfl_sync(0xffffffffu, plan.ends, r) - 1 - m) * ROWS;
+        const Kv4Seq q = warp_seq(plan.own, __shfl_sync(0xffffffffu, plan.from, r));
+        if (m < all) {
             p.rows = min(ROWS, q.n_rows - p.row0);
             kp_span(A, q, p);
+            lens[m] = p.tiles;
+            sum += p.tiles;
         }
-        if (!f(is, p)) return;
     }
-}
-// by a warp: how long pieces may be, 0 where items stay whole.  Of the even share, 4 / 3 and 2 of it that which ends first
-template <int ROWS>
-__device__ __forceinline__ int kp_limit(const Kv4Attn & A, const KpWork & W, int ctas) {
-    if (!W.cut) return 0;
-    int sum = 0;
-    kp_walk<ROWS>(A, W, [&](bool, const KpPiece & p) { sum += p.tiles; return true; });
     sum = __reduce_add_sync(0xffffffffu, sum) * A.cache.n_head_kv;
+    __syncwarp();
+    // of the even share, 4 / 3 and 2 of it that which ends first
     const int share = max(4, (sum + ctas - 1) / ctas), limits[3] = {share, share + (share + 2) / 3, 2 * share};
-    int pieces[3] = {0, 0, 0}, longest[3] = {0, 0, 0};
-    kp_walk<ROWS>(A, W, [&](bool is, const KpPiece & p) {
-#pragma unroll
-        for (int i = 0; i < 3; i++)
-            if (is) {
-                const int k = kp_pieces(p.tiles, limits[i]);
-                pieces[i] += k;
-                longest[i] = max(longest[i], (p.tiles + k - 1) / k);
-            }
-        return true;
-    });
-    int best = share, best_cost = INT_MAX;
+    int best_cost = INT_MAX;
 #pragma unroll
     for (int i = 0; i < 3; i++) {
-        const int n = __reduce_add_sync(0xffffffffu, pieces[i]) * A.cache.n_head_kv, most = __reduce_max_sync(0xffffffffu, longest[i]);
+        int n = 0, most = 0;
+        for (int m = lane; m < all; m += 32) {
+            const int k = kp_pieces(lens[m], limits[i]);
+            n += k;
+            most = max(most, (lens[m] + k - 1) / k);
+        }
+        n = __reduce_add_sync(0xffffffffu, n) * A.cache.n_head_kv;
+        most = __reduce_max_sync(0xffffffffu, most);
         // a piece's start and end are about three tiles; rounds of the longest, or, where lengths differ, long ones first: 4 / 3 of the mean at most
         const int mean4 = (int) ((4ll * (sum + 3ll * n) / 3 + ctas - 1) / ctas), cost = min((n + ctas - 1) / ctas * (most + 3), max(most + 3, mean4));
-        if (cost < best_cost) { best = limits[i]; best_cost = cost; }
+        if (cost < best_cost) { plan.limit = limits[i]; best_cost = cost; }
     }
-    return best;
+    return plan;
 }
 // by a warp: what ticket t stands for; false: there is none
 template <int ROWS>
-__device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, int limit, int t, KpPiece & out) {
+__device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, const KpPlan & plan, const int * lens, int t, KpPiece & out) {
     const int lane = threadIdx.x & 31, hks = A.cache.n_head_kv;
     int before = 0, cut = 0;
-    bool found = false;
-    if (limit > 0) {
-        kp_walk<ROWS>(A, W, [&](bool is, KpPiece & p) {
-            const int k = is ? kp_pieces(p.tiles, limit) : 0, c = k > 1 ? k : 0;
-            int x = k * hks, y = c * hks;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
-                if (lane >= o) { x += u; y += v; }
-            }
+    if (plan.limit > 0) {
+        const int all = __shfl_sync(0xffffffffu, plan.ends, 31);
+        for (int m0 = 0; m0 < all; m0 += 32) {
+            const int tiles = m0 + lane < all ? lens[m0 + lane] : 0, k = tiles > 0 ? kp_pieces(tiles, plan.limit) : 0, c = k > 1 ? k * hks : 0;
+            const int x = warp_running_sum(k * hks), y = warp_running_sum(c);
             const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
             if (!in) {
                 before += __shfl_sync(0xffffffffu, x, 31);
                 cut += __shfl_sync(0xffffffffu, y, 31);
-                return true;
+                continue;
             }
-            if (lane == __ffs((int) in) - 1) {
+            const int at = __ffs((int) in) - 1, m = m0 + at, r = __popc(__ballot_sync(0xffffffffu, plan.ends <= m));
+            KpPiece p{};
+            p.row0 = (__shfl_sync(0xffffffffu, plan.ends, r) - 1 - m) * ROWS;
+            p.s = __shfl_sync(0xffffffffu, plan.from, r);
+            const Kv4Seq q = warp_seq(plan.own, p.s);
+            if (lane == at) {
+                p.rows = min(ROWS, q.n_rows - p.row0);
+                kp_span(A, q, p);
                 const int i = t - before - (x - k * hks);
                 p.hk = i / k;
                 p.part = i - p.hk * k;
                 p.parts = k;
                 p.a = (int) ((long long) p.tiles * p.part / k);
                 p.b = (int) ((long long) p.tiles * (p.part + 1) / k);
-                p.slot = k > 1 ? cut + (y - c * hks) + i : -1;
+                p.slot = k > 1 ? cut + (y - c) + i : -1;
                 out = p;
             }
-            found = true;
-            return false;
-        });
-        __syncwarp();
-        return found;
+            __syncwarp();
+            return true;
+        }
+        return false;
     }
     for (int s0 = 0; s0 < A.n_seq; s0 += 32) {
         const Kv4Seq q = kv4_seq(A, s0 + lane, W.most_rows, true);
         const int n = q.n_q > 0 ? (q.n_rows + ROWS - 1) / ROWS * hks : 0;
-        int x = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += u;
-        }
+        const int x = warp_running_sum(n);
         const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
         if (!in) {
             before += __shfl_sync(0xffffffffu, x, 31);
@@ -257,10 +255,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
         __syncwarp();
         tmem_alloc(&S.tmem_base, 512);
     }
-    int limit = 0, ticket = blockIdx.x;
+    int ticket = blockIdx.x;
+    KpPlan plan{};
     if (warp == 12) {
-        limit = kp_limit<ROWS>(A, W, gridDim.x);
-        const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece[0]);
+        plan = kp_plan<ROWS>(A, W, gridDim.x, S.order, S.lens);
+        const bool more = kp_find<ROWS>(A, W, plan, S.lens, ticket, S.piece[0]);
         if (lane == 0) S.more[0] = more;
     }
     fence_before();
@@ -398,7 +397,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[KP_DRAWN], 1);
             ticket = __shfl_sync(0xffffffffu, ticket, 0);
             const int later = (pieces + 1) & 1;
-            const bool more = kp_find<ROWS>(A, W, limit, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
+            const bool more = kp_find<ROWS>(A, W, plan, S.lens, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
             if (lane == 0) S.more[later] = more;
         } else {
             // ---- softmax ----
