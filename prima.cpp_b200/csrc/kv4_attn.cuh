@@ -6,7 +6,7 @@
 namespace pb {
 
 constexpr int KV4_MAX_CTAS = 152;      // of a launch: the workspace has parts by CTA and warp
-constexpr int KV4_SLOTS = 256;         // and by piece of a cut item: these are 5 / 3 of the CTAs at most
+constexpr int KV4_SLOTS = 288;         // and by piece of a cut item: these are 9 / 5 of the CTAs at most
 constexpr int KV4_COUNTERS = 16384;    // in front of them
 
 // A sequence: its queries' rows, and the pages that any of them sees: the first `keep`, then those from page `from` on.  At least one page, so that rows which see

@@ -72,7 +72,7 @@ __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpP
 // 32 sequences at most, of which those with the longest items come first, and a plan of a warp's: in a lane the lane-th sequence, the one that is lane-th in that order, and how many row
 // tiles that and those in front have; in shared memory the row tiles' key tiles.
 struct KpPlan { Kv4Seq own; int from, ends, limit; };      // limit: how long pieces may be, 0 where items stay whole
-__device__ __forceinline__ int kp_pieces(int tiles, int limit) { return 2 * tiles > 3 * limit ? (tiles + limit - 1) / limit : 1; }
+__device__ __forceinline__ int kp_pieces(int tiles, int limit) { return 4 * (int64_t) tiles > 5 * (int64_t) limit ? 1 + (int) (((float) tiles - 0.5f) * __frcp_rn((float) limit)) : 1; }
 __device__ __forceinline__ int warp_running_sum(int x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -128,21 +128,22 @@ __device__ __forceinline__ KpPlan kp_plan(const Kv4Attn & A, const KpWork & W, i
     sum = __reduce_add_sync(0xffffffffu, sum) * A.cache.n_head_kv;
     __syncwarp();
     // of the even share, 4 / 3 and 2 of it that which ends first
-    const int share = max(4, (sum + ctas - 1) / ctas), limits[3] = {share, share + (share + 2) / 3, 2 * share};
+    const int share = max(4, (sum + ctas - 1) / ctas);
     int best_cost = INT_MAX;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < 3; i++) {
+        const int limit = share + (i == 0 ? 0 : i == 1 ? (share + 2) / 3 : share);
         int n = 0, most = 0;
         for (int m = lane; m < all; m += 32) {
-            const int k = kp_pieces(lens[m], limits[i]);
+            const int k = kp_pieces(lens[m], limit);
             n += k;
-            most = max(most, (lens[m] + k - 1) / k);
+            most = max(most, (int) (((float) lens[m] - 0.5f) * __frcp_rn((float) k)) + 1);
         }
         n = __reduce_add_sync(0xffffffffu, n) * A.cache.n_head_kv;
         most = __reduce_max_sync(0xffffffffu, most);
         // a piece's start and end are about three tiles; rounds of the longest, or, where lengths differ, long ones first: 4 / 3 of the mean at most
-        const int mean4 = (int) ((4ll * (sum + 3ll * n) / 3 + ctas - 1) / ctas), cost = min((n + ctas - 1) / ctas * (most + 3), max(most + 3, mean4));
-        if (cost < best_cost) { plan.limit = limits[i]; best_cost = cost; }
+        const int mean = (int) (((float) sum + 3.f * (float) n) * (4.f / 3.f) * __frcp_rn((float) ctas)) + 1, cost = min((n + ctas - 1) / ctas * (most + 3), max(most + 3, mean));
+        if (cost < best_cost) { plan.limit = limit; best_cost = cost; }
     }
     return plan;
 }
@@ -712,7 +713,9 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_prompt<T, D>, smem, true);
     if (e != cudaSuccess) return (int) e;
     const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
-    w.cut = a.n_seq <= KP_CUT_SEQ && (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv < ctas;
+    // (a plan adds up key tiles of all items: in 30 bits)
+    const int64_t items = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv, pages = a.table_ld < INT_MAX / KV4_CELLS ? a.table_ld : INT_MAX / KV4_CELLS;
+    w.cut = a.n_seq <= KP_CUT_SEQ && items < ctas && KP_CUT_TILES * (pages / 2 + 1) * a.cache.n_head_kv < 1 << 30;
     launches += w.cut ? 2 : 1;
     // Behind the kernel of few rows (most_rows > 0), CTAs start where that has none at work: it has nothing that they read, and all in front of it has ended when it starts
     cudaLaunchConfig_t cfg{};
