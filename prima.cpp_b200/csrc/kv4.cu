@@ -11,7 +11,7 @@
 namespace pb {
 namespace {
 
-constexpr int KA_THREADS = 256, KA_WARPS = KA_THREADS / 32, KA_CTAS = 4;
+constexpr int KA_THREADS = 256, KA_WARPS = KA_THREADS / 32, KA_MANY = 2;
 
 template <typename T>
 struct AppendParams {
@@ -26,13 +26,16 @@ struct AppendParams {
 __device__ __forceinline__ void raw4(const float * p, uint32_t (&w)[4]) { *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(p); }
 template <typename T> __device__ __forceinline__ void raw4(const T * p, uint32_t (&w)[2]) { *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p); }
 
-// the sum of four squares to 47 bits: products and sums of 32 bits with what their roundings left (two conversions to 64 bits where four numbers are eight operations)
+// the sum of four squares to 47 bits: products and sums of 32 bits with what their roundings left (two conversions to 64 bits where four numbers are eight operations); exact: squares of
+// numbers of T have 24 bits at most
+template <typename T>
 __device__ __forceinline__ double squares(const float (&x)[4]) {
-    float hi = 0.f, lo = 0.f;
+    constexpr bool exact = sizeof(T) == 2;
+    float hi = __fmul_rn(x[0], x[0]), lo = exact ? 0.f : fmaf(x[0], x[0], -hi);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float p = __fmul_rn(x[i], x[i]), s = __fadd_rn(hi, p), t = __fsub_rn(s, hi);
-        lo += __fadd_rn(__fsub_rn(hi, __fsub_rn(s, t)), __fsub_rn(p, t)) + fmaf(x[i], x[i], -p);
+    for (int i = 1; i < 4; i++) {
+        const float p = __fmul_rn(x[i], x[i]), big = fmaxf(hi, p), small = fminf(hi, p), s = __fadd_rn(big, small), left = __fsub_rn(small, __fsub_rn(s, big));
+        lo += exact ? left : left + fmaf(x[i], x[i], -p);
         hi = s;
     }
     if (!(hi > 1e-30f && hi < 1e38f)) {   // squares that leave the range of 32 bits
@@ -52,12 +55,13 @@ __device__ __forceinline__ float inverse_root(double v) {
 }
 
 // Bound: instructions: a row's norm and rotation, and a stored row's scale and steps, about as much again each as reading and writing a row of queries.  us, 2048 tokens of 32 heads over 8
-// of 128, bf16: 28 (and 6 for k_kv4_load; floor 8.4 of both); 64 tokens in F32 3.  With roots and quotients of 64 and 32 bits 42, a head to a warp and angles once for 8 rows 57.
+// of 128, bf16: 22 (and 6 for k_kv4_load; floor 8.4 of both); 64 tokens in F32 3.  A head to a warp and angles once for 8 rows 57; roots and quotients of 64 and 32 bits 42; four tokens to
+// a CTA (some SMs have four of these, others three), and steps by conversions, 28.
 // A CTA takes TOKENS tokens at a time and a part of their heads, a warp R heads of q, of k or of v at a time (R rows on their way together): D / 4 lanes hold a row, four neighbouring numbers
 // each.  What decides which of 16 steps a number falls to is computed so that it does not depend on an order: the mean of squares and the angles in 64 bits, rounded
 // once, products and sums of the rotation in 32 bits without contraction.
 template <typename T, int D, int TOKENS, int R>
-__global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid_constant__ AppendParams<T> P, const __grid_constant__ Kv4Rope RP) {
+__global__ void __launch_bounds__(KA_THREADS, 4) k_kv4_append(const __grid_constant__ AppendParams<T> P, const __grid_constant__ Kv4Rope RP) {
     constexpr int LPR = D / 4, RPW = 32 / LPR, HEADS = R * RPW;      // lanes to a row, rows to a warp's instruction, heads to an item
     __shared__ float2 cs[TOKENS][D / 2];
     const int lane = threadIdx.x & 31;
@@ -66,7 +70,8 @@ __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid
     const int of_q = (P.n_head + HEADS - 1) / HEADS, of_kv = (hk + HEADS - 1) / HEADS, of_token = of_q + 2 * of_kv;
     const int step = KA_WARPS * gridDim.y;
     uint32_t raw[R][sizeof(T) == 4 ? 4 : 2];
-    int t0 = blockIdx.x * TOKENS, t = 0, kind = 0, head0 = 0, heads = 0;   // of the item at hand: token, 0 q 1 k 2 v, its first head, heads there are
+    const int t0 = blockIdx.x * TOKENS;
+    int t = 0, kind = 0, head0 = 0, heads = 0;   // of the item at hand: token, 0 q 1 k 2 v, its first head, heads there are
     auto ask = [&](int item) {
         t = item / of_token;
         const int i = item - t * of_token;
@@ -83,11 +88,9 @@ __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid
                 for (uint32_t & w : raw[r]) w = 0u;
         }
     };
-    for (; t0 < P.n_tokens; t0 += gridDim.x * TOKENS) {
     const int tokens = min(TOKENS, P.n_tokens - t0), items = tokens * of_token;
     int item = blockIdx.y * KA_WARPS + (threadIdx.x >> 5);
     if (item < items) ask(item);                                     // on its way beside the angles
-    __syncthreads();                                                 // those of the tokens in front have been used
     for (int i = threadIdx.x; i < tokens * pairs; i += KA_THREADS) {
         const int at = i / pairs, pair = i - at * pairs;
         const double a = (double) P.pos[t0 + at] * RP.w[pair] / (RP.freq_factors ? (double) RP.freq_factors[pair] : 1.0);
@@ -113,7 +116,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid
                 constexpr int H = LPR / 2, Q = LPR / 4;
                 double v[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) v[r] = squares(x[r]);
+                for (int r = 0; r < 4; r++) v[r] = squares<T>(x[r]);
                 const bool h = lane & H, q = lane & Q;
 #pragma unroll
                 for (int r = 0; r < 2; r++) v[r] = (h ? v[r + 2] : v[r]) + __shfl_xor_sync(0xffffffffu, h ? v[r] : v[r + 2], H);
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid
             } else {
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    double sum = squares(x[r]);
+                    double sum = squares<T>(x[r]);
 #pragma unroll
                     for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     f[r] = inverse_root(sum * (1.0 / D) + (double) P.eps);
@@ -199,10 +202,8 @@ __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid
             for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const uint32_t who = __ballot_sync(0xffffffffu, fabsf(most) == top) & (0xffu << (lane & 24));
             const float scale = kv4_scale_of(__shfl_sync(0xffffffffu, most, __ffs((int) who) - 1));
-            const float inv = __frcp_rn(scale);
             uint32_t m[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) m[i] = kv4_bits_of(x[r][i], scale, inv);
+            kv4_bits_of(x[r], scale, scale == 0.f ? 0.f : __frcp_rn(scale), m);
             const int head = first + r * RPW + sub;
             uint8_t * chunk = page + (int64_t) head * kv4_chunk_bytes(D);
             if (is == 1) {
@@ -214,7 +215,6 @@ __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_append(const __grid
             if (head < n && (l & 7) == 0)
                 *reinterpret_cast<__half *>(chunk + 2 * kv4_rows_bytes(D) + (is == 2 ? kv4_scales_bytes(D) : 0) + kv4_scale(D, c, b)) = __float2half_rn(scale);
         }
-    }
     }
 }
 
@@ -319,11 +319,12 @@ template <typename T>
 int append(const Kv4 & cache, int D, const void * q, int64_t ldq, void * q_out, int64_t ldqo, const void * k, int64_t ldk, const void * v, int64_t ldv, int64_t n, int n_head,
            const int64_t * cells, const int32_t * pos, const float * q_norm, const float * k_norm, float eps, const Kv4Rope & rope, cudaStream_t st) {
     const AppendParams<T> p{cache, (const T *) q, (const T *) k, (const T *) v, (T *) q_out, ldq, ldqo, ldk, ldv, n_head, (int) n, cells, pos, q_norm, k_norm, eps};
-    // Many tokens: four to a CTA, so that angles are made once, and four heads to a warp.  Few: a CTA has a token's heads in part, which makes the angles again for each
-    if (n >= 4 * sm_count()) {
-        const unsigned grid = (unsigned) std::min<int64_t>((n + 3) / 4, KA_CTAS * sm_count());       // as many as are at work together
-        if (D == 128) k_kv4_append<T, 128, 4, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
-        else k_kv4_append<T, 64, 4, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
+    // Many tokens: two to a CTA, so that angles are made once, and four heads to a warp.  Few: a CTA has a token's heads in part, which makes the angles again for each.  us, many / few, bf16,
+    // 32 heads over 8, with k_kv4_load: 150 tokens 10.8 / 8.7, 200 10.9 / 10.7, 300 12.2 / 12.9, 600 15 / 20
+    if (n >= KA_MANY * sm_count()) {
+        const unsigned grid = (unsigned) ((n + 1) / 2);
+        if (D == 128) k_kv4_append<T, 128, 2, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
+        else k_kv4_append<T, 64, 2, 4><<<grid, KA_THREADS, 0, st>>>(p, rope);
     } else {
         const int64_t items = (n_head + 2 * (int64_t) cache.n_head_kv + 32 / (D / 4) - 1) / (32 / (D / 4)), parts = (items + KA_WARPS - 1) / KA_WARPS, most = (4 * sm_count() + n - 1) / n;
         const dim3 grid((unsigned) n, (unsigned) (parts < most ? parts : most));

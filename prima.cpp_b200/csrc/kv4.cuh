@@ -48,13 +48,22 @@ __device__ __forceinline__ uint8_t * kv4_chunk(const Kv4 & c, int64_t page, int 
 
 // A block's scale from its number of largest magnitude: bf16 rounds to the 8 significant bits
 __device__ __forceinline__ float kv4_scale_of(float most) { return __half2float(__float2half_rn(__bfloat162float(__float2bfloat16_rn(most * -0.125f)))); }
-// rint(x / scale) + 8, by the reciprocal of the scale: that product is within 2^-22 of the quotient (of up to 8.03), and only next to a half is the quotient itself needed
-__device__ __forceinline__ uint32_t kv4_bits_of(float x, float scale, float inv) {
-    if (scale == 0.f) return 8u;
-    const float y = x * inv;
-    float n = rintf(y);
-    if (fabsf(fabsf(y - n) - 0.5f) < 4e-6f) n = rintf(__fdiv_rn(x, scale));
-    return (uint32_t) fminf(fmaxf(n + 8.f, 0.f), 15.f);
+// rint(x / scale) + 8 within 0 .. 15, by the reciprocal of the scale (0: of a scale of 0): that product is within 2^-22 of the quotient (of up to 8.03), and only next to a half is the quotient
+// itself needed.  Sums with 1.5 * 2^23 round like rint, and hold the number in their last bits: conversions take eight times as long
+__device__ __forceinline__ void kv4_bits_of(const float (&x)[4], float scale, float inv, uint32_t (&m)[4]) {
+    float n[4];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float y = x[i] * inv;
+        n[i] = __fadd_rn(y, 12582912.f) - 12582912.f;
+        near |= fabsf(fabsf(y - n[i]) - 0.5f) < 4e-6f;
+    }
+    if (near)
+#pragma unroll
+        for (int i = 0; i < 4; i++) n[i] = rintf(__fdiv_rn(x[i], scale));
+#pragma unroll
+    for (int i = 0; i < 4; i++) m[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(n[i], -8.f), 7.f), 12582920.f)) & 15u;
 }
 // the cache holds numbers only: a value that is none would reach rows that do not see its cell (0 * NaN)
 __device__ __forceinline__ float kv4_finite(float x) { return x != x ? 0.f : fminf(fmaxf(x, -KV4_MOST), KV4_MOST); }
