@@ -27,14 +27,14 @@ __device__ __forceinline__ void raw4(const float * p, uint32_t (&w)[4]) { *reint
 template <typename T> __device__ __forceinline__ void raw4(const T * p, uint32_t (&w)[2]) { *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p); }
 
 // the sum of four squares to 47 bits: products and sums of 32 bits with what their roundings left (two conversions to 64 bits where four numbers are eight operations); exact: squares of
-// numbers of T have 24 bits at most
+// numbers of T have 24 bits at most.  (The larger and the smaller of a NaN are no NaN: the sum has it.)
 template <typename T>
 __device__ __forceinline__ double squares(const float (&x)[4]) {
     constexpr bool exact = sizeof(T) == 2;
     float hi = __fmul_rn(x[0], x[0]), lo = exact ? 0.f : fmaf(x[0], x[0], -hi);
 #pragma unroll
     for (int i = 1; i < 4; i++) {
-        const float p = __fmul_rn(x[i], x[i]), big = fmaxf(hi, p), small = fminf(hi, p), s = __fadd_rn(big, small), left = __fsub_rn(small, __fsub_rn(s, big));
+        const float p = __fmul_rn(x[i], x[i]), big = fmaxf(hi, p), small = fminf(hi, p), s = __fadd_rn(hi, p), left = __fsub_rn(small, __fsub_rn(s, big));
         lo += exact ? left : left + fmaf(x[i], x[i], -p);
         hi = s;
     }
