@@ -15,7 +15,7 @@
 // Bound: with 16 bits a key tile takes 4400 clocks for 256 rows: MMAs 2100 (S with both operands in shared memory, which also takes the expanded tiles), exponentials 2050 a scheduler, two
 // softmax groups and expansion side by side, each group waiting for a third of it on its own two products; an item adds 12000 for queries, first tile, output; a launch 4000, or 8000 where
 // items are cut.  us: 2048 tokens of 32 heads over 8 56 (610 TFLOP/s of visible pairs; over an f16 cache k_attn_prefill_tc takes 58), a plain form of elementary operations 3066; 512 behind
-// 8000 cells 104; F32, 1077 queries behind up to 5077 cells 70 (with the sequence of one query and the join), 5200.
+// 8000 cells 104; F32, 1077 queries behind up to 5077 cells 67 (with the sequence of one query and the join), 5200.
 // On the way, us at 2048 tokens: scores 32 at a time, waited for, masks within the passes 124; the next 32 on their way 102; masks in a pass of their own over edge tiles (their code was a
 // third of what was fetched and not run) 64; eight numbers of a query to a lane 57.  A row to a thread for the queries is no faster (its loads are 256 bytes apart),
 // weights handed over in halves neither (F32 70 -> 77: the issuing warp waits for one group's while the other's are there).
@@ -45,6 +45,17 @@ struct KpPiece {               // what a ticket stands for
     Kv4Seq q;                  // pages that the tile's rows see
     int p_lo, p_hi;            // positions of the tile's first and last row
 };
+// of a launch whose long items may be cut, in shared memory (in registers it takes them from all roles): a sequence's rows; which one is i-th in the order of lengths, and how many row tiles
+// that and those in front have; the row tiles' key tiles; how long pieces may be, 0 where items stay whole
+struct KpPlan {
+    int64_t q0[KP_CUT_SEQ];
+    int n_q[KP_CUT_SEQ], p0[KP_CUT_SEQ], n_rows[KP_CUT_SEQ], from[KP_CUT_SEQ], ends[KP_CUT_SEQ], lens[KP_CUT_TILES], limit;
+    __device__ __forceinline__ Kv4Seq seq(int s) const {       // without its pages
+        Kv4Seq q{};
+        q.q0 = q0[s]; q.n_q = n_q[s]; q.p0 = p0[s]; q.n_rows = n_rows[s];
+        return q;
+    }
+};
 template <int D> struct KpPart { float o[2 * KP_TILE][D]; float m[2 * KP_TILE], l[2 * KP_TILE]; };
 template <int D> struct KpSmem {
     uint8_t q[2][D / 64][KP_BLOCK];            // 16 bits: either row tile; F32: high and low
@@ -55,7 +66,7 @@ template <int D> struct KpSmem {
     int cell[4][2];            // first cells of a key tile's pages (of none: beyond everything)
     uint32_t tmem_base;
     int abort, more[2];
-    int order[KP_CUT_SEQ], lens[KP_CUT_TILES];
+    KpPlan plan;
 };
 // tickets: words that are zero between calls.  cut: long items may be
 struct KpWork { int most_rows; int * tickets; void * parts; int * abort_flag; int cut; };
@@ -71,9 +82,7 @@ __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpP
     p.tiles = (p.q.pages + 1) / 2;
 }
 // Items, their pieces and slots, in the order of tickets: sequences, tiles from the last on, heads, pieces; every CTA counts them in the same way.  Where long items may be cut there are
-// 32 sequences at most, of which those with the longest items come first, and a plan of a warp's: in a lane the lane-th sequence, the one that is lane-th in that order, and how many row
-// tiles that and those in front have; in shared memory the row tiles' key tiles.
-struct KpPlan { Kv4Seq own; int from, ends, limit; };      // limit: how long pieces may be, 0 where items stay whole
+// 32 sequences at most, of which those with the longest items come first.
 __device__ __forceinline__ int kp_pieces(int tiles, int limit) { return 4 * (int64_t) tiles > 5 * (int64_t) limit ? 1 + (int) (((float) tiles - 0.5f) * __frcp_rn((float) limit)) : 1; }
 __device__ __forceinline__ int warp_running_sum(int x) {
 #pragma unroll
@@ -83,47 +92,41 @@ __device__ __forceinline__ int warp_running_sum(int x) {
     }
     return x;
 }
-__device__ __forceinline__ Kv4Seq warp_seq(const Kv4Seq & own, int src) {       // the lane src's, without its pages
-    Kv4Seq q{};
-    q.q0 = __shfl_sync(0xffffffffu, own.q0, src);
-    q.n_q = __shfl_sync(0xffffffffu, own.n_q, src);
-    q.p0 = __shfl_sync(0xffffffffu, own.p0, src);
-    q.n_rows = __shfl_sync(0xffffffffu, own.n_rows, src);
-    return q;
-}
 template <int ROWS>
-__device__ __forceinline__ KpPlan kp_plan(const Kv4Attn & A, const KpWork & W, int ctas, int * order, int * lens) {
-    KpPlan plan{};
-    if (!W.cut) return plan;
+__device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int ctas, KpPlan & plan) {     // by a warp
     const int lane = threadIdx.x & 31;
-    plan.own = kv4_seq(A, lane, W.most_rows, true);
-    const int len = plan.own.n_q > 0 ? plan.own.p0 + plan.own.n_q : INT_MIN;
+    if (lane == 0) plan.limit = 0;
+    if (!W.cut) return;
+    const Kv4Seq own = kv4_seq(A, lane, W.most_rows, true);
+    plan.q0[lane] = own.q0; plan.n_q[lane] = own.n_q; plan.p0[lane] = own.p0; plan.n_rows[lane] = own.n_rows;
+    const int len = own.n_q > 0 ? own.p0 + own.n_q : INT_MIN;
     int rank = lane < A.n_seq ? 0 : lane;
     for (int i = 0; i < A.n_seq; i++) {
         const int other = __shfl_sync(0xffffffffu, len, i);
         if (lane < A.n_seq) rank += other > len || (other == len && i < lane);
     }
-    order[rank] = lane;
+    plan.from[rank] = lane;
     __syncwarp();
-    plan.from = order[lane];
-    plan.ends = warp_running_sum(__shfl_sync(0xffffffffu, plan.own.n_q > 0 ? (plan.own.n_rows + ROWS - 1) / ROWS : 0, plan.from));
-    const int all = __shfl_sync(0xffffffffu, plan.ends, 31);
-    if (all > KP_CUT_TILES) return plan;              // (starts that are in no order)
+    const int from = plan.from[lane], ends = warp_running_sum(__shfl_sync(0xffffffffu, own.n_q > 0 ? (own.n_rows + ROWS - 1) / ROWS : 0, from));
+    plan.ends[lane] = ends;
+    const int all = __shfl_sync(0xffffffffu, ends, 31);
+    if (all > KP_CUT_TILES) return;                   // (starts that are in no order)
     int sum = 0;
     for (int m0 = 0; m0 < all; m0 += 32) {
         const int m = m0 + lane;
         int r = 0;                                    // how many sequences end in front of tile m
 #pragma unroll
         for (int step = 16; step > 0; step >>= 1)
-            if (__shfl_sync(0xffffffffu, plan.ends, r + step - 1) <= m) r += step;
+            if (__shfl_sync(0xffffffffu, ends, r + step - 1) <= m) r += step;
         r = min(r, 31);
         KpPiece p{};
-        p.row0 = (__shfl_sync(0xffffffffu, plan.ends, r) - 1 - m) * ROWS;
-        const Kv4Seq q = warp_seq(plan.own, __shfl_sync(0xffffffffu, plan.from, r));
+        p.row0 = (__shfl_sync(0xffffffffu, ends, r) - 1 - m) * ROWS;
+        const int src = __shfl_sync(0xffffffffu, from, r);
         if (m < all) {
+            const Kv4Seq q = plan.seq(src);
             p.rows = min(ROWS, q.n_rows - p.row0);
             kp_span(A, q, p);
-            lens[m] = p.tiles;
+            plan.lens[m] = p.tiles;
             sum += p.tiles;
         }
     }
@@ -131,33 +134,33 @@ __device__ __forceinline__ KpPlan kp_plan(const Kv4Attn & A, const KpWork & W, i
     __syncwarp();
     // of the even share, 4 / 3 and 2 of it that which ends first
     const int share = max(4, (sum + ctas - 1) / ctas);
-    int best_cost = INT_MAX;
+    int best = share, best_cost = INT_MAX;
 #pragma unroll 1
     for (int i = 0; i < 3; i++) {
         const int limit = share + (i == 0 ? 0 : i == 1 ? (share + 2) / 3 : share);
         int n = 0, most = 0;
         for (int m = lane; m < all; m += 32) {
-            const int k = kp_pieces(lens[m], limit);
+            const int k = kp_pieces(plan.lens[m], limit);
             n += k;
-            most = max(most, (int) (((float) lens[m] - 0.5f) * __frcp_rn((float) k)) + 1);
+            most = max(most, (int) (((float) plan.lens[m] - 0.5f) * __frcp_rn((float) k)) + 1);
         }
         n = __reduce_add_sync(0xffffffffu, n) * A.cache.n_head_kv;
         most = __reduce_max_sync(0xffffffffu, most);
         // a piece's start and end are about three tiles; rounds of the longest, or, where lengths differ, long ones first: 4 / 3 of the mean at most
         const int mean = (int) (((float) sum + 3.f * (float) n) * (4.f / 3.f) * __frcp_rn((float) ctas)) + 1, cost = min((n + ctas - 1) / ctas * (most + 3), max(most + 3, mean));
-        if (cost < best_cost) { plan.limit = limit; best_cost = cost; }
+        if (cost < best_cost) { best = limit; best_cost = cost; }
     }
-    return plan;
+    if (lane == 0) plan.limit = best;
 }
 // by a warp: what ticket t stands for; false: there is none
 template <int ROWS>
-__device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, const KpPlan & plan, const int * lens, int t, KpPiece & out) {
+__device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, const KpPlan & plan, int t, KpPiece & out) {
     const int lane = threadIdx.x & 31, hks = A.cache.n_head_kv;
     int before = 0, cut = 0;
-    if (plan.limit > 0) {
-        const int all = __shfl_sync(0xffffffffu, plan.ends, 31);
+    if (W.cut && plan.limit > 0) {
+        const int limit = plan.limit, all = plan.ends[31];
         for (int m0 = 0; m0 < all; m0 += 32) {
-            const int tiles = m0 + lane < all ? lens[m0 + lane] : 0, k = tiles > 0 ? kp_pieces(tiles, plan.limit) : 0, c = k > 1 ? k * hks : 0;
+            const int tiles = m0 + lane < all ? plan.lens[m0 + lane] : 0, k = tiles > 0 ? kp_pieces(tiles, limit) : 0, c = k > 1 ? k * hks : 0;
             const int x = warp_running_sum(k * hks), y = warp_running_sum(c);
             const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
             if (!in) {
@@ -165,12 +168,12 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, con
                 cut += __shfl_sync(0xffffffffu, y, 31);
                 continue;
             }
-            const int at = __ffs((int) in) - 1, m = m0 + at, r = __popc(__ballot_sync(0xffffffffu, plan.ends <= m));
-            KpPiece p{};
-            p.row0 = (__shfl_sync(0xffffffffu, plan.ends, r) - 1 - m) * ROWS;
-            p.s = __shfl_sync(0xffffffffu, plan.from, r);
-            const Kv4Seq q = warp_seq(plan.own, p.s);
+            const int at = __ffs((int) in) - 1, m = m0 + at, r = __popc(__ballot_sync(0xffffffffu, plan.ends[lane] <= m));
             if (lane == at) {
+                KpPiece p{};
+                p.row0 = (plan.ends[r] - 1 - m) * ROWS;
+                p.s = plan.from[r];
+                const Kv4Seq q = plan.seq(p.s);
                 p.rows = min(ROWS, q.n_rows - p.row0);
                 kp_span(A, q, p);
                 const int i = t - before - (x - k * hks);
@@ -259,10 +262,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
         tmem_alloc(&S.tmem_base, 512);
     }
     int ticket = blockIdx.x;
-    KpPlan plan{};
     if (warp == 12) {
-        plan = kp_plan<ROWS>(A, W, gridDim.x, S.order, S.lens);
-        const bool more = kp_find<ROWS>(A, W, plan, S.lens, ticket, S.piece[0]);
+        kp_plan<ROWS>(A, W, gridDim.x, S.plan);
+        __syncwarp();
+        const bool more = kp_find<ROWS>(A, W, S.plan, ticket, S.piece[0]);
         if (lane == 0) S.more[0] = more;
     }
     fence_before();
@@ -400,7 +403,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[KP_DRAWN], 1);
             ticket = __shfl_sync(0xffffffffu, ticket, 0);
             const int later = (pieces + 1) & 1;
-            const bool more = kp_find<ROWS>(A, W, plan, S.lens, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
+            const bool more = kp_find<ROWS>(A, W, S.plan, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
             if (lane == 0) S.more[later] = more;
         } else {
             // ---- softmax ----
