@@ -170,8 +170,8 @@ PB200_API int pb200_kv4_attn(const pb200_kv4_cache * cache, int layer, int type,
 /* Copies of whole pages, all layers: page src[i] to page dst[i] (HOST arrays, not needed after the call).  A sequence that forks shares its full pages with the new one, and
  * copies the last, which both go on writing.  PB200_EINVAL where a page is written twice, or written and read. */
 PB200_API int pb200_kv4_copy_pages(const pb200_kv4_cache * cache, const int32_t * src, const int32_t * dst, int n, void * stream);
-/* Cells that a sequence keeps, to pages of their own, all layers: cell index[s * index_ld + i] of table row s becomes cell i of row s of `to`, i < count[s] <= max_count
- * (device arrays).  Bits are moved as they are: keys stay rotated for the positions that they had.  Pages of `to` are none of the pages that are read, and of one sequence each;
+/* Cells that a sequence keeps, to pages of their own, all layers: cell index[s * index_ld + i] of table row s becomes cell i of row s of `to`, i < count[s] and
+ * max_count (device arrays).  Bits are moved as they are: keys stay rotated for the positions that they had.  Pages of `to` are none of the pages that are read, and of one sequence each;
  * their other cells stay as they were.  Behind it the old pages are free. */
 PB200_API int pb200_kv4_compact(const pb200_kv4_cache * cache, int n_seq, const int32_t * table, int64_t table_ld, const int32_t * to, int64_t to_ld, const int32_t * index,
                                 int64_t index_ld, const int32_t * count, int max_count, void * stream);

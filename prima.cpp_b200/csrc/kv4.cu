@@ -268,10 +268,10 @@ __global__ void __launch_bounds__(256) k_kv4_copy_pages(uint8_t * pages, int64_t
 constexpr int KM_CHUNKS = 8;
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_compact(uint8_t * pages, int64_t n_pages, int chunks, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to,
-                                                     const int32_t * index, int64_t ld_index, const int32_t * count) {
+                                                     const int32_t * index, int64_t ld_index, const int32_t * count, int most) {
     constexpr int NB = D / 32, WORDS = D / 64;                           // 32-bit words of an eighth of a row
     const int s = blockIdx.z, i = blockIdx.x * 32 + (threadIdx.x >> 3), l = threadIdx.x & 7;
-    if (i >= count[s]) return;
+    if (i >= min(count[s], most)) return;                                // (the grid is rounded up: a count may say more than there is)
     const int32_t c = index[s * ld_index + i];
     if (c < 0 || c / KV4_CELLS >= ld_from || i / KV4_CELLS >= ld_to) return;
     const int64_t a = from[s * ld_from + c / KV4_CELLS], b = to[s * ld_to + i / KV4_CELLS];
@@ -370,9 +370,9 @@ int launch_kv4_copy_pages(uint8_t * pages, int64_t page_bytes, const int32_t * s
 
 int launch_kv4_compact(uint8_t * pages, int64_t n_pages, int rows, int D, int n_seq, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to, const int32_t * index,
                        int64_t ld_index, const int32_t * count, int most, cudaStream_t st) {
-    const dim3 grid((unsigned) ((most + 31) / 32), (unsigned) ((rows + KM_CHUNKS - 1) / KM_CHUNKS), (unsigned) n_seq);
-    if (D == 128) k_kv4_compact<128><<<grid, 256, 0, st>>>(pages, n_pages, rows, from, ld_from, to, ld_to, index, ld_index, count);
-    else k_kv4_compact<64><<<grid, 256, 0, st>>>(pages, n_pages, rows, from, ld_from, to, ld_to, index, ld_index, count);
+    const dim3 grid((unsigned) (((int64_t) most + 31) / 32), (unsigned) ((rows + KM_CHUNKS - 1) / KM_CHUNKS), (unsigned) n_seq);
+    if (D == 128) k_kv4_compact<128><<<grid, 256, 0, st>>>(pages, n_pages, rows, from, ld_from, to, ld_to, index, ld_index, count, most);
+    else k_kv4_compact<64><<<grid, 256, 0, st>>>(pages, n_pages, rows, from, ld_from, to, ld_to, index, ld_index, count, most);
     return (int) cudaGetLastError();
 }
 

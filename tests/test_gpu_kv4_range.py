@@ -1,0 +1,61 @@
+"""The 4-bit cache's operators at the ends of their ranges: counts and lengths that say too much, weights and values many binary orders apart, long prompts, buffers that interleave."""
+import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+import ref_kv4 as R
+from gpu_util import ptr
+from test_gpu_kv4 import MIXED, TORCH, Attn, random_pages
+
+
+pytestmark = pytest.mark.gpu
+BOTH = pytest.mark.parametrize("q,kv", [([1, 3, 1], [300, 64, 1000]), ([200, 40, 1], [400, 90, 70])], ids=["tokens", "prompts"])
+# The root mean square of a rounding, relative to numbers whose logarithms are spread evenly over a binary order: half a step h is h / m of a number m of [1, 2), even over -h .. h, and
+# the mean of 1 / m^2 is 3 / (8 ln 2): h * sqrt(0.541 / 3) = 0.4246 h.  16 bits round a weight, with few rows its product with a scale too, and the output; errors of weights add up over
+# cells as the (random) values do, so relative to the output's norm they are what they are relative to a weight.
+RMS = {"f16": 0.4246 * 2.0 ** -11 * 3 ** 0.5, "bf16": 0.4246 * (2 * 2.0 ** -22 + 2.0 ** -16) ** 0.5}
+ON_THE_WHOLE = {t: 1.1 * r for t, r in RMS.items()}      # a tenth for samples of some thousand numbers
+
+
+def result(a):
+    """(output, what it should be) of the rows of sequences"""
+    torch.cuda.synchronize()
+    assert a.lib.c.pb200_aborted() == 0
+    want = a.want()[0]
+    got = a.out[:, :a.heads * a.dim].double().cpu().numpy().reshape(want.shape)
+    mine = ~np.isnan(want[:, 0, 0])
+    return got[mine], want[mine]
+
+
+def off(got, want):
+    return np.linalg.norm(got - want) / np.linalg.norm(want)
+
+
+# ---------------------------------------------------------------------------------------------------------------- counts and lengths
+@pytest.mark.parametrize("layers,kv_heads,dim", [(1, 1, 64), (2, 3, 128)])
+def test_compaction_stops_at_its_most(pkg, lib, cuda, layers, kv_heads, dim):
+    """Counts above max_count are max_count: the next row's indices, and what lies behind the last row, move nothing (what a count let through would still be cells of the cache)."""
+    rng = np.random.default_rng(40)
+    n, most, per = 4, 100, 3
+    pages_np = random_pages(rng, 2 * n * per, layers * kv_heads, dim)
+    order = rng.permutation(2 * n * per).astype(np.int32)
+    table, to = order[:n * per].reshape(n, per), order[n * per:].reshape(n, per)
+    index = rng.integers(0, per * 64, n * most + 64).astype(np.int32)          # 64 behind the last row
+    count = np.array([120, 100, 2 ** 31 - 1, -7], np.int32)
+    pages = torch.from_numpy(pages_np).cuda()
+    cache = pkg.Kv4Cache(pages.data_ptr(), len(pages_np), layers, kv_heads, dim)
+    dev = [torch.from_numpy(np.ascontiguousarray(x)).cuda() for x in (table, to, index, count)]
+    lib.check(lib.c.pb200_kv4_compact(C.byref(cache), n, ptr(dev[0]), per, ptr(dev[1]), per, ptr(dev[2]), most, ptr(dev[3]), most, None))
+    torch.cuda.synchronize()
+    old, want = R.unpack(pages_np, dim), R.unpack(pages_np, dim)
+    for s in range(n):
+        for i in range(max(0, min(int(count[s]), most))):
+            c = index[s * most + i]
+            for w, o in zip(want, old):
+                w[to[s, i // 64], :, i % 64] = o[table[s, c // 64], :, c % 64]
+    assert all(np.array_equal(g, w) for g, w in zip(R.unpack(pages.cpu().numpy(), dim), want))
