@@ -63,7 +63,7 @@ template <int D> struct KpSmem {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
     KpPiece piece[2];          // the one at hand and the next
     float mult[2 * KP_TILE], other[2][KP_TILE];
-    int cell[4][2];            // first cells of a key tile's pages (of none: beyond everything)
+    int cell[4][2];            // first cells of a key tile's pages (of none: -1)
     uint32_t tmem_base;
     int abort, more[2];
     KpPlan plan;
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 const uint32_t u = tiles + (uint32_t) j;
                 const int st = (int) (u & 1);
                 const uint8_t * third = chunk_of(j + 2);
-                if (t6 == 0) S.cell[u & 3][half] = now ? kv4_page_index(P.q, 2 * (P.a + j) + half) * KV4_CELLS : 0x7fffff00;
+                if (t6 == 0) S.cell[u & 3][half] = now ? kv4_page_index(P.q, 2 * (P.a + j) + half) * KV4_CELLS : -1;
                 if (u >= 2) mbar_wait(&S.k_empty[st], (u / 2 - 1) & 1, cta_abort, W.abort_flag);
                 {
                     const uint32_t odd = t6 & 1 ? 0x3232u : 0x1010u;
@@ -468,14 +468,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     fence_after();
                     // (four of them: written for tile j + 4 behind the scores of j + 2, which come behind the weights of j)
                     const int c0 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][0], c1 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][1];
-                    const bool whole = c1 <= g_lo - 63 && c0 <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
+                    const bool whole = min(c0, c1) >= 0 && max(c0, c1) <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
                     if (!whole) {   // a score that is not seen is -inf: in its place, ahead of the passes over the tile
                         const int from = A.window > 0 ? max(0, pos - A.window + 1) : 0;
 #pragma unroll 1
                         for (int h = 0; h < 4; h++) {
-                            const int base = (h < 2 ? c0 : c1) + 32 * (h & 1);
+                            const int page = h < 2 ? c0 : c1, base = page + 32 * (h & 1);
                             auto below = [&](int cell) { const int k = cell - base; return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };     // cells in front of it
-                            const uint32_t seen = pos < 0 || base > pos ? 0u : below(pos + 1) & (~below(from) | below(A.first));
+                            const uint32_t seen = page < 0 || base > pos ? 0u : below(pos + 1) & (~below(from) | below(A.first));
                             TMEM_LD32(mine + 32 * h, t0);
                             TMEM_ARRIVED(t0);
 #pragma unroll

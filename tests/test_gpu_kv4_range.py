@@ -59,3 +59,21 @@ def test_compaction_stops_at_its_most(pkg, lib, cuda, layers, kv_heads, dim):
             for w, o in zip(want, old):
                 w[to[s, i // 64], :, i % 64] = o[table[s, c // 64], :, c % 64]
     assert all(np.array_equal(g, w) for g, w in zip(R.unpack(pages.cpu().numpy(), dim), want))
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("q", [[1, 2], [200, 70]], ids=["tokens", "prompts"])
+@pytest.mark.parametrize("pages", [1, 3, 4])
+@pytest.mark.parametrize("window,back", [(0, 0), (0, 130), (2 ** 31 - 400, 0)])
+def test_lengths_next_to_the_largest_behind_a_short_table(pkg, lib, cuda, type_, q, pages, window, back):
+    """Positions up to 2^31 - 2: cells behind the table, and pages that are none, are seen by nobody, whatever the position."""
+    a = Attn(pkg, lib, 41, type_, 8, 2, 128, q, [64 * pages] * 2, window=window, extra_cols=0)
+    if pages > 1:
+        a.table_np[1, 1] = -1
+    a.kv_np = np.array([2 ** 31 - 1 - back, 2 ** 31 - 1], np.int32)
+    a.upload()
+    a.call()
+    a.check()
+    got, want = result(a)
+    if want.any():
+        assert off(got, want) <= (1e-5 if type_ == "f32" else ON_THE_WHOLE[type_])
