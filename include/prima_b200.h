@@ -149,7 +149,8 @@ PB200_API size_t pb200_kv4_page_bytes(int n_layer, int n_head_kv, int head_dim);
 /* The rows of n_tokens tokens, one launch: queries and keys normed per head (x / sqrt(mean(x^2) + eps) * weight, weights f32 [head_dim] at 16 bytes, either may be NULL),
  * rotated by the token's position, queries to q_out (which may be q), keys and values into cell cells[t] = page * 64 + cell of the layer (negative: not stored; no two tokens
  * have the same).  type: PB200_TYPE_F32, F16 or BF16 of q, q_out, k and v; rows of ld* numbers (a multiple of 4), heads next to each other, at 4 numbers' boundaries.
- * n_head 0: keys and values alone.  q_out lies over q or over nothing that the call reads. */
+ * n_head 0: keys and values alone.  q_out lies over q (with its stride) or over nothing that the call reads; rows may lie between each other where strides are equal, as in a joint
+ * buffer (ranges of other strides have to lie apart). */
 PB200_API int pb200_kv4_append(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * q_out, int64_t ldq_out, const void * k, int64_t ldk,
                                const void * v, int64_t ldv, int64_t n_tokens, int n_head, const int64_t * cells, const int32_t * pos, const float * q_norm, const float * k_norm,
                                float eps, const pb200_rope_args * rope, void * stream);
@@ -159,7 +160,7 @@ PB200_API int pb200_kv4_load(const pb200_kv4_cache * cache, int layer, int type,
  * stands at position p = kv_len[s] - n + i and sees the cells 0 .. p; with window > 0 those of the last `window` positions and the first keep_first.  Cell j is cell j % 64 of
  * page table[s * table_ld + j / 64].  out[t][head] = sum of softmax(scale q k) v over what it sees, zeros if that is nothing; rows outside q_start[0] .. q_start[n_seq]-1, and
  * queries beyond the first max_q of a sequence, stay as they were.  n_tokens: rows of q and out; max_q: the most queries of one sequence.  q, out: rows of [n_head][head_dim] of the
- * type as in pb200_kv4_append, not overlapping.  q, softmax weights and sums have 22 bits and more with F32; with F16 and BF16 weights are rounded to f16, and
+ * type as in pb200_kv4_append, whose rows may lie between each other in the same way, but have no number in common.  q, softmax weights and sums have 22 bits and more with F32; with F16 and BF16 weights are rounded to f16, and
  * what is below 2^-38 of the largest value in a sequence's pages is lost.
  * PB200_ENOTSUP where pages, heads and tiles of rows do not fit 31 bits.
  * ws: pb200_kv4_attn_workspace_bytes, zeroed once by the caller, for calls that follow one another (one per stream, also of graphs that may run at the same time). */

@@ -31,7 +31,15 @@ Kv4 layer_of(const pb200_kv4_cache * c, int layer) {
 int elem_bytes(int type) { return type == PB200_TYPE_F32 ? 4 : type == PB200_TYPE_F16 || type == PB200_TYPE_BF16 ? 2 : 0; }
 // rows of n numbers of a type: four at a time are loaded and stored
 bool rows_ok(const void * p, int64_t ld, int64_t n, int eb) { return p && ((uintptr_t) p & (4 * eb - 1)) == 0 && ld >= n && ld % 4 == 0; }
-bool overlap(const void * a, int64_t na, const void * b, int64_t nb) { return (uintptr_t) a < (uintptr_t) b + nb && (uintptr_t) b < (uintptr_t) a + na; }
+// n rows of wa numbers every lda, n of wb every ldb (as rows_ok has them): whether they have a number in common.  With equal strides rows may lie between each other, as in a joint buffer
+// (row j of b against row i of a: what counts is j - i); with others, ranges have to lie apart.
+bool overlap(const void * a, int64_t lda, int64_t wa, const void * b, int64_t ldb, int64_t wb, int64_t n, int eb) {
+    const int64_t at = (int64_t) ((uintptr_t) b - (uintptr_t) a), ld = lda * eb, end_a = (n - 1) * ld + wa * eb, end_b = (n - 1) * ldb * eb + wb * eb;
+    if (end_a <= at || at + end_b <= 0) return false;
+    if (lda != ldb) return true;
+    const int64_t in = (at % ld + ld) % ld;     // where rows of b begin in a's stride
+    return in < wa * eb || in + wb * eb > ld;
+}
 
 }  // namespace
 
@@ -53,8 +61,8 @@ int pb200_kv4_append(const pb200_kv4_cache * c, int layer, int type, const void 
     if (n_head > 0 && (!rows_ok(q, ldq, n_head * D, eb) || !rows_ok(q_out, ldq_out, n_head * D, eb))) return PB200_EINVAL;
     if ((((uintptr_t) q_norm | (uintptr_t) k_norm) & 15) || ((q_norm || k_norm) && !(eps >= 0.f))) return PB200_EINVAL;
     if (n_head > 0 && n_tokens > 0) {   // rows that are read must not be another row's result: in place, or apart
-        const int64_t nq = ((n_tokens - 1) * ldq + n_head * D) * eb, no = ((n_tokens - 1) * ldq_out + n_head * D) * eb;
-        if (overlap(q, nq, q_out, no) && !(q == q_out && ldq == ldq_out)) return PB200_EINVAL;
+        const auto over = [&](const void * p, int64_t ld, int64_t n) { return overlap(p, ld, n, q_out, ldq_out, n_head * D, n_tokens, eb); };
+        if ((over(q, ldq, n_head * D) && !(q == q_out && ldq == ldq_out)) || over(k, ldk, kd) || over(v, ldv, kd)) return PB200_EINVAL;
     }
     Kv4Rope r{};
     if (rope && rope->n_dims != 0) {
@@ -115,7 +123,7 @@ int pb200_kv4_attn(const pb200_kv4_cache * c, int layer, int type, const void * 
     const double pages = (double) n_seq * (double) std::min<int64_t>(table_ld, INT32_MAX / PB200_KV4_CELLS) * c->n_head_kv * std::ceil(rows / 8);
     const double tiles = ((double) n_tokens * group / 128 + n_seq) * c->n_head_kv;
     if (pages >= 2147483648.0 || tiles >= 2147483648.0 || n_tokens * group >= 2147483648.0) return PB200_ENOTSUP;
-    if (overlap(q, ((n_tokens - 1) * ldq + n_head * D) * eb, out, ((n_tokens - 1) * ldo + n_head * D) * eb)) return PB200_EINVAL;
+    if (overlap(q, ldq, n_head * D, out, ldo, n_head * D, n_tokens, eb)) return PB200_EINVAL;
     const Kv4Attn a{layer_of(c, layer), q, ldq, out, ldo, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};
     int launches = 0;
     const int rc = launch_kv4_attn(a, c->head_dim, type, ws, (cudaStream_t) stream, launches);

@@ -77,3 +77,39 @@ def test_lengths_next_to_the_largest_behind_a_short_table(pkg, lib, cuda, type_,
     got, want = result(a)
     if want.any():
         assert off(got, want) <= (1e-5 if type_ == "f32" else ON_THE_WHOLE[type_])
+
+
+# ---------------------------------------------------------------------------------------------------------------- buffers and graphs
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@BOTH
+def test_queries_and_results_in_one_buffer(pkg, lib, cuda, type_, q, kv):
+    """Rows of queries with rows of results between them: ranges interleave, rows do not."""
+    a = Attn(pkg, lib, 50, type_, 8, 2, 128, q, kv)
+    alone = a.call(torch.full_like(a.out, 7.0))
+    joint = torch.full((a.tokens, 2 * 1024 + 8), 7.0, dtype=TORCH[type_], device="cuda")
+    joint[:, :1024] = a.q
+    a.q, a.ldq, a.ldo, out = joint, joint.shape[1], joint.shape[1], joint[:, 1024:]
+    queries = joint[:, :1024].clone()
+    a.call(out)
+    torch.cuda.synchronize()
+    assert torch.equal(joint[:, 1024:2048], alone) and torch.equal(joint[:, :1024], queries) and bool((joint[:, 2048:] == 7.0).all())
+
+
+@pytest.mark.parametrize("tokens", [5, 700])
+def test_append_with_its_results_in_the_same_rows(pkg, lib, cuda, tokens):
+    """Rows of queries, keys, values and turned queries: what goes out lies between what is read."""
+    H, HK, D, P = 4, 2, 128, -(-tokens // 64)
+    x = torch.randn(tokens, (2 * H + 2 * HK) * D, device="cuda").to(torch.bfloat16)
+    before, W, e = x.clone(), x.shape[1], x.element_size()
+    cells, pos = torch.arange(tokens, device="cuda"), torch.arange(tokens, dtype=torch.int32, device="cuda")
+    rope = pkg.RopeArgs(D, 2, 4096, 10000.0, 1.0, 0.0, 1.0, 32.0, 1.0, None)
+    got = []
+    for apart in (False, True):
+        pages = torch.zeros(P, HK, R.chunk_bytes(D), dtype=torch.uint8, device="cuda")
+        cache, q_out = pkg.Kv4Cache(pages.data_ptr(), P, 1, HK, D), torch.zeros(tokens, H * D, dtype=torch.bfloat16, device="cuda")
+        at = [C.c_void_p(x.data_ptr() + i * D * e) for i in (0, H, H + HK, H + 2 * HK)]
+        lib.check(lib.c.pb200_kv4_append(C.byref(cache), 0, 30, at[0], W, ptr(q_out) if apart else at[3], H * D if apart else W, at[1], W, at[2], W, tokens, H, ptr(cells), ptr(pos), None, None,
+                                         0.0, C.byref(rope), None))
+        torch.cuda.synchronize()
+        got.append((q_out if apart else x[:, (H + 2 * HK) * D:].clone(), pages))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and torch.equal(x[:, :(H + 2 * HK) * D], before[:, :(H + 2 * HK) * D])

@@ -148,3 +148,24 @@ def test_copies_have_no_order(lib, cache):
                                (1, BASE, 1, BASE, 1, BASE, 1, None, 1), (1, BASE, 1, BASE, 1, BASE, 1, BASE, -1)], ids=str)
 def test_compact_refuses(lib, cache, a):
     assert lib.c.pb200_kv4_compact(C.byref(cache), *a, None) == -1
+
+
+def test_rows_may_lie_between_each_other(lib, pkg, cache):
+    """Refused where a row that is read and one that is written have a number in common, and with equal strides only there (what is not refused ends in a launch without a GPU)."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("would run on the GPU")
+    at, n = 4 << 20, 3
+    for ld in (512, 520, 1024, 1536):
+        for off in sorted({x for r in range(-n - 1, n + 2) for x in (r * ld, r * ld - 512, r * ld + 512, r * ld - 508, r * ld + 508, r * ld + ld // 8 * 4)}):
+            common = any(abs(off + (j - i) * ld) < 512 for i in range(n) for j in range(n))
+            rc = lib.c.pb200_kv4_attn(*attn_args(cache, q=at, ldq=ld, out=at + 4 * off, ldo=ld))
+            assert (rc == -1) == common and rc != 0, (ld, off)
+            for what in ("k", "v"):
+                rc = lib.c.pb200_kv4_append(*append_args(cache, None, q=1 << 30, ldq=ld, **{what: at, "ld" + what: ld}, q_out=at + 4 * off, ldqo=ld))
+                assert (rc == -1) == common and rc != 0, (what, ld, off)
+            rc = lib.c.pb200_kv4_append(*append_args(cache, None, q=at, ldq=ld, q_out=at + 4 * off, ldqo=ld))
+            assert (rc == -1) == (common and off != 0) and rc != 0, (ld, off)
+    # other strides: ranges apart; a single row has none
+    assert lib.c.pb200_kv4_attn(*attn_args(cache, q=at, ldq=1024, out=at + 4 * 512, ldo=2048)) == -1
+    assert lib.c.pb200_kv4_attn(*attn_args(cache, q=at, ldq=1024, out=at + 4 * 512, ldo=2048, n_tokens=1)) not in (0, -1, -3)
