@@ -770,21 +770,20 @@ cudaError_t ensure_dyn_smem(FuncAttrCache & c, const void * fn, size_t bytes, bo
     c.bytes[dev] = bytes;
     return cudaSuccess;
 }
-// process-wide abort flag of the wait watchdogs: pinned, mapped host memory (UVA: same address on every device)
-static int * g_abort_flag = nullptr;
+// process-wide abort flag of the wait watchdogs: pinned, mapped host memory (UVA: same address on every device).  The call that makes it may be one that a stream is capturing: an allocation
+// would invalidate the capture in any but the relaxed mode, and is no part of it.
 int * abort_flag() {
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
+    static int * const flag = [] {
         void * p = nullptr;
-        if (cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
-            g_abort_flag = (int *) p;
-            *g_abort_flag = 0;
-        } else {
-            cudaGetLastError();
-        }
-    }
-    return g_abort_flag;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+        if (cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) p = nullptr;
+        if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+        if (p) *(int *) p = 0;
+        else cudaGetLastError();
+        return (int *) p;
+    }();
+    return flag;
 }
 int check_clear_abort() {
     int * f = abort_flag();

@@ -113,3 +113,29 @@ def test_append_with_its_results_in_the_same_rows(pkg, lib, cuda, tokens):
         torch.cuda.synchronize()
         got.append((q_out if apart else x[:, (H + 2 * HK) * D:].clone(), pages))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and torch.equal(x[:, :(H + 2 * HK) * D], before[:, :(H + 2 * HK) * D])
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+import torch
+import pkgload
+from test_gpu_kv4 import Attn
+pkg = pkgload.load()
+lib = pkg.Lib.get()
+a = Attn(pkg, lib, 51, "f32", 8, 2, 128, [1, 200], [300, 400])
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a.call()
+for _ in range(2):
+    a.out.fill_(7.0)
+    g.replay()
+    a.check()
+print("as it should be")
+"""
+
+
+def test_first_call_of_a_process_is_captured(cuda):
+    """Nothing has to be called once in front of a capture."""
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=str(Path(__file__).resolve().parent.parent))], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "as it should be" in r.stdout, r.stdout[-1000:] + r.stderr[-3000:]
