@@ -2,7 +2,7 @@
 //
 // Mathematics.  S = Q K^T, P = 2^(S c - reference), O += P V, divided by the row's sum at the end.  Keys and values are f16 numbers exactly; queries become f16 (a row by a power of two:
 // 16-bit ones exactly, F32 as two numbers, 22 bits), weights f16 (F32: two numbers).  A row's reference is the largest score of its first tile; it moves only where a
-// score lies beyond it by more than 2^8, and then its sum and O are scaled.
+// score lies beyond it (16 bits: by more than 2^6), and then its sum and O are scaled.
 //
 // Work.  An item is a (sequence, kv head, tile of query rows: tokens x heads of the group).  Two softmax groups keep the tensor cores busy in turns: with 16 bits each has 128 rows, which
 // share each expanded key tile; with F32 both have the same 128 rows and every other key tile, and their sums are joined at the end.  Key tiles are two pages.  CTAs (one to an SM) take
@@ -35,7 +35,10 @@ namespace {
 
 constexpr int KP_THREADS = 13 * 32, KP_TILE = 128, KP_BLOCK = 16384;   // a block: 128 rows of 64 entries
 constexpr int KP_CUT_SEQ = 32, KP_CUT_TILES = KV4_MAX_CTAS + KP_CUT_SEQ;     // where long items may be cut: sequences, row tiles
-constexpr float KP_UP = 6.f;            // weights are up to 2^(8 + 6)
+// A row's reference may fall behind its largest score by 2^SLACK; a weight is 2^(15 - SLACK) at its reference, so 2^15 at most, and what f16 (F32: its low part) rounds off is 2^(SLACK - 40) of the
+// row's largest weight (F32, whose references are whole numbers: 2^-39).  8, as it was with 2^6 in front of weights, lost small ones beside a large one (of weights 2^-24 of it, 2e-3); us, 512
+// tokens behind 8000 in f16, 8 / 6 / 5 / 4: 110 / 110 / 111 / 112.
+template <typename T> constexpr float kp_slack() { return std::is_same<T, float>::value ? 0.f : 6.f; }
 template <typename T> constexpr int kp_rows() { return std::is_same<T, float>::value ? KP_TILE : 2 * KP_TILE; }   // of an item
 
 struct KpPiece {               // what a ticket stands for
@@ -238,6 +241,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
     constexpr bool F32 = std::is_same<T, float>::value;
     constexpr int ROWS = kp_rows<T>(), NB = D / 32;
+    constexpr float SLACK = kp_slack<T>(), UP = 15.f - SLACK;
     extern __shared__ uint8_t smem_raw[];
     KpSmem<D> & S = *reinterpret_cast<KpSmem<D> *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
@@ -497,8 +501,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
 #pragma unroll
                         for (int i = 0; i < 32; i++) tm[i & 3] = fmaxf(tm[i & 3], x[i]);
                     }
-                    const float top = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * c;
-                    const bool move = top > m + 8.f;               // (the first: m is -inf)
+                    // rounded upwards, so that weights stay within 2^15 however large scores are.  F32: to a whole number: what weights, sums and parts are scaled by are powers of two then
+                    float top = __fmul_ru(fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])), c);
+                    if (F32) top = ceilf(top);
+                    const bool move = top > __fadd_rd(m, SLACK);   // (the first: m is -inf)
                     if (__any_sync(0xffffffffu, move)) {
                         const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2(m - top);
                         if (move) m = top;
@@ -515,7 +521,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             }
                         }
                     }
-                    const float off = m == -INFINITY ? 0.f : KP_UP - m;
+                    const float off = m == -INFINITY ? 0.f : __fsub_rd(UP, m);
                     float e4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int h = 0; h < 4; h++) {

@@ -41,7 +41,8 @@ constexpr int KR_WARPS = 12, KR_THREADS = 32 * KR_WARPS;
 // 1000 13.6 / 15.2 / 20.1, behind 4000 17.1 / 17.9 / 19.5
 constexpr int KR_LEAST = 4;
 template <int D> constexpr int kr_stages() { return D == 128 ? 2 : 4; }
-constexpr int KR_UP = 12;   // F32: weights are 2^12 larger than exp(score - maximum): those of 2^-26 are normal f16 numbers
+// Weights are 2^15 times 2^(score - reference), the largest 2^15 (F32: above 2^14): those of 2^-28 of it are normal f16 numbers, and what rounds off below them is 2^-40 (F32: of low parts, 2^-39)
+constexpr int KR_UP = 15;
 
 // a part of an item: sums of 2^(score - m) v, and of the weights
 template <int D> struct KrPart { float o[KR_ROWS][D]; float m[KR_ROWS], l[KR_ROWS]; };
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
         // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1 (16 bits: times 2^-24, and 2^-20 the odd ones)
         float o[NB][2][4], less[4] = {0.f, 0.f, 0.f, 0.f};     // less: 16 bits: row b: - 8 * 2^-24 times the sum of block b's scaled weights
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        int up = F32 ? KR_UP : 15;                      // weights are exp(score - maximum) * 2^up
+        int up = KR_UP;                                 // weights are 2^(score - reference + up)
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -452,7 +453,10 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 4));
                     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 8));
                     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 16));
-                    mx[k] = a * mult[k];
+                    // rounded upwards, so that weights stay within 2^up however large scores are.  F32: to a whole number: what weights, sums and parts are scaled by are powers of two then
+                    // (16 bits: the largest weight is a power of two, which f16 holds exactly; rounded, errors are a third larger)
+                    mx[k] = __fmul_ru(a, mult[k]);
+                    if constexpr (F32) mx[k] = ceilf(mx[k]);
                 }
                 int to = up;
                 if constexpr (!F32) {   // lane: the scales of cells 2 lane, 2 lane + 1
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                         }
                     }
                 }
-                const float off[2] = {m[0] == -INFINITY ? 0.f : (float) up - m[0], m[1] == -INFINITY ? 0.f : (float) up - m[1]};
+                const float off[2] = {m[0] == -INFINITY ? 0.f : __fsub_rd((float) up, m[0]), m[1] == -INFINITY ? 0.f : __fsub_rd((float) up, m[1])};
                 // weights, transposed: lane: row g, cells 8 x + 2 c, + 1 (x: eights of the page)
                 uint32_t pf[LO][8];
 #pragma unroll

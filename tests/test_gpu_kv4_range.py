@@ -79,6 +79,33 @@ def test_lengths_next_to_the_largest_behind_a_short_table(pkg, lib, cuda, type_,
         assert off(got, want) <= (1e-5 if type_ == "f32" else ON_THE_WHOLE[type_])
 
 
+# ---------------------------------------------------------------------------------------------------------------- magnitudes
+@pytest.mark.parametrize("gap", [12, 16, 20, 24, 28])
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@BOTH
+def test_a_cell_ahead_of_all_that_has_no_value(pkg, lib, cuda, type_, gap, q, kv):
+    """The first cell's score is `gap` binary orders above the others' and its value is zero: what comes out is the others'.  A weight is off by its own rounding or by 2^-39 of the largest
+    (prompts of 16 bits, whose reference may fall behind the largest score by 2^6: 2^-34) at most, evenly spread (root mean square: a sqrt(3)-th); scores of gap * ln 2 by two roundings of 32
+    bits."""
+    a = Attn(pkg, lib, 42, type_, 8, 2, 128, q, kv, scale=1.0)
+    rng = np.random.default_rng(43)
+    k, v = rng.standard_normal((2, len(a.pages_np), 2, 64, 128))
+    k[..., 0] = 0.0
+    for s in range(len(kv)):
+        k[a.table_np[s, 0], :, 0], v[a.table_np[s, 0], :, 0] = 0.0, 0.0
+        k[a.table_np[s, 0], :, 0, 0] = gap * np.log(2.0)
+    a.pages_np = R.pack(*R.quantize(k), *R.quantize(v))
+    a.q *= 0.05
+    a.q.view(a.tokens, 8, 128)[..., 0] = 1.0
+    a.q_np = a.q.double().cpu().numpy()
+    a.upload()
+    a.call()
+    got, want = result(a)
+    few = 1.2 / 3 ** 0.5
+    tol = 1e-6 + gap * np.log(2.0) * 2.0 ** -23 if type_ == "f32" else ON_THE_WHOLE[type_]
+    assert off(got, want) <= tol + few * 2.0 ** (gap - (34 if type_ != "f32" and sum(q) > 10 else 39))
+
+
 # ---------------------------------------------------------------------------------------------------------------- buffers and graphs
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 @BOTH
