@@ -6,7 +6,7 @@
 namespace pb {
 
 constexpr int KV4_MAX_CTAS = 152;      // of a launch: the workspace has parts by CTA and warp
-constexpr int KV4_SLOTS = 288;         // and by piece of a cut item: these are 9 / 5 of the CTAs at most
+constexpr int KV4_SLOTS = 2 * KV4_MAX_CTAS;   // and by piece of a cut item: these are 9 / 5 of the CTAs at most (F32's have half of their rows: the other half of two is a CTA's)
 constexpr int KV4_COUNTERS = 16384;    // in front of them
 
 // A sequence: its queries' rows, and the pages that any of them sees: the first `keep`, then those from page `from` on.  At least one page, so that rows which see
@@ -56,6 +56,9 @@ __device__ __forceinline__ int kv4_page(const Kv4Attn & A, const Kv4Seq & q, int
     const int id = A.table[s * A.table_ld + at];
     return id >= 0 && id < A.cache.n_pages ? id : -1;
 }
+
+// of a part with maximum m and sum l of weights, where all parts' maximum is top (a row that is no number has no maximum)
+__device__ __forceinline__ float part_factor(float m, float l, float top) { return m == -INFINITY ? (l == l ? 0.f : 1.f) : ex2(m - top); }
 
 __device__ __forceinline__ void tmem_alloc(uint32_t * at, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)), "r"(columns) : "memory");

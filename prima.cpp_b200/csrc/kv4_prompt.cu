@@ -37,8 +37,11 @@ constexpr int KP_THREADS = 13 * 32, KP_TILE = 128, KP_BLOCK = 16384;   // a bloc
 constexpr int KP_CUT_SEQ = 32, KP_CUT_TILES = KV4_MAX_CTAS + KP_CUT_SEQ;     // where long items may be cut: sequences, row tiles
 // A row's reference may fall behind its largest score by 2^SLACK; a weight is 2^(15 - SLACK) at its reference, so 2^15 at most, and what f16 (F32: its low part) rounds off is 2^(SLACK - 40) of the
 // row's largest weight (F32, whose references are whole numbers: 2^-39).  8, as it was with 2^6 in front of weights, lost small ones beside a large one (of weights 2^-24 of it, 2e-3); us, 512
-// tokens behind 8000 in f16, 8 / 6 / 5 / 4: 110 / 110 / 111 / 112.
+// tokens behind 8000 in f16, 8 / 6 / 5 / 4: 110 / 110 / 111 / 112; the ragged case in F32, 4 / 2 / 0: 75 / 77 / 77.
 template <typename T> constexpr float kp_slack() { return std::is_same<T, float>::value ? 0.f : 6.f; }
+// F32: key tiles of a group (512 cells) whose products add up in tensor memory, before they go to a sum in 32 bits: the tensor core cuts off what it adds to.  Error, 8 x 512 queries of 4096 cells
+// (elementary 32-bit operations 1.3e-6), and us: 2 1.0e-6, 343; 3 1.3e-6, 322; 4 1.6e-6, 302; 8 2.7e-6, 290; all of them 4.9e-6, 272.
+constexpr int KP_CHUNK = 4;
 template <typename T> constexpr int kp_rows() { return std::is_same<T, float>::value ? KP_TILE : 2 * KP_TILE; }   // of an item
 
 struct KpPiece {               // what a ticket stands for
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     for (int part = 0; part < (F32 ? 2 : 1); part++)
 #pragma unroll
                         for (int k = 0; k < 8; k++)
-                            mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * grp + 32 * (k >> 1) + 8 * (k & 1) + 16 * part, dv + k * (2048 >> 4), idesc_v, (uint32_t) ((i | part | k) != 0));
+                            mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * grp + 32 * (k >> 1) + 8 * (k & 1) + 16 * part, dv + k * (2048 >> 4), idesc_v, (uint32_t) (((F32 ? i % KP_CHUNK : i) | part | k) != 0));
                     if (last) mma_commit(&S.o_full[grp]);
                     if (F32 || grp == groups - 1) mma_commit(&S.v_empty[st]);
                 }
@@ -466,6 +469,20 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 float m = -INFINITY, l = 0.f;
                 float t[2][32];                                    // scores, 32 being worked on and 32 on their way
                 uint32_t * const t0 = reinterpret_cast<uint32_t *>(t[0]), * const t1 = reinterpret_cast<uint32_t *>(t[1]);
+                // F32: the sum of the chunks in front, a thread's own: numbers 4 k .. 4 k + 3 of row r at 128 k + r
+                float m_far = -INFINITY, l_far = 0.f, f_far = 0.f, f_own = 1.f;
+                float4 * const far = reinterpret_cast<float4 *>(reinterpret_cast<KpParts<D> *>(W.parts)->part[F32 ? 2 * blockIdx.x + grp : 0].o[KP_TILE]) + row;
+                auto ask_far = [&](int h) {                        // numbers h .. h + 31 of it -> t[1]
+#pragma unroll
+                    for (int k = 0; k < 8; k++) *reinterpret_cast<float4 *>(&t[1][4 * k]) = far[(h / 4 + k) * KP_TILE];
+                };
+                auto factors = [&] {                               // of the sum in front and of the chunk at hand, which become one
+                    const float top = fmaxf(m_far, m);
+                    f_far = part_factor(m_far, l_far, top);
+                    f_own = part_factor(m, l, top);
+                    l_far = l_far * f_far + l * f_own;
+                    m_far = top;
+                };
                 for (int j = F32 ? grp : 0, i = 0; j < n; j += F32 ? 2 : 1, i++) {
                     mbar_wait(&S.s_full[grp], (of_group[grp] + (uint32_t) i) & 1, cta_abort, W.abort_flag);
                     __syncwarp();
@@ -489,6 +506,21 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         }
                         tmem_wait_st();
                     }
+                    if (F32 && i > 0 && i % KP_CHUNK == 0) {       // a chunk ends
+                        factors();
+#pragma unroll 1
+                        for (int h = 0; h < D; h += 32) {
+                            TMEM_LD32(mine + 128 + h, t0);
+                            if (i > KP_CHUNK) ask_far(h);
+                            TMEM_ARRIVED(t0);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) t[0][k] = i > KP_CHUNK ? fmaf(t[1][k], f_far, t[0][k] * f_own) : t[0][k] * f_own;
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) far[(h + k) / 4 * KP_TILE] = make_float4(t[0][k], t[0][k + 1], t[0][k + 2], t[0][k + 3]);
+                        }
+                        m = -INFINITY;
+                        l = 0.f;
+                    }
                     float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     TMEM_LD32(mine, t0);
 #pragma unroll
@@ -509,7 +541,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2(m - top);
                         if (move) m = top;
                         l *= f;
-                        if (i > 0) {
+                        if (F32 ? i % KP_CHUNK != 0 : i > 0) {
 #pragma unroll
                             for (int h = 0; h < D; h += 32) {
                                 TMEM_LD32(mine + 128 + h, t1);
@@ -560,14 +592,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 __syncwarp();
                 fence_after();
                 constexpr int PIECE = 4, PIECES = D / PIECE;       // numbers to a piece; row r's pieces are rotated by r
-                float mine_f = 1.f, other = 0.f;                    // F32: factors of the groups' sums
+                float other = 0.f;                                  // F32: factor of the other group's sum
+                const bool folded = F32 && (n - grp + 1) / 2 > KP_CHUNK;
+                if (folded) {
+                    factors();
+                    m = m_far;
+                    l = l_far;
+                }
+                auto own_sum = [&](int h) {                         // numbers h .. h + 31 of the row's sum -> t[0]
+                    TMEM_LD32(mine + 128 + h, t0);
+                    if (folded) ask_far(h);
+                    TMEM_ARRIVED(t0);
+                    if (F32)
+#pragma unroll
+                        for (int k = 0; k < 32; k++) t[0][k] = folded ? fmaf(t[1][k], f_far, t[0][k] * f_own) : t[0][k] * f_own;
+                };
                 float * const os32 = reinterpret_cast<float *>(&S.q[0][0][0]) + row * D;
                 if (F32 && groups == 2) {                           // the second group's sums go to the first through the queries' memory
                     if (grp == 1) {
-#pragma unroll
+#pragma unroll 1
                         for (int h = 0; h < D; h += 32) {
-                            TMEM_LD32(mine + 128 + h, t0);
-                            TMEM_ARRIVED(t0);
+                            own_sum(h);
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) store4(os32 + ((h + i) / 4 + row) % PIECES * 4, make_float4(t[0][i], t[0][i + 1], t[0][i + 2], t[0][i + 3]));
                         }
@@ -577,12 +622,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     asm volatile("bar.sync 5, 256;" ::: "memory");
                     if (grp == 0) {
                         const float m2 = S.other[0][row], l2 = S.other[1][row], top = fmaxf(m, m2);
-                        // a row that is no number has no maximum
-                        const float f = m == -INFINITY ? (l == l ? 0.f : 1.f) : ex2(m - top);
-                        other = m2 == -INFINITY ? (l2 == l2 ? 0.f : 1.f) : ex2(m2 - top);
+                        const float f = part_factor(m, l, top);
+                        other = part_factor(m2, l2, top);
                         l = l * f + l2 * other;
                         m = top;
-                        mine_f = f;
+                        f_own *= f;
+                        f_far *= f;
                     }
                 }
                 if (!F32 || grp == 0) {
@@ -598,16 +643,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     T * os = reinterpret_cast<T *>(&S.q[F32 ? 0 : grp][0][0]) + row * D;
 #pragma unroll
                     for (int h = 0; h < D; h += 32) {
-                        TMEM_LD32(mine + 128 + h, t0);
-                        TMEM_ARRIVED(t0);
+                        own_sum(h);
                         if (F32 && groups == 2) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) {
                                 const float4 y = *reinterpret_cast<const float4 *>(os32 + ((h + i) / 4 + row) % PIECES * 4);
-                                t[0][i] = t[0][i] * mine_f + y.x * other;
-                                t[0][i + 1] = t[0][i + 1] * mine_f + y.y * other;
-                                t[0][i + 2] = t[0][i + 2] * mine_f + y.z * other;
-                                t[0][i + 3] = t[0][i + 3] * mine_f + y.w * other;
+                                t[0][i] += y.x * other;
+                                t[0][i + 1] += y.y * other;
+                                t[0][i + 2] += y.z * other;
+                                t[0][i + 3] += y.w * other;
                             }
                         }
 #pragma unroll
@@ -679,7 +723,7 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
             float f = 0.f, fl = 0.f;
             if (i0 + lane < n) {
                 const float mi = parts[i0 + lane].m[r], li = parts[i0 + lane].l[r];
-                f = mi == -INFINITY ? (li == li ? 0.f : 1.f) : ex2(mi - top);     // a row that is no number has no maximum
+                f = part_factor(mi, li, top);
                 fl = li * f;
             }
             l += warp_sum(fl);

@@ -106,6 +106,43 @@ def test_a_cell_ahead_of_all_that_has_no_value(pkg, lib, cuda, type_, gap, q, kv
     assert off(got, want) <= tol + few * 2.0 ** (gap - (34 if type_ != "f32" and sum(q) > 10 else 39))
 
 
+# ---------------------------------------------------------------------------------------------------------------- long and mixed batches
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kv,beside", [(2130, 0), (2130, 33), (16130, 0), (16130, 33)])
+def test_prompts_in_f32_behind_many_cells(pkg, lib, cuda, dim, kv, beside):
+    """An error that does not grow with the length, also where items stay whole (more than 32 sequences): tensor cores cut off half a step of 2^-23 in the mean of what they add to, 64 times
+    (16 cells, high and low parts) before the sum goes to one of 32 bits, and that sum grows from nothing: 2 / 3 * 64 * 2^-24 = 2.5e-6; a score is added up in 16 such steps, 0.6e-6."""
+    a = Attn(pkg, lib, 48, "f32", 4, 1, dim, [130] + [1] * beside, [kv] + [0] * beside)
+    a.call()
+    a.check()
+    assert off(*result(a)) <= (2.5e-6 ** 2 + 0.6e-6 ** 2) ** 0.5
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,kv", [(40, 500), (200, 16000)])
+def test_tokens_in_f32_behind_many_cells(pkg, lib, cuda, dim, n, kv):
+    """The same for single tokens (which share their pages here), where a warp has up to 225 pages of a sequence: 16 cells are added up in 4 steps that cut off, their sums in 32 bits."""
+    a = Attn(pkg, lib, 52, "f32", 8, 8, dim, [n], [kv])
+    a.table_np, a.q_start_np, a.kv_np, a.max_q = np.repeat(a.table_np, n, 0), np.arange(n + 1, dtype=np.int32), np.full(n, kv, np.int32), 1
+    a.upload()
+    a.call()
+    torch.cuda.synchronize()
+    k, v = (torch.from_numpy(np.ascontiguousarray(x.transpose(1, 0, 2, 3).reshape(8, -1, dim)[:, :kv])).cuda() for x in R.unpack(a.pages_np[a.table_np[0, :-(-kv // 64)]], dim))
+    q = torch.from_numpy(a.q_np).cuda().view(n, 8, dim).transpose(0, 1)
+    want = torch.softmax(q @ k.transpose(1, 2) * a.scale, -1) @ v
+    assert off(a.out.double().view(n, 8, dim).transpose(0, 1).cpu().numpy(), want.cpu().numpy()) <= 1e-6
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [20, 40])
+def test_a_prompt_beside_many_tokens(pkg, lib, cuda, type_, tokens):
+    """Long items are cut with up to 32 sequences, and stay whole with more."""
+    a = Attn(pkg, lib, 49, type_, 8, 2, 128, [1] * tokens + [200] + [1], [100 + 30 * i for i in range(tokens)] + [6000, 77])
+    a.call()
+    a.check()
+    assert off(*result(a)) <= (3e-6 if type_ == "f32" else ON_THE_WHOLE[type_])
+
+
 # ---------------------------------------------------------------------------------------------------------------- buffers and graphs
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 @BOTH
