@@ -5,9 +5,12 @@
 // nibble further up, exactly.
 //   scores    with d a block's scale: q . k = sum over blocks b of d_b (sum_i q_i n_i - 8 sum_i q_i).  The sum over i is the product, which starts from what the 8 adds; scales go
 //             onto the block's sums in 32 bits.  Numbers of the upper nibble meet queries of a 16th.
-//   values    sum over cells of w d_b (n - 8): weights become the other operand transposed (movmatrix), times the scales of their cells, the sum of which times 8 is a product with
-//             constants.  The power of two by which weights are larger than exp(score - maximum) follows the largest scale seen, so that neither they nor small products leave f16.
-// With F32, queries and weights are two f16 numbers each (22 bits), and the 4-bit operand is made signed (and values scaled, exactly): products of n as it is, up to 15, lose 3e-6 to
+//   values    sum over cells of w d_b (n - 8): weights become the other operand transposed (movmatrix).  BF16: times the scales of their cells, the sum of which times 8 is a product with
+//             constants; the power of two by which weights are larger than 2^(score - reference) follows the largest scale seen, so that neither they nor small products leave f16.  That rounds a
+//             weight twice, an eighth of BF16's own rounding each.  F16 and F32: the 4-bit operand is made signed and scaled, exactly, and a weight is rounded once.  us, carried by the weights / by
+//             the values: bf16, 32 sequences 52 / 53, two long ones 57.6 / 62, 40 of 8192 cells over 8 heads 82 / 91; f16, 256 of 1000 to 3000 132 / 145, and errors 3.05e-4 / 2.6e-4 (elementary
+//             32-bit operations 2.1e-4, the output's rounding).
+// With F32, queries and weights are two f16 numbers each (22 bits), and keys are made signed, too: products of n as it is, up to 15, lose 3e-6 to
 // the tensor core's alignment of its 16 terms.  16-bit queries are one f16 number, exactly: a row is scaled by a power of two.
 // Softmax by running maximum and sum, per page of 64 cells.
 //
@@ -137,7 +140,7 @@ __device__ __forceinline__ T * kr_row(const Kv4Attn & A, const KrSegment & at, i
 template <typename T, int D>
 __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_constant__ Kv4Attn A, const __grid_constant__ KrWork W) {
     constexpr int NB = D / 32, STAGES = kr_stages<D>(), CHUNK = kv4_chunk_bytes(D);
-    constexpr bool F32 = std::is_same<T, float>::value;
+    constexpr bool F32 = std::is_same<T, float>::value, SCALED = std::is_same<T, __nv_bfloat16>::value;   // SCALED: weights carry the values' scales
     constexpr int LO = F32 ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     KrSmem<D> & S = *reinterpret_cast<KrSmem<D> *>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
@@ -369,8 +372,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             for (int k = 0; k < STAGES; k++) fetch(u0 + k);
         const int p_lo = q.p0 + row0 / A.group, p_hi = q.p0 + (row0 + rows - 1) / A.group;   // of the tile's rows
 
-        // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1 (16 bits: times 2^-24, and 2^-20 the odd ones)
-        float o[NB][2][4], less[4] = {0.f, 0.f, 0.f, 0.f};     // less: 16 bits: row b: - 8 * 2^-24 times the sum of block b's scaled weights
+        // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1 (SCALED: times 2^-24, and 2^-20 the odd ones)
+        float o[NB][2][4], less[4] = {0.f, 0.f, 0.f, 0.f};     // less: SCALED: row b: - 8 * 2^-24 times the sum of block b's scaled weights
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
         int up = KR_UP;                                 // weights are 2^(score - reference + up)
 #pragma unroll
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                     if constexpr (F32) mx[k] = ceilf(mx[k]);
                 }
                 int to = up;
-                if constexpr (!F32) {   // lane: the scales of cells 2 lane, 2 lane + 1
+                if constexpr (SCALED) {   // lane: the scales of cells 2 lane, 2 lane + 1
                     uint32_t w[NB], top = 0;
                     const uint8_t * src = vs + 4 * NB * lane;
                     if constexpr (NB == 4) *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(src);
@@ -484,7 +487,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                             o[b][h][0] *= f[0]; o[b][h][1] *= f[1];
                             o[b][h][2] *= f[0]; o[b][h][3] *= f[1];
                         }
-                        if (!F32 && b == 0) {
+                        if (SCALED && b == 0) {
                             less[0] *= f[0]; less[1] *= f[1];
                         }
                     }
@@ -526,7 +529,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                         uint32_t u[2];   // of an eight: numbers of the two cells
 #pragma unroll
                         for (int k = 0; k < 2; k++) u[k] = __byte_perm(w[2 * k][b / 2], w[2 * k + 1][b / 2], b & 1 ? 0x7632 : 0x5410);
-                        if constexpr (F32) {
+                        if constexpr (!SCALED) {
                             uint32_t v[2][4];
 #pragma unroll
                             for (int k = 0; k < 2; k++) {
@@ -536,15 +539,17 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                                 v[k][2] = h2u(__hfma2(u2h((u[k] >> 2 & 0x03c003c0u) | 0x4c004c00u), sd, s24));                                         // 16 + n: 24 scales are an f16
                                 v[k][3] = h2u(__hfma2(u2h((u[k] >> 6 & 0x03c003c0u) | 0x4c004c00u), sd, s24));
                             }
-                            // 16 cells' products start from zero, low parts of the weights first, and are added to the sums in 32 bits: the tensor core cuts off what it adds to, and a sum that
-                            // ran through all cells lost with their number (40 sequences of 8192 cells 3.9e-6)
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
-                                float t[4];
-                                mma16816_from(t, 0.f, 0.f, v[0][2 * h], v[0][2 * h + 1], v[1][2 * h], v[1][2 * h + 1], pf[LO - 1][2 * j], pf[LO - 1][2 * j + 1]);
-                                mma16816(t, v[0][2 * h], v[0][2 * h + 1], v[1][2 * h], v[1][2 * h + 1], pf[0][2 * j], pf[0][2 * j + 1]);
+                                if constexpr (F32) {
+                                    // 16 cells' products start from zero, low parts of the weights first, and are added to the sums in 32 bits: the tensor core cuts off what it adds to, and a sum
+                                    // that ran through all cells lost with their number (40 sequences of 8192 cells 3.9e-6)
+                                    float t[4];
+                                    mma16816_from(t, 0.f, 0.f, v[0][2 * h], v[0][2 * h + 1], v[1][2 * h], v[1][2 * h + 1], pf[LO - 1][2 * j], pf[LO - 1][2 * j + 1]);
+                                    mma16816(t, v[0][2 * h], v[0][2 * h + 1], v[1][2 * h], v[1][2 * h + 1], pf[0][2 * j], pf[0][2 * j + 1]);
 #pragma unroll
-                                for (int i = 0; i < 4; i++) o[b][h][i] += t[i];
+                                    for (int i = 0; i < 4; i++) o[b][h][i] += t[i];
+                                } else mma16816(o[b][h], v[0][2 * h], v[0][2 * h + 1], v[1][2 * h], v[1][2 * h + 1], pf[0][2 * j], pf[0][2 * j + 1]);
                             }
                         } else {
                             const uint32_t p0 = h2u(__hmul2(u2h(pf[0][2 * j]), u2h(d[0][b]))), p1 = h2u(__hmul2(u2h(pf[0][2 * j + 1]), u2h(d[1][b])));
@@ -568,7 +573,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             l[k] += __shfl_xor_sync(0xffffffffu, l[k], 8);
             l[k] += __shfl_xor_sync(0xffffffffu, l[k], 16);
         }
-        if constexpr (!F32)
+        if constexpr (SCALED)
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll

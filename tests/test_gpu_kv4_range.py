@@ -16,9 +16,9 @@ from test_gpu_kv4 import MIXED, TORCH, Attn, random_pages
 pytestmark = pytest.mark.gpu
 BOTH = pytest.mark.parametrize("q,kv", [([1, 3, 1], [300, 64, 1000]), ([200, 40, 1], [400, 90, 70])], ids=["tokens", "prompts"])
 # The root mean square of a rounding, relative to numbers whose logarithms are spread evenly over a binary order: half a step h is h / m of a number m of [1, 2), even over -h .. h, and
-# the mean of 1 / m^2 is 3 / (8 ln 2): h * sqrt(0.541 / 3) = 0.4246 h.  16 bits round a weight, with few rows its product with a scale too, and the output; errors of weights add up over
-# cells as the (random) values do, so relative to the output's norm they are what they are relative to a weight.
-RMS = {"f16": 0.4246 * 2.0 ** -11 * 3 ** 0.5, "bf16": 0.4246 * (2 * 2.0 ** -22 + 2.0 ** -16) ** 0.5}
+# the mean of 1 / m^2 is 3 / (8 ln 2): h * sqrt(0.541 / 3) = 0.4246 h.  16 bits round a weight to f16, BF16 with few rows its product with a scale too, and the output; errors of weights add up
+# over cells as the (random) values do, so relative to the output's norm they are what they are relative to a weight.
+RMS = {"f16": 0.4246 * 2.0 ** -11 * 2 ** 0.5, "bf16": 0.4246 * (2 * 2.0 ** -22 + 2.0 ** -16) ** 0.5}
 ON_THE_WHOLE = {t: 1.1 * r for t, r in RMS.items()}      # a tenth for samples of some thousand numbers
 
 
@@ -104,6 +104,36 @@ def test_a_cell_ahead_of_all_that_has_no_value(pkg, lib, cuda, type_, gap, q, kv
     few = 1.2 / 3 ** 0.5
     tol = 1e-6 + gap * np.log(2.0) * 2.0 ** -23 if type_ == "f32" else ON_THE_WHOLE[type_]
     assert off(got, want) <= tol + few * 2.0 ** (gap - (34 if type_ != "f32" and sum(q) > 10 else 39))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prompt", [False, True], ids=["tokens", "prompts"])
+def test_weights_of_f16_are_rounded_once(pkg, lib, cuda, dim, prompt):
+    """One cell is ahead of the others, which have equal scores and equal scales, so that their weights are rounded alike: what comes out is off by that rounding, which is known, and the output's
+    own; not by one of a weight's product with a scale."""
+    rng, n, kv = np.random.default_rng(53), 128, 300 if prompt else 60     # (tokens: a page, so that all cells go by the same reference)
+    a = Attn(pkg, lib, 53, "f16", 8, 2, dim, [n], [kv], scale=1.0)
+    if not prompt:
+        a.table_np, a.q_start_np, a.kv_np, a.max_q = np.repeat(a.table_np, n, 0), np.arange(n + 1, dtype=np.int32), np.full(n, kv, np.int32), 1
+    shape = (len(a.pages_np), 2, 64)
+    vn, vs = rng.integers(0, 16, shape + (dim,)), np.full(shape + (dim // 32,), 181.0 / 128.0)
+    kn, ks, first = np.full(shape + (dim,), 8), np.zeros(shape + (dim // 32,)), a.table_np[0, 0]
+    kn[first, :, 0, 0], ks[first, :, 0, 0], vs[first, :, 0] = 0, -0.125, 0.0     # a key of 1, a value of 0
+    a.pages_np = R.pack(kn.astype(np.uint8), ks, vn.astype(np.uint8), vs)
+    x = rng.uniform(0.05, 6.0, (n, 8))
+    a.q.view(n, 8, dim)[..., 0] = torch.from_numpy(x).cuda().half()
+    a.q_np = a.q.double().cpu().numpy()
+    a.upload()
+    a.call()
+    got, want = result(a)
+    w = 2.0 ** 15 * np.exp(-a.q_np.reshape(n, 8, dim)[..., 0])
+    # not next to the middle of two f16 numbers: a score of 16 bits is a sum of up to 8 * 32 magnitudes of queries in 4 steps of 2^-23, an eighth of which it is: 1e-4 at most
+    sure = np.float16(w * (1 - 1e-4)) == np.float16(w * (1 + 1e-4))
+    want = want * (np.float16(w).astype(np.float64) / w)[..., None]
+    assert sure.mean() > 0.5
+    # sums of some hundred numbers of up to 8 * 1.5 in 32 bits: 1e-5
+    beyond = np.abs(got - want) - R.HALF_STEP["f16"] * 1.001 * np.abs(want) - 2.0 ** -24 - 1e-5
+    assert beyond[sure].max() <= 0.0
 
 
 # ---------------------------------------------------------------------------------------------------------------- long and mixed batches
