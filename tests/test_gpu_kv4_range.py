@@ -136,6 +136,97 @@ def test_weights_of_f16_are_rounded_once(pkg, lib, cuda, dim, prompt):
     assert beyond[sure].max() <= 0.0
 
 
+@pytest.mark.parametrize("type_", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q,kv,heads,kv_heads,window,first", [([1] * 8, [400 + 90 * i for i in range(8)], 16, 4, 0, 0), ([1] * 4, [5000, 700, 90, 2000], 32, 8, 0, 0),
+                                                              ([4, 5, 3], [500, 320, 900], 8, 2, 200, 4), ([300], [900], 8, 2, 0, 0), ([150, 200, 1], [700, 2000, 800], 4, 2, 0, 0),
+                                                              ([400], [1500], 4, 4, 300, 10)], ids=str)
+def test_sixteen_bits_on_the_whole(pkg, lib, cuda, type_, dim, q, kv, heads, kv_heads, window, first):
+    a = Attn(pkg, lib, 44, type_, heads, kv_heads, dim, q, kv, window, first)
+    a.call()
+    a.check()
+    assert off(*result(a)) <= ON_THE_WHOLE[type_]
+
+
+@pytest.mark.parametrize("type_", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("per", ["block", "page", "cell"])
+@pytest.mark.parametrize("largest", [4.0, 21760.0])
+@BOTH
+def test_values_of_very_different_scales(pkg, lib, cuda, type_, dim, per, largest, q, kv):
+    """Values 2^12 apart between blocks, pages or cells, up to the largest that a cache holds, and a page of zeros: each block of the output as near as if it were alone."""
+    a = Attn(pkg, lib, 45, type_, 8, 2, dim, q, kv)
+    rng, n = np.random.default_rng(46), len(a.pages_np)
+    shape = {"block": (1, 1, 1, dim // 32, 1), "page": (n, 1, 1, dim // 32, 1), "cell": (n, 2, 64, dim // 32, 1)}[per]
+    small = np.arange(dim // 32).reshape(shape) % 2 if per == "block" else rng.random(shape) < 0.5
+    v = np.clip(rng.standard_normal((n, 2, 64, dim // 32, 32)), -2.5, 2.5) * (largest / 2.5) * np.where(small, 2.0 ** -12, 1.0)
+    v[a.table_np[0, 1]] = 0.0
+    a.pages_np = R.pack(*R.quantize(rng.standard_normal((n, 2, 64, dim))), *R.quantize(v.reshape(n, 2, 64, dim)))
+    a.upload()
+    a.call()
+    got, want = result(a)
+    for b in range(dim // 32):
+        g, w = got[..., 32 * b:32 * b + 32], want[..., 32 * b:32 * b + 32]
+        # f16 results below its normal range have steps of 2^-24
+        assert np.linalg.norm(g - w) <= (3e-6 if type_ == "f32" else ON_THE_WHOLE[type_]) * np.linalg.norm(w) + (2.0 ** -25 * w.size ** 0.5 if type_ == "f16" else 0.0), b
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("q,kv", MIXED, ids=["tokens", "prompts"])
+def test_rows_of_any_magnitude_one_by_one(pkg, lib, cuda, type_, q, kv):
+    """Queries from 1e-30 to 1e5: rows whose best score leads by more than all scores' errors give that cell's value, others are near on their own."""
+    a = Attn(pkg, lib, 47, type_, 8, 2, 128, q, kv)
+    a.q = (a.q.double() * torch.from_numpy((10.0 ** np.linspace(-30, 5, a.tokens))[:, None]).cuda()).to(TORCH[type_])
+    a.q_np = a.q.double().cpu().numpy()
+    a.call()
+    got, want = result(a)
+    half, single = R.HALF_STEP[type_] * 1.01, 0
+    for s in range(len(q)):
+        k, v = (x.transpose(1, 0, 2, 3).reshape(2, -1, 128) for x in R.unpack(a.pages_np[a.table_np[s, :-(-kv[s] // 64)]], 128))
+        for i in range(q[s]):
+            row, see = a.q_np[a.q_start_np[s] + i].reshape(2, 4, 128), kv[s] - q[s] + i + 1
+            for h in range(8):
+                kk, qq = k[h // 4, :see], row[h // 4, h % 4]
+                z = kk @ qq * a.scale
+                mag, g, w = np.abs(kk) @ np.abs(qq) * a.scale, got[a.q_start_np[s] + i, h], want[a.q_start_np[s] + i, h]
+                best = np.sort(z)[::-1]
+                err = 2 * 136 * 2.0 ** -23 * mag.max()
+                if see > 1 and best[0] - best[1] > 2 * err + 30.0:
+                    chosen = v[h // 4, z.argmax()]
+                    assert np.all(np.abs(g - chosen) <= half * np.abs(chosen) + 1e-5 * np.abs(chosen).max())
+                    single += 1
+                elif err < 1e-3:
+                    few = 1e-5 + 2.0 ** -22 * mag.max() if type_ == "f32" else 3 * ON_THE_WHOLE[type_]      # (of 128 numbers)
+                    assert np.linalg.norm(g - w) <= few * np.linalg.norm(w) + 1e-6 * (type_ != "f32")
+    assert single >= (8 if sum(q) < 10 else 100)
+
+
+@pytest.mark.parametrize("type_", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q,kv", MIXED, ids=["tokens", "prompts"])
+@pytest.mark.parametrize("scale", [1e4, 3e5])
+def test_large_scores(pkg, lib, cuda, type_, q, kv, scale):
+    """Scores whose own rounding is more than a binary order: weights stay finite, and the cell that is ahead by more than all errors is what comes out, but for the roundings of a weight that is no
+    power of two then and of the output."""
+    a = Attn(pkg, lib, 54, type_, 8, 2, 128, q, kv, scale=scale)
+    a.call()
+    got, want = result(a)
+    single, half = 0, R.HALF_STEP[type_] + (2.0 ** -11 if type_ != "f32" else 0.0)
+    for s in range(len(q)):
+        k, v = (x.transpose(1, 0, 2, 3).reshape(2, -1, 128) for x in R.unpack(a.pages_np[a.table_np[s, :-(-kv[s] // 64)]], 128))
+        for i in range(q[s]):
+            row, see = a.q_np[a.q_start_np[s] + i].reshape(8, 128), kv[s] - q[s] + i + 1
+            for h in range(8):
+                z, mag = k[h // 4, :see] @ row[h] * scale, (np.abs(k[h // 4, :see]) @ np.abs(row[h])).max() * scale
+                assert mag < 2e9 and np.abs(z).max() < 4e7
+                g, best = got[a.q_start_np[s] + i, h], np.sort(z)[::-1]
+                assert np.all(np.abs(g) <= np.abs(v[h // 4, :see]).max(0) * (1 + 1.01 * half + 1e-5))
+                if see == 1 or best[0] - best[1] > 4 * 136 * 2.0 ** -23 * mag + 30.0:
+                    chosen = v[h // 4, z.argmax()]
+                    assert np.all(np.abs(g - chosen) <= half * 1.01 * np.abs(chosen) + 1e-5 * np.abs(chosen).max())
+                    single += 1
+    assert single >= sum(q) * 4
+
+
 # ---------------------------------------------------------------------------------------------------------------- long and mixed batches
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("kv,beside", [(2130, 0), (2130, 33), (16130, 0), (16130, 33)])
