@@ -11,15 +11,17 @@
 //   warps 4 - 11   softmax, groups of four: a thread has a row of S, which is also a lane of tensor memory
 //   warp 12        MMA issuer, owner of the tensor memory, and of the tickets
 // Tensor memory: S / P of either group at 0 and 256, O at 128 and 384.  Weights lie over their scores: 16 columns for 32, F32's low parts in the other 16.
+// F32: every 512 cells of a group O is added to a sum in the workspace, and begins anew with a reference of its own.
 //
 // Bound: with 16 bits a key tile takes 4400 clocks for 256 rows: MMAs 2100 (S with both operands in shared memory, which also takes the expanded tiles), exponentials 2050 a scheduler, two
 // softmax groups and expansion side by side, each group waiting for a third of it on its own two products; an item adds 12000 for queries, first tile, output; a launch 4000, or 8000 where
 // items are cut.  us: 2048 tokens of 32 heads over 8 56 (610 TFLOP/s of visible pairs; over an f16 cache k_attn_prefill_tc takes 58), a plain form of elementary operations 3066; 512 behind
-// 8000 cells 104; F32, 1077 queries behind up to 5077 cells 67 (with the sequence of one query and the join), 5200.
+// 8000 cells 109 (F32 166); F32, 1077 queries behind up to 5077 cells 77 (with the sequence of one query and the join; 69 with sums that stay in tensor memory), 5200.
 // On the way, us at 2048 tokens: scores 32 at a time, waited for, masks within the passes 124; the next 32 on their way 102; masks in a pass of their own over edge tiles (their code was a
 // third of what was fetched and not run) 64; eight numbers of a query to a lane 57.  A row to a thread for the queries is no faster (its loads are 256 bytes apart),
-// weights handed over in halves neither (F32 70 -> 77: the issuing warp waits for one group's while the other's are there).
-// Error against 64 bits with F32: 4e-7 at 128 cells, 1.1e-6 at 5000: MMAs cut off what they add to O, and O is the sum of all tiles.
+// weights handed over in halves neither (F32, with sums that stay, 70 -> 77: the issuing warp waits for one group's while the other's are there).
+// Error against 64 bits with F32: 3.5e-7 at 128 cells, 1.6e-6 at 4000 and more (KP_CHUNK).  With 16 bits O is the sum of all tiles, of which MMAs cut off what they add to: 2e-4 at 131 000 cells.
+// A chunk's sum goes through L2: 128 KB read and written by an SM for both groups, 2.5 us; asking for it ahead of the wait for scores changes nothing.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
