@@ -164,7 +164,7 @@ PB200_API int pb200_kv4_load(const pb200_kv4_cache * cache, int layer, int type,
  * Precision.  Scores: 32 bits, up to 4e7 of them.  q: F16 and BF16 as it is, F32 22 bits of a number or 2^-39 of its row's largest.  Weights: F32 22 bits or 2^-39 of the row's largest weight, F16 and BF16 11 bits or 2^-34;
  * BF16 with few rows (up to 48 queries x heads of a group) 11 bits of a weight and of its product with its block's scale, or 2^-39 of the largest weight, 2^-36 of it in what they add to the
  * output, both times the largest value in the sequence's pages / 8 where that is more than 1.  Sums: 32 bits; prompts' are the tensor core's, which cuts off what it adds to:
- * F32 for 512 cells at a time (2e-6 of the output's norm, whatever the length), 16 bits for all (2e-4 at 131 000 cells, which is F16's own rounding).
+ * F32 for 256 cells at a time (1e-6 of the output's norm, whatever the length), 16 bits for all (2e-4 at 131 000 cells, which is F16's own rounding).
  * PB200_ENOTSUP where pages, heads and tiles of rows do not fit 31 bits.
  * ws: pb200_kv4_attn_workspace_bytes, zeroed once by the caller, for calls that follow one another (one per stream, also of graphs that may run at the same time). */
 PB200_API size_t pb200_kv4_attn_workspace_bytes(int n_head, int n_head_kv, int head_dim);

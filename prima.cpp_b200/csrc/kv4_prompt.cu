@@ -11,17 +11,17 @@
 //   warps 4 - 11   softmax, groups of four: a thread has a row of S, which is also a lane of tensor memory
 //   warp 12        MMA issuer, owner of the tensor memory, and of the tickets
 // Tensor memory: S / P of either group at 0 and 256, O at 128 and 384.  Weights lie over their scores: 16 columns for 32, F32's low parts in the other 16.
-// F32: every 512 cells of a group O is added to a sum in the workspace, and begins anew with a reference of its own.
+// F32: every 256 cells of a group O is added to a sum in the workspace, and begins anew with a reference of its own.
 //
 // Bound: with 16 bits a key tile takes 4400 clocks for 256 rows: MMAs 2100 (S with both operands in shared memory, which also takes the expanded tiles), exponentials 2050 a scheduler, two
 // softmax groups and expansion side by side, each group waiting for a third of it on its own two products; an item adds 12000 for queries, first tile, output; a launch 4000, or 8000 where
 // items are cut.  us: 2048 tokens of 32 heads over 8 56 (610 TFLOP/s of visible pairs; over an f16 cache k_attn_prefill_tc takes 58), a plain form of elementary operations 3066; 512 behind
-// 8000 cells 109 (F32 166); F32, 1077 queries behind up to 5077 cells 77 (with the sequence of one query and the join; 69 with sums that stay in tensor memory), 5200.
+// 8000 cells 109 (F32 178); F32, 1077 queries behind up to 5077 cells 82 (with the sequence of one query and the join; 69 with sums that stay in tensor memory), 5200.
 // On the way, us at 2048 tokens: scores 32 at a time, waited for, masks within the passes 124; the next 32 on their way 102; masks in a pass of their own over edge tiles (their code was a
 // third of what was fetched and not run) 64; eight numbers of a query to a lane 57.  A row to a thread for the queries is no faster (its loads are 256 bytes apart),
 // weights handed over in halves neither (F32, with sums that stay, 70 -> 77: the issuing warp waits for one group's while the other's are there).
-// Error against 64 bits with F32: 3.5e-7 at 128 cells, 1.6e-6 at 4000 and more (KP_CHUNK).  With 16 bits O is the sum of all tiles, of which MMAs cut off what they add to: 2e-4 at 131 000 cells.
-// A chunk's sum goes through L2: 128 KB read and written by an SM for both groups, 2.5 us; asking for it ahead of the wait for scores changes nothing.
+// Error against 64 bits with F32: 3.5e-7 at 128 cells, 1.1e-6 at 4000 and more (KP_CHUNK).  With 16 bits O is the sum of all tiles, of which MMAs cut off what they add to: 2e-4 at 131 000 cells.
+// A chunk's sum goes through L2, 128 KB read and written by an SM for both groups; asking for it ahead of a wait changes nothing.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -39,11 +39,11 @@ constexpr int KP_THREADS = 13 * 32, KP_TILE = 128, KP_BLOCK = 16384;   // a bloc
 constexpr int KP_CUT_SEQ = 32, KP_CUT_TILES = KV4_MAX_CTAS + KP_CUT_SEQ;     // where long items may be cut: sequences, row tiles
 // A row's reference may fall behind its largest score by 2^SLACK; a weight is 2^(15 - SLACK) at its reference, so 2^15 at most, and what f16 (F32: its low part) rounds off is 2^(SLACK - 40) of the
 // row's largest weight (F32, whose references are whole numbers: 2^-39).  8, as it was with 2^6 in front of weights, lost small ones beside a large one (of weights 2^-24 of it, 2e-3); us, 512
-// tokens behind 8000 in f16, 8 / 6 / 5 / 4: 110 / 110 / 111 / 112; the ragged case in F32, 4 / 2 / 0: 75 / 77 / 77.
+// tokens behind 8000 in f16, 8 / 6 / 5 / 4: 110 / 110 / 111 / 112; the ragged case in F32, with four tiles to a chunk (below), 4 / 2 / 0: 75 / 77 / 77.
 template <typename T> constexpr float kp_slack() { return std::is_same<T, float>::value ? 0.f : 6.f; }
-// F32: key tiles of a group (512 cells) whose products add up in tensor memory, before they go to a sum in 32 bits: the tensor core cuts off what it adds to.  Error, 8 x 512 queries of 4096 cells
-// (elementary 32-bit operations 1.3e-6), and us: 2 1.0e-6, 343; 3 1.3e-6, 322; 4 1.6e-6, 302; 8 2.7e-6, 290; all of them 4.9e-6, 272.
-constexpr int KP_CHUNK = 4;
+// F32: key tiles of a group (256 cells) whose products add up in tensor memory, before they go to a sum in 32 bits: the tensor core cuts off what it adds to.  Error, 8 x 512 queries of 4096 cells
+// (elementary 32-bit operations 1.3e-6), and us: 1 0.8e-6, 400; 2 1.1e-6, 335; 3 1.3e-6, 318; 4 1.6e-6, 308; all of them 4.9e-6, 272.  779 queries of up to 1260 cells (0.7e-6): 2 0.9e-6, 4 1.3e-6.
+constexpr int KP_CHUNK = 2;
 template <typename T> constexpr int kp_rows() { return std::is_same<T, float>::value ? KP_TILE : 2 * KP_TILE; }   // of an item
 
 struct KpPiece {               // what a ticket stands for
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     __syncthreads();
     fence_after();
     const uint32_t tmem = *(volatile uint32_t *) &S.tmem_base;
-    uint32_t tiles = 0, pieces = 0, of_group[2] = {0, 0}, ends[2] = {0, 0};   // key tiles and pieces in front; key tiles and pieces of either group (all roles count them)
+    uint32_t tiles = 0, pieces = 0, of_group[2] = {0, 0}, ends[2] = {0, 0};   // key tiles and pieces in front; key tiles and ends of chunks of either group (all roles count them)
     while (*(volatile int *) &S.more[pieces & 1]) {
         const KpPiece & P = S.piece[pieces & 1];
         const int n = P.b - P.a, groups = (F32 ? n > 1 : P.rows > KP_TILE) ? 2 : 1;      // groups at work
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
 #pragma unroll
                         for (int k = 0; k < 8; k++)
                             mma_f16_ts(tmem + 256 * grp + 128, tmem + 256 * grp + 32 * (k >> 1) + 8 * (k & 1) + 16 * part, dv + k * (2048 >> 4), idesc_v, (uint32_t) (((F32 ? i % KP_CHUNK : i) | part | k) != 0));
-                    if (last) mma_commit(&S.o_full[grp]);
+                    if (last || (F32 && i % KP_CHUNK == KP_CHUNK - 1)) mma_commit(&S.o_full[grp]);
                     if (F32 || grp == groups - 1) mma_commit(&S.v_empty[st]);
                 }
                 __syncwarp();
@@ -508,21 +508,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                         }
                         tmem_wait_st();
                     }
-                    if (F32 && i > 0 && i % KP_CHUNK == 0) {       // a chunk ends
-                        factors();
-#pragma unroll 1
-                        for (int h = 0; h < D; h += 32) {
-                            TMEM_LD32(mine + 128 + h, t0);
-                            if (i > KP_CHUNK) ask_far(h);
-                            TMEM_ARRIVED(t0);
-#pragma unroll
-                            for (int k = 0; k < 32; k++) t[0][k] = i > KP_CHUNK ? fmaf(t[1][k], f_far, t[0][k] * f_own) : t[0][k] * f_own;
-#pragma unroll
-                            for (int k = 0; k < 32; k += 4) far[(h + k) / 4 * KP_TILE] = make_float4(t[0][k], t[0][k + 1], t[0][k + 2], t[0][k + 3]);
-                        }
-                        m = -INFINITY;
-                        l = 0.f;
-                    }
                     float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     TMEM_LD32(mine, t0);
 #pragma unroll
@@ -587,10 +572,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&S.p_full[grp]);
+                    if (F32 && i % KP_CHUNK == KP_CHUNK - 1 && j + 2 < n) {       // a chunk ends: beside the next scores
+                        mbar_wait(&S.o_full[grp], (ends[grp] + (uint32_t) (i / KP_CHUNK)) & 1, cta_abort, W.abort_flag);
+                        __syncwarp();
+                        fence_after();
+                        factors();
+#pragma unroll 1
+                        for (int h = 0; h < D; h += 32) {
+                            TMEM_LD32(mine + 128 + h, t0);
+                            if (i >= KP_CHUNK) ask_far(h);
+                            TMEM_ARRIVED(t0);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) t[0][k] = i >= KP_CHUNK ? fmaf(t[1][k], f_far, t[0][k] * f_own) : t[0][k] * f_own;
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) far[(h + k) / 4 * KP_TILE] = make_float4(t[0][k], t[0][k + 1], t[0][k + 2], t[0][k + 3]);
+                        }
+                        m = -INFINITY;
+                        l = 0.f;
+                    }
                 }
-                // F32: all scores are made before the queries' memory is used again
-                for (int k = 0; k < 2; k++)
-                    if (F32 ? k < groups : k == grp) mbar_wait(&S.o_full[k], ends[k] & 1, cta_abort, W.abort_flag);
+                // (all scores are made, too, before the queries' memory is used again: they come in front of the last products)
+                mbar_wait(&S.o_full[grp], (ends[grp] + (uint32_t) (F32 ? ((n - grp + 1) / 2 - 1) / KP_CHUNK : 0)) & 1, cta_abort, W.abort_flag);
                 __syncwarp();
                 fence_after();
                 constexpr int PIECE = 4, PIECES = D / PIECE;       // numbers to a piece; row r's pieces are rotated by r
@@ -694,7 +696,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
         pieces++;
         for (int grp = 0; grp < groups; grp++) {
             of_group[grp] += (uint32_t) (F32 ? (n - grp + 1) / 2 : n);
-            ends[grp]++;
+            ends[grp] += (uint32_t) (F32 ? ((n - grp + 1) / 2 - 1) / KP_CHUNK + 1 : 1);
         }
         fence_after();
     }
