@@ -115,8 +115,8 @@ struct Kv4Attn {
 };
 // A sequence with up to so many rows (queries x heads of a group) goes to the kernel of few rows, which walks its pages once for every eight of them; the other one has tiles of 128 and
 // 256 rows whatever there are.  us, 32 heads over 8, few rows / prompt: bf16, 8 sequences of 4096 cells, 32 rows 48 / 66, 48 60 / 66, 56 69 / 63; 64 of 1000, 32 rows 86 / 113, 48 111 / 113,
-// 64 141 / 114; f16, 8 of 4096, 40 rows 57 / 61, 48 65 / 61; 64 of 1000, 40 rows 104 / 111, 48 122 / 111; 4 of 500, 48 rows 25 / 30; F32, 8 of 4096, 20 rows 54 / 64, 32 69 / 63, 40 77 / 64;
-// 64 of 1000, 20 rows 109 / 121, 32 135 / 123; 4 of 500, 32 rows 20 / 32, which is why F32's bound is not lower.
+// 64 141 / 114; f16, 8 of 4096, 40 rows 57 / 61, 48 65 / 61; 64 of 1000, 40 rows 104 / 111, 48 122 / 111; 4 of 500, 48 rows 25 / 30; F32, 8 of 4096, 20 rows 54 / 68, 32 70 / 69, 40 77 / 69;
+// 64 of 1000, 20 rows 107 / 130, 32 135 / 131, 40 154 / 132; 4 of 500, 32 rows 20 / 32.
 constexpr int KV4_FEW_ROWS = 48, KV4_FEW_ROWS_F32 = 32;
 size_t kv4_attn_workspace(int D);
 int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t st, int & launches);   // launches: kernels, added up
