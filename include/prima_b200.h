@@ -171,6 +171,32 @@ PB200_API size_t pb200_kv4_attn_workspace_bytes(int n_head, int n_head_kv, int h
 PB200_API int pb200_kv4_attn(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
                              const int32_t * kv_len, const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, void * ws,
                              size_t ws_bytes, void * stream);
+/* The same, and lse[t * ld_lse + head] = the natural logarithm of the sum of exp(scale q k) over what the query sees (f32; -inf where that is nothing). */
+PB200_API int pb200_kv4_attn_lse(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
+                                 const int32_t * kv_len, const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, float * lse,
+                                 int64_t ld_lse, void * ws, size_t ws_bytes, void * stream);
+/* Attention of a batch whose sequences come in groups with a prefix in common, whose pages are read once for the group.  Group g has the sequences group_start[g] .. group_start[g+1]-1 (device
+ * [n_group + 1], rising; sequences outside of group_start[0] .. group_start[n_group]-1 have no prefix), whose queries all see the prefix_len[g] cells of row g of prefix_table (as table's,
+ * prefix_ld pages a row) in front of their own, which are those of pb200_kv4_attn without a window: kv_len counts them alone, and rotations count from the prefix's start.  A prefix may end
+ * inside a page.  lse: as in pb200_kv4_attn_lse, or NULL.  Precision: as in pb200_kv4_attn; a prefix goes to the kernel of few rows where its groups have few rows on the average.
+ * ws: pb200_kv4_attn_shared_workspace_bytes, zeroed once, as pb200_kv4_attn's, for which it serves, too. */
+PB200_API size_t pb200_kv4_attn_shared_workspace_bytes(int n_head, int n_head_kv, int head_dim, int64_t n_tokens);
+PB200_API int pb200_kv4_attn_shared(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
+                                    const int32_t * kv_len, const int32_t * table, int64_t table_ld, int n_group, const int32_t * group_start, const int32_t * prefix_len,
+                                    const int32_t * prefix_table, int64_t prefix_ld, int64_t n_tokens, int max_q, float scale, float * lse, int64_t ld_lse, void * ws, size_t ws_bytes,
+                                    void * stream);
+/* What the cells are worth: sums[s * ld_sums + j] = decay * old[s * ld_old + j] + the weights of cell j, exp(scale q k - lse), added up over the queries of sequence s that see it and all heads,
+ * for j below kv_len[s] and ld_sums; other sums stay as they were.  The arguments as in pb200_kv4_attn, lse as pb200_kv4_attn_lse gives it.  q_start may name the last few queries of a prompt
+ * alone: their positions are the last ones.  old: NULL counts as zeros (and is not read with a decay of 0); sums may lie over old (with its stride), otherwise apart from it.
+ * Precision: scores and sums in 32 bits (q: F16 and BF16 as it is, F32 22 bits of a number).  Equal calls give equal bits. */
+PB200_API int pb200_kv4_weigh(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, int n_head, int n_seq, const int32_t * q_start, const int32_t * kv_len,
+                              const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, const float * lse, int64_t ld_lse, float decay,
+                              const float * old, int64_t ld_old, float * sums, int64_t ld_sums, void * stream);
+/* Which cells a sequence keeps, for pb200_kv4_compact: of its len = kv_len[s] cells (max_len and ld_sums at most) count[s] = min(len, budget[s], ld_index): the last keep_last, the first keep_first
+ * (as far as count[s] goes, the last ones first), and of those between the ones with the largest sums, of equal ones the lowest; a sum that is no number counts as -inf, -0 as 0.
+ * index[s * ld_index + i]: the i-th, ascending; kept (or NULL)[s * ld_kept + i]: its sum, for the compacted sequence.  What lies behind count[s] stays as it was.  kept lies apart from sums. */
+PB200_API int pb200_kv4_select(int n_seq, const float * sums, int64_t ld_sums, const int32_t * kv_len, int max_len, const int32_t * budget, int keep_first, int keep_last, int32_t * index,
+                               int64_t ld_index, int32_t * count, float * kept, int64_t ld_kept, void * stream);
 /* Copies of whole pages, all layers: page src[i] to page dst[i] (HOST arrays, not needed after the call).  A sequence that forks shares its full pages with the new one, and
  * copies the last, which both go on writing.  PB200_EINVAL where a page is written twice, or written and read. */
 PB200_API int pb200_kv4_copy_pages(const pb200_kv4_cache * cache, const int32_t * src, const int32_t * dst, int n, void * stream);
@@ -179,6 +205,20 @@ PB200_API int pb200_kv4_copy_pages(const pb200_kv4_cache * cache, const int32_t 
  * their other cells stay as they were.  Behind it the old pages are free. */
 PB200_API int pb200_kv4_compact(const pb200_kv4_cache * cache, int n_seq, const int32_t * table, int64_t table_ld, const int32_t * to, int64_t to_ld, const int32_t * index,
                                 int64_t index_ld, const int32_t * count, int max_count, void * stream);
+
+/* ---- verification of drafted tokens ----
+ * Sequence s has the drafts start[s] .. start[s+1]-1 (device [n_seq + 1], rising from 0 to n_drafts): tokens and, in rows of n_vocab logits of a type (PB200_TYPE_F32, F16 or BF16; any stride), what
+ * the draft model had: row i of `draft` for draft i, or draft NULL: the tokens come from elsewhere, as if with probability 1.  target: for each of its drafts and for the token behind the last one
+ * a row: start[s] + s .. start[s+1] + s.  p and q: softmax of logits times inv_temp[s] (NULL: 1; infinite: all on the largest, of several the lowest; 0: even over all finite logits).
+ * Draft x with its number u = u_accept[i] is accepted where u q(x) < p(x); n_accepted[s]: how many are, up to the first that is not.  Behind them comes a token drawn by u_draw[s]: with weights
+ * w = max(p - q, 0) of the first that is not accepted (p, where these are all 0), with p behind the last: the lowest i with w_0 + .. + w_i > u_draw[s] * (sum of w), in 64 bits.
+ * out[s * ld_out + ..]: the accepted tokens and that one (as far as ld_out goes; what lies behind stays as it was).  kv_len_out[s] = kv_len[s] less the drafts that were not accepted (both NULL:
+ * not wanted; may be the same): the cells of these are free.  Logits that are no number count as -inf, +inf takes all weight; tokens outside the vocabulary are not accepted; where a row has no
+ * weights at all, or inv_temp[s] is below 0 or no number, the token is -1.  Numbers u lie in [0, 1).  ws: pb200_verify_drafts_workspace_bytes, for calls that follow one another. */
+PB200_API size_t pb200_verify_drafts_workspace_bytes(int64_t n_drafts);
+PB200_API int pb200_verify_drafts(int type, const void * target, int64_t ld_target, const void * draft, int64_t ld_draft, int n_vocab, int n_seq, const int32_t * start, int64_t n_drafts,
+                                  const int32_t * tokens, const float * inv_temp, const float * u_accept, const float * u_draw, int32_t * n_accepted, int32_t * out, int64_t ld_out,
+                                  const int32_t * kv_len, int32_t * kv_len_out, void * ws, size_t ws_bytes, void * stream);
 
 /* ---- fused decode launches (what the engine is made of), for graph-level fusion in a host such as the ggml-backend plugin ---- */
 typedef struct pb200_gemv_mat {

@@ -102,6 +102,17 @@ int launch_kv4_load(const Kv4 & cache, int D, int type, const int64_t * cells, i
 int launch_kv4_copy_pages(uint8_t * pages, int64_t page_bytes, const int32_t * src, const int32_t * dst, int n, cudaStream_t st);   // src, dst: host
 int launch_kv4_compact(uint8_t * pages, int64_t n_pages, int rows, int D, int n_seq, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to,
                        const int32_t * index, int64_t ld_index, const int32_t * count, int most, cudaStream_t st);   // rows: chunks of a page
+// What attention may do besides (kernels with X): rows' logarithms; results as parts, of which a second call makes one result with its own
+struct Kv4Ext {
+    float * lse; int64_t ld_lse;          // of each query and head; NULL: not wanted
+    int part;                             // KV4_PUT: results are sums and what belongs to them, into o and ml; KV4_FOLD: those are added to the results of the sequences in groups
+    float * o;                            // [token][head][D]
+    float2 * ml;                          // [token][head]: reference and sum of weights
+    const int32_t * group_start;          // the groups' first sequences
+    int n_group, n_seq;
+    int all;                              // a sequence is a group of them: the queries of all, each of which sees all cells
+};
+enum { KV4_PUT = 1, KV4_FOLD = 2 };
 struct Kv4Attn {
     Kv4 cache;
     const void * q; int64_t ldq;
@@ -112,6 +123,7 @@ struct Kv4Attn {
     int64_t n_tokens;
     int max_q, window, first;
     float scale;
+    Kv4Ext x;
 };
 // A sequence with up to so many rows (queries x heads of a group) goes to the kernel of few rows, which walks its pages once for every eight of them; the other one has tiles of 128 and
 // 256 rows whatever there are.  us, 32 heads over 8, few rows / prompt: bf16, 8 sequences of 4096 cells, 32 rows 48 / 66, 48 60 / 66, 56 69 / 63; 64 of 1000, 32 rows 86 / 113, 48 111 / 113,
@@ -120,5 +132,16 @@ struct Kv4Attn {
 constexpr int KV4_FEW_ROWS = 48, KV4_FEW_ROWS_F32 = 32;
 size_t kv4_attn_workspace(int D);
 int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t st, int & launches);   // launches: kernels, added up
+struct Kv4Groups { int n; const int32_t * start; const int32_t * kv_len; const int32_t * table; int64_t table_ld; };
+size_t kv4_attn_shared_workspace(int64_t rows, int D);
+int launch_kv4_attn_shared(const Kv4Attn & a, const Kv4Groups & g, int D, int type, void * ws, cudaStream_t st, int & launches);
+struct Kv4Weigh {
+    Kv4Attn attn;
+    const float * lse; int64_t ld_lse;
+    float decay;
+    const float * old; int64_t ld_old;    // NULL: nothing
+    float * sums; int64_t ld_sums;
+};
+int launch_kv4_weigh(const Kv4Weigh & w, int D, int type, cudaStream_t st);
 
 }  // namespace pb

@@ -41,6 +41,38 @@ bool overlap(const void * a, int64_t lda, int64_t wa, const void * b, int64_t ld
     return in < wa * eb || in + wb * eb > ld;
 }
 
+int attend(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start, const int32_t * kv_len,
+           const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, float * lse, int64_t ld_lse, const Kv4Groups * groups, void * ws,
+           size_t ws_bytes, void * stream) {
+    const int e = check(c);
+    if (e) return e;
+    const int eb = elem_bytes(type);
+    const int64_t D = c->head_dim;
+    if (!eb || layer < 0 || layer >= c->n_layer || n_head <= 0 || n_head % c->n_head_kv || n_seq < 0 || n_tokens < 0 || n_tokens > INT32_MAX || max_q < 0) return PB200_EINVAL;
+    if (!q_start || !kv_len || !table || table_ld <= 0 || !std::isfinite(scale) || window < 0 || keep_first < 0) return PB200_EINVAL;
+    if (!rows_ok(q, ldq, n_head * D, eb) || !rows_ok(out, ldo, n_head * D, eb)) return PB200_EINVAL;
+    if (lse && (((uintptr_t) lse & 3) || ld_lse < n_head)) return PB200_EINVAL;
+    const size_t least = groups ? pb200_kv4_attn_shared_workspace_bytes(n_head, c->n_head_kv, c->head_dim, n_tokens) : pb200_kv4_attn_workspace_bytes(n_head, c->n_head_kv, c->head_dim);
+    if (!ws || ((uintptr_t) ws & 15) || ws_bytes < least) return PB200_EINVAL;
+    if (n_seq == 0 || n_tokens == 0 || max_q == 0) return 0;
+    // what the kernels count in 31 bits: pages of all sequences, heads and tiles of eight rows where rows are few, tiles of all prompts otherwise
+    const double group = n_head / c->n_head_kv, rows = std::min(std::min<double>(max_q, (double) n_tokens) * group, (double) KV4_FEW_ROWS);
+    const auto pages_of = [&](int64_t ld) { return (double) std::min<int64_t>(ld, INT32_MAX / PB200_KV4_CELLS) * c->n_head_kv; };
+    const double pages = n_seq * pages_of(table_ld) * std::ceil(rows / 8);
+    const double tiles = ((double) n_tokens * group / 128 + n_seq) * c->n_head_kv;
+    if (pages >= 2147483648.0 || tiles >= 2147483648.0 || n_tokens * group >= 2147483648.0) return PB200_ENOTSUP;
+    // (of prefixes the kernel of few rows takes up to so many rows a group on the average)
+    if (groups && (groups->n * pages_of(groups->table_ld) * (KV4_FEW_ROWS / 8 + 1) >= 2147483648.0 || ((double) n_tokens * group / 128 + groups->n) * c->n_head_kv >= 2147483648.0)) return PB200_ENOTSUP;
+    if (overlap(q, ldq, n_head * D, out, ldo, n_head * D, n_tokens, eb)) return PB200_EINVAL;
+    Kv4Attn a{layer_of(c, layer), q, ldq, out, ldo, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};
+    a.x.lse = lse;
+    a.x.ld_lse = ld_lse;
+    int launches = 0;
+    const int rc = groups ? launch_kv4_attn_shared(a, *groups, c->head_dim, type, ws, (cudaStream_t) stream, launches) : launch_kv4_attn(a, c->head_dim, type, ws, (cudaStream_t) stream, launches);
+    g_launches += launches;
+    return rc;
+}
+
 }  // namespace
 
 extern "C" {
@@ -109,26 +141,51 @@ size_t pb200_kv4_attn_workspace_bytes(int n_head, int n_head_kv, int head_dim) {
 int pb200_kv4_attn(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
                    const int32_t * kv_len, const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, void * ws,
                    size_t ws_bytes, void * stream) {
+    return attend(c, layer, type, q, ldq, out, ldo, n_head, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, scale, window, keep_first, nullptr, 0, nullptr, ws, ws_bytes, stream);
+}
+
+int pb200_kv4_attn_lse(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
+                       const int32_t * kv_len, const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, float * lse, int64_t ld_lse,
+                       void * ws, size_t ws_bytes, void * stream) {
+    if (!lse) return PB200_EINVAL;
+    return attend(c, layer, type, q, ldq, out, ldo, n_head, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, scale, window, keep_first, lse, ld_lse, nullptr, ws, ws_bytes, stream);
+}
+
+size_t pb200_kv4_attn_shared_workspace_bytes(int n_head, int n_head_kv, int head_dim, int64_t n_tokens) {
+    if (!pb200_kv4_attn_workspace_bytes(n_head, n_head_kv, head_dim) || n_tokens < 0 || n_tokens > INT32_MAX) return 0;
+    return kv4_attn_shared_workspace(n_tokens * n_head, head_dim);
+}
+
+int pb200_kv4_attn_shared(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
+                          const int32_t * kv_len, const int32_t * table, int64_t table_ld, int n_group, const int32_t * group_start, const int32_t * prefix_len, const int32_t * prefix_table,
+                          int64_t prefix_ld, int64_t n_tokens, int max_q, float scale, float * lse, int64_t ld_lse, void * ws, size_t ws_bytes, void * stream) {
+    if (n_group < 0 || (n_group > 0 && (!group_start || !prefix_len || !prefix_table || prefix_ld <= 0))) return PB200_EINVAL;
+    const Kv4Groups g{n_group, group_start, prefix_len, prefix_table, prefix_ld};
+    return attend(c, layer, type, q, ldq, out, ldo, n_head, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, scale, 0, 0, lse, ld_lse, n_group > 0 ? &g : nullptr, ws, ws_bytes, stream);
+}
+
+int pb200_kv4_weigh(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, int n_head, int n_seq, const int32_t * q_start, const int32_t * kv_len, const int32_t * table,
+                    int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, const float * lse, int64_t ld_lse, float decay, const float * old, int64_t ld_old,
+                    float * sums, int64_t ld_sums, void * stream) {
     const int e = check(c);
     if (e) return e;
     const int eb = elem_bytes(type);
     const int64_t D = c->head_dim;
     if (!eb || layer < 0 || layer >= c->n_layer || n_head <= 0 || n_head % c->n_head_kv || n_seq < 0 || n_tokens < 0 || n_tokens > INT32_MAX || max_q < 0) return PB200_EINVAL;
-    if (!q_start || !kv_len || !table || table_ld <= 0 || !std::isfinite(scale) || window < 0 || keep_first < 0) return PB200_EINVAL;
-    if (!rows_ok(q, ldq, n_head * D, eb) || !rows_ok(out, ldo, n_head * D, eb)) return PB200_EINVAL;
-    if (!ws || ((uintptr_t) ws & 15) || ws_bytes < pb200_kv4_attn_workspace_bytes(n_head, c->n_head_kv, c->head_dim)) return PB200_EINVAL;
-    if (n_seq == 0 || n_tokens == 0 || max_q == 0) return 0;
-    // what the kernels count in 31 bits: pages of all sequences, heads and tiles of eight rows where rows are few, tiles of all prompts otherwise
-    const double group = n_head / c->n_head_kv, rows = std::min(std::min<double>(max_q, (double) n_tokens) * group, (double) KV4_FEW_ROWS);
-    const double pages = (double) n_seq * (double) std::min<int64_t>(table_ld, INT32_MAX / PB200_KV4_CELLS) * c->n_head_kv * std::ceil(rows / 8);
-    const double tiles = ((double) n_tokens * group / 128 + n_seq) * c->n_head_kv;
-    if (pages >= 2147483648.0 || tiles >= 2147483648.0 || n_tokens * group >= 2147483648.0) return PB200_ENOTSUP;
-    if (overlap(q, ldq, n_head * D, out, ldo, n_head * D, n_tokens, eb)) return PB200_EINVAL;
-    const Kv4Attn a{layer_of(c, layer), q, ldq, out, ldo, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};
-    int launches = 0;
-    const int rc = launch_kv4_attn(a, c->head_dim, type, ws, (cudaStream_t) stream, launches);
-    g_launches += launches;
-    return rc;
+    if (!q_start || !kv_len || !table || table_ld <= 0 || !std::isfinite(scale) || window < 0 || keep_first < 0 || !std::isfinite(decay)) return PB200_EINVAL;
+    if (n_tokens > 0 && (!rows_ok(q, ldq, n_head * D, eb) || !lse || ((uintptr_t) lse & 3) || ld_lse < n_head)) return PB200_EINVAL;
+    if (!sums || ((uintptr_t) sums & 3) || ld_sums <= 0 || (old && (((uintptr_t) old & 3) || ld_old < ld_sums))) return PB200_EINVAL;
+    // a sum is read and written by the same thread: in place, or apart
+    if (old && n_seq > 0 && !(old == sums && ld_old == ld_sums) && overlap(old, ld_old, ld_sums, sums, ld_sums, ld_sums, n_seq, 4)) return PB200_EINVAL;
+    // what the kernel counts in 31 bits: items (256 cells of a sequence), rows, blocks of rows of all heads
+    const double rows = std::min((double) max_q, (double) n_tokens) * (n_head / c->n_head_kv);
+    if ((double) n_seq * (std::min<double>((double) ld_sums, (double) INT32_MAX) / 256 + 1) >= 2147483648.0 - 65536 || rows >= 2147483648.0 || (rows / 64 + 1) * c->n_head_kv >= 2147483648.0)
+        return PB200_ENOTSUP;
+    if (n_seq == 0) return 0;
+    Kv4Attn a{layer_of(c, layer), q, ldq, nullptr, 0, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};
+    const Kv4Weigh w{a, lse, ld_lse, decay, decay == 0.f ? nullptr : old, ld_old, sums, ld_sums};
+    g_launches++;
+    return launch_kv4_weigh(w, c->head_dim, type, (cudaStream_t) stream);
 }
 
 int pb200_kv4_copy_pages(const pb200_kv4_cache * c, const int32_t * src, const int32_t * dst, int n, void * stream) {

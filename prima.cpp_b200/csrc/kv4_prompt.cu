@@ -82,9 +82,10 @@ enum { KP_DRAWN, KP_DONE, KP_CUT, KP_JOINED };             // tickets drawn, CTA
 template <int D> struct KpParts { KpPart<D> part[KV4_SLOTS]; KpPiece item[KV4_SLOTS]; };   // item: those that were cut, their first pieces
 
 // the tile's rows [row0, row0 + rows) of a sequence: positions and pages
+template <bool X>
 __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpPiece & p) {
-    p.p_lo = q.p0 + p.row0 / A.group;
-    p.p_hi = q.p0 + (p.row0 + p.rows - 1) / A.group;
+    p.p_lo = kv4_pos<X>(A, q, p.row0 / A.group);
+    p.p_hi = kv4_pos<X>(A, q, (p.row0 + p.rows - 1) / A.group);
     p.q = q;
     kv4_pages(A, p.p_lo, p.p_hi, p.q);
     p.tiles = (p.q.pages + 1) / 2;
@@ -100,12 +101,12 @@ __device__ __forceinline__ int warp_running_sum(int x) {
     }
     return x;
 }
-template <int ROWS>
+template <int ROWS, bool X>
 __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int ctas, KpPlan & plan) {     // by a warp
     const int lane = threadIdx.x & 31;
     if (lane == 0) plan.limit = 0;
     if (!W.cut) return;
-    const Kv4Seq own = kv4_seq(A, lane, W.most_rows, true);
+    const Kv4Seq own = kv4_seq<X>(A, lane, W.most_rows, true);
     plan.q0[lane] = own.q0; plan.n_q[lane] = own.n_q; plan.p0[lane] = own.p0; plan.n_rows[lane] = own.n_rows;
     const int len = own.n_q > 0 ? own.p0 + own.n_q : INT_MIN;
     int rank = lane < A.n_seq ? 0 : lane;
@@ -133,7 +134,7 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
         if (m < all) {
             const Kv4Seq q = plan.seq(src);
             p.rows = min(ROWS, q.n_rows - p.row0);
-            kp_span(A, q, p);
+            kp_span<X>(A, q, p);
             plan.lens[m] = p.tiles;
             sum += p.tiles;
         }
@@ -161,7 +162,7 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
     if (lane == 0) plan.limit = best;
 }
 // by a warp: what ticket t stands for; false: there is none
-template <int ROWS>
+template <int ROWS, bool X>
 __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, const KpPlan & plan, int t, KpPiece & out) {
     const int lane = threadIdx.x & 31, hks = A.cache.n_head_kv;
     int before = 0, cut = 0;
@@ -183,7 +184,7 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, con
                 p.s = plan.from[r];
                 const Kv4Seq q = plan.seq(p.s);
                 p.rows = min(ROWS, q.n_rows - p.row0);
-                kp_span(A, q, p);
+                kp_span<X>(A, q, p);
                 const int i = t - before - (x - k * hks);
                 p.hk = i / k;
                 p.part = i - p.hk * k;
@@ -199,7 +200,7 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, con
         return false;
     }
     for (int s0 = 0; s0 < A.n_seq; s0 += 32) {
-        const Kv4Seq q = kv4_seq(A, s0 + lane, W.most_rows, true);
+        const Kv4Seq q = kv4_seq<X>(A, s0 + lane, W.most_rows, true);
         const int n = q.n_q > 0 ? (q.n_rows + ROWS - 1) / ROWS * hks : 0;
         const int x = warp_running_sum(n);
         const uint32_t in = __ballot_sync(0xffffffffu, t < before + x);
@@ -213,7 +214,7 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, con
             p.s = s0 + lane;
             p.row0 = ((q.n_rows + ROWS - 1) / ROWS - 1 - tile) * ROWS;
             p.rows = min(ROWS, q.n_rows - p.row0);
-            kp_span(A, q, p);
+            kp_span<X>(A, q, p);
             p.hk = i - tile * hks;
             p.b = p.tiles;
             p.parts = 1;
@@ -242,7 +243,7 @@ __device__ __forceinline__ uint4 expand(uint32_t w, __half2 d) {
     return make_uint4(hu(__hmul2(__hsub2(uh((w & 0x000f000fu) | 0x64006400u), e), d)), hu(__hmul2(__hsub2(uh((w & 0x00f000f0u) | 0x54005400u), o), d)),
                       hu(__hmul2(__hsub2(uh((s & 0x000f000fu) | 0x64006400u), e), d)), hu(__hmul2(__hsub2(uh((s & 0x00f000f0u) | 0x54005400u), o), d)));
 }
-template <typename T, int D>
+template <typename T, int D, bool X>
 __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
     constexpr bool F32 = std::is_same<T, float>::value;
     constexpr int ROWS = kp_rows<T>(), NB = D / 32;
@@ -272,9 +273,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     }
     int ticket = blockIdx.x;
     if (warp == 12) {
-        kp_plan<ROWS>(A, W, gridDim.x, S.plan);
+        kp_plan<ROWS, X>(A, W, gridDim.x, S.plan);
         __syncwarp();
-        const bool more = kp_find<ROWS>(A, W, S.plan, ticket, S.piece[0]);
+        const bool more = kp_find<ROWS, X>(A, W, S.plan, ticket, S.piece[0]);
         if (lane == 0) S.more[0] = more;
     }
     fence_before();
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             uint32_t kw[4][WORDS], vw[4][WORDS], ks[NB], vs[NB];
             auto chunk_of = [&](int j) {                          // this half's page of tile j, none: null
                 const int i = 2 * (P.a + j) + half;
-                const int id = j < n && i < P.q.pages ? kv4_page(A, P.q, P.s, i) : -1;
+                const int id = j < n && i < P.q.pages ? kv4_page<X>(A, P.q, P.s, i) : -1;
                 return id >= 0 ? kv4_chunk<D>(A.cache, id, P.hk) : nullptr;
             };
             auto rows_of = [&](const uint8_t * row, const uint8_t * scales, uint32_t (&w)[4][WORDS], uint32_t (&d)[NB]) {
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             if (lane == 0) ticket = (int) gridDim.x + atomicAdd(&W.tickets[KP_DRAWN], 1);
             ticket = __shfl_sync(0xffffffffu, ticket, 0);
             const int later = (pieces + 1) & 1;
-            const bool more = kp_find<ROWS>(A, W, S.plan, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
+            const bool more = kp_find<ROWS, X>(A, W, S.plan, ticket, S.piece[later]);         // beside the piece's end; earlier, and CTAs with long pieces would draw more
             if (lane == 0) S.more[later] = more;
         } else {
             // ---- softmax ----
@@ -464,10 +465,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("bar.sync 4, 288;" ::: "memory");
             if (grp < groups) {
-                const int pos = mine_is ? P.q.p0 + tok : -1;
+                const int pos = mine_is ? kv4_pos<X>(A, P.q, tok) : -1;
                 const float c = S.mult[rows0 + row];
                 const uint32_t mine = tmem + ((uint32_t) (quad * 32) << 16) + 256 * grp;
-                const int g_lo = P.q.p0 + (P.row0 + rows0) / A.group;              // of the group's first row
+                const int g_lo = kv4_pos<X>(A, P.q, (P.row0 + rows0) / A.group);              // of the group's first row
                 float m = -INFINITY, l = 0.f;
                 float t[2][32];                                    // scores, 32 being worked on and 32 on their way
                 uint32_t * const t0 = reinterpret_cast<uint32_t *>(t[0]), * const t1 = reinterpret_cast<uint32_t *>(t[1]);
@@ -637,6 +638,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 if (!F32 || grp == 0) {
                     const float inv = P.slot >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
                     KpPart<D> * part = nullptr;
+                    Kv4Row w{inv, 0.f, nullptr, nullptr};
+                    if (X && P.slot < 0 && mine_is) w = kv4_row<D>(A, P.s, P.q.q0 + tok, head, m - UP, l, true);
+                    const bool put = X && P.slot < 0 && A.x.part == KV4_PUT;
                     if (P.slot >= 0) {
                         part = &reinterpret_cast<KpParts<D> *>(W.parts)->part[P.slot];
                         part->m[rows0 + row] = m;
@@ -659,20 +663,30 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; i++) t[0][i] *= inv;
+                        for (int i = 0; i < 32; i++) t[0][i] *= X ? w.own : inv;
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {           // columns 0 2 4 6 | 1 3 5 7 of an eight are numbers 0 1 2 3 | 4 5 6 7
-                            const float4 a = make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]), b = make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]);
-                            if (part) {
+                            float4 a = make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]), b = make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]);
+                            if (X && put) {
+                                if (mine_is) {
+                                    *reinterpret_cast<float4 *>(w.put + h + i) = a;
+                                    *reinterpret_cast<float4 *>(w.put + h + i + 4) = b;
+                                }
+                            } else if (part) {
                                 *reinterpret_cast<float4 *>(&part->o[rows0 + row][h + i]) = a;
                                 *reinterpret_cast<float4 *>(&part->o[rows0 + row][h + i + 4]) = b;
                             } else {
+                                if (X && w.from) {
+                                    const Kv4Row r{1.f, w.other, w.from, nullptr};
+                                    a = kv4_mix(r, a, h + i);
+                                    b = kv4_mix(r, b, h + i + 4);
+                                }
                                 store4(os + ((h + i) / 4 + row) % PIECES * 4, a);
                                 store4(os + ((h + i) / 4 + 1 + row) % PIECES * 4, b);
                             }
                         }
                     }
-                    if (!part) {
+                    if (!part && !put) {
                         constexpr int LPR = D / 4, RPW = 32 / LPR;
                         const int sub = lane / LPR, l4 = lane % LPR;
                         __syncwarp();                               // a warp reads its own rows
@@ -708,7 +722,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
 }
 
 // Items that were cut, eight rows to a CTA at a time: a warp adds a row's parts in their order, a lane D / 32 numbers.
-template <typename T, int D>
+template <typename T, int D, bool X>
 __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
     constexpr int PER = D / 32, ONCE = 8, EIGHTS = kp_rows<T>() / 8;
     const int lane = threadIdx.x & 31, items = *(volatile int *) &W.tickets[KP_CUT];
@@ -748,9 +762,19 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
                 }
             }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = X ? 1.f : l == 0.f ? 0.f : 1.f / l;
         const int at = p.row0 + r, tt = at / A.group;
         T * out = (T *) A.out + (p.q.q0 + tt) * A.ldo + (int64_t) (p.hk * A.group + at - tt * A.group) * D + lane * PER;
+        if constexpr (X) {
+            const Kv4Row w = kv4_row<D>(A, p.s, p.q.q0 + tt, p.hk * A.group + at - tt * A.group, top - (15.f - kp_slack<T>()), l, lane == 0);
+            if (w.put) {
+#pragma unroll
+                for (int e = 0; e < PER; e++) w.put[lane * PER + e] = x[e];
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < PER; e++) x[e] = w.from ? fmaf(w.from[lane * PER + e], w.other, x[e] * w.own) : x[e] * w.own;
+        }
         if constexpr (PER == 4) store4(out, make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv));
         else
 #pragma unroll
@@ -764,12 +788,12 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
     if (threadIdx.x == 0 && atomicAdd(&W.tickets[KP_JOINED], 1) == (int) gridDim.x - 1) W.tickets[KP_CUT] = W.tickets[KP_JOINED] = 0;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool X>
 int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) {
     constexpr size_t smem = sizeof(KpSmem<D>) + 1024;
     static_assert(smem <= 232448, "shared memory of an SM");
     static FuncAttrCache cache;
-    cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_prompt<T, D>, smem, true);
+    cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_prompt<T, D, X>, smem, true);
     if (e != cudaSuccess) return (int) e;
     const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
     // (a plan adds up key tiles of all items: in 30 bits)
@@ -784,9 +808,9 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = w.most_rows > 0 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, k_kv4_attn_prompt<T, D>, a, w);
+    e = cudaLaunchKernelEx(&cfg, k_kv4_attn_prompt<T, D, X>, a, w);
     if (e != cudaSuccess || !w.cut) return (int) e;
-    k_kv4_join<T, D><<<4 * sm_count(), 256, 0, st>>>(a, w);
+    k_kv4_join<T, D, X><<<4 * sm_count(), 256, 0, st>>>(a, w);
     return (int) cudaGetLastError();
 }
 
@@ -794,10 +818,16 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
 
 size_t kv4_prompt_workspace(int D) { return D == 128 ? sizeof(KpParts<128>) : sizeof(KpParts<64>); }
 
-int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st, int & launches) {
+template <int D, bool X>
+static int prompt_launch(const Kv4Attn & a, const KpWork & w, int type, cudaStream_t st, int & launches) {
+    return type == PB200_TYPE_F32   ? prompt_launch<float, D, X>(a, w, st, launches)
+           : type == PB200_TYPE_F16 ? prompt_launch<__half, D, X>(a, w, st, launches)
+                                    : prompt_launch<__nv_bfloat16, D, X>(a, w, st, launches);
+}
+int launch_kv4_attn_prompt(const Kv4Attn & a, int D, int type, int most_rows, int * tickets, void * parts, cudaStream_t st, bool ext, int & launches) {
     const KpWork w{most_rows, tickets, parts, abort_flag(), 0};
-    if (D == 128) return type == PB200_TYPE_F32 ? prompt_launch<float, 128>(a, w, st, launches) : type == PB200_TYPE_F16 ? prompt_launch<__half, 128>(a, w, st, launches) : prompt_launch<__nv_bfloat16, 128>(a, w, st, launches);
-    return type == PB200_TYPE_F32 ? prompt_launch<float, 64>(a, w, st, launches) : type == PB200_TYPE_F16 ? prompt_launch<__half, 64>(a, w, st, launches) : prompt_launch<__nv_bfloat16, 64>(a, w, st, launches);
+    if (ext) return D == 128 ? prompt_launch<128, true>(a, w, type, st, launches) : prompt_launch<64, true>(a, w, type, st, launches);
+    return D == 128 ? prompt_launch<128, false>(a, w, type, st, launches) : prompt_launch<64, false>(a, w, type, st, launches);
 }
 
 }  // namespace pb

@@ -129,6 +129,10 @@ struct KrSum {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         store4(to, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
     }
+    template <typename T> __device__ __forceinline__ void write(T * to, const Kv4Row & r, int d4) const {
+        if (r.put) store4(r.put + d4, x);
+        else store4(to, kv4_mix(r, x, d4));
+    }
 };
 // row r of a segment's tile in the output
 template <typename T, int D>
@@ -136,8 +140,13 @@ __device__ __forceinline__ T * kr_row(const Kv4Attn & A, const KrSegment & at, i
     const int row = at.tile * KR_ROWS + r, t = row / A.group;
     return (T *) A.out + (at.q.q0 + t) * A.ldo + (int64_t) (at.hk * A.group + row - t * A.group) * D;
 }
+template <int D>
+__device__ __forceinline__ Kv4Row kr_ext(const Kv4Attn & A, const KrSegment & at, int r, float m, float l, bool writes) {
+    const int row = at.tile * KR_ROWS + r, t = row / A.group;
+    return kv4_row<D>(A, at.s, at.q.q0 + t, at.hk * A.group + row - t * A.group, m, l, writes);
+}
 
-template <typename T, int D>
+template <typename T, int D, bool X>
 __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_constant__ Kv4Attn A, const __grid_constant__ KrWork W) {
     constexpr int NB = D / 32, STAGES = kr_stages<D>(), CHUNK = kv4_chunk_bytes(D);
     constexpr bool F32 = std::is_same<T, float>::value, SCALED = std::is_same<T, __nv_bfloat16>::value;   // SCALED: weights carry the values' scales
@@ -151,7 +160,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
     pdl_trigger();                                      // the prompts' kernel may start where this one has no work
 
     // ---- shares: units (pages of items) in the order of sequences, tiles, heads, pages; a thread has a sequence ----
-    Kv4Seq mine = kv4_seq(A, tid, W.most_rows, false);
+    Kv4Seq mine = kv4_seq<X>(A, tid, W.most_rows, false);
     int n = mine.units(hks, KR_ROWS), units = n;
     if (lane < STAGES) {
         mbar_init(&S.full[warp][lane], 1);
@@ -159,7 +168,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (tid == 0) S.abort = 0;
-    for (int s = tid + KR_THREADS; s < A.n_seq; s += KR_THREADS) units += kv4_seq(A, s, W.most_rows, false).units(hks, KR_ROWS);
+    for (int s = tid + KR_THREADS; s < A.n_seq; s += KR_THREADS) units += kv4_seq<X>(A, s, W.most_rows, false).units(hks, KR_ROWS);
     auto upto = [&](int x) {                   // sum over the lanes up to this one
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
     else {
         int before = 0;
         for (int s0 = 0; s0 < A.n_seq; s0 += KR_THREADS) {
-            mine = kv4_seq(A, s0 + tid, W.most_rows, false);
+            mine = kv4_seq<X>(A, s0 + tid, W.most_rows, false);
             n = mine.units(hks, KR_ROWS);
             x = upto(n);
             __syncthreads();
@@ -225,7 +234,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
         while (p.u - p.before >= p.q.units(hks, KR_ROWS)) {
             p.before += p.q.units(hks, KR_ROWS);
             if (++p.s >= A.n_seq) return false;
-            p.q = kv4_seq(A, p.s, W.most_rows, false);
+            p.q = kv4_seq<X>(A, p.s, W.most_rows, false);
         }
         const int in = p.u - p.before, item = in / p.q.pages;
         p.pa = in - item * p.q.pages;
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             ids0 = u;
             ids1 = min(u + 32, p.u);
             f_hk = p.hk;
-            ids = u + lane < ids1 ? kv4_page(A, p.q, p.s, p.pa + u + lane - p.k0) : -1;
+            ids = u + lane < ids1 ? kv4_page<X>(A, p.q, p.s, p.pa + u + lane - p.k0) : -1;
         }
         const int id = __shfl_sync(0xffffffffu, ids, u - ids0), st = (u - u0) % STAGES;
         none = id >= 0 ? none & ~(1u << st) : none | 1u << st;
@@ -358,7 +367,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             }
             // of a row's sums: the power of two, n * 2^-24, and scores in units of log2; never 0: a masked score stays -inf
             const float down = fmaxf(fabsf(A.scale) * (F32 ? 1.4426950408889634f : 1.4426950408889634f * 16777216.f) * __int_as_float((127 - ex) << 23), FLT_MIN);
-            const int p = q.p0 + row / A.group;
+            const int p = kv4_pos<X>(A, q, row / A.group);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int from = 4 * (2 * c + i);                               // a lane of row 2 c + i
@@ -370,7 +379,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
         }
         if (at.k0 == u0)                                // the first pages, behind the queries: these would wait for all that is on its way to this SM
             for (int k = 0; k < STAGES; k++) fetch(u0 + k);
-        const int p_lo = q.p0 + row0 / A.group, p_hi = q.p0 + (row0 + rows - 1) / A.group;   // of the tile's rows
+        const int p_lo = kv4_pos<X>(A, q, row0 / A.group), p_hi = kv4_pos<X>(A, q, (row0 + rows - 1) / A.group);   // of the tile's rows
 
         // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1 (SCALED: times 2^-24, and 2^-20 the odd ones)
         float o[NB][2][4], less[4] = {0.f, 0.f, 0.f, 0.f};     // less: SCALED: row b: - 8 * 2^-24 times the sum of block b's scaled weights
@@ -590,7 +599,16 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             for (int k = 0; k < 2; k++) {
                 const int r = 2 * c + k;
                 const float inv = l[k] == 0.f ? 0.f : 1.f / l[k];
-                if (r < rows) {
+                if (X && r < rows) {
+                    const Kv4Row w = kr_ext<D>(A, at, r, m[k] - (float) up, l[k], g == 0);
+                    T * to = kr_row<T, D>(A, at, r) + 4 * g;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const float4 x = make_float4(o[b][0][k], o[b][0][2 + k], o[b][1][k], o[b][1][2 + k]);
+                        if (w.put) store4(w.put + 32 * b + 4 * g, x);
+                        else store4(to + 32 * b, kv4_mix(w, x, 32 * b + 4 * g));
+                    }
+                } else if (r < rows) {
                     T * to = kr_row<T, D>(A, at, r) + 4 * g;
 #pragma unroll
                     for (int b = 0; b < NB; b++) store4(to + 32 * b, make_float4(o[b][0][k] * inv, o[b][0][2 + k] * inv, o[b][1][k] * inv, o[b][1][2 + k] * inv));
@@ -646,7 +664,9 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             KrSum sum;
             sum.add<KR_WARPS, false>(to - f0 + 1, r, d4, [&](int i) { return S.part[f0 - first + i][f0 + i == v0 ? 1 : 0]; });
             if (v0 >= first && v1 < first + at_work) {
-                if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
+                if (r >= rows) return;
+                if constexpr (X) sum.write(kr_row<T, D>(A, at, r) + d4, kr_ext<D>(A, at, r, sum.top, sum.l, d4 == 0), d4);
+                else sum.write(kr_row<T, D>(A, at, r) + d4);
                 return;
             }
             KrPart<D> & mid = parts.cta[blockIdx.x][f0 == v0 ? 1 : 0];
@@ -677,19 +697,21 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             const int c0 = v0 / at_work, c1 = v1 / at_work;
             KrSum sum;
             sum.add<16, true>(c1 - c0 + 1, r, d4, [&](int i) { return &parts.cta[c0 + i][i == 0 ? 1 : 0]; });
-            if (r < rows) sum.write(kr_row<T, D>(A, at, r) + d4);
+            if (r >= rows) return;
+                if constexpr (X) sum.write(kr_row<T, D>(A, at, r) + d4, kr_ext<D>(A, at, r, sum.top, sum.l, d4 == 0), d4);
+                else sum.write(kr_row<T, D>(A, at, r) + d4);
         });
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool X>
 int rows_launch(const Kv4Attn & a, const KrWork & w, cudaStream_t st) {
     constexpr size_t smem = sizeof(KrSmem<D>) + 128;
     static_assert(smem <= 232448, "shared memory of an SM");
     static FuncAttrCache cache;
-    const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_rows<T, D>, smem, true);
+    const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_rows<T, D, X>, smem, true);
     if (e != cudaSuccess) return (int) e;
-    k_kv4_attn_rows<T, D><<<sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS, KR_THREADS, smem, st>>>(a, w);
+    k_kv4_attn_rows<T, D, X><<<sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS, KR_THREADS, smem, st>>>(a, w);
     return (int) cudaGetLastError();
 }
 
@@ -699,10 +721,14 @@ size_t kv4_rows_workspace(int D) { return D == 128 ? sizeof(KrParts<128>) : size
 static_assert(sizeof(KrPart<128>) <= kv4_chunk_bytes(128) && sizeof(KrPart<64>) <= kv4_chunk_bytes(64), "a part goes through a stage");
 static_assert(KV4_COUNTERS >= KV4_MAX_CTAS * KR_WARPS * KR_ROWS, "a counter for each slice of a warp's item");
 
-int launch_kv4_attn_rows(const Kv4Attn & a, int D, int type, int most_rows, int * counters, void * parts, cudaStream_t st) {
+template <int D, bool X>
+static int rows_launch(const Kv4Attn & a, const KrWork & w, int type, cudaStream_t st) {
+    return type == PB200_TYPE_F32 ? rows_launch<float, D, X>(a, w, st) : type == PB200_TYPE_F16 ? rows_launch<__half, D, X>(a, w, st) : rows_launch<__nv_bfloat16, D, X>(a, w, st);
+}
+int launch_kv4_attn_rows(const Kv4Attn & a, int D, int type, int most_rows, int * counters, void * parts, cudaStream_t st, bool ext) {
     const KrWork w{most_rows, counters, parts, abort_flag()};
-    if (D == 128) return type == PB200_TYPE_F32 ? rows_launch<float, 128>(a, w, st) : type == PB200_TYPE_F16 ? rows_launch<__half, 128>(a, w, st) : rows_launch<__nv_bfloat16, 128>(a, w, st);
-    return type == PB200_TYPE_F32 ? rows_launch<float, 64>(a, w, st) : type == PB200_TYPE_F16 ? rows_launch<__half, 64>(a, w, st) : rows_launch<__nv_bfloat16, 64>(a, w, st);
+    if (ext) return D == 128 ? rows_launch<128, true>(a, w, type, st) : rows_launch<64, true>(a, w, type, st);
+    return D == 128 ? rows_launch<128, false>(a, w, type, st) : rows_launch<64, false>(a, w, type, st);
 }
 
 }  // namespace pb

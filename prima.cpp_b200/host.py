@@ -151,6 +151,16 @@ class Lib:
         c.pb200_kv4_attn.argtypes = [cache, C.c_int, C.c_int, vp, i64, vp, i64, C.c_int, C.c_int, vp, vp, vp, i64, i64, C.c_int, f32, C.c_int, C.c_int, vp, st, vp]
         c.pb200_kv4_copy_pages.argtypes = [cache, vp, vp, C.c_int, vp]
         c.pb200_kv4_compact.argtypes = [cache, C.c_int, vp, i64, vp, i64, vp, i64, vp, C.c_int, vp]
+        attn = c.pb200_kv4_attn.argtypes
+        c.pb200_kv4_attn_lse.argtypes = attn[:18] + [vp, i64] + attn[18:]
+        c.pb200_kv4_attn_shared_workspace_bytes.restype = st
+        c.pb200_kv4_attn_shared_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int, i64]
+        c.pb200_kv4_attn_shared.argtypes = attn[:13] + [C.c_int, vp, vp, vp, i64, i64, C.c_int, f32, vp, i64, vp, st, vp]
+        c.pb200_kv4_weigh.argtypes = attn[:5] + attn[7:18] + [vp, i64, f32, vp, i64, vp, i64, vp]
+        c.pb200_kv4_select.argtypes = [C.c_int, vp, i64, vp, C.c_int, vp, C.c_int, C.c_int, vp, i64, vp, vp, i64, vp]
+        c.pb200_verify_drafts_workspace_bytes.restype = st
+        c.pb200_verify_drafts_workspace_bytes.argtypes = [i64]
+        c.pb200_verify_drafts.argtypes = [C.c_int, vp, i64, vp, i64, C.c_int, C.c_int, vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, st, vp]
         c.pb200_dense.argtypes = [C.c_int, vp, i64, vp, i64, vp, i64, C.c_int, C.c_int, C.c_int, vp, vp, i64, f32, vp]
 
     @classmethod
