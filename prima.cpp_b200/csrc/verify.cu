@@ -4,8 +4,9 @@
 // token from max(p - q, 0) at the place of the rejection, from p behind the last draft: by the inverse of the cumulative sum at v times the whole.  What is emitted then has the target's
 // distribution, whatever the draft's.
 //   rows    a CTA has a chunk of a row: its largest logit m and the sum of 2^((l - m) t log2 e), in 32 bits: a decision u q < p changes where they are within 1e-7 of each other
-//   draw    a cluster has a sequence.  It joins its rows' chunks, decides, and takes the one row (two, with draft logits) that the token is drawn from into shared memory.  Weights and sums are in
-//           64 bits: a cumulative sum of 100 000 weights with errors of 1e-8 each would give another token once in a thousand draws.  A row's sum is that of its tiles, of which one is scanned.
+//   draw    a cluster has a sequence.  It joins its rows' chunks, decides, and adds up the weights that the token is drawn with, of one row, or of two with draft logits.  Weights and sums are in
+//           64 bits: a cumulative sum of 100 000 weights with errors of 1e-8 each would give another token once in a thousand draws.  Each warp has the sum of a contiguous part; that in which the
+//           token lies goes to all warps of its CTA once more, and a part of that is scanned.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -13,6 +14,7 @@
 #include <atomic>
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "../../include/prima_b200.h"
 #include "cluster.cuh"
@@ -23,9 +25,8 @@ extern std::atomic<uint64_t> g_launches;
 namespace pb {
 namespace {
 
-constexpr int VR_THREADS = 256, VR_ONCE = 4;           // rows: vectors of 16 bytes to a thread on their way
-constexpr int VD_THREADS = 512, VD_EACH = 4, VD_TILE = VD_THREADS * VD_EACH, VD_TILES = 64;
-constexpr size_t VD_SMEM = 220 * 1024;
+constexpr int VERIFY_CHUNKS = 64;      // of a row, at most
+constexpr int VR_THREADS = 256, VR_CTAS = 4, VR_ONCE = 4;      // rows: CTAs of an SM; vectors of 16 bytes to a thread at a time
 
 struct Verify {
     const void * target, * draft;
@@ -44,22 +45,20 @@ struct Verify {
 };
 
 __device__ __forceinline__ float number(float x) { return fmaxf(x, -INFINITY); }      // a logit that is none counts as -inf
-__device__ __forceinline__ float get(const float * p) { return number(*p); }
-__device__ __forceinline__ float get(const __half * p) { return number(__half2float(*p)); }
-__device__ __forceinline__ float get(const __nv_bfloat16 * p) { return number(__bfloat162float(*p)); }
+__device__ __forceinline__ float raw(const float * p) { return *p; }
+__device__ __forceinline__ float raw(const __half * p) { return __half2float(*p); }
+__device__ __forceinline__ float raw(const __nv_bfloat16 * p) { return __bfloat162float(*p); }
+template <typename T> __device__ __forceinline__ float get(const T * p) { return number(raw(p)); }
 template <typename T> constexpr int vec() { return 16 / (int) sizeof(T); }
 // vector v of a row of n: entries v * vec - skew and on, those outside -inf.  skew: entries between a 16-byte boundary and the row's first
 template <typename T>
-__device__ __forceinline__ void get_vec(const T * row, int n, int skew, int v, float (&x)[vec<T>()]) {
+__device__ __forceinline__ void get_vec(const T * row, int n, int skew, int v, uint4 & w) {
     const int at = v * vec<T>() - skew;
-    if (at >= 0 && at + vec<T>() <= n) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(row + at));
-        const T * e = reinterpret_cast<const T *>(&w);
+    if (at >= 0 && at + vec<T>() <= n) w = __ldg(reinterpret_cast<const uint4 *>(row + at));
+    else {
+        T * e = reinterpret_cast<T *>(&w);
 #pragma unroll
-        for (int i = 0; i < vec<T>(); i++) x[i] = get(e + i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < vec<T>(); i++) x[i] = at + i >= 0 && at + i < n ? get(row + at + i) : -INFINITY;
+        for (int i = 0; i < vec<T>(); i++) e[i] = at + i >= 0 && at + i < n ? row[at + i] : T(-INFINITY);
     }
 }
 template <typename T> __device__ __forceinline__ int skew_of(const T * row) { return (int) (((uintptr_t) row & 15) / sizeof(T)); }
@@ -98,7 +97,7 @@ struct Sum {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(VR_THREADS) k_verify_rows(const __grid_constant__ Verify A) {
+__global__ void __launch_bounds__(VR_THREADS, VR_CTAS) k_verify_rows(const __grid_constant__ Verify A) {
     constexpr int VEC = vec<T>();
     const int64_t row = blockIdx.x / A.chunks;
     const int chunk = (int) (blockIdx.x - row * A.chunks), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -114,36 +113,58 @@ __global__ void __launch_bounds__(VR_THREADS) k_verify_rows(const __grid_constan
     Sum sum;
     int arg = INT_MAX;
     const bool greedy = t == INFINITY;
-    for (int v0 = from + tid; v0 < to; v0 += VR_ONCE * VR_THREADS) {
-        float x[VR_ONCE][VEC], top = -INFINITY;
+    auto take = [&](auto once, int v0, const uint4 * w) {   // so many vectors from v0 on
+        constexpr int ONCE = decltype(once)::value;
+        float top = -INFINITY;
+        auto entry = [&](int k, int e) { return number(raw(reinterpret_cast<const T *>(&w[k]) + e)); };
 #pragma unroll
-        for (int k = 0; k < VR_ONCE; k++) {
-            if (v0 + k * VR_THREADS < to) get_vec(src, A.vocab, skew, v0 + k * VR_THREADS, x[k]);
-            else
+        for (int k = 0; k < ONCE; k++)
 #pragma unroll
-                for (int e = 0; e < VEC; e++) x[k][e] = -INFINITY;
-        }
-#pragma unroll
-        for (int k = 0; k < VR_ONCE; k++)
-#pragma unroll
-            for (int e = 0; e < VEC; e++) top = fmaxf(top, x[k][e]);
+            for (int e = 0; e < VEC; e++) top = fmaxf(top, entry(k, e));
         if (greedy) {
             if (top > sum.m) {
                 sum.m = top;
 #pragma unroll
-                for (int k = VR_ONCE - 1; k >= 0; k--)
+                for (int k = ONCE - 1; k >= 0; k--)
 #pragma unroll
                     for (int e = VEC - 1; e >= 0; e--)
-                        if (x[k][e] == top) arg = (v0 + k * VR_THREADS) * VEC - skew + e;
+                        if (entry(k, e) == top) arg = (v0 + k * VR_THREADS) * VEC - skew + e;
             }
         } else if (top > -INFINITY) {
             float l = 0.f;
+            if (top == INFINITY) {
 #pragma unroll
-            for (int k = 0; k < VR_ONCE; k++)
+                for (int k = 0; k < ONCE; k++)
 #pragma unroll
-                for (int e = 0; e < VEC; e++) l += top == INFINITY ? (x[k][e] == INFINITY ? 1.f : 0.f) : ex2((x[k][e] - top) * c);
+                    for (int e = 0; e < VEC; e++) l += entry(k, e) == INFINITY ? 1.f : 0.f;
+            } else {
+#pragma unroll
+                for (int k = 0; k < ONCE; k++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) l += ex2((entry(k, e) - top) * c);
+            }
             sum.add(top, l, c);
         }
+    };
+    // whole batches, the next one on its way beside the one at hand
+    const int batch = VR_ONCE * VR_THREADS;
+    int v0 = from + tid, whole = (to - from) / batch;
+    uint4 now[VR_ONCE];
+    auto ask = [&](int v, uint4 (&w)[VR_ONCE]) {
+#pragma unroll
+        for (int k = 0; k < VR_ONCE; k++) get_vec(src, A.vocab, skew, v + k * VR_THREADS, w[k]);
+    };
+    if (whole > 0) ask(v0, now);
+    for (; whole > 0; whole--, v0 += batch) {
+        uint4 next[VR_ONCE];
+        if (whole > 1) ask(v0 + batch, next);
+        take(std::integral_constant<int, VR_ONCE>(), v0, now);
+#pragma unroll
+        for (int k = 0; k < VR_ONCE; k++) now[k] = next[k];
+    }
+    for (; v0 < to; v0 += VR_THREADS) {
+        get_vec(src, A.vocab, skew, v0, now[0]);
+        take(std::integral_constant<int, 1>(), v0, now);
     }
     __shared__ Sum sums[VR_THREADS / 32];
     __shared__ int args[VR_THREADS / 32];
@@ -166,269 +187,312 @@ __global__ void __launch_bounds__(VR_THREADS) k_verify_rows(const __grid_constan
     }
 }
 
-struct VdSmem {
-    double warp[VD_THREADS / 32][2];
-    double mine[8];            // what the other CTAs read: largest logits, indices, sums
-    double tile[2][VD_TILES];
-    int first, found;
+// 2^(y / 16) in 64 bits for y from -16 * 1001 to about 0: the whole part of y goes to the exponent and to one of 16 roots, 2^(r / 16) of the rest (up to a half) is the polynomial that agrees
+// with it at the six Chebyshev nodes: within 2^-47 of it.  (Without roots nine products instead of five: 64 sequences of 128 256 logits 70 us where this takes 66.)
+__device__ __forceinline__ double power_of_two(double y, const double * roots) {
+    constexpr double ROUND = 6755399441055744.0;          // 1.5 * 2^52: a sum with it has the whole number in its last bits
+    const double z = y + ROUND, r = y - (z - ROUND);
+    const int k = __double2loint(z);
+    double p = 1.2716085030349987e-09;
+    p = fma(p, r, 1.467644462189871e-07);
+    p = fma(p, r, 1.355080777749983e-05);
+    p = fma(p, r, 0.000938384792486206);
+    p = fma(p, r, 0.04332169878499661);
+    p = fma(p, r, 1.0000000000000044) * roots[k & 15];
+    return __hiloint2double(__double2hiint(p) + ((k & ~15) << 16), __double2loint(p));
+}
+// The weights of a row's logits, the largest of them m; none is taken for less than 2^-1000, masked entries and what is no number among them: NOTHING is less than that, and a sum of them
+constexpr double NOTHING = 1e-290;
+struct Weights {
+    double c, mc;
+    float least;
+    bool step;                 // the same weight for all from `least` on: a largest logit of +inf, or an infinite temperature
+    const double * roots;      // 2^(i / 16)
+    __device__ __forceinline__ Weights(float m, float t, const double * roots) : c((double) t * (16 * 1.4426950408889634)), mc((double) m * c), roots(roots) {
+        step = m == INFINITY || t < 1e-30f;
+        least = m == INFINITY ? INFINITY : t < 1e-30f ? -FLT_MAX : fmaxf((float) ((double) m - 16000.0 / c), -FLT_MAX);
+    }
+    template <int N> __device__ __forceinline__ void operator()(const float (&l)[N], double (&w)[N]) const {
+        if (step) {
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = l[i] >= least ? 1.0 : 0.0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = power_of_two(fma((double) fmaxf(l[i], least), c, -mc), roots);
+        }
+    }
+    __device__ __forceinline__ double operator()(float l) const {
+        const float x[1] = {l};
+        double w[1];
+        (*this)(x, w);
+        return w[0];
+    }
 };
 
-// p(x) of a row from its chunks, by a warp
-__device__ __forceinline__ double chance(const float4 * parts, int chunks, int x, float lx, float t) {
+template <int WARPS> struct VdSmem {
+    double warp[WARPS][2], roots[16];
+    double z[2], all[2];       // what the other CTAs read: sums of either row, of the weights
+    float top;
+    int arg, first;
+};
+
+// sum of the warp's numbers in the lanes' order, of the first parts: `front` and the lanes up to the one that ends beyond x (where rounding leaves none, the last that has any) -> that lane
+__device__ __forceinline__ int find(double w, double x, double & front) {
     const int lane = threadIdx.x & 31;
-    float m = -INFINITY;
-    for (int k = lane; k < chunks; k += 32) m = fmaxf(m, __ldcg(&parts[k]).x);
-    m = warp_max(m);
-    if (m == -INFINITY || !(t >= 0.f)) return 0.0;
-    if (t == INFINITY) {
-        int arg = INT_MAX;
-        for (int k = lane; k < chunks; k += 32) {
-            const float4 p = __ldcg(&parts[k]);
-            if (p.x == m) arg = min(arg, __float_as_int(p.z));
-        }
-        return __reduce_min_sync(0xffffffffu, arg) == x ? 1.0 : 0.0;
+    double upto = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
     }
-    double l = 0.0;
-    for (int k = lane; k < chunks; k += 32) {
-        const float4 p = __ldcg(&parts[k]);
-        l += m == INFINITY ? (p.x == INFINITY ? p.y : 0.0) : p.y * exp(((double) p.x - m) * t);
-    }
-    l = warp_sum_d(l);
-    return (m == INFINITY ? (lx == INFINITY ? 1.0 : 0.0) : exp(((double) lx - m) * t)) / l;
+    const uint32_t some = __ballot_sync(0xffffffffu, w > NOTHING), above = __ballot_sync(0xffffffffu, w > NOTHING && front + upto > x);
+    const int at = above ? __ffs((int) above) - 1 : some ? 31 - __clz((int) some) : 0;
+    front += __shfl_sync(0xffffffffu, upto - w, at);
+    return at;
 }
 
-template <typename T, bool HELD>     // HELD: the rows lie in shared memory
-__global__ void __launch_bounds__(VD_THREADS) k_verify_draw(const __grid_constant__ Verify A) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ VdSmem S;
-    float * const held = reinterpret_cast<float *>(smem_raw);
+// a row's chunks, two to a lane of a warp
+struct Chunks {
+    float4 p[VERIFY_CHUNKS / 32];
+    __device__ __forceinline__ Chunks(const float4 * parts, int chunks) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int k = 0; k < VERIFY_CHUNKS / 32; k++) p[k] = lane + 32 * k < chunks ? __ldcg(&parts[lane + 32 * k]) : make_float4(-INFINITY, 0.f, __int_as_float(INT_MAX), 0.f);
+    }
+    __device__ __forceinline__ float top() const {
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < VERIFY_CHUNKS / 32; k++) m = fmaxf(m, p[k].x);
+        return warp_max(m);
+    }
+    __device__ __forceinline__ int first(float m) const {           // of the largest
+        int arg = INT_MAX;
+#pragma unroll
+        for (int k = 0; k < VERIFY_CHUNKS / 32; k++)
+            if (p[k].x == m) arg = min(arg, __float_as_int(p[k].z));
+        return __reduce_min_sync(0xffffffffu, arg);
+    }
+    __device__ __forceinline__ double chance(int x, float lx, float t, const double * roots) const {   // p(x)
+        const float m = top();
+        if (m == -INFINITY || !(t >= 0.f)) return 0.0;
+        if (t == INFINITY) return first(m) == x ? 1.0 : 0.0;
+        const Weights w(m, t, roots);
+        double l = 0.0;
+#pragma unroll
+        for (int k = 0; k < VERIFY_CHUNKS / 32; k++)
+            if (p[k].x > -INFINITY) l += p[k].y * w(p[k].x);
+        l = warp_sum_d(l);
+        return lx > -INFINITY ? w(lx) / l : 0.0;
+    }
+};
+
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) k_verify_draw(const __grid_constant__ Verify A) {
+    constexpr int THREADS = 32 * WARPS;
+    __shared__ VdSmem<WARPS> S;
     const uint32_t rank = cluster_rank(), ctas = cluster_size();
     const int s = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // this CTA's tiles of the vocabulary: as many to each
-    const int tiles = (A.vocab + VD_TILE - 1) / VD_TILE, t0 = (int) ((int64_t) tiles * rank / ctas), t1 = (int) ((int64_t) tiles * (rank + 1) / ctas);
-    const int base = t0 * VD_TILE, n = max(0, min(A.vocab, t1 * VD_TILE) - base);
     const int64_t a = A.start[s], b = A.start[s + 1];
     const bool good = a >= 0 && b >= a && b <= A.n_drafts;
     const int drafts = good ? (int) (b - a) : 0;
     const float t = inv_temp_of(A, s);
     if (tid == 0) S.first = drafts;
+    if (tid < 16) S.roots[tid] = exp2(tid * 0.0625);
+    // this warp's first draft: what is known of it ahead of the rows' sums
+    int token = -1;
+    float of_p = -INFINITY, of_q = -INFINITY, u = 0.f;
+    auto ask = [&](int i) {
+        token = A.tokens[a + i];
+        u = A.u[a + i];
+        if (token < 0 || token >= A.vocab) return;
+        of_p = get((const T *) A.target + (a + i + s) * A.ld_target + token);
+        if (A.draft) of_q = get((const T *) A.draft + (a + i) * A.ld_draft + token);
+    };
+    if (warp < drafts) ask(warp);
     __syncthreads();
     pdl_wait();                                             // the rows' sums
-    if (good)
-        for (int i = warp; i < drafts; i += VD_THREADS / 32) {
-            const int64_t d = a + i;
-            const int x = A.tokens[d];
-            bool ok = false;
-            if (x >= 0 && x < A.vocab) {
-                const double p = chance(A.parts + d * A.chunks, A.chunks, x, get((const T *) A.target + (d + s) * A.ld_target + x), t);
-                const double q = A.draft ? chance(A.parts + (A.n_drafts + d) * A.chunks, A.chunks, x, get((const T *) A.draft + d * A.ld_draft + x), t) : 1.0;
-                ok = (double) A.u[d] * q < p;
-            }
-            if (!ok && lane == 0) atomicMin(&S.first, i);
+    if (!good) return;                                      // (all CTAs of the cluster)
+    for (int i = warp; i < drafts; i += WARPS) {
+        if (i != warp) ask(i);
+        bool ok = false;
+        if (token >= 0 && token < A.vocab) {
+            const Chunks p(A.parts + (a + i) * A.chunks, A.chunks), q(A.parts + (A.draft ? A.n_drafts + a + i : a + i) * A.chunks, A.chunks);
+            ok = (double) u * (A.draft ? q.chance(token, of_q, t, S.roots) : 1.0) < p.chance(token, of_p, t, S.roots);
         }
+        if (!ok && lane == 0) atomicMin(&S.first, i);
+    }
     __syncthreads();
     const int acc = S.first;
-    if (!good) return;                                      // (all CTAs of the cluster)
-    const bool rejected = acc < drafts, two = rejected && A.draft;
+    const bool rejected = acc < drafts;
     const int out_of = rejected && !A.draft ? A.tokens[a + acc] : -1;       // a token whose weight is 0
-    const T * const row_p = (const T *) A.target + (a + s + acc) * A.ld_target, * const row_q = two ? (const T *) A.draft + (a + acc) * A.ld_draft : nullptr;
-
-    // ---- the rows, and their largest logits ----
-    auto block_max = [&](float & x, float & y) {
-        x = warp_max(x);
-        y = warp_max(y);
-        if (lane == 0) { S.warp[warp][0] = x; S.warp[warp][1] = y; }
-        __syncthreads();
-        for (int w = 0; w < VD_THREADS / 32; w++) { x = fmaxf(x, (float) S.warp[w][0]); y = fmaxf(y, (float) S.warp[w][1]); }
-        __syncthreads();
-    };
-    float m[2] = {-INFINITY, -INFINITY};
-    int arg = INT_MAX;
-    auto take = [&](const T * row, float * to, float & top) {
-        constexpr int VEC = vec<T>();
-        const T * src = row + base;
-        const int skew = skew_of(src), vecs = n > 0 ? (n + skew + VEC - 1) / VEC : 0;
-        for (int v0 = tid; v0 < vecs; v0 += 4 * VD_THREADS) {
-            float x[4][VEC];
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (v0 + k * VD_THREADS < vecs) get_vec(src, n, skew, v0 + k * VD_THREADS, x[k]);
-                else
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) x[k][e] = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const int at = (v0 + k * VD_THREADS) * VEC - skew + e;
-                    if (at < 0 || at >= n) continue;
-                    if (x[k][e] > top) {
-                        top = x[k][e];
-                        if (row == row_p) arg = base + at;
-                    }
-                    if (HELD) to[at] = x[k][e];
-                }
-        }
-    };
-    const int room = (n + 3) & ~3;
-    take(row_p, held, m[0]);
-    const float mine = m[0];
-    if (two) take(row_q, held + room, m[1]);
-    block_max(m[0], m[1]);
-    if (t == INFINITY) {       // the first of the largest: (that of a thread is the first of its own)
-        int first = mine == m[0] ? arg : INT_MAX;
-        first = __reduce_min_sync(0xffffffffu, first);
-        if (lane == 0) S.warp[warp][0] = first;
-        __syncthreads();
-        for (int w = 0; w < VD_THREADS / 32; w++) first = min(first, (int) S.warp[w][0]);
-        arg = first;
-    }
-    if (tid == 0) { S.mine[0] = m[0]; S.mine[1] = m[1]; S.mine[2] = arg; }
-    cluster_sync();
-    int first = INT_MAX;
-    for (uint32_t r = 0; r < ctas; r++) { m[0] = fmaxf(m[0], (float) remote(&S.mine[0], r)); m[1] = fmaxf(m[1], (float) remote(&S.mine[1], r)); }
-    for (uint32_t r = 0; r < ctas; r++)
-        if ((float) remote(&S.mine[0], r) == m[0]) first = min(first, (int) remote(&S.mine[2], r));
-    auto finish = [&](int token) {                          // by one thread of the cluster
-        if (acc < A.ld_out) A.out[s * A.ld_out + acc] = token;
-    };
+    const T * const row_p = (const T *) A.target + (a + s + acc) * A.ld_target, * const row_q = rejected && A.draft ? (const T *) A.draft + (a + acc) * A.ld_draft : nullptr;
     if (rank == 0) {
-        for (int64_t i = tid; i < acc && i < A.ld_out; i += VD_THREADS) A.out[s * A.ld_out + i] = A.tokens[a + i];
+        for (int64_t i = tid; i < acc && i < A.ld_out; i += THREADS) A.out[s * A.ld_out + i] = A.tokens[a + i];
         if (tid == 0) {
             A.accepted[s] = acc;
             if (A.kv_len) A.kv_len_out[s] = A.kv_len[s] - (drafts - acc);
         }
     }
+    // this CTA's part of the vocabulary, and this warp's, both even to a load of a warp
+    const int loads = (A.vocab + 31) / 32, l0 = (int) ((int64_t) loads * rank / ctas), l1 = (int) ((int64_t) loads * (rank + 1) / ctas);
+    const int from = 32 * (l0 + (int) ((int64_t) (l1 - l0) * warp / WARPS)), to = min(A.vocab, 32 * (l0 + (int) ((int64_t) (l1 - l0) * (warp + 1) / WARPS)));
+
+    // ---- the rows' largest logits: of those that were looked at, from their chunks ----
+    float m[2] = {-INFINITY, -INFINITY};
+    int arg = INT_MAX;
+    if (rejected) {
+        const Chunks p(A.parts + (a + acc) * A.chunks, A.chunks), q(A.parts + (row_q ? A.n_drafts + a + acc : a + acc) * A.chunks, A.chunks);
+        m[0] = p.top();
+        m[1] = q.top();
+        arg = p.first(m[0]);
+    } else {
+        constexpr int ONCE = 8;
+            for (int i0 = from + lane; i0 < to; i0 += 32 * ONCE) {
+                float x[ONCE];
+#pragma unroll
+                for (int k = 0; k < ONCE; k++) x[k] = i0 + 32 * k < to ? raw(row_p + i0 + 32 * k) : -INFINITY;
+#pragma unroll
+                for (int k = 0; k < ONCE; k++)
+                    if (x[k] > m[0]) { m[0] = x[k]; arg = i0 + 32 * k; }
+            }
+    }
+    if (!rejected) {
+        const float own = m[0];
+        m[0] = warp_max(m[0]);
+        arg = __reduce_min_sync(0xffffffffu, own == m[0] && own > -INFINITY ? arg : INT_MAX);
+        if (lane == 0) { S.warp[warp][0] = m[0]; S.warp[warp][1] = arg; }
+        __syncthreads();
+        const float top = lane < WARPS ? (float) S.warp[lane % WARPS][0] : -INFINITY, most = warp_max(top);
+        const int first = __reduce_min_sync(0xffffffffu, top == most && lane < WARPS ? (int) S.warp[lane % WARPS][1] : INT_MAX);
+        if (tid == 0) { S.top = most; S.arg = first; }
+        cluster_sync();
+        const float far = lane < ctas ? remote(&S.top, lane % ctas) : -INFINITY;
+        m[0] = warp_max(far);
+        arg = __reduce_min_sync(0xffffffffu, far == m[0] && lane < ctas ? remote(&S.arg, lane % ctas) : INT_MAX);
+    }
     if (m[0] == -INFINITY || !(t >= 0.f) || t == INFINITY) {       // no weights; all of it on one
-        if (rank == 0 && tid == 0) finish(m[0] == -INFINITY || !(t >= 0.f) ? -1 : first);
-        cluster_sync();                                     // (the others read this CTA's numbers)
+        if (rank == 0 && tid == 0 && acc < A.ld_out) A.out[s * A.ld_out + acc] = t == INFINITY && m[0] > -INFINITY ? arg : -1;
+        cluster_sync();                                     // (others read this CTA's numbers)
         return;
     }
 
     // ---- weights ----
-    auto weight = [&](float x, float top) { return top == INFINITY ? (x == INFINITY ? 1.0 : 0.0) : exp(((double) x - top) * t); };
-    auto load = [&](int which, int i) {                     // logit i of this CTA's
-        if (HELD) return held[which * room + i];
-        return get((which ? row_q : row_p) + base + i);
+    const Weights wp(m[0], t, S.roots), wq(m[1], t, S.roots);
+    const bool minus_q = row_q && m[1] > -INFINITY;         // (a draft row without a number takes nothing away)
+    constexpr int ONCE = 4;
+    // f(first entry, logits of p, of q) for the entries i0 .. i1 - 1, ONCE of a lane at a time, 32 entries from each other; those outside are -inf
+    auto walk = [&](int i0, int i1, auto && f) {
+        for (i0 += lane; i0 < i1; i0 += 32 * ONCE) {
+            float lp[ONCE], lq[ONCE];
+#pragma unroll
+            for (int k = 0; k < ONCE; k++) {
+                lp[k] = i0 + 32 * k < i1 ? raw(row_p + i0 + 32 * k) : -INFINITY;
+                lq[k] = minus_q && i0 + 32 * k < i1 ? raw(row_q + i0 + 32 * k) : -INFINITY;
+            }
+            f(i0, lp, lq);
+        }
     };
-    auto block_sum = [&](double & x, double & y) {
+    auto add_up = [&](const double (&w)[ONCE]) {
+        double x = w[0];
+#pragma unroll
+        for (int k = 1; k < ONCE; k++) x += w[k];
+        return x;
+    };
+    double z[2] = {1.0, 0.0};
+    if (minus_q) {
+        double x = 0.0, y = 0.0;
+        walk(from, to, [&](int, const float (&lp)[ONCE], const float (&lq)[ONCE]) {
+            double p[ONCE], q[ONCE];
+            wp(lp, p);
+            wq(lq, q);
+            x += add_up(p);
+            y += add_up(q);
+        });
         x = warp_sum_d(x);
         y = warp_sum_d(y);
-        __syncthreads();
         if (lane == 0) { S.warp[warp][0] = x; S.warp[warp][1] = y; }
         __syncthreads();
-        x = y = 0.0;
-        for (int w = 0; w < VD_THREADS / 32; w++) { x += S.warp[w][0]; y += S.warp[w][1]; }
-    };
-    double z[2] = {0.0, 0.0};
-    const bool residual_q = two && m[1] > -INFINITY;        // (a draft row without a number takes nothing away)
-    if (residual_q) {
-        for (int i = tid; i < n; i += VD_THREADS) {
-            z[0] += weight(load(0, i), m[0]);
-            z[1] += weight(load(1, i), m[1]);
+        if (warp == 0) {
+            x = warp_sum_d(lane < WARPS ? S.warp[lane % WARPS][0] : 0.0);
+            y = warp_sum_d(lane < WARPS ? S.warp[lane % WARPS][1] : 0.0);
+            if (lane == 0) { S.z[0] = x; S.z[1] = y; }
         }
-        block_sum(z[0], z[1]);
-        if (tid == 0) { S.mine[3] = z[0]; S.mine[4] = z[1]; }
         cluster_sync();
-        z[0] = z[1] = 0.0;
-        for (uint32_t r = 0; r < ctas; r++) { z[0] += remote(&S.mine[3], r); z[1] += remote(&S.mine[4], r); }
+        z[0] = warp_sum_d(lane < ctas ? remote(&S.z[0], lane % ctas) : 0.0);
+        z[1] = warp_sum_d(lane < ctas ? remote(&S.z[1], lane % ctas) : 0.0);
     }
-    // entry i's weight, of the distribution at hand and of p
-    auto entry = [&](int i, bool rest) {
-        const double e = weight(load(0, i), m[0]);
-        if (!rest) return e;
-        if (residual_q) return fmax(e * z[1] - weight(load(1, i), m[1]) * z[0], 0.0);
-        return base + i == out_of ? 0.0 : e;
+    bool rest = minus_q || out_of >= 0;                     // max(p - q, 0), or p
+    auto weights = [&](int i0, int step, const float (&lp)[ONCE], const float (&lq)[ONCE], double (&w)[ONCE]) {
+        wp(lp, w);
+        if (rest && minus_q) {
+            double q[ONCE];
+            wq(lq, q);
+#pragma unroll
+            for (int k = 0; k < ONCE; k++) w[k] = fmax(fma(w[k], z[1], -q[k] * z[0]), 0.0);
+        } else if (rest)
+#pragma unroll
+            for (int k = 0; k < ONCE; k++) w[k] = i0 + step * k == out_of ? 0.0 : w[k];
     };
-    bool rest = residual_q || out_of >= 0;
-    for (;;) {
-        double all = 0.0;
-        for (int k = 0; k < t1 - t0; k++) {                 // (tiles beyond the first VD_TILES are added to the last)
-            double x = 0.0, y = 0.0;
-            for (int i = k * VD_TILE + tid; i < min(n, (k + 1) * VD_TILE); i += VD_THREADS) x += entry(i, rest);
-            block_sum(x, y);
-            if (tid == 0) S.tile[0][min(k, VD_TILES - 1)] = k < VD_TILES ? x : S.tile[0][VD_TILES - 1] + x;
-            all += x;
-        }
+    // The warps' sums; the CTA and the warp in whose entries the token is; that warp's entries, in as many pieces, once more; the piece
+    double x = 0.0, front = 0.0;
+    int lo = from, hi = to, w0 = 0, w1 = 0, piece = 0;
+    for (int round = 0;; round++) {
+        double mine = 0.0;
+        walk(lo, hi, [&](int at, const float (&lp)[ONCE], const float (&lq)[ONCE]) {
+            double w[ONCE];
+            weights(at, 32, lp, lq, w);
+            mine += add_up(w);
+        });
+        mine = warp_sum_d(mine);
         __syncthreads();
-        if (tid == 0) S.mine[rest ? 5 : 6] = all;
+        if (lane == 0) S.warp[warp][0] = mine;
+        __syncthreads();
+        mine = lane < WARPS ? S.warp[lane % WARPS][0] : 0.0;
+        if (piece > 0) {
+            lo = w0 + piece * find(mine, x, front);
+            hi = min(w1, lo + piece);
+            break;
+        }
+        const double all = warp_sum_d(mine);
+        if (tid == 0) S.all[round] = all;
         cluster_sync();
-        double total = 0.0, front = 0.0;
-        for (uint32_t r = 0; r < ctas; r++) total += remote(&S.mine[rest ? 5 : 6], r);
-        if (rest && !(total > 0.0)) {                        // nothing is left: from p
+        const double far = lane < ctas ? remote(&S.all[round], lane % ctas) : 0.0, total = warp_sum_d(far);
+        if (!(total > NOTHING) && rest) {                   // nothing is left: from p
             rest = false;
             continue;
         }
-        const double x = (double) A.v[s] * total;
-        int owner = 0;
-        double cum = 0.0;
-        // the first CTA whose end lies beyond x; where rounding leaves none, the last that has any
-        for (uint32_t r = 0; r < ctas; r++) {
-            const double w = remote(&S.mine[rest ? 5 : 6], r);
-            if (w > 0.0) {
-                owner = (int) r;
-                front = cum;
-                if (cum + w > x) break;
-            }
-            cum += w;
-        }
+        x = (double) A.v[s] * total;
+        const int owner = find(far, x, front);
         cluster_sync();                                     // nobody reads this CTA's numbers from here on
         if (owner != (int) rank) return;
-        // the tile, in the same way
-        int tile = 0;
-        double before = front;
-        cum = front;
-        for (int k = 0; k < min(t1 - t0, VD_TILES); k++) {
-            const double w = S.tile[0][k];
-            if (w > 0.0) {
-                tile = k;
-                before = cum;
-                if (cum + w > x) break;
-            }
-            cum += w;
-        }
-        // the entry
-        if (tid == 0) { S.first = INT_MAX; S.found = 0; }
-        for (int k = tile;; k++) {
-            double w[VD_EACH], sum = 0.0;
-            const int i0 = k * VD_TILE + tid * VD_EACH;
-#pragma unroll
-            for (int e = 0; e < VD_EACH; e++) {
-                w[e] = i0 + e < n ? entry(i0 + e, rest) : 0.0;
-                sum += w[e];
-            }
-            double upto = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
-            __syncthreads();
-            if (lane == 31) S.warp[warp][0] = upto;
-            __syncthreads();
-            double c = before, end = before;
-            for (int j = 0; j < VD_THREADS / 32; j++) {
-                if (j < warp) c += S.warp[j][0];
-                end += S.warp[j][0];
-            }
-            c += upto - sum;
-#pragma unroll
-            for (int e = 0; e < VD_EACH; e++) {
-                c += w[e];
-                if (w[e] > 0.0) {
-                    atomicMax(&S.found, i0 + e);
-                    if (c > x) atomicMin(&S.first, i0 + e);
-                }
-            }
-            __syncthreads();
-            const bool last = tile < VD_TILES - 1 || k == t1 - t0 - 1;
-            if (S.first != INT_MAX || last) {
-                if (tid == 0) finish(base + (S.first != INT_MAX ? S.first : S.found));
-                return;
-            }
-            before = end;
-        }
+        const int w = find(mine, x, front);
+        w0 = 32 * (l0 + (int) ((int64_t) (l1 - l0) * w / WARPS));
+        w1 = min(A.vocab, 32 * (l0 + (int) ((int64_t) (l1 - l0) * (w + 1) / WARPS)));
+        piece = ((w1 - w0 + WARPS - 1) / WARPS + 31) & ~31;
+        lo = w0 + warp * piece;
+        hi = min(w1, lo + piece);
     }
+    if (warp != 0) return;
+    // an even part of them to each lane, until a part is one entry
+    while (hi - lo > 1) {
+        const int each = (hi - lo + 31) / 32, i0 = min(hi, lo + lane * each), i1 = min(hi, i0 + each);
+        double own = 0.0;
+        for (int i = i0; i < i1; i += ONCE) {
+            float lp[ONCE], lq[ONCE];
+            double some[ONCE];
+#pragma unroll
+            for (int k = 0; k < ONCE; k++) {
+                lp[k] = i + k < i1 ? raw(row_p + i + k) : -INFINITY;
+                lq[k] = i + k < i1 && minus_q ? raw(row_q + i + k) : -INFINITY;
+            }
+            weights(i, 1, lp, lq, some);
+            own += add_up(some);
+        }
+        const int at = find(own, x, front);
+        lo += at * each;
+        hi = min(hi, lo + each);
+    }
+    if (lane == 0 && acc < A.ld_out) A.out[s * A.ld_out + acc] = lo;
 }
 
 template <typename T>
@@ -440,14 +504,11 @@ int verify_launch(const Verify & A, cudaStream_t st) {
         if (e != cudaSuccess) return (int) e;
         g_launches++;
     }
-    const int tiles = (A.vocab + VD_TILE - 1) / VD_TILE, ctas = tiles >= 8 ? 8 : tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
-    const size_t rows = (size_t) ((tiles + ctas - 1) / ctas) * VD_TILE * sizeof(float), smem = rows * (A.draft ? 2 : 1);
-    const bool held = smem <= VD_SMEM;
-    static FuncAttrCache cache[2];
-    const void * fn = held ? (const void *) k_verify_draw<T, true> : (const void *) k_verify_draw<T, false>;
-    cudaError_t e = ensure_dyn_smem(cache[held], fn, held ? VD_SMEM : 0, false);
-    if (e != cudaSuccess) return (int) e;
-    e = held ? launch_clusters(k_verify_draw<T, true>, A.n_seq, ctas, VD_THREADS, smem, A.n_drafts > 0, st, A) : launch_clusters(k_verify_draw<T, false>, A.n_seq, ctas, VD_THREADS, 0, A.n_drafts > 0, st, A);
+    const int ctas = A.vocab > 16384 ? 8 : A.vocab > 8192 ? 4 : A.vocab > 4096 ? 2 : 1;
+    const int64_t warps = 32 * sm_count() / ((int64_t) A.n_seq * ctas);
+    const bool after = A.n_drafts > 0;
+    const cudaError_t e = warps >= 16 ? launch_clusters(k_verify_draw<T, 16>, A.n_seq, ctas, 512, 0, after, st, A)
+                                      : launch_clusters(k_verify_draw<T, 8>, A.n_seq, ctas, 256, 0, after, st, A);
     if (e == cudaSuccess) g_launches++;
     return (int) e;
 }
@@ -458,12 +519,15 @@ int verify_launch(const Verify & A, cudaStream_t st) {
 using namespace pb;
 
 namespace {
-constexpr int VERIFY_CHUNKS = 64;      // of a row, at most
-// rows over enough CTAs to fill the GPU, each with a batch of loads at least
+// Chunks of a row: as many CTAs as the GPU runs at once take a round; that number of chunks whose rounds of whole batches of loads, and a batch's time for each CTA's start and end, are fewest
 int chunks_of(int64_t rows, int vocab, int elem) {
-    const int64_t least = (int64_t) VR_ONCE * VR_THREADS * 16 / elem, most = (vocab + least - 1) / least, want = (16 * sm_count() + rows - 1) / rows;
-    const int64_t n = want < most ? want : most;
-    return (int) (n < 1 ? 1 : n > VERIFY_CHUNKS ? VERIFY_CHUNKS : n);
+    const int64_t batch = (int64_t) VR_ONCE * VR_THREADS * 16 / elem, batches = (vocab + batch - 1) / batch, at_once = VR_CTAS * sm_count();
+    int64_t best = 1, cost = INT64_MAX;
+    for (int64_t n = 1; n <= VERIFY_CHUNKS && n <= batches; n++) {
+        const int64_t k = (rows * n + at_once - 1) / at_once * ((batches + n - 1) / n + 1);
+        if (k < cost) { cost = k; best = n; }
+    }
+    return (int) best;
 }
 }  // namespace
 
