@@ -177,9 +177,9 @@ int pb200_kv4_weigh(const pb200_kv4_cache * c, int layer, int type, const void *
     if (!sums || ((uintptr_t) sums & 3) || ld_sums <= 0 || (old && (((uintptr_t) old & 3) || ld_old < ld_sums))) return PB200_EINVAL;
     // a sum is read and written by the same thread: in place, or apart
     if (old && n_seq > 0 && !(old == sums && ld_old == ld_sums) && overlap(old, ld_old, ld_sums, sums, ld_sums, ld_sums, n_seq, 4)) return PB200_EINVAL;
-    // what the kernel counts in 31 bits: items (256 cells of a sequence), rows, blocks of rows of all heads
+    // what the kernels count in 31 bits: cells, pages of all sequences, rows, blocks of rows of all heads
     const double rows = std::min((double) max_q, (double) n_tokens) * (n_head / c->n_head_kv);
-    if ((double) n_seq * (std::min<double>((double) ld_sums, (double) INT32_MAX) / 256 + 1) >= 2147483648.0 - 65536 || rows >= 2147483648.0 || (rows / 64 + 1) * c->n_head_kv >= 2147483648.0)
+    if (ld_sums > INT32_MAX - 4096 || (double) n_seq * ((double) ld_sums / PB200_KV4_CELLS + 1) >= 2147483648.0 - 65536 || rows >= 2147483648.0 || (rows / 64 + 1) * c->n_head_kv >= 2147483648.0)
         return PB200_ENOTSUP;
     if (n_seq == 0) return 0;
     Kv4Attn a{layer_of(c, layer), q, ldq, nullptr, 0, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};

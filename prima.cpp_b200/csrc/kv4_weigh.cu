@@ -41,6 +41,83 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// ---- a query row in shared memory, a part of it to each of four threads next to each other ----
+// its power of two: the largest number comes to 2^13 .. 2^14
+template <int EACH>
+__device__ __forceinline__ float row_power(const float (&x)[EACH], float top) {
+#pragma unroll
+    for (int i = 0; i < EACH; i++) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int ex = top > 0.f && top < INFINITY ? min(126, 140 - (int) (__float_as_uint(top) >> 23)) : 0;
+    return __int_as_float((ex + 127) << 23);
+}
+template <typename T, int EACH>
+__device__ __forceinline__ void row_store(const float (&x)[EACH], float up, uint8_t * high, uint8_t * low) {
+#pragma unroll
+    for (int i = 0; i < EACH; i += 8) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = x[i + 2 * e] * up, b = x[i + 2 * e + 1] * up;
+            const __half2 h = __floats2half2_rn(a, b);
+            hi[e] = hu(h);
+            if constexpr (std::is_same<T, float>::value) {
+                const float2 back = __half22float2(h);
+                lo[e] = hu(__floats2half2_rn(a - back.x, b - back.y));
+            }
+        }
+        *reinterpret_cast<uint4 *>(high + 2 * i) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (std::is_same<T, float>::value) *reinterpret_cast<uint4 *>(low + 2 * i) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+// of a score to the power of two (never 0: a masked score stays -inf), and the logarithm of the row's sum; a row that saw nothing has no weights
+__device__ __forceinline__ float2 row_factors(float scale, float up, float lse) {
+    return make_float2(fmaxf(fabsf(scale) * 1.4426950408889634f * __int_as_float((254 << 23) - (__float_as_int(up) & 0x7f800000)), FLT_MIN), lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f);
+}
+// ---- keys: eight numbers of each block of a cell, as the rows h of an A operand of 16 cells; odd: the cell, whose scales lie behind its even neighbour's ----
+template <int D>
+__device__ __forceinline__ void key_halves(const uint8_t * row, const uint8_t * scales, int odd, uint32_t (&kf)[D / 32][2][4], int h) {
+    constexpr int NB = D / 32;
+    uint32_t w[NB], d[NB];
+    if constexpr (NB == 4) {
+        *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(row);
+        *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(scales);
+    } else {
+        *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(row);
+        *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(scales);
+    }
+    const __half2 e = __float2half2_rn(1032.f), o = __float2half2_rn(72.f);        // 1024 + 8, 64 + 8
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const __half2 sc = uh(__byte_perm(d[b], 0u, odd ? 0x3232u : 0x1010u));
+        const uint32_t x = w[b], y = w[b] >> 8;
+        kf[b][0][h] = hu(__hmul2(__hsub2(uh((x & 0x000f000fu) | 0x64006400u), e), sc));
+        kf[b][0][2 + h] = hu(__hmul2(__hsub2(uh((x & 0x00f000f0u) | 0x54005400u), o), sc));
+        kf[b][1][h] = hu(__hmul2(__hsub2(uh((y & 0x000f000fu) | 0x64006400u), e), sc));
+        kf[b][1][2 + h] = hu(__hmul2(__hsub2(uh((y & 0x00f000f0u) | 0x54005400u), o), sc));
+    }
+}
+// scores of 32 cells and eight rows: lane: cells 16 m + g, + 8 of rows 2 c, 2 c + 1; q: this lane's part of row g, the low parts `low` bytes further on: these first (what is added to a sum is cut off)
+template <int LO, int NB>
+__device__ __forceinline__ void scores(const uint32_t (&kf)[2][NB][2][4], const uint8_t * q, size_t low, float (&acc)[2][4]) {
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[m][i] = 0.f;
+#pragma unroll
+    for (int part = LO - 1; part >= 0; part--)
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(q + part * low + 64 * b);
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                mma16816(acc[m], kf[m][b][0], x.x, x.y);
+                mma16816(acc[m], kf[m][b][1], x.z, x.w);
+            }
+        }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_constant__ Kv4Weigh W) {
     constexpr bool F32 = std::is_same<T, float>::value;
@@ -118,23 +195,7 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const int t = in_page + 16 * m + 8 * h + g;
-                        uint32_t w[NB], d[NB];
-                        if constexpr (NB == 4) {
-                            *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(chunk + t * (D / 2) + 16 * c);
-                            *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(scales + kv4_scale(D, t & ~1, 0));
-                        } else {
-                            *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(chunk + t * (D / 2) + 8 * c);
-                            *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(scales + kv4_scale(D, t & ~1, 0));
-                        }
-#pragma unroll
-                        for (int b = 0; b < NB; b++) {
-                            const __half2 sc = uh(__byte_perm(d[b], 0u, t & 1 ? 0x3232u : 0x1010u)), e = __float2half2_rn(1032.f), o = __float2half2_rn(72.f);
-                            const uint32_t x = w[b], y = w[b] >> 8;
-                            kf[m][b][0][h] = hu(__hmul2(__hsub2(uh((x & 0x000f000fu) | 0x64006400u), e), sc));
-                            kf[m][b][0][2 + h] = hu(__hmul2(__hsub2(uh((x & 0x00f000f0u) | 0x54005400u), o), sc));
-                            kf[m][b][1][h] = hu(__hmul2(__hsub2(uh((y & 0x000f000fu) | 0x64006400u), e), sc));
-                            kf[m][b][1][2 + h] = hu(__hmul2(__hsub2(uh((y & 0x00f000f0u) | 0x54005400u), o), sc));
-                        }
+                        key_halves<D>(chunk + t * (D / 2) + 4 * NB * c, scales + kv4_scale(D, t & ~1, 0), t & 1, kf[m], h);
                     }
                 held = hk;
             }
@@ -152,32 +213,10 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
                     x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
                 }
                 const float lse = have ? W.lse[(q0 + t) * W.ld_lse + head] : -INFINITY;
-#pragma unroll
-                for (int i = 0; i < EACH; i++) top = fmaxf(top, fabsf(x[i]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // the row's power of two: its largest number comes to 2^13 .. 2^14
-                const int ex = top > 0.f && top < INFINITY ? min(126, 140 - (int) (__float_as_uint(top) >> 23)) : 0;
-                const float up = __int_as_float((ex + 127) << 23) * (A.scale < 0.f ? -1.f : 1.f);
-#pragma unroll
-                for (int i = 0; i < EACH; i += 8) {
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float a = x[i + 2 * e] * up, b = x[i + 2 * e + 1] * up;
-                        const __half2 h = __floats2half2_rn(a, b);
-                        hi[e] = hu(h);
-                        if constexpr (F32) {
-                            const float2 back = __half22float2(h);
-                            lo[e] = hu(__floats2half2_rn(a - back.x, b - back.y));
-                        }
-                    }
-                    *reinterpret_cast<uint4 *>(&S.q[0][r][2 * (quarter * EACH + i)]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (F32) *reinterpret_cast<uint4 *>(&S.q[LO - 1][r][2 * (quarter * EACH + i)]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
+                const float up = row_power<EACH>(x, top) * (A.scale < 0.f ? -1.f : 1.f);
+                row_store<T, EACH>(x, up, &S.q[0][r][2 * quarter * EACH], &S.q[LO - 1][r][2 * quarter * EACH]);
                 if (quarter == 0) {
-                    // a row that saw nothing has no weights
-                    S.row[r] = make_float2(fmaxf(fabsf(A.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23), FLT_MIN), lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f);
+                    S.row[r] = row_factors(A.scale, up, lse);
                     S.pos[r] = have ? p0 + t : -1;
                 }
             }
@@ -187,18 +226,8 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
             const bool whole = cell0 + 31 <= p_lo && (A.window <= 0 || p_hi - cell0 < A.window || cell0 + 31 < A.first);
 #pragma unroll 1
             for (int j = 0; j < n; j += 8) {
-                float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                for (int part = LO - 1; part >= 0; part--)
-#pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        const uint4 q = *reinterpret_cast<const uint4 *>(&S.q[part][j + g][64 * b + 16 * c]);
-#pragma unroll
-                        for (int m = 0; m < 2; m++) {
-                            mma16816(acc[m], kf[m][b][0], q.x, q.y);
-                            mma16816(acc[m], kf[m][b][1], q.z, q.w);
-                        }
-                    }
+                float acc[2][4];
+                scores<LO, NB>(kf, &S.q[0][j + g][16 * c], sizeof(S.q[0]), acc);
                 const float4 r = *reinterpret_cast<const float4 *>(&S.row[j + 2 * c]);
                 float e[2][4];
 #pragma unroll
@@ -243,13 +272,281 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
     }
 }
 
+// ---- few rows ----
+// Pages stream through shared memory, by bulk copies: a warp has the keys of a page and a kv head at a time, the next ones on their way.  A unit is as many pages of a sequence as give each warp a
+// kv head of one; a CTA has a contiguous share of all units.  The queries of all heads lie in shared memory while it is at their sequence.
+constexpr int KF_WARPS = 16, KF_THREADS = 32 * KF_WARPS;
+__host__ __device__ constexpr int kf_bytes(int D) { return kv4_rows_bytes(D) + kv4_scales_bytes(D); }     // of a page's keys
+template <int D> constexpr int kf_stages() { return D == 128 ? 2 : 4; }
+constexpr size_t KF_QUERIES = 64 * 1024;
+
+template <int D> struct __align__(128) KfSmem {
+    __align__(128) uint8_t ring[KF_WARPS][kf_stages<D>()][kf_bytes(D)];
+    uint64_t full[KF_WARPS][kf_stages<D>()];
+    float part[2][KF_WARPS][KV4_CELLS];
+    int scan[KF_WARPS], begin_s, begin_unit, abort;
+};
+// behind it: of all rows (kv head by kv head) and eight more the numbers (F32: high, then low parts), what makes their weights, the positions of a kv head's
+template <typename T, int D> __host__ __device__ constexpr size_t kf_row_bytes() { return (std::is_same<T, float>::value ? 2 : 1) * (2 * D + 64) + sizeof(float2); }
+
+// a sequence: its queries, positions, cells and units
+struct KfSeq {
+    int64_t q0;
+    int n_q, p0, len, units;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_constant__ Kv4Weigh W, int * abort_flag, int most_rows) {
+    constexpr bool F32 = std::is_same<T, float>::value;
+    constexpr int NB = D / 32, LO = F32 ? 2 : 1, STAGES = kf_stages<D>(), STRIDE = 2 * D + 64;
+    extern __shared__ uint8_t smem_raw[];
+    KfSmem<D> & S = *reinterpret_cast<KfSmem<D> *>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
+    const Kv4Attn & A = W.attn;
+    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp(), g = lane >> 2, c = lane & 3, hks = A.cache.n_head_kv;
+    uint8_t * const queries = reinterpret_cast<uint8_t *>(&S + 1);
+    const int room = hks * most_rows + 8;                   // rows
+    float2 * const factors = reinterpret_cast<float2 *>(queries + (size_t) room * STRIDE * LO);
+    int * const pos = reinterpret_cast<int *>(factors + room);
+    volatile int * cta_abort = &S.abort;
+    // pages of a unit; this warp's page of them and its first kv head (hks and more: none)
+    const int P = max(1, KF_WARPS / hks), my_page = P > 1 ? warp / hks : 0, my_head = P > 1 ? (my_page < P ? warp % hks : hks) : warp;
+
+    auto seq = [&](int s) {
+        KfSeq q{};
+        if (s >= A.n_seq) return q;
+        const int64_t a = A.q_start[s], b = A.q_start[s + 1];
+        const int cells = max(A.kv_len[s], 0);
+        q.len = (int) min((int64_t) cells, W.ld_sums);
+        q.units = ((q.len + KV4_CELLS - 1) / KV4_CELLS + P - 1) / P;
+        q.q0 = a;
+        q.p0 = cells;
+        if (a >= 0 && b > a && b <= A.n_tokens) {
+            q.p0 = cells - (int) (b - a);
+            q.n_q = min((int) (b - a), A.max_q);
+        }
+        return q;
+    };
+    // ---- the share: units in the order of sequences ----
+    if (lane < STAGES) {
+        mbar_init(&S.full[warp][lane], 1);
+        mbar_fence_init();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (tid == 0) S.abort = 0;
+    auto upto = [&](int x) {                                // sum over the threads up to this one, all: over all
+        int y = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) y += z;
+        }
+        __syncthreads();
+        if (lane == 31) S.scan[warp] = y;
+        __syncthreads();
+        return y;
+    };
+    int mine = 0;
+    for (int s = tid; s < A.n_seq; s += KF_THREADS) mine += seq(s).units;
+    upto(mine);
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < KF_WARPS; w++) total += S.scan[w];
+    const int u0 = (int) (total * blockIdx.x / gridDim.x), u1 = (int) (total * (blockIdx.x + 1) / gridDim.x);
+    if (u0 == u1) return;
+    for (int s0 = 0, before = 0; s0 < A.n_seq; s0 += KF_THREADS) {
+        const int n = seq(s0 + tid).units;
+        int x = upto(n) - n + before;
+#pragma unroll
+        for (int w = 0; w < KF_WARPS; w++) {
+            if (w < warp) x += S.scan[w];
+            before += S.scan[w];
+        }
+        if (u0 >= x && u0 < x + n) { S.begin_s = s0 + tid; S.begin_unit = u0 - x; }
+        if (u0 < before) break;
+    }
+    __syncthreads();
+
+    // ---- this warp's keys on their way: by units and, where there are more heads than warps, heads ----
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    int f_s = S.begin_s, f_unit = S.begin_unit, f_u = u0, f_head = my_head, f_n = 0;
+    KfSeq f_q = seq(f_s);
+    int ids = -1, ids0 = 0, ids1 = 0;                       // pages of the units ids0 .. ids1 - 1 of the sequence, one to a lane
+    uint32_t none = 0;                                      // stages whose page nobody sees, or that is none
+    auto sees = [&](const KfSeq & q, int base) {            // any query any of the page's cells
+        return q.n_q > 0 && base <= q.p0 + q.n_q - 1 && (A.window <= 0 || q.p0 - (base + KV4_CELLS - 1) < A.window || base < A.first);
+    };
+    auto fetch = [&] {
+        if (f_u >= u1 || f_head >= hks) return;
+        while (f_unit >= f_q.units) {
+            f_q = seq(++f_s);
+            f_unit = 0;
+            ids1 = 0;
+        }
+        if (f_unit >= ids1) {
+            const int at = (f_unit + lane) * P + my_page;
+            ids = at < A.table_ld && f_unit + lane < f_q.units && at * KV4_CELLS < f_q.len ? A.table[f_s * A.table_ld + at] : -1;
+            ids0 = f_unit;
+            ids1 = f_unit + 32;
+        }
+        int id = __shfl_sync(0xffffffffu, ids, f_unit - ids0);
+        if (id >= A.cache.n_pages || !sees(f_q, (f_unit * P + my_page) * KV4_CELLS)) id = -1;
+        const int st = f_n % STAGES;
+        none = id >= 0 ? none & ~(1u << st) : none | 1u << st;
+        if (elect_one()) {
+            if (id >= 0) {
+                const uint8_t * chunk = kv4_chunk<D>(A.cache, id, f_head);
+                mbar_arrive_expect_tx(&S.full[warp][st], kf_bytes(D));
+                bulk_g2s(S.ring[warp][st], chunk, kv4_rows_bytes(D), &S.full[warp][st], policy);
+                bulk_g2s(S.ring[warp][st] + kv4_rows_bytes(D), chunk + 2 * kv4_rows_bytes(D), kv4_scales_bytes(D), &S.full[warp][st], policy);
+            } else mbar_arrive(&S.full[warp][st]);
+        }
+        __syncwarp();
+        f_n++;
+        f_head += KF_WARPS;
+        if (P > 1 || f_head >= hks) {
+            f_head = my_head;
+            f_unit++;
+            f_u++;
+        }
+    };
+    for (int k = 0; k < STAGES; k++) fetch();
+
+    int s = S.begin_s, unit = S.begin_unit, n = 0;
+    bool fresh = true;
+    KfSeq q = seq(s);
+    for (int u = u0; u < u1; u++, unit++) {
+        while (unit >= q.units) {
+            q = seq(++s);
+            unit = 0;
+            fresh = true;
+        }
+        const int rows = q.n_q * A.group;
+        if (fresh) {   // ---- the sequence's queries: four threads to a row ----  (everybody is through with the last one's: behind the barrier of its last unit)
+            fresh = false;
+            for (int i0 = 0; i0 < hks * rows; i0 += KF_THREADS / 4) {
+                const int i = i0 + (tid >> 2), quarter = tid & 3, hk = i / max(rows, 1), r = i - hk * rows, t = r / A.group, head = hk * A.group + r - t * A.group;
+                const bool have = i < hks * rows;
+                constexpr int EACH = D / 4;
+                float x[EACH], top = 0.f;
+                const T * src = (const T *) A.q + (q.q0 + t) * A.ldq + (int64_t) head * D + quarter * EACH;
+#pragma unroll
+                for (int k = 0; k < EACH; k += 4) {
+                    const float4 v = have ? load4(src + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
+                }
+                const float lse = have ? W.lse[(q.q0 + t) * W.ld_lse + head] : -INFINITY;
+                const float up = row_power<EACH>(x, top) * (A.scale < 0.f ? -1.f : 1.f);
+                if (have) {
+                    row_store<T, EACH>(x, up, queries + (size_t) i * STRIDE + 2 * quarter * EACH, queries + (size_t) (room + i) * STRIDE + 2 * quarter * EACH);
+                    if (quarter == 0) {
+                        factors[i] = row_factors(A.scale, up, lse);
+                        if (hk == 0) pos[r] = q.p0 + t;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        float sum[4][2];
+#pragma unroll
+        for (int m = 0; m < 4; m++) sum[m][0] = sum[m][1] = 0.f;
+        const int base = (unit * P + my_page) * KV4_CELLS;
+        for (int hk = my_head; hk < hks; hk += P > 1 ? hks : KF_WARPS, n++) {
+            const int st = n % STAGES;
+            const bool have = !(none >> st & 1);
+            mbar_wait(&S.full[warp][st], (uint32_t) (n / STAGES) & 1, cta_abort, abort_flag);
+            if (have) {
+                const uint8_t * chunk = S.ring[warp][st], * scales = chunk + kv4_rows_bytes(D);
+                const int p_lo = q.p0, p_hi = q.p0 + q.n_q - 1;
+                const bool whole = base + KV4_CELLS - 1 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + KV4_CELLS - 1 < A.first);
+#pragma unroll 1
+                for (int m2 = 0; m2 < 2; m2++) {            // 32 cells at a time
+                    uint32_t kf[2][NB][2][4];
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int t = 32 * m2 + 16 * m + 8 * h + g;
+                            key_halves<D>(chunk + t * (D / 2) + 4 * NB * c, scales + kv4_scale(D, t & ~1, 0), t & 1, kf[m], h);
+                        }
+                    float acc2[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll 1
+                    for (int j = 0; j < rows; j += 8) {
+                        const int i = hk * rows + j;
+                        float e[2][4];
+                        scores<LO, NB>(kf, queries + (size_t) (i + g) * STRIDE + 16 * c, (size_t) room * STRIDE, e);
+                        const float2 r0 = factors[i + 2 * c], r1 = factors[i + 2 * c + 1];
+#pragma unroll
+                        for (int m = 0; m < 2; m++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) e[m][k] = ex2(fmaf(e[m][k], k & 1 ? r1.x : r0.x, k & 1 ? -r1.y : -r0.y));
+                        if (!whole || j + 8 > rows) {
+                            const int pa = j + 2 * c < rows ? pos[j + 2 * c] : INT_MIN, pb = j + 2 * c + 1 < rows ? pos[j + 2 * c + 1] : INT_MIN;
+#pragma unroll
+                            for (int m = 0; m < 2; m++)
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const int cell = base + 32 * m2 + 16 * m + 8 * (k >> 1) + g, p = k & 1 ? pb : pa;
+                                    if (!(cell <= p && (A.window <= 0 || p - cell < A.window || cell < A.first))) e[m][k] = 0.f;
+                                }
+                        }
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            acc2[m][0] += e[m][0] + e[m][1];
+                            acc2[m][1] += e[m][2] + e[m][3];
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            if (m2 == 0) sum[m][h] += acc2[m][h];
+                            else sum[2 + m][h] += acc2[m][h];
+                        }
+                }
+            }
+            __syncwarp();
+            fetch();
+        }
+        // ---- the warps' sums: of a page those of its kv heads, in their order ----
+        const int flip = u & 1;
+        if (my_head < hks)
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float x = sum[m][h];
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    if (c == 0) S.part[flip][warp][16 * m + 8 * h + g] = x;
+                }
+        __syncthreads();                                    // (of the unit behind the next one's, nobody reads these any more)
+        for (int i = tid; i < P * KV4_CELLS; i += KF_THREADS) {
+            const int page = i / KV4_CELLS, j = unit * P * KV4_CELLS + i, w0 = P > 1 ? page * hks : 0, w1 = P > 1 ? w0 + hks : min(KF_WARPS, hks);
+            float x = 0.f;
+            for (int w = w0; w < w1; w++) x += S.part[flip][w][i % KV4_CELLS];
+            if (j < q.len) W.sums[s * W.ld_sums + j] = W.old ? fmaf(W.decay, W.old[s * W.ld_old + j], x) : x;
+        }
+    }
+}
+
 template <typename T, int D>
 int weigh_launch(const Kv4Weigh & w, cudaStream_t st) {
+    const int hks = w.attn.cache.n_head_kv;
+    const int64_t rows = std::min<int64_t>(w.attn.max_q, w.attn.n_tokens) * w.attn.group, few = (hks * rows + 8) * (int64_t) kf_row_bytes<T, D>() + 4 * rows;
+    if (few <= (int64_t) KF_QUERIES) {
+        const size_t smem = sizeof(KfSmem<D>) + 128 + (size_t) few;
+        static FuncAttrCache cache;
+        const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D>, sizeof(KfSmem<D>) + 128 + KF_QUERIES, true);
+        if (e != cudaSuccess) return (int) e;
+        k_kv4_weigh_few<T, D><<<sm_count(), KF_THREADS, smem, st>>>(w, abort_flag(), (int) rows);
+        return (int) cudaGetLastError();
+    }
     constexpr size_t smem = sizeof(KwSmem<D, std::is_same<T, float>::value>);
     static FuncAttrCache cache;
     cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh<T, D>, smem, false);
     if (e != cudaSuccess) return (int) e;
-    const int64_t rows = std::min<int64_t>(w.attn.max_q, w.attn.n_tokens) * w.attn.group, units = w.attn.cache.n_head_kv * ((rows + KW_ROWS - 1) / KW_ROWS);
+    const int64_t units = hks * ((rows + KW_ROWS - 1) / KW_ROWS);
     const int ctas = units >= 8 ? 8 : units >= 4 ? 4 : units >= 2 ? 2 : 1;
     return (int) launch_clusters(k_kv4_weigh<T, D>, std::max(1, 2 * sm_count() / ctas), ctas, KW_THREADS, smem, false, st, w);
 }
