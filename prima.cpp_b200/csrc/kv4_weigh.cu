@@ -480,7 +480,14 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                         for (int m = 0; m < 2; m++)
 #pragma unroll
                             for (int k = 0; k < 4; k++) e[m][k] = ex2(fmaf(e[m][k], k & 1 ? r1.x : r0.x, k & 1 ? -r1.y : -r0.y));
-                        if (!whole || j + 8 > rows) {
+                        if (j + 8 > rows) {                 // rows of nobody's
+                            const bool ra = j + 2 * c < rows, rb = j + 2 * c + 1 < rows;
+#pragma unroll
+                            for (int m = 0; m < 2; m++)
+#pragma unroll
+                                for (int k = 0; k < 4; k++) e[m][k] = (k & 1 ? rb : ra) ? e[m][k] : 0.f;
+                        }
+                        if (!whole) {
                             const int pa = j + 2 * c < rows ? pos[j + 2 * c] : INT_MIN, pb = j + 2 * c + 1 < rows ? pos[j + 2 * c + 1] : INT_MIN;
 #pragma unroll
                             for (int m = 0; m < 2; m++)
