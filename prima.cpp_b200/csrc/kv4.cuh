@@ -102,17 +102,21 @@ int launch_kv4_load(const Kv4 & cache, int D, int type, const int64_t * cells, i
 int launch_kv4_copy_pages(uint8_t * pages, int64_t page_bytes, const int32_t * src, const int32_t * dst, int n, cudaStream_t st);   // src, dst: host
 int launch_kv4_compact(uint8_t * pages, int64_t n_pages, int rows, int D, int n_seq, const int32_t * from, int64_t ld_from, const int32_t * to, int64_t ld_to,
                        const int32_t * index, int64_t ld_index, const int32_t * count, int most, cudaStream_t st);   // rows: chunks of a page
-// What attention may do besides (kernels with X): rows' logarithms; results as parts, of which a second call makes one result with its own
+// What attention may do besides (kernels with X): rows' logarithms; prefixes that groups of sequences have in common
 struct Kv4Ext {
     float * lse; int64_t ld_lse;          // of each query and head; NULL: not wanted
-    int part;                             // KV4_PUT: results are sums and what belongs to them, into o and ml; KV4_FOLD: those are added to the results of the sequences in groups
-    float * o;                            // [token][head][D]
-    float2 * ml;                          // [token][head]: reference and sum of weights
+    int mode;
     const int32_t * group_start;          // the groups' first sequences
-    int n_group, n_seq;
-    int all;                              // a sequence is a group of them: the queries of all, each of which sees all cells
+    const int32_t * prefix_len, * prefix_table;
+    int64_t prefix_ld;
+    int n_group, n_own;                   // groups, sequences
+    int64_t least, of_page;               // groups whose sequences walk as many pages in front of their own have them by themselves; what a page of a prefix counts for a sequence: tiles x kv heads
+    float * o; float4 * ml;               // parts of rows [token][head]: sums [D]; reference, sum of weights, and the mark of the call
+    int * sync;                           // calls that have ended, CTAs of a call's last kernel that have
 };
-enum { KV4_PUT = 1, KV4_FOLD = 2 };
+// SHARED: a sequence's cells are the prefix's pages and its own behind them, or, where that is much work for the group, its own alone: sums and what belongs to them go into o and ml.  FRONT, behind
+// it: a group is a sequence whose queries, those of all its sequences, see all cells of the prefix; what the others left is added
+enum { KV4_PLAIN = 0, KV4_SHARED = 1, KV4_FRONT = 2 };
 struct Kv4Attn {
     Kv4 cache;
     const void * q; int64_t ldq;

@@ -58,11 +58,9 @@ int attend(const pb200_kv4_cache * c, int layer, int type, const void * q, int64
     // what the kernels count in 31 bits: pages of all sequences, heads and tiles of eight rows where rows are few, tiles of all prompts otherwise
     const double group = n_head / c->n_head_kv, rows = std::min(std::min<double>(max_q, (double) n_tokens) * group, (double) KV4_FEW_ROWS);
     const auto pages_of = [&](int64_t ld) { return (double) std::min<int64_t>(ld, INT32_MAX / PB200_KV4_CELLS) * c->n_head_kv; };
-    const double pages = n_seq * pages_of(table_ld) * std::ceil(rows / 8);
-    const double tiles = ((double) n_tokens * group / 128 + n_seq) * c->n_head_kv;
+    const double pages = n_seq * (pages_of(table_ld) + (groups ? pages_of(groups->table_ld) : 0.0)) * std::ceil(rows / 8);
+    const double tiles = ((double) n_tokens * group / 128 + std::max(n_seq, groups ? groups->n : 0)) * c->n_head_kv;
     if (pages >= 2147483648.0 || tiles >= 2147483648.0 || n_tokens * group >= 2147483648.0) return PB200_ENOTSUP;
-    // (of prefixes the kernel of few rows takes up to so many rows a group on the average)
-    if (groups && (groups->n * pages_of(groups->table_ld) * (KV4_FEW_ROWS / 8 + 1) >= 2147483648.0 || ((double) n_tokens * group / 128 + groups->n) * c->n_head_kv >= 2147483648.0)) return PB200_ENOTSUP;
     if (overlap(q, ldq, n_head * D, out, ldo, n_head * D, n_tokens, eb)) return PB200_EINVAL;
     Kv4Attn a{layer_of(c, layer), q, ldq, out, ldo, n_head, n_head / c->n_head_kv, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, window, keep_first, scale};
     a.x.lse = lse;
@@ -159,7 +157,7 @@ size_t pb200_kv4_attn_shared_workspace_bytes(int n_head, int n_head_kv, int head
 int pb200_kv4_attn_shared(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
                           const int32_t * kv_len, const int32_t * table, int64_t table_ld, int n_group, const int32_t * group_start, const int32_t * prefix_len, const int32_t * prefix_table,
                           int64_t prefix_ld, int64_t n_tokens, int max_q, float scale, float * lse, int64_t ld_lse, void * ws, size_t ws_bytes, void * stream) {
-    if (n_group < 0 || (n_group > 0 && (!group_start || !prefix_len || !prefix_table || prefix_ld <= 0))) return PB200_EINVAL;
+    if (n_group < 0 || n_group > 1 << 24 || (n_group > 0 && (!group_start || !prefix_len || !prefix_table || prefix_ld <= 0))) return PB200_EINVAL;
     const Kv4Groups g{n_group, group_start, prefix_len, prefix_table, prefix_ld};
     return attend(c, layer, type, q, ldq, out, ldo, n_head, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, scale, 0, 0, lse, ld_lse, n_group > 0 ? &g : nullptr, ws, ws_bytes, stream);
 }

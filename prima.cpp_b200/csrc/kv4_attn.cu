@@ -11,7 +11,8 @@
 namespace pb {
 
 // counters (rows: one per warp and slice), tickets and a word for each slot, all zero between calls; then the parts of either kernel, which may run at the same time
-static size_t counters() { return (KV4_COUNTERS + 64 + KV4_SLOTS) * sizeof(int); }
+constexpr int KV4_SYNC = KV4_COUNTERS + 64 + KV4_SLOTS;      // and the words of calls with prefixes, which keep their place whatever a call's sizes
+static size_t counters() { return (KV4_SYNC + 64) * sizeof(int); }
 size_t kv4_attn_workspace(int D) { return counters() + kv4_rows_workspace(D) + kv4_prompt_workspace(D); }
 
 static int few_rows(int type) { return type == PB200_TYPE_F32 ? KV4_FEW_ROWS_F32 : KV4_FEW_ROWS; }
@@ -21,7 +22,7 @@ int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t 
     void * parts = (char *) ws + counters();
     const int64_t most = std::min<int64_t>(a.max_q, a.n_tokens) * a.group;
     const int few = few_rows(type);
-    const bool ext = a.x.lse || a.x.part;
+    const bool ext = a.x.lse || a.x.mode != KV4_PLAIN;
     if (most <= few || a.n_seq > 1) {   // of several sequences, each goes where its rows belong
         launches++;
         const int e = launch_kv4_attn_rows(a, D, type, few, words, parts, st, ext);
@@ -31,35 +32,41 @@ int launch_kv4_attn(const Kv4Attn & a, int D, int type, void * ws, cudaStream_t 
     return launch_kv4_attn_prompt(a, D, type, a.n_seq > 1 ? few : 0, words + KV4_COUNTERS, (char *) parts + kv4_rows_workspace(D), st, ext, launches);
 }
 
-// Rows' parts lie behind the workspace of a call without groups.
-static size_t part_rows(int64_t rows, int D) { return ((size_t) rows * D * sizeof(float) + 255) / 256 * 256; }
-size_t kv4_attn_shared_workspace(int64_t rows, int D) { return (kv4_attn_workspace(D) + 255) / 256 * 256 + part_rows(rows, D) + (size_t) rows * sizeof(float2); }
+// Rows' parts lie behind the workspace of a call without groups
+static size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
+size_t kv4_attn_shared_workspace(int64_t rows, int D) { return round_up(kv4_attn_workspace(D)) + round_up((size_t) rows * D * sizeof(float)) + (size_t) rows * sizeof(float4); }
 
-// The prefixes first: a group is a sequence whose rows all see all cells.  Which kernel takes them is decided for the call: by the rows that a group has on the average.
+// A prefix is read once for the rows of all its sequences, by the prompts' kernel, where each sequence has few and these would walk many pages in front of their own; otherwise they do: nothing
+// has to be added up, and there is one launch.  How many pages (times kv heads and tiles of eight rows) is decided group by group on the device, where lengths are; the prompts' kernel is launched
+// where tables have room for as many.  us, pages in front of the own ones / by themselves, n sequences of one token, 32 heads over 8, bf16: 1000 cells, 64 39 / 45, 128 55 / 46; 4000, 16 33 / 36,
+// 24 41 / 40, 32 47 / 41, 128 123 / 63; 16 000, 8 46 / 49, 12 56 / 49, 32 117 / 51, 128 405 / 90; 16 heads over 2: 4000, 64 34 / 39, 128 47 / 46; F32, 32 over 8: 1000, 32 37 / 43, 64 56 / 46;
+// 4000, 8 36 / 37, 12 39 / 38, 16 45 / 38; 16 000, 4 43 / 49, 8 67 / 54
+constexpr int KV4_APART = 14000, KV4_APART_F32 = 8500;
 int launch_kv4_attn_shared(const Kv4Attn & a, const Kv4Groups & g, int D, int type, void * ws, cudaStream_t st, int & launches) {
-    Kv4Attn own = a, front = a;
-    own.x.o = front.x.o = (float *) ((char *) ws + (kv4_attn_workspace(D) + 255) / 256 * 256);
-    own.x.ml = front.x.ml = (float2 *) ((char *) own.x.o + part_rows(a.n_tokens * a.n_head, D));
-    own.x.group_start = front.x.group_start = g.start;
-    own.x.n_group = front.x.n_group = g.n;
-    own.x.n_seq = front.x.n_seq = a.n_seq;
-    own.x.part = KV4_FOLD;
-    front.x.part = KV4_PUT;
-    front.x.all = 1;
-    front.x.lse = nullptr;
-    front.n_seq = g.n;
-    front.kv_len = g.kv_len;
-    front.table = g.table;
-    front.table_ld = g.table_ld;
-    front.max_q = INT_MAX;
+    Kv4Attn b = a;
     int * words = (int *) ws;
     void * parts = (char *) ws + counters();
-    int e;
-    if (a.n_tokens * a.group <= (int64_t) few_rows(type) * g.n) {
-        launches++;
-        e = launch_kv4_attn_rows(front, D, type, INT_MAX, words, parts, st, true);
-    } else e = launch_kv4_attn_prompt(front, D, type, 0, words + KV4_COUNTERS, (char *) parts + kv4_rows_workspace(D), st, true, launches);
-    return e ? e : launch_kv4_attn(own, D, type, ws, st, launches);
+    b.x.sync = words + KV4_SYNC;
+    b.x.o = (float *) ((char *) ws + round_up(kv4_attn_workspace(D)));
+    b.x.ml = (float4 *) ((char *) b.x.o + round_up((size_t) a.n_tokens * a.n_head * D * sizeof(float)));
+    b.x.group_start = g.start;
+    b.x.prefix_len = g.kv_len;
+    b.x.prefix_table = g.table;
+    b.x.prefix_ld = g.table_ld;
+    b.x.n_group = g.n;
+    b.x.n_own = a.n_seq;
+    const int few = few_rows(type);
+    const int64_t rows = std::min<int64_t>(a.max_q, a.n_tokens) * a.group;
+    b.x.mode = KV4_SHARED;
+    b.x.of_page = (rows + 7) / 8 * a.cache.n_head_kv;
+    b.x.least = std::max<int64_t>(1, (type == PB200_TYPE_F32 ? KV4_APART_F32 : KV4_APART) / g.n);
+    const bool apart = rows <= few && (double) a.n_seq * g.table_ld * b.x.of_page >= (double) b.x.least;
+    if (!apart) b.x.least = INT64_MAX;
+    const int e = launch_kv4_attn(b, D, type, ws, st, launches);
+    if (e || !apart) return e;
+    b.x.mode = KV4_FRONT;
+    b.n_seq = g.n;
+    return launch_kv4_attn_prompt(b, D, type, 0, words + KV4_COUNTERS, (char *) parts + kv4_rows_workspace(D), st, true, launches);
 }
 
 }  // namespace pb

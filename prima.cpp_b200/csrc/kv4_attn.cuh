@@ -16,15 +16,17 @@ struct Kv4Seq {
     int n_q, p0;               // queries; position of the first
     int pages, keep, from;
     int n_rows;                // queries x heads of a group
+    // with prefixes there are no windows: KV4_SHARED has in `keep` the pages of the prefix that come first (a query stands 64 * keep further on), in `from` 64 times the group and the cells that
+    // the last of them has not; -1 where the prefix is by itself
     __device__ __forceinline__ int items(int n_head_kv, int tile) const { return n_q > 0 ? n_head_kv * ((n_rows + tile - 1) / tile) : 0; }
     __device__ __forceinline__ int units(int n_head_kv, int tile) const { return items(n_head_kv, tile) * pages; }
 };
-// the pages that queries at the positions lo .. hi see
-__device__ __forceinline__ void kv4_pages(const Kv4Attn & A, int lo, int hi, Kv4Seq & q) {
+// the pages that queries at the positions lo .. hi see, of a table with ld pages to a row
+__device__ __forceinline__ void kv4_pages(const Kv4Attn & A, int64_t table_ld, int lo, int hi, Kv4Seq & q) {
     q.pages = 1;
     q.keep = q.from = 0;
     if (hi < 0) return;
-    const int ld = (int) (A.table_ld < 0x1ffffff ? A.table_ld : 0x1ffffff);   // cells have 31 bits
+    const int ld = (int) (table_ld < 0x1ffffff ? table_ld : 0x1ffffff);   // cells have 31 bits
     const int last = min(hi / KV4_CELLS, ld - 1);
     if (A.window > 0 && lo >= A.window) {
         q.from = (lo - A.window + 1) / KV4_CELLS;
@@ -32,64 +34,130 @@ __device__ __forceinline__ void kv4_pages(const Kv4Attn & A, int lo, int hi, Kv4
     }
     q.pages = max(1, q.keep + max(0, last + 1 - q.from));
 }
+template <bool X> __device__ __forceinline__ bool kv4_shared(const Kv4Attn & A) { return X && A.x.mode == KV4_SHARED; }
+template <bool X>
+__device__ __forceinline__ void kv4_span(const Kv4Attn & A, int lo, int hi, Kv4Seq & q) {
+    if (kv4_shared<X>(A)) {
+        const int front = q.keep, from = q.from, own = hi - KV4_CELLS * front;
+        kv4_pages(A, A.table_ld, own, own, q);
+        q.pages = front + (own < 0 && front > 0 ? 0 : q.pages);
+        q.keep = front;
+        q.from = from;
+    } else kv4_pages(A, X && A.x.mode == KV4_FRONT ? A.x.prefix_ld : A.table_ld, lo, hi, q);
+}
+// the group of a sequence, -1: none
+__device__ __forceinline__ int kv4_group_of(const Kv4Attn & A, int s) {
+    const int n = A.x.n_group;
+    if (s < A.x.group_start[0] || s >= A.x.group_start[n]) return -1;
+    int lo = 0, hi = n;                        // group_start[lo] <= s < group_start[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (A.x.group_start[mid] <= s) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// cells of a prefix (30 bits), and whether it is by itself
+__device__ __forceinline__ int kv4_prefix(const Kv4Attn & A, int g, bool & apart) {
+    const int cells = min(max(A.x.prefix_len[g], 0), 1 << 30), sequences = A.x.group_start[g + 1] - A.x.group_start[g];
+    apart = (int64_t) sequences * ((cells + KV4_CELLS - 1) / KV4_CELLS) * A.x.of_page >= A.x.least;
+    return cells;
+}
+// position of query t of a sequence
+template <bool X> __device__ __forceinline__ int kv4_pos(const Kv4Attn & A, const Kv4Seq & q, int t) {
+    if (X && A.x.mode == KV4_FRONT) return q.p0;
+    return kv4_shared<X>(A) ? max(q.p0 + t, KV4_CELLS * q.keep - 1) : q.p0 + t;
+}
 // many: sequences with more than most_rows rows, otherwise the others
 template <bool X>
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_rows, bool many) {
     Kv4Seq q{};
     if (s >= A.n_seq) return q;
-    int s0 = s, s1 = s + 1;
-    if (X && A.x.all) {
+    const bool front = X && A.x.mode == KV4_FRONT;
+    int s0 = s, s1 = s + 1, prefix = 0;
+    if (front) {
         s0 = A.x.group_start[s];
         s1 = A.x.group_start[s + 1];
-        if (s0 < 0 || s1 <= s0 || s1 > A.x.n_seq) return q;
+        bool apart;
+        prefix = kv4_prefix(A, s, apart);
+        if (!apart || s0 < 0 || s1 <= s0 || s1 > A.x.n_own) return q;
     }
-    const long long a = A.q_start[s0], b = A.q_start[s1], cells = A.kv_len[s];     // (all on their way)
+    const long long a = A.q_start[s0], b = A.q_start[s1], cells = front ? prefix : A.kv_len[s];     // (all on their way)
     if (a < 0 || b <= a || b > A.n_tokens) return q;
-    const int all = (int) (b - a), n = min(all, A.max_q);
+    const int all = (int) (b - a), n = front ? all : min(all, A.max_q);
     if (((long long) n * A.group > most_rows) != many) return q;
     q.q0 = a;
     q.n_q = n;
     q.n_rows = n * A.group;
     const int len = max((int) cells, 0);
-    if (X && A.x.all) {
-        q.p0 = len - 1;
-        kv4_pages(A, q.p0, q.p0, q);
-        return q;
+    q.p0 = front ? len - 1 : len - all;
+    if (kv4_shared<X>(A)) {
+        const int g = kv4_group_of(A, s);
+        q.p0 = min(len, 1 << 30) - all;
+        if (g >= 0) {
+            bool apart;
+            const int in_front = kv4_prefix(A, g, apart);
+            q.keep = apart ? 0 : (in_front + KV4_CELLS - 1) / KV4_CELLS;
+            q.from = apart ? -1 : KV4_CELLS * g + (KV4_CELLS * q.keep - in_front);
+            q.p0 += KV4_CELLS * q.keep;
+        }
     }
-    q.p0 = len - all;
-    kv4_pages(A, q.p0, q.p0 + n - 1, q);
+    kv4_span<X>(A, kv4_pos<X>(A, q, 0), kv4_pos<X>(A, q, n - 1), q);
     return q;
 }
-// position of a sequence's query
-template <bool X> __device__ __forceinline__ int kv4_pos(const Kv4Attn & A, const Kv4Seq & q, int t) { return X && A.x.all ? q.p0 : q.p0 + t; }
 // the i-th of its pages: which one of the sequence, and its number in the pool (-1: none)
-__device__ __forceinline__ int kv4_page_index(const Kv4Seq & q, int i) { return i < q.keep ? i : i - q.keep + q.from; }
+template <bool X> __device__ __forceinline__ int kv4_page_index(const Kv4Attn & A, const Kv4Seq & q, int i) { return kv4_shared<X>(A) || i < q.keep ? i : i - q.keep + q.from; }
 template <bool X>
 __device__ __forceinline__ int kv4_page(const Kv4Attn & A, const Kv4Seq & q, int s, int i) {
-    const int at = kv4_page_index(q, i);
-    if ((X && A.x.all ? q.p0 < 0 : q.p0 + q.n_q <= 0) || at >= A.table_ld) return -1;
-    const int id = A.table[s * A.table_ld + at];
+    int at = kv4_page_index<X>(A, q, i), id, own = q.p0 + q.n_q;           // (own cells, if it is more than 0)
+    if (X && A.x.mode == KV4_FRONT) {
+        if (q.p0 < 0 || at >= A.x.prefix_ld) return -1;
+        id = A.x.prefix_table[s * A.x.prefix_ld + at];
+    } else if (kv4_shared<X>(A) && at < q.keep) {
+        if (at >= A.x.prefix_ld) return -1;
+        id = A.x.prefix_table[q.from / KV4_CELLS * A.x.prefix_ld + at];
+    } else {
+        if (kv4_shared<X>(A)) {
+            at -= q.keep;
+            own -= KV4_CELLS * q.keep;
+        }
+        if (own <= 0 || at >= A.table_ld) return -1;
+        id = A.table[s * A.table_ld + at];
+    }
     return id >= 0 && id < A.cache.n_pages ? id : -1;
+}
+// cells behind the end of a prefix, in its last page
+template <bool X> __device__ __forceinline__ int kv4_hole_from(const Kv4Seq & q) { return KV4_CELLS * q.keep - q.from % KV4_CELLS; }
+template <bool X> __device__ __forceinline__ bool kv4_hole(const Kv4Attn & A, const Kv4Seq & q, int cell) {
+    return kv4_shared<X>(A) && q.keep > 0 && cell >= kv4_hole_from<X>(q) && cell < KV4_CELLS * q.keep;
+}
+template <bool X> __device__ __forceinline__ bool kv4_has_hole(const Kv4Attn & A, const Kv4Seq & q, int base) {      // a page from cell `base` on
+    return kv4_shared<X>(A) && q.keep > 0 && base < KV4_CELLS * q.keep && base + KV4_CELLS > kv4_hole_from<X>(q);
 }
 
 // of a part with maximum m and sum l of weights, where all parts' maximum is top (a row that is no number has no maximum)
 __device__ __forceinline__ float part_factor(float m, float l, float top) { return m == -INFINITY ? (l == l ? 0.f : 1.f) : ex2(m - top); }
 
-// What becomes of a row's sum of values x, times 2^-m and with l the sum of its weights: own * x + other * from, into `to` or, as a part, into `put`
-struct Kv4Row { float own, other; const float * from; float * put; };
+// What becomes of a row's sum of values x, times 2^-m and with l the sum of its weights: own * x + other * from, or, as a part, x goes to `put`; skip: nothing (the row is nobody's)
+struct Kv4Row { float own, other; const float * from; float * put; bool skip; };
 template <int D>
-__device__ __forceinline__ Kv4Row kv4_row(const Kv4Attn & A, int s, int64_t token, int head, float m, float l, bool writes) {
+__device__ __forceinline__ Kv4Row kv4_row(const Kv4Attn & A, const Kv4Seq & q, int64_t token, int head, float m, float l, bool writes) {
     const int64_t at = token * A.n_head + head;
-    Kv4Row r{0.f, 0.f, nullptr, nullptr};
-    if (A.x.part == KV4_PUT) {
-        if (writes) A.x.ml[at] = make_float2(m, l);
-        r.own = 1.f;
-        r.put = A.x.o + at * D;
-        return r;
-    }
+    Kv4Row r{0.f, 0.f, nullptr, nullptr, false};
     float all = l, top = m, f = 1.f;
-    if (A.x.part == KV4_FOLD && s >= A.x.group_start[0] && s < A.x.group_start[A.x.n_group]) {
-        const float2 p = A.x.ml[at];
+    if (A.x.mode == KV4_FRONT || (A.x.mode == KV4_SHARED && q.from < 0)) {
+        const int tag = *(volatile int *) &A.x.sync[0] + 1;        // of this call; what earlier ones left has others
+        if (A.x.mode == KV4_SHARED) {
+            if (writes) A.x.ml[at] = make_float4(m, l, __int_as_float(tag), __int_as_float(~tag));
+            r.own = 1.f;
+            r.put = A.x.o + at * D;
+            return r;
+        }
+        const float4 p = A.x.ml[at];
+        if (__float_as_int(p.z) != tag || __float_as_int(p.w) != ~tag) {           // a query beyond the first max_q of its sequence
+            r.skip = true;
+            return r;
+        }
         top = fmaxf(m, p.x);
         f = part_factor(m, l, top);
         r.other = part_factor(p.x, p.y, top);
@@ -109,6 +177,15 @@ __device__ __forceinline__ float4 kv4_mix(const Kv4Row & r, float4 x, int d) {  
         y.x = fmaf(z.x, r.other, y.x); y.y = fmaf(z.y, r.other, y.y); y.z = fmaf(z.z, r.other, y.z); y.w = fmaf(z.w, r.other, y.w);
     }
     return y;
+}
+// KV4_FRONT: a CTA of the call's last kernel has ended (one thread says so, and its others behind a barrier): behind the last of them the call has
+__device__ __forceinline__ void kv4_leave(const Kv4Attn & A) {
+    if (A.x.mode != KV4_FRONT) return;
+    __threadfence();
+    if (atomicAdd(&A.x.sync[1], 1) == (int) gridDim.x - 1) {
+        A.x.sync[1] = 0;
+        A.x.sync[0] = A.x.sync[0] + 1;
+    }
 }
 
 __device__ __forceinline__ void tmem_alloc(uint32_t * at, uint32_t columns) {

@@ -58,9 +58,11 @@ struct KpPiece {               // what a ticket stands for
 struct KpPlan {
     int64_t q0[KP_CUT_SEQ];
     int n_q[KP_CUT_SEQ], p0[KP_CUT_SEQ], n_rows[KP_CUT_SEQ], from[KP_CUT_SEQ], ends[KP_CUT_SEQ], lens[KP_CUT_TILES], limit;
-    __device__ __forceinline__ Kv4Seq seq(int s) const {       // without its pages
+    int2 front[KP_CUT_SEQ];                                    // with X: `keep` and `from`
+    template <bool X> __device__ __forceinline__ Kv4Seq seq(int s) const {       // without its pages
         Kv4Seq q{};
         q.q0 = q0[s]; q.n_q = n_q[s]; q.p0 = p0[s]; q.n_rows = n_rows[s];
+        if (X) { q.keep = front[s].x; q.from = front[s].y; }
         return q;
     }
 };
@@ -87,7 +89,7 @@ __device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpP
     p.p_lo = kv4_pos<X>(A, q, p.row0 / A.group);
     p.p_hi = kv4_pos<X>(A, q, (p.row0 + p.rows - 1) / A.group);
     p.q = q;
-    kv4_pages(A, p.p_lo, p.p_hi, p.q);
+    kv4_span<X>(A, p.p_lo, p.p_hi, p.q);
     p.tiles = (p.q.pages + 1) / 2;
 }
 // Items, their pieces and slots, in the order of tickets: sequences, tiles from the last on, heads, pieces; every CTA counts them in the same way.  Where long items may be cut there are
@@ -108,6 +110,7 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
     if (!W.cut) return;
     const Kv4Seq own = kv4_seq<X>(A, lane, W.most_rows, true);
     plan.q0[lane] = own.q0; plan.n_q[lane] = own.n_q; plan.p0[lane] = own.p0; plan.n_rows[lane] = own.n_rows;
+    if (X) plan.front[lane] = make_int2(own.keep, own.from);
     const int len = own.n_q > 0 ? own.p0 + own.n_q : INT_MIN;
     int rank = lane < A.n_seq ? 0 : lane;
     for (int i = 0; i < A.n_seq; i++) {
@@ -132,7 +135,7 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
         p.row0 = (__shfl_sync(0xffffffffu, ends, r) - 1 - m) * ROWS;
         const int src = __shfl_sync(0xffffffffu, from, r);
         if (m < all) {
-            const Kv4Seq q = plan.seq(src);
+            const Kv4Seq q = plan.seq<X>(src);
             p.rows = min(ROWS, q.n_rows - p.row0);
             kp_span<X>(A, q, p);
             plan.lens[m] = p.tiles;
@@ -141,12 +144,12 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
     }
     sum = __reduce_add_sync(0xffffffffu, sum) * A.cache.n_head_kv;
     __syncwarp();
-    // of the even share, 4 / 3 and 2 of it that which ends first
+    // of the even share, 4 / 3 and 2 of it (with X also 2 / 3 and a half, as far as there are slots) that which ends first
     const int share = max(4, (sum + ctas - 1) / ctas);
     int best = share, best_cost = INT_MAX;
 #pragma unroll 1
-    for (int i = 0; i < 3; i++) {
-        const int limit = share + (i == 0 ? 0 : i == 1 ? (share + 2) / 3 : share);
+    for (int i = 0; i < (X ? 5 : 3); i++) {
+        const int limit = X && i > 2 ? max(4, i == 3 ? (2 * share + 2) / 3 : (share + 1) / 2) : share + (i == 0 ? 0 : i == 1 ? (share + 2) / 3 : share);
         int n = 0, most = 0;
         for (int m = lane; m < all; m += 32) {
             const int k = kp_pieces(plan.lens[m], limit);
@@ -155,6 +158,7 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
         }
         n = __reduce_add_sync(0xffffffffu, n) * A.cache.n_head_kv;
         most = __reduce_max_sync(0xffffffffu, most);
+        if (X && i > 2 && n > KV4_SLOTS) break;
         // a piece's start and end are about three tiles; rounds of the longest, or, where lengths differ, long ones first: 4 / 3 of the mean at most
         const int mean = (int) (((float) sum + 3.f * (float) n) * (4.f / 3.f) * __frcp_rn((float) ctas)) + 1, cost = min((n + ctas - 1) / ctas * (most + 3), max(most + 3, mean));
         if (cost < best_cost) { best = limit; best_cost = cost; }
@@ -182,7 +186,7 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, con
                 KpPiece p{};
                 p.row0 = (plan.ends[r] - 1 - m) * ROWS;
                 p.s = plan.from[r];
-                const Kv4Seq q = plan.seq(p.s);
+                const Kv4Seq q = plan.seq<X>(p.s);
                 p.rows = min(ROWS, q.n_rows - p.row0);
                 kp_span<X>(A, q, p);
                 const int i = t - before - (x - k * hks);
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 const uint32_t u = tiles + (uint32_t) j;
                 const int st = (int) (u & 1);
                 const uint8_t * third = chunk_of(j + 2);
-                if (t6 == 0) S.cell[u & 3][half] = now ? kv4_page_index(P.q, 2 * (P.a + j) + half) * KV4_CELLS : -1;
+                if (t6 == 0) S.cell[u & 3][half] = now ? kv4_page_index<X>(A, P.q, 2 * (P.a + j) + half) * KV4_CELLS : -1;
                 if (u >= 2) mbar_wait(&S.k_empty[st], (u / 2 - 1) & 1, cta_abort, W.abort_flag);
                 {
                     const uint32_t odd = t6 & 1 ? 0x3232u : 0x1010u;
@@ -333,9 +337,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 ask_k(later);
                 if (u >= 2) mbar_wait(&S.v_empty[st], (u / 2 - 1) & 1, cta_abort, W.abort_flag);
                 {
-                    const int i = 2 * (P.a + j) + half, cell = kv4_page_index(P.q, i) * KV4_CELLS + tv, t = half * 64 + tv;
+                    const int i = 2 * (P.a + j) + half, cell = kv4_page_index<X>(A, P.q, i) * KV4_CELLS + tv, t = half * 64 + tv;
                     // a weight of zero does not silence a scale that is no number: cells nobody sees may hold anything
-                    const bool seen = cell <= P.p_hi && (A.window <= 0 || P.p_lo - cell < A.window || cell < A.first);
+                    const bool seen = cell <= P.p_hi && (A.window <= 0 || P.p_lo - cell < A.window || cell < A.first) && !kv4_hole<X>(A, P.q, cell);
                     const uint32_t odd = tv & 1 ? 0x3232u : 0x1010u;
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
@@ -492,14 +496,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     fence_after();
                     // (four of them: written for tile j + 4 behind the scores of j + 2, which come behind the weights of j)
                     const int c0 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][0], c1 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][1];
-                    const bool whole = min(c0, c1) >= 0 && max(c0, c1) <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first));
+                    const bool whole = min(c0, c1) >= 0 && max(c0, c1) <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first)) && !kv4_has_hole<X>(A, P.q, c0) && !kv4_has_hole<X>(A, P.q, c1);
                     if (!whole) {   // a score that is not seen is -inf: in its place, ahead of the passes over the tile
                         const int from = A.window > 0 ? max(0, pos - A.window + 1) : 0;
 #pragma unroll 1
                         for (int h = 0; h < 4; h++) {
                             const int page = h < 2 ? c0 : c1, base = page + 32 * (h & 1);
                             auto below = [&](int cell) { const int k = cell - base; return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };     // cells in front of it
-                            const uint32_t seen = page < 0 || base > pos ? 0u : below(pos + 1) & (~below(from) | below(A.first));
+                            uint32_t seen = page < 0 || base > pos ? 0u : below(pos + 1) & (~below(from) | below(A.first));
+                            if (kv4_shared<X>(A) && P.q.keep > 0) seen &= below(kv4_hole_from<X>(P.q)) | ~below(KV4_CELLS * P.q.keep);
                             TMEM_LD32(mine + 32 * h, t0);
                             TMEM_ARRIVED(t0);
 #pragma unroll
@@ -638,9 +643,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 if (!F32 || grp == 0) {
                     const float inv = P.slot >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
                     KpPart<D> * part = nullptr;
-                    Kv4Row w{inv, 0.f, nullptr, nullptr};
-                    if (X && P.slot < 0 && mine_is) w = kv4_row<D>(A, P.s, P.q.q0 + tok, head, m - UP, l, true);
-                    const bool put = X && P.slot < 0 && A.x.part == KV4_PUT;
+                    Kv4Row w{inv, 0.f, nullptr, nullptr, false};
+                    if (X && A.x.mode == KV4_FRONT) pdl_wait();        // the kernel in front has the sequences' own parts
+                    if (X && P.slot < 0 && mine_is) w = kv4_row<D>(A, P.q, P.q.q0 + tok, head, m - UP, l, true);
+                    const uint32_t write = X ? __ballot_sync(0xffffffffu, mine_is && !w.skip) : valid;
                     if (P.slot >= 0) {
                         part = &reinterpret_cast<KpParts<D> *>(W.parts)->part[P.slot];
                         part->m[rows0 + row] = m;
@@ -667,17 +673,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {           // columns 0 2 4 6 | 1 3 5 7 of an eight are numbers 0 1 2 3 | 4 5 6 7
                             float4 a = make_float4(t[0][i], t[0][i + 2], t[0][i + 4], t[0][i + 6]), b = make_float4(t[0][i + 1], t[0][i + 3], t[0][i + 5], t[0][i + 7]);
-                            if (X && put) {
-                                if (mine_is) {
-                                    *reinterpret_cast<float4 *>(w.put + h + i) = a;
-                                    *reinterpret_cast<float4 *>(w.put + h + i + 4) = b;
-                                }
-                            } else if (part) {
+                            if (part) {
                                 *reinterpret_cast<float4 *>(&part->o[rows0 + row][h + i]) = a;
                                 *reinterpret_cast<float4 *>(&part->o[rows0 + row][h + i + 4]) = b;
                             } else {
                                 if (X && w.from) {
-                                    const Kv4Row r{1.f, w.other, w.from, nullptr};
+                                    const Kv4Row r{1.f, w.other, w.from, nullptr, false};
                                     a = kv4_mix(r, a, h + i);
                                     b = kv4_mix(r, b, h + i + 4);
                                 }
@@ -686,7 +687,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             }
                         }
                     }
-                    if (!part && !put) {
+                    if (!part) {
                         constexpr int LPR = D / 4, RPW = 32 / LPR;
                         const int sub = lane / LPR, l4 = lane % LPR;
                         __syncwarp();                               // a warp reads its own rows
@@ -697,7 +698,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             const int rr = i * RPW + sub;
                             const float4 v = load4(rows + rr * D + (l4 + quad * 32 + rr) % PIECES * 4);
                             const int64_t to = __shfl_sync(0xffffffffu, o_at, rr);
-                            if (valid >> rr & 1) store4((T *) A.out + to + 4 * l4, v);
+                            if (write >> rr & 1) store4((T *) A.out + to + 4 * l4, v);
                         }
                     }
                 }
@@ -718,6 +719,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     if (warp == 12) {
         tmem_free(tmem, 512);
         if (lane == 0 && atomicAdd(&W.tickets[KP_DONE], 1) == (int) gridDim.x - 1) W.tickets[KP_DRAWN] = W.tickets[KP_DONE] = 0;   // the last CTA: every ticket has been drawn
+        if (X && lane == 0 && !W.cut) kv4_leave(A);
     }
 }
 
@@ -766,12 +768,8 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
         const int at = p.row0 + r, tt = at / A.group;
         T * out = (T *) A.out + (p.q.q0 + tt) * A.ldo + (int64_t) (p.hk * A.group + at - tt * A.group) * D + lane * PER;
         if constexpr (X) {
-            const Kv4Row w = kv4_row<D>(A, p.s, p.q.q0 + tt, p.hk * A.group + at - tt * A.group, top - (15.f - kp_slack<T>()), l, lane == 0);
-            if (w.put) {
-#pragma unroll
-                for (int e = 0; e < PER; e++) w.put[lane * PER + e] = x[e];
-                continue;
-            }
+            const Kv4Row w = kv4_row<D>(A, p.q, p.q.q0 + tt, p.hk * A.group + at - tt * A.group, top - (15.f - kp_slack<T>()), l, lane == 0);
+            if (w.skip) continue;
 #pragma unroll
             for (int e = 0; e < PER; e++) x[e] = w.from ? fmaf(w.from[lane * PER + e], w.other, x[e] * w.own) : x[e] * w.own;
         }
@@ -786,6 +784,7 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
     }
     __syncthreads();
     if (threadIdx.x == 0 && atomicAdd(&W.tickets[KP_JOINED], 1) == (int) gridDim.x - 1) W.tickets[KP_CUT] = W.tickets[KP_JOINED] = 0;
+    if (X && threadIdx.x == 0) kv4_leave(A);
 }
 
 template <typename T, int D, bool X>
@@ -807,7 +806,7 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = w.most_rows > 0 ? 1 : 0;
+    cfg.numAttrs = w.most_rows > 0 || a.x.mode == KV4_FRONT ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, k_kv4_attn_prompt<T, D, X>, a, w);
     if (e != cudaSuccess || !w.cut) return (int) e;
     k_kv4_join<T, D, X><<<4 * sm_count(), 256, 0, st>>>(a, w);

@@ -143,7 +143,7 @@ __device__ __forceinline__ T * kr_row(const Kv4Attn & A, const KrSegment & at, i
 template <int D>
 __device__ __forceinline__ Kv4Row kr_ext(const Kv4Attn & A, const KrSegment & at, int r, float m, float l, bool writes) {
     const int row = at.tile * KR_ROWS + r, t = row / A.group;
-    return kv4_row<D>(A, at.s, at.q.q0 + t, at.hk * A.group + row - t * A.group, m, l, writes);
+    return kv4_row<D>(A, at.q, at.q.q0 + t, at.hk * A.group + row - t * A.group, m, l, writes);
 }
 
 template <typename T, int D, bool X>
@@ -396,13 +396,13 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             if (have) {
                 uint8_t * chunk = S.ring[warp][st];
                 uint8_t * const vs = chunk + 2 * kv4_rows_bytes(D) + kv4_scales_bytes(D);
-                const int base = kv4_page_index(q, at.pa + u - at.k0) * KV4_CELLS;
-                const bool whole = base + 63 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + 63 < A.first);
+                const int base = kv4_page_index<X>(A, q, at.pa + u - at.k0) * KV4_CELLS;
+                const bool whole = base + 63 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + 63 < A.first) && !kv4_has_hole<X>(A, q, base);
                 if (!whole) {   // a weight of zero does not silence a scale that is no number: cells nobody sees may hold anything
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int t = 2 * lane + e, cell = base + t;
-                        if (!(cell <= p_hi && (A.window <= 0 || p_lo - cell < A.window || cell < A.first)))
+                        if (!(cell <= p_hi && (A.window <= 0 || p_lo - cell < A.window || cell < A.first)) || kv4_hole<X>(A, q, cell))
 #pragma unroll
                             for (int b = 0; b < NB; b++) *reinterpret_cast<uint16_t *>(vs + kv4_scale(D, t, b)) = 0;
                     }
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const int cell = base + 16 * j + g + (k >> 1) * 8, p = pos[k & 1];
-                            if (!(cell <= p && (A.window <= 0 || p - cell < A.window || cell < A.first))) sc[j][k] = -INFINITY;
+                            if (!(cell <= p && (A.window <= 0 || p - cell < A.window || cell < A.first)) || kv4_hole<X>(A, q, cell)) sc[j][k] = -INFINITY;
                         }
                 }
                 float mx[2];
