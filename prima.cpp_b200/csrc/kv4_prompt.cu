@@ -144,12 +144,12 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
     }
     sum = __reduce_add_sync(0xffffffffu, sum) * A.cache.n_head_kv;
     __syncwarp();
-    // of the even share, 4 / 3 and 2 of it (with X also 2 / 3 and a half, as far as there are slots) that which ends first
+    // of the even share, 4 / 3 and 2 of it that which ends first
     const int share = max(4, (sum + ctas - 1) / ctas);
     int best = share, best_cost = INT_MAX;
 #pragma unroll 1
-    for (int i = 0; i < (X ? 5 : 3); i++) {
-        const int limit = X && i > 2 ? max(4, i == 3 ? (2 * share + 2) / 3 : (share + 1) / 2) : share + (i == 0 ? 0 : i == 1 ? (share + 2) / 3 : share);
+    for (int i = 0; i < 3; i++) {
+        const int limit = share + (i == 0 ? 0 : i == 1 ? (share + 2) / 3 : share);
         int n = 0, most = 0;
         for (int m = lane; m < all; m += 32) {
             const int k = kp_pieces(plan.lens[m], limit);
@@ -158,7 +158,6 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
         }
         n = __reduce_add_sync(0xffffffffu, n) * A.cache.n_head_kv;
         most = __reduce_max_sync(0xffffffffu, most);
-        if (X && i > 2 && n > KV4_SLOTS) break;
         // a piece's start and end are about three tiles; rounds of the longest, or, where lengths differ, long ones first: 4 / 3 of the mean at most
         const int mean = (int) (((float) sum + 3.f * (float) n) * (4.f / 3.f) * __frcp_rn((float) ctas)) + 1, cost = min((n + ctas - 1) / ctas * (most + 3), max(most + 3, mean));
         if (cost < best_cost) { best = limit; best_cost = cost; }
@@ -286,6 +285,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     __syncthreads();
     fence_after();
     const uint32_t tmem = *(volatile uint32_t *) &S.tmem_base;
+    if (X) pdl_trigger();                          // the join's CTAs may come where this kernel has none at work any more
     uint32_t tiles = 0, pieces = 0, of_group[2] = {0, 0}, ends[2] = {0, 0};   // key tiles and pieces in front; key tiles and ends of chunks of either group (all roles count them)
     while (*(volatile int *) &S.more[pieces & 1]) {
         const KpPiece & P = S.piece[pieces & 1];
@@ -726,7 +726,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
 // Items that were cut, eight rows to a CTA at a time: a warp adds a row's parts in their order, a lane D / 32 numbers.
 template <typename T, int D, bool X>
 __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Attn A, const __grid_constant__ KpWork W) {
-    constexpr int PER = D / 32, ONCE = 8, EIGHTS = kp_rows<T>() / 8;
+    constexpr int PER = D / 32, ONCE = X ? 4 : 8, EIGHTS = kp_rows<T>() / 8;
+    if (X) pdl_wait();
     const int lane = threadIdx.x & 31, items = *(volatile int *) &W.tickets[KP_CUT];
     const KpParts<D> & all = *reinterpret_cast<const KpParts<D> *>(W.parts);
     for (int task = blockIdx.x; task < items * EIGHTS; task += gridDim.x) {
@@ -809,8 +810,11 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     cfg.numAttrs = w.most_rows > 0 || a.x.mode == KV4_FRONT ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, k_kv4_attn_prompt<T, D, X>, a, w);
     if (e != cudaSuccess || !w.cut) return (int) e;
-    k_kv4_join<T, D, X><<<4 * sm_count(), 256, 0, st>>>(a, w);
-    return (int) cudaGetLastError();
+    cudaLaunchConfig_t join{};
+    join.gridDim = dim3(4 * sm_count()); join.blockDim = dim3(256); join.stream = st;
+    join.attrs = attr;
+    join.numAttrs = X ? 1 : 0;
+    return (int) cudaLaunchKernelEx(&join, k_kv4_join<T, D, X>, a, w);
 }
 
 }  // namespace

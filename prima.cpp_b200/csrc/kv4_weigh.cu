@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (tid == 0) S.abort = 0;
+    pdl_wait();                                             // what attention, or whatever stands in front, has written
     auto upto = [&](int x) {                                // sum over the threads up to this one, all: over all
         int y = x;
 #pragma unroll
@@ -546,8 +547,14 @@ int weigh_launch(const Kv4Weigh & w, cudaStream_t st) {
         static FuncAttrCache cache;
         const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D>, sizeof(KfSmem<D>) + 128 + KF_QUERIES, true);
         if (e != cudaSuccess) return (int) e;
-        k_kv4_weigh_few<T, D><<<sm_count(), KF_THREADS, smem, st>>>(w, abort_flag(), (int) rows);
-        return (int) cudaGetLastError();
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(sm_count()); cfg.blockDim = dim3(KF_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return (int) cudaLaunchKernelEx(&cfg, k_kv4_weigh_few<T, D>, w, abort_flag(), (int) rows);
     }
     constexpr size_t smem = sizeof(KwSmem<D, std::is_same<T, float>::value>);
     static FuncAttrCache cache;
