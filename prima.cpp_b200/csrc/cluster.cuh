@@ -39,9 +39,9 @@ __device__ __forceinline__ int remote(const int * at, uint32_t cta) {
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote_addr(at, cta)) : "memory");
     return v;
 }
-__device__ __forceinline__ uint4 remote(const uint4 * at, uint32_t cta) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote_addr(at, cta)) : "memory");
+__device__ __forceinline__ uint2 remote(const uint2 * at, uint32_t cta) {
+    uint2 v;
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(remote_addr(at, cta)) : "memory");
     return v;
 }
 
