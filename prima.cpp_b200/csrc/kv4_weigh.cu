@@ -273,43 +273,49 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
 }
 
 // ---- few rows ----
-// Pages stream through shared memory, by bulk copies: a warp has the keys of a page and a kv head at a time, the next ones on their way.  A unit is as many pages of a sequence as give each warp a
-// kv head of one; a CTA has a contiguous share of all units.  The queries of all heads lie in shared memory while it is at their sequence.
+// Pages stream through shared memory, by bulk copies: a warp has the keys of a page and a kv head at a time, the next ones on their way, and all of the head's rows or a part of them.  A unit is as
+// many pages of a sequence as give each warp such a turn; a CTA has a contiguous share of all units.  The queries lie in shared memory while it is at their sequence: where those of all heads do not fit, a cluster has the share, and each
+// CTA of it some of the heads, and some of the rows.
 constexpr int KF_WARPS = 16, KF_THREADS = 32 * KF_WARPS;
 __host__ __device__ constexpr int kf_bytes(int D) { return kv4_rows_bytes(D) + kv4_scales_bytes(D); }     // of a page's keys
-template <int D> constexpr int kf_stages() { return D == 128 ? 2 : 4; }
-constexpr size_t KF_QUERIES = 64 * 1024;
+constexpr int KF_STAGES = 2;
 
-template <int D> struct __align__(128) KfSmem {
-    __align__(128) uint8_t ring[KF_WARPS][kf_stages<D>()][kf_bytes(D)];
-    uint64_t full[KF_WARPS][kf_stages<D>()];
-    float part[2][KF_WARPS][KV4_CELLS];
-    int scan[KF_WARPS], begin_s, begin_unit, abort;
-};
-// behind it: of all rows (kv head by kv head) and eight more the numbers (F32: high, then low parts), what makes their weights, the positions of a kv head's
-template <typename T, int D> __host__ __device__ constexpr size_t kf_row_bytes() { return (std::is_same<T, float>::value ? 2 : 1) * (2 * D + 64) + sizeof(float2); }
-
+// heads and rows of a cluster's CTAs: so many parts of either (heads: evenly), a part's heads and rows at most; into how many turns a warp's rows are cut
+struct KfSplit { int heads, rows, n_head, most_rows, turns; int * abort_flag; };
 // a sequence: its queries, positions, cells and units
 struct KfSeq {
     int64_t q0;
     int n_q, p0, len, units;
 };
+template <int D> struct __align__(128) KfSmem {
+    __align__(128) uint8_t ring[KF_WARPS][KF_STAGES][kf_bytes(D)];
+    uint64_t full[KF_WARPS][KF_STAGES];
+    float part[2][KF_WARPS][KV4_CELLS], sums[2][KF_WARPS * KV4_CELLS];       // of the warps; of the CTA, for the cluster's others
+    int scan[KF_WARPS], begin_s, begin_unit, abort;
+    KfSeq begin;
+};
+// behind it: of all rows (kv head by kv head) and eight more the numbers (F32: high, then low parts), what makes their weights, the positions of a kv head's
+template <typename T, int D> __host__ __device__ constexpr size_t kf_row_bytes() { return (std::is_same<T, float>::value ? 2 : 1) * (2 * D + 64) + sizeof(float2); }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_constant__ Kv4Weigh W, int * abort_flag, int most_rows) {
+// MANY: a cluster has a share, or rows are cut into turns
+template <typename T, int D, bool MANY>
+__global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_constant__ Kv4Weigh W, const __grid_constant__ KfSplit X) {
     constexpr bool F32 = std::is_same<T, float>::value;
-    constexpr int NB = D / 32, LO = F32 ? 2 : 1, STAGES = kf_stages<D>(), STRIDE = 2 * D + 64;
+    constexpr int NB = D / 32, LO = F32 ? 2 : 1, STAGES = KF_STAGES, STRIDE = 2 * D + 64;
     extern __shared__ uint8_t smem_raw[];
     KfSmem<D> & S = *reinterpret_cast<KfSmem<D> *>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
     const Kv4Attn & A = W.attn;
-    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp(), g = lane >> 2, c = lane & 3, hks = A.cache.n_head_kv;
+    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp(), g = lane >> 2, c = lane & 3;
     uint8_t * const queries = reinterpret_cast<uint8_t *>(&S + 1);
-    const int room = hks * most_rows + 8;                   // rows
+    // kv heads of this CTA, its part of their rows, turns over a page
+    const int ctas = MANY ? X.heads * X.rows : 1, rank = MANY ? (int) cluster_rank() : 0, head0 = MANY ? rank % X.heads * X.n_head : 0, part = MANY ? rank / X.heads : 0, hks = X.n_head;
+    const int row_parts = MANY ? X.rows : 1, cuts = MANY ? X.turns : 1, turns = hks * cuts;
+    const int room = hks * X.most_rows + 8;                 // rows
     float2 * const factors = reinterpret_cast<float2 *>(queries + (size_t) room * STRIDE * LO);
     int * const pos = reinterpret_cast<int *>(factors + room);
     volatile int * cta_abort = &S.abort;
-    // pages of a unit; this warp's page of them and its first kv head (hks and more: none)
-    const int P = max(1, KF_WARPS / hks), my_page = P > 1 ? warp / hks : 0, my_head = P > 1 ? (my_page < P ? warp % hks : hks) : warp;
+    // pages of a unit; this warp's page of them and its first turn (`turns` and more: none)
+    const int P = max(1, KF_WARPS / turns), my_page = P > 1 ? warp / turns : 0, my_turn = P > 1 ? (my_page < P ? warp % turns : turns) : warp;
 
     auto seq = [&](int s) {
         KfSeq q{};
@@ -346,39 +352,47 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         __syncthreads();
         return y;
     };
-    int mine = 0;
-    for (int s = tid; s < A.n_seq; s += KF_THREADS) mine += seq(s).units;
-    upto(mine);
+    const KfSeq first = seq(tid);
+    int mine = first.units;
+    for (int s = tid + KF_THREADS; s < A.n_seq; s += KF_THREADS) mine += seq(s).units;
+    int ends = upto(mine);
     long long total = 0;
 #pragma unroll
-    for (int w = 0; w < KF_WARPS; w++) total += S.scan[w];
-    const int u0 = (int) (total * blockIdx.x / gridDim.x), u1 = (int) (total * (blockIdx.x + 1) / gridDim.x);
-    if (u0 == u1) return;
-    for (int s0 = 0, before = 0; s0 < A.n_seq; s0 += KF_THREADS) {
-        const int n = seq(s0 + tid).units;
-        int x = upto(n) - n + before;
-#pragma unroll
-        for (int w = 0; w < KF_WARPS; w++) {
-            if (w < warp) x += S.scan[w];
-            before += S.scan[w];
-        }
-        if (u0 >= x && u0 < x + n) { S.begin_s = s0 + tid; S.begin_unit = u0 - x; }
-        if (u0 < before) break;
+    for (int w = 0; w < KF_WARPS; w++) {
+        if (w < warp) ends += S.scan[w];
+        total += S.scan[w];
     }
+    const int shares = (int) gridDim.x / ctas, share = (int) blockIdx.x / ctas, u0 = (int) (total * share / shares), u1 = (int) (total * (share + 1) / shares);
+    if (u0 == u1) return;                                   // (all CTAs of a cluster)
+    auto begins = [&](int s, const KfSeq & q, int before) {
+        if (u0 >= before && u0 < before + q.units) { S.begin_s = s; S.begin_unit = u0 - before; S.begin = q; }
+    };
+    if (A.n_seq <= KF_THREADS) begins(tid, first, ends - mine);
+    else
+        for (int s0 = 0, before = 0; s0 < A.n_seq && before <= u0; s0 += KF_THREADS) {
+            const KfSeq q = seq(s0 + tid);
+            int x = upto(q.units) - q.units + before;
+#pragma unroll
+            for (int w = 0; w < KF_WARPS; w++) {
+                if (w < warp) x += S.scan[w];
+                before += S.scan[w];
+            }
+            begins(s0 + tid, q, x);
+        }
     __syncthreads();
 
-    // ---- this warp's keys on their way: by units and, where there are more heads than warps, heads ----
+    // ---- this warp's keys on their way: by units and, where there are more turns than warps, turns ----
     uint64_t policy;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    int f_s = S.begin_s, f_unit = S.begin_unit, f_u = u0, f_head = my_head, f_n = 0;
-    KfSeq f_q = seq(f_s);
+    int f_s = S.begin_s, f_unit = S.begin_unit, f_u = u0, f_turn = my_turn, f_n = 0;
+    KfSeq f_q = S.begin;
     int ids = -1, ids0 = 0, ids1 = 0;                       // pages of the units ids0 .. ids1 - 1 of the sequence, one to a lane
     uint32_t none = 0;                                      // stages whose page nobody sees, or that is none
     auto sees = [&](const KfSeq & q, int base) {            // any query any of the page's cells
         return q.n_q > 0 && base <= q.p0 + q.n_q - 1 && (A.window <= 0 || q.p0 - (base + KV4_CELLS - 1) < A.window || base < A.first);
     };
     auto fetch = [&] {
-        if (f_u >= u1 || f_head >= hks) return;
+        if (f_u >= u1 || f_turn >= turns) return;
         while (f_unit >= f_q.units) {
             f_q = seq(++f_s);
             f_unit = 0;
@@ -396,7 +410,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         none = id >= 0 ? none & ~(1u << st) : none | 1u << st;
         if (elect_one()) {
             if (id >= 0) {
-                const uint8_t * chunk = kv4_chunk<D>(A.cache, id, f_head);
+                const uint8_t * chunk = kv4_chunk<D>(A.cache, id, head0 + (MANY ? f_turn / cuts : f_turn));
                 mbar_arrive_expect_tx(&S.full[warp][st], kf_bytes(D));
                 bulk_g2s(S.ring[warp][st], chunk, kv4_rows_bytes(D), &S.full[warp][st], policy);
                 bulk_g2s(S.ring[warp][st] + kv4_rows_bytes(D), chunk + 2 * kv4_rows_bytes(D), kv4_scales_bytes(D), &S.full[warp][st], policy);
@@ -404,61 +418,84 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         }
         __syncwarp();
         f_n++;
-        f_head += KF_WARPS;
-        if (P > 1 || f_head >= hks) {
-            f_head = my_head;
+        f_turn += KF_WARPS;
+        if (P > 1 || f_turn >= turns) {
+            f_turn = my_turn;
             f_unit++;
             f_u++;
         }
     };
-    for (int k = 0; k < STAGES; k++) fetch();
-
     int s = S.begin_s, unit = S.begin_unit, n = 0;
     bool fresh = true;
-    KfSeq q = seq(s);
+    // the k-th cell of a unit that this thread stores (a cluster's CTAs have them in turns), at most two; beyond the unit's: none
+    auto own_cell = [&](int k) { return (k * KF_THREADS + tid) * ctas + rank; };
+    KfSeq q = S.begin;
     for (int u = u0; u < u1; u++, unit++) {
         while (unit >= q.units) {
             q = seq(++s);
             unit = 0;
             fresh = true;
         }
-        const int rows = q.n_q * A.group;
-        if (fresh) {   // ---- the sequence's queries: four threads to a row ----  (everybody is through with the last one's: behind the barrier of its last unit)
+        const int all_rows = q.n_q * A.group, row0 = MANY ? (int) ((int64_t) all_rows * part / row_parts) : 0, rows = MANY ? (int) ((int64_t) all_rows * (part + 1) / row_parts) - row0 : all_rows;
+        if (fresh) {   // ---- the sequence's queries: four threads to a row, two rows of theirs at once ----  (everybody is through with the last one's: behind the barrier of its last unit)
             fresh = false;
-            for (int i0 = 0; i0 < hks * rows; i0 += KF_THREADS / 4) {
-                const int i = i0 + (tid >> 2), quarter = tid & 3, hk = i / max(rows, 1), r = i - hk * rows, t = r / A.group, head = hk * A.group + r - t * A.group;
-                const bool have = i < hks * rows;
-                constexpr int EACH = D / 4;
-                float x[EACH], top = 0.f;
-                const T * src = (const T *) A.q + (q.q0 + t) * A.ldq + (int64_t) head * D + quarter * EACH;
+            constexpr int EACH = D / 4, ONCE = 2, ROWS = KF_THREADS / 4;
+            for (int i0 = 0; i0 < hks * rows; i0 += ONCE * ROWS) {
+                float x[ONCE][EACH], lse[ONCE];
 #pragma unroll
-                for (int k = 0; k < EACH; k += 4) {
-                    const float4 v = have ? load4(src + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
+                for (int o = 0; o < ONCE; o++) {
+                    const int i = i0 + o * ROWS + (tid >> 2), hk = i / max(rows, 1), r = row0 + i - hk * rows, t = r / A.group, head = (head0 + hk) * A.group + r - t * A.group;
+                    const bool have = i < hks * rows;
+                    const T * src = (const T *) A.q + (q.q0 + t) * A.ldq + (int64_t) head * D + (tid & 3) * EACH;
+#pragma unroll
+                    for (int k = 0; k < EACH; k += 4) {
+                        const float4 v = have ? load4(src + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[o][k] = v.x; x[o][k + 1] = v.y; x[o][k + 2] = v.z; x[o][k + 3] = v.w;
+                    }
+                    lse[o] = have ? W.lse[(q.q0 + t) * W.ld_lse + head] : -INFINITY;
                 }
-                const float lse = have ? W.lse[(q.q0 + t) * W.ld_lse + head] : -INFINITY;
-                const float up = row_power<EACH>(x, top) * (A.scale < 0.f ? -1.f : 1.f);
-                if (have) {
-                    row_store<T, EACH>(x, up, queries + (size_t) i * STRIDE + 2 * quarter * EACH, queries + (size_t) (room + i) * STRIDE + 2 * quarter * EACH);
+                if (f_n == 0)                               // the first keys, behind the first queries
+                    for (int k = 0; k < STAGES; k++) fetch();
+#pragma unroll
+                for (int o = 0; o < ONCE; o++) {
+                    const int i = i0 + o * ROWS + (tid >> 2), quarter = tid & 3;
+                    const float up = row_power<EACH>(x[o], 0.f) * (A.scale < 0.f ? -1.f : 1.f);
+                    if (i >= hks * rows) continue;
+                    row_store<T, EACH>(x[o], up, queries + (size_t) i * STRIDE + 2 * quarter * EACH, queries + (size_t) (room + i) * STRIDE + 2 * quarter * EACH);
                     if (quarter == 0) {
-                        factors[i] = row_factors(A.scale, up, lse);
-                        if (hk == 0) pos[r] = q.p0 + t;
+                        factors[i] = row_factors(A.scale, up, lse[o]);
+                        if (i < rows) pos[i] = q.p0 + (row0 + i) / A.group;
                     }
                 }
             }
+            if (f_n == 0)
+                for (int k = 0; k < STAGES; k++) fetch();
             __syncthreads();
         }
+        // what the sums are added to, on its way
+        const int cells = P * KV4_CELLS;
+        float past[2] = {0.f, 0.f};
+        if (W.old)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int i = own_cell(k);
+                const int64_t j = (int64_t) unit * cells + i;
+                if (i < cells && j < q.len) past[k] = W.decay * W.old[s * W.ld_old + j];
+            }
+        const int t_lo = row0 / A.group, t_hi = rows > 0 ? (row0 + rows - 1) / A.group : t_lo;      // this CTA's queries
         float sum[4][2];
 #pragma unroll
         for (int m = 0; m < 4; m++) sum[m][0] = sum[m][1] = 0.f;
         const int base = (unit * P + my_page) * KV4_CELLS;
-        for (int hk = my_head; hk < hks; hk += P > 1 ? hks : KF_WARPS, n++) {
+        for (int turn = my_turn; turn < turns; turn += P > 1 ? turns : KF_WARPS, n++) {
+            // rows j0 .. j1 - 1 of kv head hk
+            const int hk = MANY ? turn / cuts : turn, cut = MANY ? turn - hk * cuts : 0, j0 = MANY ? (rows + 7) / 8 * cut / cuts * 8 : 0, j1 = !MANY || cut == cuts - 1 ? rows : (rows + 7) / 8 * (cut + 1) / cuts * 8;
             const int st = n % STAGES;
             const bool have = !(none >> st & 1);
-            mbar_wait(&S.full[warp][st], (uint32_t) (n / STAGES) & 1, cta_abort, abort_flag);
+            mbar_wait(&S.full[warp][st], (uint32_t) (n / STAGES) & 1, cta_abort, X.abort_flag);
             if (have) {
                 const uint8_t * chunk = S.ring[warp][st], * scales = chunk + kv4_rows_bytes(D);
-                const int p_lo = q.p0, p_hi = q.p0 + q.n_q - 1;
+                const int p_lo = q.p0 + t_lo, p_hi = q.p0 + t_hi;
                 const bool whole = base + KV4_CELLS - 1 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + KV4_CELLS - 1 < A.first);
 #pragma unroll 1
                 for (int m2 = 0; m2 < 2; m2++) {            // 32 cells at a time
@@ -471,25 +508,22 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                             key_halves<D>(chunk + t * (D / 2) + 4 * NB * c, scales + kv4_scale(D, t & ~1, 0), t & 1, kf[m], h);
                         }
                     float acc2[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll 1
-                    for (int j = 0; j < rows; j += 8) {
+                    auto weights = [&](int j, float (&e)[2][4]) {       // of rows j .. j + 7, from their scores
                         const int i = hk * rows + j;
-                        float e[2][4];
-                        scores<LO, NB>(kf, queries + (size_t) (i + g) * STRIDE + 16 * c, (size_t) room * STRIDE, e);
                         const float2 r0 = factors[i + 2 * c], r1 = factors[i + 2 * c + 1];
 #pragma unroll
                         for (int m = 0; m < 2; m++)
 #pragma unroll
                             for (int k = 0; k < 4; k++) e[m][k] = ex2(fmaf(e[m][k], k & 1 ? r1.x : r0.x, k & 1 ? -r1.y : -r0.y));
-                        if (j + 8 > rows) {                 // rows of nobody's
-                            const bool ra = j + 2 * c < rows, rb = j + 2 * c + 1 < rows;
+                        if (j + 8 > j1) {                   // rows of nobody's
+                            const bool ra = j + 2 * c < j1, rb = j + 2 * c + 1 < j1;
 #pragma unroll
                             for (int m = 0; m < 2; m++)
 #pragma unroll
                                 for (int k = 0; k < 4; k++) e[m][k] = (k & 1 ? rb : ra) ? e[m][k] : 0.f;
                         }
                         if (!whole) {
-                            const int pa = j + 2 * c < rows ? pos[j + 2 * c] : INT_MIN, pb = j + 2 * c + 1 < rows ? pos[j + 2 * c + 1] : INT_MIN;
+                            const int pa = j + 2 * c < j1 ? pos[j + 2 * c] : INT_MIN, pb = j + 2 * c + 1 < j1 ? pos[j + 2 * c + 1] : INT_MIN;
 #pragma unroll
                             for (int m = 0; m < 2; m++)
 #pragma unroll
@@ -503,6 +537,21 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                             acc2[m][0] += e[m][0] + e[m][1];
                             acc2[m][1] += e[m][2] + e[m][3];
                         }
+                    };
+                    const uint8_t * const q_at = queries + (size_t) (hk * rows + g) * STRIDE + 16 * c;
+                    int j = j0;
+#pragma unroll 1
+                    for (; j + 8 < j1; j += 16) {           // two tiles of rows at once: one's products beside the other's weights
+                        float e0[2][4], e1[2][4];
+                        scores<LO, NB>(kf, q_at + (size_t) j * STRIDE, (size_t) room * STRIDE, e0);
+                        scores<LO, NB>(kf, q_at + (size_t) (j + 8) * STRIDE, (size_t) room * STRIDE, e1);
+                        weights(j, e0);
+                        weights(j + 8, e1);
+                    }
+                    if (j < j1) {
+                        float e0[2][4];
+                        scores<LO, NB>(kf, q_at + (size_t) j * STRIDE, (size_t) room * STRIDE, e0);
+                        weights(j, e0);
                     }
 #pragma unroll
                     for (int m = 0; m < 2; m++)
@@ -518,7 +567,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         }
         // ---- the warps' sums: of a page those of its kv heads, in their order ----
         const int flip = u & 1;
-        if (my_head < hks)
+        if (my_turn < turns)
 #pragma unroll
             for (int m = 0; m < 4; m++)
 #pragma unroll
@@ -529,32 +578,76 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                     if (c == 0) S.part[flip][warp][16 * m + 8 * h + g] = x;
                 }
         __syncthreads();                                    // (of the unit behind the next one's, nobody reads these any more)
-        for (int i = tid; i < P * KV4_CELLS; i += KF_THREADS) {
-            const int page = i / KV4_CELLS, j = unit * P * KV4_CELLS + i, w0 = P > 1 ? page * hks : 0, w1 = P > 1 ? w0 + hks : min(KF_WARPS, hks);
+        auto store = [&](int k, float x) {
+            const int64_t j = (int64_t) unit * cells + own_cell(k);
+            if (j < q.len) W.sums[s * W.ld_sums + j] = x + past[k];
+        };
+        for (int k = 0, i = tid; i < cells; k++, i += KF_THREADS) {
+            const int page = i / KV4_CELLS, w0 = P > 1 ? page * turns : 0, w1 = P > 1 ? w0 + turns : min(KF_WARPS, turns);
             float x = 0.f;
             for (int w = w0; w < w1; w++) x += S.part[flip][w][i % KV4_CELLS];
-            if (j < q.len) W.sums[s * W.ld_sums + j] = W.old ? fmaf(W.decay, W.old[s * W.ld_old + j], x) : x;
+            if (MANY) S.sums[flip][i] = x;
+            else store(k, x);
+        }
+        if (MANY) {   // the cluster's CTAs each add up some of the cells, in the CTAs' order
+            cluster_sync();
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int i = own_cell(k);
+                if (i >= cells) continue;
+                float far[8], x = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; r++) far[r] = r < ctas ? remote(&S.sums[flip][i], r) : 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; r++) x += far[r];
+                store(k, x);
+            }
         }
     }
+    if (MANY) cluster_sync();                               // nobody reads a CTA's sums that has ended
+}
+
+template <typename T, int D, bool MANY>
+int weigh_few_launch(const Kv4Weigh & w, const KfSplit & x, size_t rows_bytes, cudaStream_t st) {
+    const size_t smem = sizeof(KfSmem<D>) + 128 + rows_bytes;
+    static FuncAttrCache cache;
+    const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D, MANY>, 232448, true);
+    if (e != cudaSuccess) return (int) e;
+    const int ctas = x.heads * x.rows;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(sm_count() / ctas * ctas); cfg.blockDim = dim3(KF_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned) ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = MANY ? 2 : 1;
+    return (int) cudaLaunchKernelEx(&cfg, k_kv4_weigh_few<T, D, MANY>, w, x);
 }
 
 template <typename T, int D>
 int weigh_launch(const Kv4Weigh & w, cudaStream_t st) {
     const int hks = w.attn.cache.n_head_kv;
-    const int64_t rows = std::min<int64_t>(w.attn.max_q, w.attn.n_tokens) * w.attn.group, few = (hks * rows + 8) * (int64_t) kf_row_bytes<T, D>() + 4 * rows;
-    if (few <= (int64_t) KF_QUERIES) {
-        const size_t smem = sizeof(KfSmem<D>) + 128 + (size_t) few;
-        static FuncAttrCache cache;
-        const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D>, sizeof(KfSmem<D>) + 128 + KF_QUERIES, true);
-        if (e != cudaSuccess) return (int) e;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(sm_count()); cfg.blockDim = dim3(KF_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        return (int) cudaLaunchKernelEx(&cfg, k_kv4_weigh_few<T, D>, w, abort_flag(), (int) rows);
+    const int64_t rows = std::min<int64_t>(w.attn.max_q, w.attn.n_tokens) * w.attn.group;
+    // as few CTAs to a cluster as hold the rows; heads are split first
+    KfSplit x{1, 1, hks, 0, 1, abort_flag()};
+    constexpr size_t least = sizeof(KfSmem<D>) + 128, room = 232448 - least;      // an SM's shared memory
+    size_t few;
+    for (;;) {
+        x.n_head = hks / x.heads;
+        const int64_t most = (rows + x.rows - 1) / x.rows;
+        few = (size_t) (x.n_head * most + 8) * kf_row_bytes<T, D>() + 4 * (size_t) most;
+        x.most_rows = (int) most;
+        if (few <= room || x.heads * x.rows == 8) break;
+        if (x.n_head % 2 == 0) x.heads *= 2;
+        else x.rows *= 2;
+    }
+    if (few <= room) {
+        // many rows of a head are cut into turns of 64 and more, so that units are smaller
+        while (x.n_head * x.turns * 2 <= KF_WARPS && x.most_rows >= 128 * x.turns) x.turns *= 2;
+        return x.heads * x.rows * x.turns > 1 ? weigh_few_launch<T, D, true>(w, x, few, st) : weigh_few_launch<T, D, false>(w, x, few, st);
     }
     constexpr size_t smem = sizeof(KwSmem<D, std::is_same<T, float>::value>);
     static FuncAttrCache cache;
