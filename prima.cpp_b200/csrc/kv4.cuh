@@ -110,7 +110,7 @@ struct Kv4Ext {
     const int32_t * prefix_len, * prefix_table;
     int64_t prefix_ld;
     int n_group, n_own;                   // groups, sequences
-    int64_t least, of_page;               // groups whose sequences walk as many pages in front of their own have them by themselves; what a page of a prefix counts for a sequence: tiles x kv heads
+    int64_t least, of_page;               // where sequences would walk as many pages in front of their own, prefixes are by themselves; what a page of a prefix counts for a sequence: tiles x kv heads
     float * o; float4 * ml;               // parts of rows [token][head]: sums [D]; reference, sum of weights, and the mark of the call
     int * sync;                           // calls that have ended, CTAs of a call's last kernel that have
 };

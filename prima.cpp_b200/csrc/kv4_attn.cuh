@@ -45,23 +45,32 @@ __device__ __forceinline__ void kv4_span(const Kv4Attn & A, int lo, int hi, Kv4S
         q.from = from;
     } else kv4_pages(A, X && A.x.mode == KV4_FRONT ? A.x.prefix_ld : A.table_ld, lo, hi, q);
 }
-// the group of a sequence, -1: none
-__device__ __forceinline__ int kv4_group_of(const Kv4Attn & A, int s) {
-    const int n = A.x.n_group;
-    if (s < A.x.group_start[0] || s >= A.x.group_start[n]) return -1;
-    int lo = 0, hi = n;                        // group_start[lo] <= s < group_start[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (A.x.group_start[mid] <= s) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-// cells of a prefix (30 bits), and whether it is by itself
+// cells of group g's prefix (30 bits), and whether it is by itself: what counts are all groups' pages, up to KV4_FEW_GROUPS of them; of more, the group's times their number
+constexpr int KV4_FEW_GROUPS = 8;
 __device__ __forceinline__ int kv4_prefix(const Kv4Attn & A, int g, bool & apart) {
-    const int cells = min(max(A.x.prefix_len[g], 0), 1 << 30), sequences = A.x.group_start[g + 1] - A.x.group_start[g];
-    apart = (int64_t) sequences * ((cells + KV4_CELLS - 1) / KV4_CELLS) * A.x.of_page >= A.x.least;
-    return cells;
+    auto cells = [&](int i) { return min(max(A.x.prefix_len[i], 0), 1 << 30); };
+    auto pages = [&](int i) { return (int64_t) (A.x.group_start[i + 1] - A.x.group_start[i]) * ((cells(i) + KV4_CELLS - 1) / KV4_CELLS); };
+    int64_t all = 0;
+    if (A.x.n_group <= KV4_FEW_GROUPS)
+#pragma unroll 1
+        for (int i = 0; i < A.x.n_group; i++) all += pages(i);
+    else all = pages(g) * A.x.n_group;
+    apart = all * A.x.of_page >= A.x.least;
+    return cells(g);
+}
+// KV4_SHARED: a sequence's `keep` and `from`.  A call, not code in its place: kernels have it in many, and what they are short of is the time to fetch code (a token behind 1000 cells 16 -> 14 us)
+static __device__ __noinline__ int2 kv4_in_front(const Kv4Attn & A, int s) {
+    const int n = A.x.n_group;
+    if (s < A.x.group_start[0] || s >= A.x.group_start[n]) return make_int2(0, 0);
+    int g = 0, end = n;                        // group_start[g] <= s < group_start[end]
+    while (end - g > 1) {
+        const int mid = (g + end) / 2;
+        if (A.x.group_start[mid] <= s) g = mid;
+        else end = mid;
+    }
+    bool apart;
+    const int cells = kv4_prefix(A, g, apart), pages = (cells + KV4_CELLS - 1) / KV4_CELLS;
+    return apart ? make_int2(0, -1) : make_int2(pages, KV4_CELLS * g + (KV4_CELLS * pages - cells));
 }
 // position of query t of a sequence
 template <bool X> __device__ __forceinline__ int kv4_pos(const Kv4Attn & A, const Kv4Seq & q, int t) {
@@ -92,15 +101,10 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_row
     const int len = max((int) cells, 0);
     q.p0 = front ? len - 1 : len - all;
     if (kv4_shared<X>(A)) {
-        const int g = kv4_group_of(A, s);
-        q.p0 = min(len, 1 << 30) - all;
-        if (g >= 0) {
-            bool apart;
-            const int in_front = kv4_prefix(A, g, apart);
-            q.keep = apart ? 0 : (in_front + KV4_CELLS - 1) / KV4_CELLS;
-            q.from = apart ? -1 : KV4_CELLS * g + (KV4_CELLS * q.keep - in_front);
-            q.p0 += KV4_CELLS * q.keep;
-        }
+        const int2 front = kv4_in_front(A, s);
+        q.keep = front.x;
+        q.from = front.y;
+        q.p0 = min(len, 1 << 30) - all + KV4_CELLS * q.keep;
     }
     kv4_span<X>(A, kv4_pos<X>(A, q, 0), kv4_pos<X>(A, q, n - 1), q);
     return q;
@@ -126,14 +130,12 @@ __device__ __forceinline__ int kv4_page(const Kv4Attn & A, const Kv4Seq & q, int
     }
     return id >= 0 && id < A.cache.n_pages ? id : -1;
 }
-// cells behind the end of a prefix, in its last page
-template <bool X> __device__ __forceinline__ int kv4_hole_from(const Kv4Seq & q) { return KV4_CELLS * q.keep - q.from % KV4_CELLS; }
-template <bool X> __device__ __forceinline__ bool kv4_hole(const Kv4Attn & A, const Kv4Seq & q, int cell) {
-    return kv4_shared<X>(A) && q.keep > 0 && cell >= kv4_hole_from<X>(q) && cell < KV4_CELLS * q.keep;
+// cells behind the end of a prefix, in its last page: [x, y)
+template <bool X> __device__ __forceinline__ int2 kv4_hole(const Kv4Attn & A, const Kv4Seq & q) {
+    return kv4_shared<X>(A) && q.keep > 0 ? make_int2(KV4_CELLS * q.keep - q.from % KV4_CELLS, KV4_CELLS * q.keep) : make_int2(0, 0);
 }
-template <bool X> __device__ __forceinline__ bool kv4_has_hole(const Kv4Attn & A, const Kv4Seq & q, int base) {      // a page from cell `base` on
-    return kv4_shared<X>(A) && q.keep > 0 && base < KV4_CELLS * q.keep && base + KV4_CELLS > kv4_hole_from<X>(q);
-}
+template <bool X> __device__ __forceinline__ bool kv4_in_hole(int2 hole, int cell) { return X && cell >= hole.x && cell < hole.y; }
+template <bool X> __device__ __forceinline__ bool kv4_has_hole(int2 hole, int base) { return X && base < hole.y && base + KV4_CELLS > hole.x; }      // a page from cell `base` on
 
 // of a part with maximum m and sum l of weights, where all parts' maximum is top (a row that is no number has no maximum)
 __device__ __forceinline__ float part_factor(float m, float l, float top) { return m == -INFINITY ? (l == l ? 0.f : 1.f) : ex2(m - top); }

@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
     uint32_t tiles = 0, pieces = 0, of_group[2] = {0, 0}, ends[2] = {0, 0};   // key tiles and pieces in front; key tiles and ends of chunks of either group (all roles count them)
     while (*(volatile int *) &S.more[pieces & 1]) {
         const KpPiece & P = S.piece[pieces & 1];
+        const int2 hole = kv4_hole<X>(A, P.q);
         const int n = P.b - P.a, groups = (F32 ? n > 1 : P.rows > KP_TILE) ? 2 : 1;      // groups at work
         if (warp < 4) {
             // ---- expand ----
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                 {
                     const int i = 2 * (P.a + j) + half, cell = kv4_page_index<X>(A, P.q, i) * KV4_CELLS + tv, t = half * 64 + tv;
                     // a weight of zero does not silence a scale that is no number: cells nobody sees may hold anything
-                    const bool seen = cell <= P.p_hi && (A.window <= 0 || P.p_lo - cell < A.window || cell < A.first) && !kv4_hole<X>(A, P.q, cell);
+                    const bool seen = cell <= P.p_hi && (A.window <= 0 || P.p_lo - cell < A.window || cell < A.first) && !kv4_in_hole<X>(hole, cell);
                     const uint32_t odd = tv & 1 ? 0x3232u : 0x1010u;
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                     fence_after();
                     // (four of them: written for tile j + 4 behind the scores of j + 2, which come behind the weights of j)
                     const int c0 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][0], c1 = *(volatile int *) &S.cell[(tiles + (uint32_t) j) & 3][1];
-                    const bool whole = min(c0, c1) >= 0 && max(c0, c1) <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first)) && !kv4_has_hole<X>(A, P.q, c0) && !kv4_has_hole<X>(A, P.q, c1);
+                    const bool whole = min(c0, c1) >= 0 && max(c0, c1) <= g_lo - 63 && (A.window <= 0 || (P.p_hi - c0 < A.window || c0 + 63 < A.first) && (P.p_hi - c1 < A.window || c1 + 63 < A.first)) && !kv4_has_hole<X>(hole, c0) && !kv4_has_hole<X>(hole, c1);
                     if (!whole) {   // a score that is not seen is -inf: in its place, ahead of the passes over the tile
                         const int from = A.window > 0 ? max(0, pos - A.window + 1) : 0;
 #pragma unroll 1
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_prompt(const __grid_
                             const int page = h < 2 ? c0 : c1, base = page + 32 * (h & 1);
                             auto below = [&](int cell) { const int k = cell - base; return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };     // cells in front of it
                             uint32_t seen = page < 0 || base > pos ? 0u : below(pos + 1) & (~below(from) | below(A.first));
-                            if (kv4_shared<X>(A) && P.q.keep > 0) seen &= below(kv4_hole_from<X>(P.q)) | ~below(KV4_CELLS * P.q.keep);
+                            if (X && hole.y > 0) seen &= below(hole.x) | ~below(hole.y);
                             TMEM_LD32(mine + 32 * h, t0);
                             TMEM_ARRIVED(t0);
 #pragma unroll

@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
         }
         if (at.k0 == u0)                                // the first pages, behind the queries: these would wait for all that is on its way to this SM
             for (int k = 0; k < STAGES; k++) fetch(u0 + k);
+        const int2 hole = kv4_hole<X>(A, q);
         const int p_lo = kv4_pos<X>(A, q, row0 / A.group), p_hi = kv4_pos<X>(A, q, (row0 + rows - 1) / A.group);   // of the tile's rows
 
         // out^T: lane: numbers 32 b + 4 g + 2 h, + 1 of rows 2 c, 2 c + 1 (SCALED: times 2^-24, and 2^-20 the odd ones)
@@ -397,12 +398,12 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
                 uint8_t * chunk = S.ring[warp][st];
                 uint8_t * const vs = chunk + 2 * kv4_rows_bytes(D) + kv4_scales_bytes(D);
                 const int base = kv4_page_index<X>(A, q, at.pa + u - at.k0) * KV4_CELLS;
-                const bool whole = base + 63 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + 63 < A.first) && !kv4_has_hole<X>(A, q, base);
+                const bool whole = base + 63 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + 63 < A.first) && !kv4_has_hole<X>(hole, base);
                 if (!whole) {   // a weight of zero does not silence a scale that is no number: cells nobody sees may hold anything
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int t = 2 * lane + e, cell = base + t;
-                        if (!(cell <= p_hi && (A.window <= 0 || p_lo - cell < A.window || cell < A.first)) || kv4_hole<X>(A, q, cell))
+                        if (!(cell <= p_hi && (A.window <= 0 || p_lo - cell < A.window || cell < A.first)) || kv4_in_hole<X>(hole, cell))
 #pragma unroll
                             for (int b = 0; b < NB; b++) *reinterpret_cast<uint16_t *>(vs + kv4_scale(D, t, b)) = 0;
                     }
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const int cell = base + 16 * j + g + (k >> 1) * 8, p = pos[k & 1];
-                            if (!(cell <= p && (A.window <= 0 || p - cell < A.window || cell < A.first)) || kv4_hole<X>(A, q, cell)) sc[j][k] = -INFINITY;
+                            if (!(cell <= p && (A.window <= 0 || p - cell < A.window || cell < A.first)) || kv4_in_hole<X>(hole, cell)) sc[j][k] = -INFINITY;
                         }
                 }
                 float mx[2];

@@ -52,7 +52,7 @@ __device__ __forceinline__ float row_power(const float (&x)[EACH], float top) {
     const int ex = top > 0.f && top < INFINITY ? min(126, 140 - (int) (__float_as_uint(top) >> 23)) : 0;
     return __int_as_float((ex + 127) << 23);
 }
-template <typename T, int EACH>
+template <typename T, int EACH, bool RAW = false>      // RAW: pairs 1 and 3 of eight numbers a 16th
 __device__ __forceinline__ void row_store(const float (&x)[EACH], float up, uint8_t * high, uint8_t * low) {
 #pragma unroll
     for (int i = 0; i < EACH; i += 8) {
@@ -61,7 +61,7 @@ __device__ __forceinline__ void row_store(const float (&x)[EACH], float up, uint
         for (int e = 0; e < 4; e++) {
             const float a = x[i + 2 * e] * up, b = x[i + 2 * e + 1] * up;
             const __half2 h = __floats2half2_rn(a, b);
-            hi[e] = hu(h);
+            hi[e] = hu(RAW && e % 2 ? __hmul2(h, __float2half2_rn(0.0625f)) : h);
             if constexpr (std::is_same<T, float>::value) {
                 const float2 back = __half22float2(h);
                 lo[e] = hu(__floats2half2_rn(a - back.x, b - back.y));
@@ -97,6 +97,21 @@ __device__ __forceinline__ void key_halves(const uint8_t * row, const uint8_t * 
         kf[b][1][h] = hu(__hmul2(__hsub2(uh((y & 0x000f000fu) | 0x64006400u), e), sc));
         kf[b][1][2 + h] = hu(__hmul2(__hsub2(uh((y & 0x00f000f0u) | 0x54005400u), o), sc));
     }
+}
+// a cell's words as they are, and the blocks' scales
+template <int D>
+__device__ __forceinline__ void key_words(const uint8_t * row, const uint8_t * scales, int odd, uint32_t (&w)[D / 32], float (&sc)[D / 32]) {
+    constexpr int NB = D / 32;
+    uint32_t d[NB];
+    if constexpr (NB == 4) {
+        *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(row);
+        *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(scales);
+    } else {
+        *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(row);
+        *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(scales);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++) sc[b] = __half2float(__ushort_as_half((unsigned short) (odd ? d[b] >> 16 : d[b])));
 }
 // scores of 32 cells and eight rows: lane: cells 16 m + g, + 8 of rows 2 c, 2 c + 1; q: this lane's part of row g, the low parts `low` bytes further on: these first (what is added to a sum is cut off)
 template <int LO, int NB>
@@ -278,7 +293,7 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
 // CTA of it some of the heads, and some of the rows.
 constexpr int KF_WARPS = 16, KF_THREADS = 32 * KF_WARPS;
 __host__ __device__ constexpr int kf_bytes(int D) { return kv4_rows_bytes(D) + kv4_scales_bytes(D); }     // of a page's keys
-constexpr int KF_STAGES = 2;
+constexpr int KF_STAGES = 2, KF_RAW_ROWS = 16;
 
 // heads and rows of a cluster's CTAs: so many parts of either (heads: evenly), a part's heads and rows at most; into how many turns a warp's rows are cut
 struct KfSplit { int heads, rows, n_head, most_rows, turns; int * abort_flag; };
@@ -297,10 +312,14 @@ template <int D> struct __align__(128) KfSmem {
 // behind it: of all rows (kv head by kv head) and eight more the numbers (F32: high, then low parts), what makes their weights, the positions of a kv head's
 template <typename T, int D> __host__ __device__ constexpr size_t kf_row_bytes() { return (std::is_same<T, float>::value ? 2 : 1) * (2 * D + 64) + sizeof(float2); }
 
-// MANY: a cluster has a share, or rows are cut into turns
-template <typename T, int D, bool MANY>
+// How: MANY: a cluster has a share, or rows are cut into turns.  RAW: 16 bits, up to two tiles of rows to a kv head: the numbers' 4 bits go into the products as they are, as the f16 n * 2^-24 (n * 2^-20
+// a nibble further up, which meets a 16th of the query), and scales onto the sums of blocks, which start from -8 times the query's; making them f16 keys takes twice as many instructions (32
+// sequences of up to 8192 cells 38 us where this takes 33)
+enum { KF_PLAIN = 0, KF_RAW = 1, KF_MANY = 2 };
+template <typename T, int D, int HOW>
 __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_constant__ Kv4Weigh W, const __grid_constant__ KfSplit X) {
     constexpr bool F32 = std::is_same<T, float>::value;
+    constexpr bool MANY = HOW == KF_MANY, RAW = HOW == KF_RAW;
     constexpr int NB = D / 32, LO = F32 ? 2 : 1, STAGES = KF_STAGES, STRIDE = 2 * D + 64;
     extern __shared__ uint8_t smem_raw[];
     KfSmem<D> & S = *reinterpret_cast<KfSmem<D> *>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
@@ -312,7 +331,8 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
     const int row_parts = MANY ? X.rows : 1, cuts = MANY ? X.turns : 1, turns = hks * cuts;
     const int room = hks * X.most_rows + 8;                 // rows
     float2 * const factors = reinterpret_cast<float2 *>(queries + (size_t) room * STRIDE * LO);
-    int * const pos = reinterpret_cast<int *>(factors + room);
+    float * const starts = reinterpret_cast<float *>(factors + room);        // RAW: of each row and block
+    int * const pos = reinterpret_cast<int *>(starts + (RAW ? room * NB : 0));
     volatile int * cta_abort = &S.abort;
     // pages of a unit; this warp's page of them and its first turn (`turns` and more: none)
     const int P = max(1, KF_WARPS / turns), my_page = P > 1 ? warp / turns : 0, my_turn = P > 1 ? (my_page < P ? warp % turns : turns) : warp;
@@ -437,9 +457,9 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
             fresh = true;
         }
         const int all_rows = q.n_q * A.group, row0 = MANY ? (int) ((int64_t) all_rows * part / row_parts) : 0, rows = MANY ? (int) ((int64_t) all_rows * (part + 1) / row_parts) - row0 : all_rows;
-        if (fresh) {   // ---- the sequence's queries: four threads to a row, two rows of theirs at once ----  (everybody is through with the last one's: behind the barrier of its last unit)
+        if (fresh) {   // ---- the sequence's queries: four threads to a row, with MANY two rows of theirs at once ----  (everybody is through with the last one's: behind the barrier of its last unit)
             fresh = false;
-            constexpr int EACH = D / 4, ONCE = 2, ROWS = KF_THREADS / 4;
+            constexpr int EACH = D / 4, ONCE = MANY ? 2 : 1, ROWS = KF_THREADS / 4;
             for (int i0 = 0; i0 < hks * rows; i0 += ONCE * ROWS) {
                 float x[ONCE][EACH], lse[ONCE];
 #pragma unroll
@@ -460,10 +480,18 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                 for (int o = 0; o < ONCE; o++) {
                     const int i = i0 + o * ROWS + (tid >> 2), quarter = tid & 3;
                     const float up = row_power<EACH>(x[o], 0.f) * (A.scale < 0.f ? -1.f : 1.f);
+                    float block = 0.f;                      // sum of the block's numbers
+                    if (RAW) {
+#pragma unroll
+                        for (int k = 0; k < EACH; k++) block += x[o][k];
+                        if (EACH == 16) block += __shfl_xor_sync(0xffffffffu, block, 1);
+                    }
                     if (i >= hks * rows) continue;
-                    row_store<T, EACH>(x[o], up, queries + (size_t) i * STRIDE + 2 * quarter * EACH, queries + (size_t) (room + i) * STRIDE + 2 * quarter * EACH);
+                    row_store<T, EACH, RAW>(x[o], up, queries + (size_t) i * STRIDE + 2 * quarter * EACH, queries + (size_t) (room + i) * STRIDE + 2 * quarter * EACH);
+                    if (RAW && (EACH == 32 || quarter % 2 == 0)) starts[i * NB + quarter * EACH / 32] = block * (up * (-8.f / 16777216.f));
                     if (quarter == 0) {
                         factors[i] = row_factors(A.scale, up, lse[o]);
+                        if (RAW) factors[i].x *= 16777216.f;
                         if (i < rows) pos[i] = q.p0 + (row0 + i) / A.group;
                     }
                 }
@@ -480,7 +508,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
             for (int k = 0; k < 2; k++) {
                 const int i = own_cell(k);
                 const int64_t j = (int64_t) unit * cells + i;
-                if (i < cells && j < q.len) past[k] = W.decay * W.old[s * W.ld_old + j];
+                if (i < cells && j < q.len) past[k] = W.old[s * W.ld_old + j];
             }
         const int t_lo = row0 / A.group, t_hi = rows > 0 ? (row0 + rows - 1) / A.group : t_lo;      // this CTA's queries
         float sum[4][2];
@@ -497,6 +525,53 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                 const uint8_t * chunk = S.ring[warp][st], * scales = chunk + kv4_rows_bytes(D);
                 const int p_lo = q.p0 + t_lo, p_hi = q.p0 + t_hi;
                 const bool whole = base + KV4_CELLS - 1 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + KV4_CELLS - 1 < A.first);
+                if constexpr (RAW) {
+#pragma unroll 1
+                    for (int j = 0; j < rows; j += 8) {
+                        const int i = hk * rows + j;
+                        const float2 r0 = factors[i + 2 * c], r1 = factors[i + 2 * c + 1];
+                        uint4 qf[NB];
+                        float from[NB][2];
+#pragma unroll
+                        for (int b = 0; b < NB; b++) {
+                            qf[b] = *reinterpret_cast<const uint4 *>(queries + (size_t) (i + g) * STRIDE + 64 * b + 16 * c);
+                            from[b][0] = starts[(i + 2 * c) * NB + b];
+                            from[b][1] = starts[(i + 2 * c + 1) * NB + b];
+                        }
+                        const bool ra = j + 2 * c < rows, rb = j + 2 * c + 1 < rows;
+                        const int pa = whole || !ra ? INT_MIN : pos[j + 2 * c], pb = whole || !rb ? INT_MIN : pos[j + 2 * c + 1];
+#pragma unroll
+                        for (int m = 0; m < 4; m++) {       // 16 cells at a time
+                            uint32_t w[2][NB];
+                            float sc[2][NB], e[4];
+#pragma unroll
+                            for (int h = 0; h < 2; h++) key_words<D>(chunk + (16 * m + 8 * h + g) * (D / 2) + 4 * NB * c, scales + kv4_scale(D, (16 * m + 8 * h + g) & ~1, 0), g & 1, w[h], sc[h]);
+#pragma unroll
+                            for (int b = 0; b < NB; b++) {
+                                const uint32_t x = w[0][b], y = w[1][b], x8 = x >> 8, y8 = y >> 8;
+                                const uint32_t a0[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u}, a1[4] = {x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u};
+                                float acc[4] = {from[b][0], from[b][1], from[b][0], from[b][1]};
+                                mma16816(acc, a0, qf[b].x, qf[b].y);
+                                mma16816(acc, a1, qf[b].z, qf[b].w);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) e[k] = b == 0 ? acc[k] * sc[k >> 1][b] : fmaf(acc[k], sc[k >> 1][b], e[k]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const float x = ex2(fmaf(e[k], k & 1 ? r1.x : r0.x, k & 1 ? -r1.y : -r0.y));
+                                e[k] = (k & 1 ? rb : ra) ? x : 0.f;
+                            }
+                            if (!whole)
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const int cell = base + 16 * m + 8 * (k >> 1) + g, p = k & 1 ? pb : pa;
+                                    if (!(cell <= p && (A.window <= 0 || p - cell < A.window || cell < A.first))) e[k] = 0.f;
+                                }
+                            sum[m][0] += e[0] + e[1];
+                            sum[m][1] += e[2] + e[3];
+                        }
+                    }
+                } else
 #pragma unroll 1
                 for (int m2 = 0; m2 < 2; m2++) {            // 32 cells at a time
                     uint32_t kf[2][NB][2][4];
@@ -580,7 +655,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         __syncthreads();                                    // (of the unit behind the next one's, nobody reads these any more)
         auto store = [&](int k, float x) {
             const int64_t j = (int64_t) unit * cells + own_cell(k);
-            if (j < q.len) W.sums[s * W.ld_sums + j] = x + past[k];
+            if (j < q.len) W.sums[s * W.ld_sums + j] = fmaf(W.decay, past[k], x);
         };
         for (int k = 0, i = tid; i < cells; k++, i += KF_THREADS) {
             const int page = i / KV4_CELLS, w0 = P > 1 ? page * turns : 0, w1 = P > 1 ? w0 + turns : min(KF_WARPS, turns);
@@ -607,11 +682,11 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
     if (MANY) cluster_sync();                               // nobody reads a CTA's sums that has ended
 }
 
-template <typename T, int D, bool MANY>
+template <typename T, int D, int HOW>
 int weigh_few_launch(const Kv4Weigh & w, const KfSplit & x, size_t rows_bytes, cudaStream_t st) {
     const size_t smem = sizeof(KfSmem<D>) + 128 + rows_bytes;
     static FuncAttrCache cache;
-    const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D, MANY>, 232448, true);
+    const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D, HOW>, 232448, true);
     if (e != cudaSuccess) return (int) e;
     const int ctas = x.heads * x.rows;
     cudaLaunchConfig_t cfg{};
@@ -623,8 +698,8 @@ int weigh_few_launch(const Kv4Weigh & w, const KfSplit & x, size_t rows_bytes, c
     attr[1].val.clusterDim.x = (unsigned) ctas;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = MANY ? 2 : 1;
-    return (int) cudaLaunchKernelEx(&cfg, k_kv4_weigh_few<T, D, MANY>, w, x);
+    cfg.numAttrs = HOW == KF_MANY ? 2 : 1;
+    return (int) cudaLaunchKernelEx(&cfg, k_kv4_weigh_few<T, D, HOW>, w, x);
 }
 
 template <typename T, int D>
@@ -647,7 +722,12 @@ int weigh_launch(const Kv4Weigh & w, cudaStream_t st) {
     if (few <= room) {
         // many rows of a head are cut into turns of 64 and more, so that units are smaller
         while (x.n_head * x.turns * 2 <= KF_WARPS && x.most_rows >= 128 * x.turns) x.turns *= 2;
-        return x.heads * x.rows * x.turns > 1 ? weigh_few_launch<T, D, true>(w, x, few, st) : weigh_few_launch<T, D, false>(w, x, few, st);
+        if (x.heads * x.rows * x.turns > 1) return weigh_few_launch<T, D, KF_MANY>(w, x, few, st);
+        if constexpr (!std::is_same<T, float>::value) {
+            const size_t raw = few + (size_t) (hks * rows + 8) * (D / 32) * sizeof(float);
+            if (rows <= KF_RAW_ROWS && raw <= room) return weigh_few_launch<T, D, KF_RAW>(w, x, raw, st);
+        }
+        return weigh_few_launch<T, D, KF_PLAIN>(w, x, few, st);
     }
     constexpr size_t smem = sizeof(KwSmem<D, std::is_same<T, float>::value>);
     static FuncAttrCache cache;
