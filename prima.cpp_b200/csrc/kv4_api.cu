@@ -157,7 +157,8 @@ size_t pb200_kv4_attn_shared_workspace_bytes(int n_head, int n_head_kv, int head
 int pb200_kv4_attn_shared(const pb200_kv4_cache * c, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
                           const int32_t * kv_len, const int32_t * table, int64_t table_ld, int n_group, const int32_t * group_start, const int32_t * prefix_len, const int32_t * prefix_table,
                           int64_t prefix_ld, int64_t n_tokens, int max_q, float scale, float * lse, int64_t ld_lse, void * ws, size_t ws_bytes, void * stream) {
-    if (n_group < 0 || n_group > 1 << 24 || (n_group > 0 && (!group_start || !prefix_len || !prefix_table || prefix_ld <= 0))) return PB200_EINVAL;
+    if (n_group < 0 || (n_group > 0 && (!group_start || !prefix_len || !prefix_table || prefix_ld <= 0))) return PB200_EINVAL;
+    if (n_group > 1 << 24) return PB200_ENOTSUP;      // (a group's number and a cell of a page in 31 bits)
     const Kv4Groups g{n_group, group_start, prefix_len, prefix_table, prefix_ld};
     return attend(c, layer, type, q, ldq, out, ldo, n_head, n_seq, q_start, kv_len, table, table_ld, n_tokens, max_q, scale, 0, 0, lse, ld_lse, n_group > 0 ? &g : nullptr, ws, ws_bytes, stream);
 }

@@ -28,14 +28,16 @@ def attend(q, pages, table, q_start, kv_len, n_head_kv, dim, scale, window=0, fi
     group = q.shape[1] // n_head_kv
     out, bound = np.full(q.shape, np.nan), np.zeros(q.shape)
     lse, lse_bound = (np.full(q.shape[:2], x) for x in (np.nan, 0.0))
-    sums, sums_bound = [], []
+    sums, sums_bound, fronts = [], [], {}
     for s in range(len(kv_len)):
         n, length = q_start[s + 1] - q_start[s], max(int(kv_len[s]), 0)
         k, v, here = read(pages, table[s], length, dim)
         at = np.arange(k.shape[1])
         if group_start is not None and group_start[0] <= s < group_start[-1]:
             g = int(np.searchsorted(group_start, s, side="right")) - 1
-            pk, pv, ph = read(pages, prefix_table[g], prefix_len[g], dim)
+            if g not in fronts:
+                fronts[g] = read(pages, prefix_table[g], prefix_len[g], dim)
+            pk, pv, ph = fronts[g]
             k, v, here, at = np.concatenate((pk, k), 1), np.concatenate((pv, v), 1), np.concatenate((ph, here)), np.concatenate((np.full(pk.shape[1], -2 ** 40), at))
         worth, worth_bound = np.zeros(length), np.zeros(length)
         for i in range(n):

@@ -152,6 +152,75 @@ def test_attention_behind_prefixes(pkg, lib, cuda, type_, dim, case):
     b.check()
 
 
+# prefixes that are much work for sequences of few rows, which then are read once for all of a group's: one group, several (one of them without cells, one without sequences), more than eight, tiles of rows
+# that are full, one more, and nearly empty; cells of a prefix cut into pieces or not
+APART_CASES = [
+    ([64], [4000], [1] * 64, [1 + 3 * i for i in range(64)], 8, 8), ([32, 0, 33, 3], [3000, 500, 2049, 0], [1] * 68, [i % 70 for i in range(68)], 16, 8), ([9] * 12, [1024 + i for i in range(12)], [1] * 108, [5] * 108, 16, 8),
+    ([65], [3500], [2] * 65, [2 + i for i in range(65)], 8, 4), ([130], [640], [3, 1] * 65, [3 + i % 9 for i in range(130)], 32, 8), ([14], [20000], [4] * 14, [40] * 14, 4, 4), ([520], [500], [1] * 520, [1 + i % 5 for i in range(520)], 4, 4),
+]
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("case", APART_CASES, ids=lambda c: f"g{'_'.join(map(str, c[0][:6]))}_p{max(c[1])}_q{sum(c[2])}_kv{max(c[3])}_h{c[4]}over{c[5]}")
+def test_prefixes_by_themselves(pkg, lib, cuda, type_, dim, case):
+    groups, prefix, q, kv, heads, kv_heads = case
+    b = Batch(pkg, lib, 60, type_, heads, kv_heads, dim, q, kv, groups, prefix)
+    before = lib.c.pb200_kernel_launches()
+    b.attend()
+    assert lib.c.pb200_kernel_launches() - before >= 2, "the prefix has no kernel of its own"
+    b.check()
+    first = b.out.clone()
+    b.out.fill_(7.0)
+    assert torch.equal(b.attend(), first)
+
+
+def test_prefixes_by_themselves_with_strides_and_rows_of_nobody(pkg, lib, cuda):
+    """Sequences in front of the groups and behind them, rows around them, queries beyond the first three of a sequence, longer rows than there have to be, a layer, no logarithms."""
+    n = 70
+    b = Batch(pkg, lib, 61, "bf16", 16, 8, 128, [1, 2] + [1 + i % 5 for i in range(n)] + [3], [70, 3] + [5 + i for i in range(n)] + [200], [30, 40], [2000, 1777], group_at=2, layers=2, layer=1, pad=4, front=3, behind=2)
+    b.attend(max_q=3)
+    b.check(most=3)
+    b.out.fill_(7.0)
+    b.lse.fill_(7.0)
+    b.attend(max_q=3, lse=False)
+    b.check(most=3, lse=False)
+
+
+def test_prefixes_by_themselves_keep_what_is_no_number_in_its_rows(pkg, lib, cuda):
+    b = Batch(pkg, lib, 62, "f32", 8, 8, 128, [1] * 64, [40] * 64, [64], [3000])
+    want = b.attend().clone()
+    b.q[3, 5], b.q[50, 200] = float("nan"), float("inf")
+    b.attend()
+    torch.cuda.synchronize()
+    other = [i for i in range(64) if i not in (3, 50)]
+    assert torch.equal(b.out[other], want[other]) and torch.isnan(b.out[3, :128]).all() and torch.equal(b.out[3, 128:], want[3, 128:])
+
+
+def test_graph_follows_prefixes_from_one_way_to_the_other(pkg, lib, cuda):
+    """One graph: prefixes long enough to be by themselves, then not, then again; workspaces of other calls' sizes and other head sizes between them."""
+    b = Batch(pkg, lib, 63, "f16", 16, 8, 128, [1] * 64, [50 + i for i in range(64)], [24, 40], [3000, 2500])
+    small = Batch(pkg, lib, 64, "f32", 8, 8, 64, [1] * 64, [30] * 64, [64], [2000])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            b.attend()
+        for prefix, groups in (([3000, 2500], [24, 40]), ([64, 70], [24, 40]), ([0, 2500], [1, 63]), ([2999, 0], [64, 0])):
+            b.prefix_np[:], b.group_np[:] = prefix, np.concatenate(([0], np.cumsum(groups)))
+            for t, x in ((b.prefix, b.prefix_np), (b.group, b.group_np)):
+                t.copy_(torch.from_numpy(x))
+            b.out.fill_(7.0)
+            b.lse.fill_(7.0)
+            graph.replay()
+            b.check()
+            small.out.fill_(7.0)
+            small.lse.fill_(7.0)
+            small.attend(ws=b.ws)
+            small.check()
+
+
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 def test_sequences_outside_of_groups_strides_and_layers(pkg, lib, cuda, type_):
     """Two sequences in front of the groups and one behind; rows that are nobody's around them; rows longer than they have to be; the second of three layers."""
@@ -278,7 +347,9 @@ def check_weights(b, sums_before, got, decay, old, width=None):
 
 @pytest.mark.parametrize("type_", TYPES)
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("case", LSE_CASES + [([1] * 70, [3 * i for i in range(70)], 4, 1, 0, 0), ([1] * 600, [1 + i % 5 for i in range(600)], 2, 1, 0, 0), ([300], [300], 6, 2, 1, 0), ([9] * 3, [900, 256, 257], 12, 3, 0, 0)],
+@pytest.mark.parametrize("case", LSE_CASES + [([1] * 70, [3 * i for i in range(70)], 4, 1, 0, 0), ([1] * 600, [1 + i % 5 for i in range(600)], 2, 1, 0, 0), ([300], [300], 6, 2, 1, 0), ([9] * 3, [900, 256, 257], 12, 3, 0, 0),
+                                              # more rows than a cluster holds; more kv heads than warps; a kv head whose rows are cut between CTAs; three kv heads
+                                              ([600, 20], [900, 300], 16, 2, 0, 0), ([2, 1], [300, 77], 40, 20, 0, 0), ([90], [400], 16, 1, 0, 0), ([130, 7], [500, 90], 12, 3, 70, 5)],
                          ids=lambda c: f"q{sum(c[0])}of{len(c[0])}_kv{max(c[1])}_h{c[2]}over{c[3]}_w{c[4]}_{c[5]}")
 def test_weights(pkg, lib, cuda, type_, dim, case):
     q, kv, heads, kv_heads, window, first = case
@@ -490,7 +561,14 @@ def test_verification_of_many_sequences(lib, cuda):
     verify(lib, "f32", target, draft, drafts, tokens, None, u, v)
 
 
-def test_a_vocabulary_that_shared_memory_does_not_hold(lib, cuda):
+def test_verification_of_more_sequences_than_fill_the_gpu(lib, cuda):
+    rng = np.random.default_rng(49)
+    drafts = [int(x) for x in rng.integers(0, 3, 60)]
+    target, draft, tokens, u, v = drafted(rng, "bf16", 20001, drafts)
+    verify(lib, "bf16", target, draft, drafts, tokens, None, u, v)
+
+
+def test_a_large_vocabulary(lib, cuda):
     rng = np.random.default_rng(42)
     for with_draft in (True, False):
         target, draft, tokens, u, v = drafted(rng, "f16", 600001, [2, 1], apart=3.0)
