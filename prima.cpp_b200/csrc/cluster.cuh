@@ -1,5 +1,7 @@
 // prima.cpp_b200/csrc/cluster.cuh — a cluster's CTAs: their places, their barrier, reads of each other's shared memory.
 #pragma once
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace pb {
@@ -45,9 +47,12 @@ __device__ __forceinline__ uint2 remote(const uint2 * at, uint32_t cta) {
     return v;
 }
 
+// clusters of 1, 2, 4 or 8 CTAs that run at the same time where a CTA takes an SM: a cluster stays within a group of SMs.  What cudaOccupancyMaxActiveClusters says on a B200 with 148 SMs, 8 from
+// below; persistent kernels launch no more, since the rest of a grid would start where these have ended
+inline int clusters_at_once(int ctas, int sms) { return std::max(1, (ctas >= 8 ? 15 : ctas >= 4 ? 33 : ctas >= 2 ? 74 : 148) * sms / 148); }
 // kernel of n clusters of so many CTAs; dependent: it may start while the kernel in front of it ends, and waits for that itself
-template <typename K, typename A>
-cudaError_t launch_clusters(K * kernel, int64_t n, int ctas, int threads, size_t smem, bool dependent, cudaStream_t st, const A & args) {
+template <typename K, typename... A>
+cudaError_t launch_clusters(K * kernel, int64_t n, int ctas, int threads, size_t smem, bool dependent, cudaStream_t st, const A &... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned) (n * ctas)); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -58,7 +63,7 @@ cudaError_t launch_clusters(K * kernel, int64_t n, int ctas, int threads, size_t
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace pb
