@@ -4,8 +4,9 @@
 // has to be looked at as a whole: a cell's sum is that of its own column.  Scores are m16n8k16 products, cells x rows: a thread holds two rows' scores of a cell next to each other, and adds
 // them up without asking others.  Keys are f16 numbers exactly and go to registers once for all rows; a query row is f16 times a power of two (F32: two of them, 22 bits, low parts first).
 //
-// Work.  An item is 256 cells of a sequence, 32 to each of a CTA's warps.  A cluster has an item; its CTAs share the kv heads, and the rows in blocks of 64; their sums meet in shared memory, in
-// the CTAs' order (equal calls give equal bits).
+// Work.  Two kernels.  Few rows (tokens that decode): keys stream through shared memory, rows stay there.  Many rows: an item is 256, 128 or 64 cells of a sequence, 32 to each of a CTA's warps (128 and
+// 64: two or four warps have the same cells, and each a part of the rows).  A cluster has an item; its CTAs share the kv heads, and the rows in blocks of 64; their sums meet in shared memory, in the
+// CTAs' order (equal calls give equal bits).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp(), g = lane >> 2, c = lane & 3, hks = A.cache.n_head_kv;
     const int ctas = (int) cluster_size(), rank = (int) cluster_rank();
 
+    pdl_wait();                                             // what attention, or whatever stands in front, has written
     auto length = [&](int s) { return s < A.n_seq ? (int) max((int64_t) 0, min((int64_t) A.kv_len[s], W.ld_sums)) : 0; };
     // items of 256 sequences at a time: where each one's end; the items in front of them
     int at = -1, before = 0, all = 0;
@@ -302,15 +304,13 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
 }
 
 // ---- few rows ----
-// Pages stream through shared memory, by bulk copies: a warp has the keys of a page and a kv head at a time, the next ones on their way, and all of the head's rows or a part of them.  A unit is as
-// many pages of a sequence as give each warp such a turn; a CTA has a contiguous share of all units.  The queries lie in shared memory while it is at their sequence: where those of all heads do not fit, a cluster has the share, and each
-// CTA of it some of the heads, and some of the rows.
+// Pages stream through shared memory, by bulk copies: a warp has the keys of a page and a kv head at a time, the next ones on their way, and all of the head's rows.  A unit is as many pages of a
+// sequence as give each warp such a turn; a CTA has a contiguous share of all units.  The queries of all heads lie in shared memory while it is at their sequence.
 constexpr int KF_WARPS = 16, KF_THREADS = 32 * KF_WARPS;
 __host__ __device__ constexpr int kf_bytes(int D) { return kv4_rows_bytes(D) + kv4_scales_bytes(D); }     // of a page's keys
-constexpr int KF_STAGES = 2, KF_RAW_ROWS = 16;
+constexpr int KF_STAGES = 2, KF_ROWS = 16;
 
-// heads and rows of a cluster's CTAs: so many parts of either (heads: evenly), a part's heads and rows at most; into how many turns a warp's rows are cut
-struct KfSplit { int heads, rows, n_head, most_rows, turns; int * abort_flag; };
+struct KfSplit { int most_rows; int * abort_flag; };      // rows of a kv head at most
 // a sequence: its queries, positions, cells and units
 struct KfSeq {
     int64_t q0;
@@ -319,37 +319,35 @@ struct KfSeq {
 template <int D> struct __align__(128) KfSmem {
     __align__(128) uint8_t ring[KF_WARPS][KF_STAGES][kf_bytes(D)];
     uint64_t full[KF_WARPS][KF_STAGES];
-    float part[2][KF_WARPS][KV4_CELLS], sums[2][KF_WARPS * KV4_CELLS];       // of the warps; of the CTA, for the cluster's others
+    float part[2][KF_WARPS][KV4_CELLS];        // of the warps
     int scan[KF_WARPS], begin_s, begin_unit, abort;
     KfSeq begin;
 };
-// behind it: of all rows (kv head by kv head) and eight more the numbers (F32: high, then low parts), what makes their weights, the positions of a kv head's
-template <typename T, int D> __host__ __device__ constexpr size_t kf_row_bytes() { return (std::is_same<T, float>::value ? 2 : 1) * (2 * D + 64) + sizeof(float2); }
+// behind it: of all rows (kv head by kv head) and eight more the numbers (F32: high, then low parts), what makes their weights, RAW: where their sums start; the positions of a kv head's
+template <typename T, int D> __host__ __device__ constexpr size_t kf_row_bytes() {
+    return (std::is_same<T, float>::value ? 2 * (2 * D + 64) : 2 * D + 64 + D / 32 * sizeof(float)) + sizeof(float2);
+}
 
-// How: MANY: a cluster has a share, or rows are cut into turns.  RAW: 16 bits, up to two tiles of rows to a kv head: the numbers' 4 bits go into the products as they are, as the f16 n * 2^-24 (n * 2^-20
-// a nibble further up, which meets a 16th of the query), and scales onto the sums of blocks, which start from -8 times the query's; making them f16 keys takes twice as many instructions (32
-// sequences of up to 8192 cells 38 us where this takes 33)
-enum { KF_PLAIN = 0, KF_RAW = 1, KF_MANY = 2 };
-template <typename T, int D, int HOW>
+// RAW: 16 bits: the numbers' 4 bits go into the products as they are, as the f16 n * 2^-24 (n * 2^-20 a nibble further up, which meets a 16th of the query), and scales onto the sums of blocks, which
+// start from -8 times the query's; making them f16 keys takes twice as many instructions (32 sequences of up to 8192 cells 38 us where this takes 33).  F32 has
+// twice the products as it is, and keeps the f16 keys
+template <typename T, int D>
 __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_constant__ Kv4Weigh W, const __grid_constant__ KfSplit X) {
     constexpr bool F32 = std::is_same<T, float>::value;
-    constexpr bool MANY = HOW == KF_MANY, RAW = HOW == KF_RAW;
+    constexpr bool RAW = !F32;
     constexpr int NB = D / 32, LO = F32 ? 2 : 1, STAGES = KF_STAGES, STRIDE = 2 * D + 64;
     extern __shared__ uint8_t smem_raw[];
     KfSmem<D> & S = *reinterpret_cast<KfSmem<D> *>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
     const Kv4Attn & A = W.attn;
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp(), g = lane >> 2, c = lane & 3;
     uint8_t * const queries = reinterpret_cast<uint8_t *>(&S + 1);
-    // kv heads of this CTA, its part of their rows, turns over a page
-    const int ctas = MANY ? X.heads * X.rows : 1, rank = MANY ? (int) cluster_rank() : 0, head0 = MANY ? rank % X.heads * X.n_head : 0, part = MANY ? rank / X.heads : 0, hks = X.n_head;
-    const int row_parts = MANY ? X.rows : 1, cuts = MANY ? X.turns : 1, turns = hks * cuts;
-    const int room = hks * X.most_rows + 8;                 // rows
+    const int hks = A.cache.n_head_kv, room = hks * X.most_rows + 8;                // rows
     float2 * const factors = reinterpret_cast<float2 *>(queries + (size_t) room * STRIDE * LO);
     float * const starts = reinterpret_cast<float *>(factors + room);        // RAW: of each row and block
     int * const pos = reinterpret_cast<int *>(starts + (RAW ? room * NB : 0));
     volatile int * cta_abort = &S.abort;
-    // pages of a unit; this warp's page of them and its first turn (`turns` and more: none)
-    const int P = max(1, KF_WARPS / turns), my_page = P > 1 ? warp / turns : 0, my_turn = P > 1 ? (my_page < P ? warp % turns : turns) : warp;
+    // pages of a unit; this warp's page of them and its first head (`hks` and more: none)
+    const int P = max(1, KF_WARPS / hks), my_page = P > 1 ? warp / hks : 0, my_head = P > 1 ? (my_page < P ? warp % hks : hks) : warp;
 
     auto seq = [&](int s) {
         KfSeq q{};
@@ -396,8 +394,8 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         if (w < warp) ends += S.scan[w];
         total += S.scan[w];
     }
-    const int shares = (int) gridDim.x / ctas, share = (int) blockIdx.x / ctas, u0 = (int) (total * share / shares), u1 = (int) (total * (share + 1) / shares);
-    if (u0 == u1) return;                                   // (all CTAs of a cluster)
+    const int u0 = (int) (total * blockIdx.x / gridDim.x), u1 = (int) (total * (blockIdx.x + 1) / gridDim.x);
+    if (u0 == u1) return;
     auto begins = [&](int s, const KfSeq & q, int before) {
         if (u0 >= before && u0 < before + q.units) { S.begin_s = s; S.begin_unit = u0 - before; S.begin = q; }
     };
@@ -415,10 +413,10 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         }
     __syncthreads();
 
-    // ---- this warp's keys on their way: by units and, where there are more turns than warps, turns ----
+    // ---- this warp's keys on their way: by units and, where there are more heads than warps, heads ----
     uint64_t policy;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    int f_s = S.begin_s, f_unit = S.begin_unit, f_u = u0, f_turn = my_turn, f_n = 0;
+    int f_s = S.begin_s, f_unit = S.begin_unit, f_u = u0, f_head = my_head, f_n = 0;
     KfSeq f_q = S.begin;
     int ids = -1, ids0 = 0, ids1 = 0;                       // pages of the units ids0 .. ids1 - 1 of the sequence, one to a lane
     uint32_t none = 0;                                      // stages whose page nobody sees, or that is none
@@ -426,7 +424,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         return q.n_q > 0 && base <= q.p0 + q.n_q - 1 && (A.window <= 0 || q.p0 - (base + KV4_CELLS - 1) < A.window || base < A.first);
     };
     auto fetch = [&] {
-        if (f_u >= u1 || f_turn >= turns) return;
+        if (f_u >= u1 || f_head >= hks) return;
         while (f_unit >= f_q.units) {
             f_q = seq(++f_s);
             f_unit = 0;
@@ -444,7 +442,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         none = id >= 0 ? none & ~(1u << st) : none | 1u << st;
         if (elect_one()) {
             if (id >= 0) {
-                const uint8_t * chunk = kv4_chunk<D>(A.cache, id, head0 + (MANY ? f_turn / cuts : f_turn));
+                const uint8_t * chunk = kv4_chunk<D>(A.cache, id, f_head);
                 mbar_arrive_expect_tx(&S.full[warp][st], kf_bytes(D));
                 bulk_g2s(S.ring[warp][st], chunk, kv4_rows_bytes(D), &S.full[warp][st], policy);
                 bulk_g2s(S.ring[warp][st] + kv4_rows_bytes(D), chunk + 2 * kv4_rows_bytes(D), kv4_scales_bytes(D), &S.full[warp][st], policy);
@@ -452,17 +450,15 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         }
         __syncwarp();
         f_n++;
-        f_turn += KF_WARPS;
-        if (P > 1 || f_turn >= turns) {
-            f_turn = my_turn;
+        f_head += KF_WARPS;
+        if (P > 1 || f_head >= hks) {
+            f_head = my_head;
             f_unit++;
             f_u++;
         }
     };
     int s = S.begin_s, unit = S.begin_unit, n = 0;
     bool fresh = true;
-    // the k-th cell of a unit that this thread stores (a cluster's CTAs have them in turns), at most two; beyond the unit's: none
-    auto own_cell = [&](int k) { return (k * KF_THREADS + tid) * ctas + rank; };
     KfSeq q = S.begin;
     for (int u = u0; u < u1; u++, unit++) {
         while (unit >= q.units) {
@@ -470,44 +466,37 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
             unit = 0;
             fresh = true;
         }
-        const int all_rows = q.n_q * A.group, row0 = MANY ? (int) ((int64_t) all_rows * part / row_parts) : 0, rows = MANY ? (int) ((int64_t) all_rows * (part + 1) / row_parts) - row0 : all_rows;
-        if (fresh) {   // ---- the sequence's queries: four threads to a row, with MANY two rows of theirs at once ----  (everybody is through with the last one's: behind the barrier of its last unit)
+        const int rows = q.n_q * A.group;
+        if (fresh) {   // ---- the sequence's queries: four threads to a row ----  (everybody is through with the last one's: behind the barrier of its last unit)
             fresh = false;
-            constexpr int EACH = D / 4, ONCE = MANY ? 2 : 1, ROWS = KF_THREADS / 4;
-            for (int i0 = 0; i0 < hks * rows; i0 += ONCE * ROWS) {
-                float x[ONCE][EACH], lse[ONCE];
+            constexpr int EACH = D / 4, ROWS = KF_THREADS / 4;
+            for (int i0 = 0; i0 < hks * rows; i0 += ROWS) {
+                const int i = i0 + (tid >> 2), quarter = tid & 3, hk = i / rows, r = i - hk * rows, t = r / A.group, head = hk * A.group + r - t * A.group;
+                const bool have = i < hks * rows;
+                const T * src = (const T *) A.q + (q.q0 + t) * A.ldq + (int64_t) head * D + quarter * EACH;
+                float x[EACH];
 #pragma unroll
-                for (int o = 0; o < ONCE; o++) {
-                    const int i = i0 + o * ROWS + (tid >> 2), hk = i / max(rows, 1), r = row0 + i - hk * rows, t = r / A.group, head = (head0 + hk) * A.group + r - t * A.group;
-                    const bool have = i < hks * rows;
-                    const T * src = (const T *) A.q + (q.q0 + t) * A.ldq + (int64_t) head * D + (tid & 3) * EACH;
-#pragma unroll
-                    for (int k = 0; k < EACH; k += 4) {
-                        const float4 v = have ? load4(src + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[o][k] = v.x; x[o][k + 1] = v.y; x[o][k + 2] = v.z; x[o][k + 3] = v.w;
-                    }
-                    lse[o] = have ? W.lse[(q.q0 + t) * W.ld_lse + head] : -INFINITY;
+                for (int k = 0; k < EACH; k += 4) {
+                    const float4 v = have ? load4(src + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
                 }
+                const float lse = have ? W.lse[(q.q0 + t) * W.ld_lse + head] : -INFINITY;
                 if (f_n == 0)                               // the first keys, behind the first queries
                     for (int k = 0; k < STAGES; k++) fetch();
+                const float up = row_power<EACH>(x, 0.f) * (A.scale < 0.f ? -1.f : 1.f);
+                float block = 0.f;                          // sum of the block's numbers
+                if (RAW) {
 #pragma unroll
-                for (int o = 0; o < ONCE; o++) {
-                    const int i = i0 + o * ROWS + (tid >> 2), quarter = tid & 3;
-                    const float up = row_power<EACH>(x[o], 0.f) * (A.scale < 0.f ? -1.f : 1.f);
-                    float block = 0.f;                      // sum of the block's numbers
-                    if (RAW) {
-#pragma unroll
-                        for (int k = 0; k < EACH; k++) block += x[o][k];
-                        if (EACH == 16) block += __shfl_xor_sync(0xffffffffu, block, 1);
-                    }
-                    if (i >= hks * rows) continue;
-                    row_store<T, EACH, RAW>(x[o], up, queries + (size_t) i * STRIDE + 2 * quarter * EACH, queries + (size_t) (room + i) * STRIDE + 2 * quarter * EACH);
-                    if (RAW && (EACH == 32 || quarter % 2 == 0)) starts[i * NB + quarter * EACH / 32] = block * (up * (-8.f / 16777216.f));
-                    if (quarter == 0) {
-                        factors[i] = row_factors(A.scale, up, lse[o]);
-                        if (RAW) factors[i].x *= 16777216.f;
-                        if (i < rows) pos[i] = max(q.p0 + (row0 + i) / A.group, -1);
-                    }
+                    for (int k = 0; k < EACH; k++) block += x[k];
+                    if (EACH == 16) block += __shfl_xor_sync(0xffffffffu, block, 1);
+                }
+                if (!have) continue;
+                row_store<T, EACH, RAW>(x, up, queries + (size_t) i * STRIDE + 2 * quarter * EACH, queries + (size_t) (room + i) * STRIDE + 2 * quarter * EACH);
+                if (RAW && (EACH == 32 || quarter % 2 == 0)) starts[i * NB + quarter * EACH / 32] = block * (up * (-8.f / 16777216.f));
+                if (quarter == 0) {
+                    factors[i] = row_factors(A.scale, up, lse);
+                    if (RAW) factors[i].x *= 16777216.f;
+                    if (i < rows) pos[i] = max(q.p0 + t, -1);
                 }
             }
             if (f_n == 0)
@@ -520,24 +509,21 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         if (W.old)
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const int i = own_cell(k);
+                const int i = k * KF_THREADS + tid;
                 const int64_t j = (int64_t) unit * cells + i;
                 if (i < cells && j < q.len) past[k] = W.old[s * W.ld_old + j];
             }
-        const int t_lo = row0 / A.group, t_hi = rows > 0 ? (row0 + rows - 1) / A.group : t_lo;      // this CTA's queries
         float sum[4][2];
 #pragma unroll
         for (int m = 0; m < 4; m++) sum[m][0] = sum[m][1] = 0.f;
         const int base = (unit * P + my_page) * KV4_CELLS;
-        for (int turn = my_turn; turn < turns; turn += P > 1 ? turns : KF_WARPS, n++) {
-            // rows j0 .. j1 - 1 of kv head hk
-            const int hk = MANY ? turn / cuts : turn, cut = MANY ? turn - hk * cuts : 0, j0 = MANY ? (rows + 7) / 8 * cut / cuts * 8 : 0, j1 = !MANY || cut == cuts - 1 ? rows : (rows + 7) / 8 * (cut + 1) / cuts * 8;
+        for (int hk = my_head; hk < hks; hk += P > 1 ? hks : KF_WARPS, n++) {
             const int st = n % STAGES;
             const bool have = !(none >> st & 1);
             mbar_wait(&S.full[warp][st], (uint32_t) (n / STAGES) & 1, cta_abort, X.abort_flag);
             if (have) {
                 const uint8_t * chunk = S.ring[warp][st], * scales = chunk + kv4_rows_bytes(D);
-                const int p_lo = q.p0 + t_lo, p_hi = q.p0 + t_hi;
+                const int p_lo = q.p0, p_hi = q.p0 + q.n_q - 1;
                 const bool whole = base + KV4_CELLS - 1 <= p_lo && (A.window <= 0 || p_hi - base < A.window || base + KV4_CELLS - 1 < A.first);
                 if constexpr (RAW) {
 #pragma unroll 1
@@ -604,15 +590,15 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                         for (int m = 0; m < 2; m++)
 #pragma unroll
                             for (int k = 0; k < 4; k++) e[m][k] = ex2(fmaf(e[m][k], k & 1 ? r1.x : r0.x, k & 1 ? -r1.y : -r0.y));
-                        if (j + 8 > j1) {                   // rows of nobody's
-                            const bool ra = j + 2 * c < j1, rb = j + 2 * c + 1 < j1;
+                        if (j + 8 > rows) {                   // rows of nobody's
+                            const bool ra = j + 2 * c < rows, rb = j + 2 * c + 1 < rows;
 #pragma unroll
                             for (int m = 0; m < 2; m++)
 #pragma unroll
                                 for (int k = 0; k < 4; k++) e[m][k] = (k & 1 ? rb : ra) ? e[m][k] : 0.f;
                         }
                         if (!whole) {
-                            const int pa = j + 2 * c < j1 ? pos[j + 2 * c] : -1, pb = j + 2 * c + 1 < j1 ? pos[j + 2 * c + 1] : -1;
+                            const int pa = j + 2 * c < rows ? pos[j + 2 * c] : -1, pb = j + 2 * c + 1 < rows ? pos[j + 2 * c + 1] : -1;
 #pragma unroll
                             for (int m = 0; m < 2; m++)
 #pragma unroll
@@ -628,16 +614,16 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                         }
                     };
                     const uint8_t * const q_at = queries + (size_t) (hk * rows + g) * STRIDE + 16 * c;
-                    int j = j0;
+                    int j = 0;
 #pragma unroll 1
-                    for (; j + 8 < j1; j += 16) {           // two tiles of rows at once: one's products beside the other's weights
+                    for (; j + 8 < rows; j += 16) {           // two tiles of rows at once: one's products beside the other's weights
                         float e0[2][4], e1[2][4];
                         scores<LO, NB>(kf, q_at + (size_t) j * STRIDE, (size_t) room * STRIDE, e0);
                         scores<LO, NB>(kf, q_at + (size_t) (j + 8) * STRIDE, (size_t) room * STRIDE, e1);
                         weights(j, e0);
                         weights(j + 8, e1);
                     }
-                    if (j < j1) {
+                    if (j < rows) {
                         float e0[2][4];
                         scores<LO, NB>(kf, q_at + (size_t) j * STRIDE, (size_t) room * STRIDE, e0);
                         weights(j, e0);
@@ -656,7 +642,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
         }
         // ---- the warps' sums: of a page those of its kv heads, in their order ----
         const int flip = u & 1;
-        if (my_turn < turns)
+        if (my_head < hks)
 #pragma unroll
             for (int m = 0; m < 4; m++)
 #pragma unroll
@@ -667,81 +653,33 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                     if (c == 0) S.part[flip][warp][16 * m + 8 * h + g] = x;
                 }
         __syncthreads();                                    // (of the unit behind the next one's, nobody reads these any more)
-        auto store = [&](int k, float x) {
-            const int64_t j = (int64_t) unit * cells + own_cell(k);
-            if (j < q.len) W.sums[s * W.ld_sums + j] = fmaf(W.decay, past[k], x);
-        };
-        for (int k = 0, i = tid; i < cells; k++, i += KF_THREADS) {
-            const int page = i / KV4_CELLS, w0 = P > 1 ? page * turns : 0, w1 = P > 1 ? w0 + turns : min(KF_WARPS, turns);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int i = k * KF_THREADS + tid, page = i / KV4_CELLS, w0 = P > 1 ? page * hks : 0, w1 = P > 1 ? w0 + hks : min(KF_WARPS, hks);
+            const int64_t j = (int64_t) unit * cells + i;
+            if (i >= cells || j >= q.len) continue;
             float x = 0.f;
             for (int w = w0; w < w1; w++) x += S.part[flip][w][i % KV4_CELLS];
-            if (MANY) S.sums[flip][i] = x;
-            else store(k, x);
-        }
-        if (MANY) {   // the cluster's CTAs each add up some of the cells, in the CTAs' order
-            cluster_sync();
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int i = own_cell(k);
-                if (i >= cells) continue;
-                float far[8], x = 0.f;
-#pragma unroll
-                for (int r = 0; r < 8; r++) far[r] = r < ctas ? remote(&S.sums[flip][i], r) : 0.f;
-#pragma unroll
-                for (int r = 0; r < 8; r++) x += far[r];
-                store(k, x);
-            }
+            W.sums[s * W.ld_sums + j] = fmaf(W.decay, past[k], x);
         }
     }
-    if (MANY) cluster_sync();                               // nobody reads a CTA's sums that has ended
-}
-
-template <typename T, int D, int HOW>
-int weigh_few_launch(const Kv4Weigh & w, const KfSplit & x, size_t rows_bytes, cudaStream_t st) {
-    const size_t smem = sizeof(KfSmem<D>) + 128 + rows_bytes;
-    static FuncAttrCache cache;
-    const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D, HOW>, 232448, true);
-    if (e != cudaSuccess) return (int) e;
-    const int ctas = x.heads * x.rows;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(clusters_at_once(ctas, sm_count()) * ctas); cfg.blockDim = dim3(KF_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned) ctas;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = HOW == KF_MANY ? 2 : 1;
-    return (int) cudaLaunchKernelEx(&cfg, k_kv4_weigh_few<T, D, HOW>, w, x);
 }
 
 template <typename T, int D>
 int weigh_launch(const Kv4Weigh & w, cudaStream_t st) {
     const int hks = w.attn.cache.n_head_kv;
     const int64_t rows = std::min<int64_t>(w.attn.max_q, w.attn.n_tokens) * w.attn.group;
-    // as few CTAs to a cluster as hold the rows; heads are split first
-    KfSplit x{1, 1, hks, 0, 1, abort_flag()};
-    constexpr size_t least = sizeof(KfSmem<D>) + 128, room = 232448 - least;      // an SM's shared memory
-    size_t few;
-    for (;;) {
-        x.n_head = hks / x.heads;
-        const int64_t most = (rows + x.rows - 1) / x.rows;
-        few = (size_t) (x.n_head * most + 8) * kf_row_bytes<T, D>() + 4 * (size_t) most;
-        x.most_rows = (int) most;
-        if (few <= room || x.heads * x.rows == 8) break;
-        if (x.n_head % 2 == 0) x.heads *= 2;
-        else x.rows *= 2;
-    }
-    if (few <= room) {
-        // many rows of a head are cut into turns of 64 and more, so that units are smaller
-        while (x.n_head * x.turns * 2 <= KF_WARPS && x.most_rows >= 128 * x.turns) x.turns *= 2;
-        if (x.heads * x.rows * x.turns > 1) return weigh_few_launch<T, D, KF_MANY>(w, x, few, st);
-        if constexpr (!std::is_same<T, float>::value) {
-            const size_t raw = few + (size_t) (hks * rows + 8) * (D / 32) * sizeof(float);
-            if (rows <= KF_RAW_ROWS && raw <= room) return weigh_few_launch<T, D, KF_RAW>(w, x, raw, st);
+    // Few rows: those of all heads lie in an SM's shared memory, beside the keys that stream through it; keys are read once, where the other kernel's CTAs each load and convert 64 rows whatever there are.
+    // bf16, 32 query heads of 8, D = 128, 20 sequences of 100 .. 4000 cells: 4 rows to a kv head 16 us against 27, 16 rows 23 against 28; 32 sequences, 20 rows 33 against 35.  One kv head, 5000 cells: 32
+    // rows 10.9 against 6.9
+    if (rows <= KF_ROWS) {
+        const size_t few = sizeof(KfSmem<D>) + 128 + (size_t) (hks * rows + 8) * kf_row_bytes<T, D>() + 4 * (size_t) rows;
+        if (few <= 232448) {
+            static FuncAttrCache cache;
+            const cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_weigh_few<T, D>, 232448, true);
+            if (e != cudaSuccess) return (int) e;
+            return (int) launch_clusters(k_kv4_weigh_few<T, D>, sm_count(), 1, KF_THREADS, few, true, st, w, KfSplit{(int) rows, abort_flag()});
         }
-        return weigh_few_launch<T, D, KF_PLAIN>(w, x, few, st);
     }
     constexpr size_t smem = sizeof(KwSmem<D, std::is_same<T, float>::value>);
     static FuncAttrCache cache;
@@ -759,7 +697,7 @@ int weigh_launch(const Kv4Weigh & w, cudaStream_t st) {
             const double t = rounds * ((units + n - 1) / n * std::max(1.2 + 2.0 / k, per_sm * (0.8 + 2.0 / k)) + 6);
             if (t < best) { best = t; ctas = n; cuts = k; }
         }
-    return (int) launch_clusters(k_kv4_weigh<T, D>, 2 * clusters_at_once(ctas, sm_count()), ctas, KW_THREADS, smem, false, st, w, KwSplit{KW_CELLS / cuts, cuts});
+    return (int) launch_clusters(k_kv4_weigh<T, D>, 2 * clusters_at_once(ctas, sm_count()), ctas, KW_THREADS, smem, true, st, w, KwSplit{KW_CELLS / cuts, cuts});
 }
 
 }  // namespace
