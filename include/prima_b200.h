@@ -178,7 +178,8 @@ PB200_API int pb200_kv4_attn_lse(const pb200_kv4_cache * cache, int layer, int t
 /* Attention of a batch whose sequences come in groups with a prefix in common, whose pages are read once for the group.  Group g has the sequences group_start[g] .. group_start[g+1]-1 (device
  * [n_group + 1], rising; sequences outside of group_start[0] .. group_start[n_group]-1 have no prefix), whose queries all see the prefix_len[g] cells of row g of prefix_table (as table's,
  * prefix_ld pages a row) in front of their own, which are those of pb200_kv4_attn without a window: kv_len counts them alone, and rotations count from the prefix's start.  A prefix may end
- * inside a page.  lse: as in pb200_kv4_attn_lse, or NULL.  Precision: as in pb200_kv4_attn; a prefix goes to the kernel of few rows where its groups have few rows on the average.
+ * inside a page.  lse: as in pb200_kv4_attn_lse, or NULL.  Precision: as in pb200_kv4_attn, of one sequence with all the cells; a prefix
+ * that is read once for many rows has a prompt's.  A prefix and the cells behind it lie within 2^30, groups within 2^24.
  * ws: pb200_kv4_attn_shared_workspace_bytes, zeroed once, as pb200_kv4_attn's, for which it serves, too. */
 PB200_API size_t pb200_kv4_attn_shared_workspace_bytes(int n_head, int n_head_kv, int head_dim, int64_t n_tokens);
 PB200_API int pb200_kv4_attn_shared(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
@@ -213,8 +214,9 @@ PB200_API int pb200_kv4_compact(const pb200_kv4_cache * cache, int n_seq, const 
  * Draft x with its number u = u_accept[i] is accepted where u q(x) < p(x); n_accepted[s]: how many are, up to the first that is not.  Behind them comes a token drawn by u_draw[s]: with weights
  * w = max(p - q, 0) of the first that is not accepted (p, where these are all 0), with p behind the last: the lowest i with w_0 + .. + w_i > u_draw[s] * (sum of w), in 64 bits.
  * out[s * ld_out + ..]: the accepted tokens and that one (as far as ld_out goes; what lies behind stays as it was).  kv_len_out[s] = kv_len[s] less the drafts that were not accepted (both NULL:
- * not wanted; may be the same): the cells of these are free.  Logits that are no number count as -inf, +inf takes all weight; tokens outside the vocabulary are not accepted; where a row has no
- * weights at all, or inv_temp[s] is below 0 or no number, the token is -1.  Numbers u lie in [0, 1).  ws: pb200_verify_drafts_workspace_bytes, for calls that follow one another. */
+ * not wanted; may be the same): the cells of these are free.  Logits that are no number count as -inf, +inf takes all weight; tokens outside the vocabulary are not accepted; weights below 2^-960
+ * of a row's largest count as 0; where a row has no weights at all, or inv_temp[s] is below 0 or no number, the token is -1.  Numbers u lie in [0, 1).
+ * ws: pb200_verify_drafts_workspace_bytes, for calls that follow one another. */
 PB200_API size_t pb200_verify_drafts_workspace_bytes(int64_t n_drafts);
 PB200_API int pb200_verify_drafts(int type, const void * target, int64_t ld_target, const void * draft, int64_t ld_draft, int n_vocab, int n_seq, const int32_t * start, int64_t n_drafts,
                                   const int32_t * tokens, const float * inv_temp, const float * u_accept, const float * u_draw, int32_t * n_accepted, int32_t * out, int64_t ld_out,

@@ -37,10 +37,11 @@ static size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 size_t kv4_attn_shared_workspace(int64_t rows, int D) { return round_up(kv4_attn_workspace(D)) + round_up((size_t) rows * D * sizeof(float)) + (size_t) rows * sizeof(float4); }
 
 // A prefix is read once for the rows of all its sequences, by the prompts' kernel, where each sequence has few and these would walk many pages in front of their own; otherwise they do: nothing
-// has to be added up, and there is one launch.  How many pages (times kv heads and tiles of eight rows) is decided twice: the prompts' kernel is launched
-// where tables have room for that many; it has work where there are half as many, as lengths, on the device, say: by then its launch, and the join's, have to be paid for anyway (8 us).  us, pages in front of the own ones / by themselves, n sequences of one token, 32 heads over 8, bf16: 1000 cells, 64 39 / 45, 128 55 / 46; 4000, 16 33 / 36,
-// 24 41 / 40, 32 47 / 41, 128 123 / 63; 16 000, 8 46 / 49, 12 56 / 49, 32 117 / 51, 128 405 / 90; 16 heads over 2: 4000, 64 34 / 39, 128 47 / 46; F32, 32 over 8: 1000, 32 37 / 43, 64 56 / 46;
-// 4000, 8 36 / 37, 12 39 / 38, 16 45 / 38; 16 000, 4 43 / 49, 8 67 / 54
+// has to be added up, and there is one launch.  How many pages (times kv heads and tiles of eight rows) is decided twice: the prompts' kernel is launched where tables have room for that many; it has
+// work where there are half as many, as lengths, on the device, say: by then its launch, and the join's, have to be paid for anyway (8 us).
+// us, pages in front of the own ones / by themselves, n sequences of one token, 32 heads over 8, bf16: 1000 cells, 64 39 / 45, 128 55 / 46; 4000, 16 33 / 36, 24 41 / 40, 32 47 / 41, 128 123 / 63;
+// 16 000, 8 46 / 49, 12 56 / 49, 32 117 / 51, 128 405 / 90; 16 heads over 2: 4000, 64 34 / 39, 128 47 / 46; F32, 32 over 8: 1000, 32 37 / 43, 64 56 / 46; 4000, 8 36 / 37, 12 39 / 38, 16 45 / 38;
+// 16 000, 4 43 / 49, 8 67 / 54.  128 requests behind 16 009 cells, 5 to 900 of their own: 119 us, about 52 for the own cells, 55 for the prefix (0.4 of the tensor cores' rate) and 12 for the join
 constexpr int KV4_APART = 14000, KV4_APART_F32 = 8500;
 int launch_kv4_attn_shared(const Kv4Attn & a, const Kv4Groups & g, int D, int type, void * ws, cudaStream_t st, int & launches) {
     Kv4Attn b = a;

@@ -7,6 +7,9 @@
 // Work.  Two kernels.  Few rows (tokens that decode): keys stream through shared memory, rows stay there.  Many rows: an item is 256, 128 or 64 cells of a sequence, 32 to each of a CTA's warps (128 and
 // 64: two or four warps have the same cells, and each a part of the rows).  A cluster has an item; its CTAs share the kv heads, and the rows in blocks of 64; their sums meet in shared memory, in the
 // CTAs' order (equal calls give equal bits).
+//
+// Bound: instructions.  Few rows: a key's numbers are taken apart once for up to 16 rows (32 sequences of up to 8192 cells 33 us; their keys' bytes take 12).  Many rows: of a block of 64 rows 1.2 us go into
+// loading and converting, 2 into the products' chains and exponentials (64 queries of 32 heads behind 16 000 cells 45 us, 0.07 of the tensor cores' rate; 2048 of a prompt, on 128 CTAs, 293).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

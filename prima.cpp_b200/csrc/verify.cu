@@ -7,6 +7,10 @@
 //   draw    a cluster has a sequence.  It joins its rows' chunks, decides, and adds up the weights that the token is drawn with, of one row, or of two with draft logits.  Weights and sums are in
 //           64 bits: a cumulative sum of 100 000 weights with errors of 1e-8 each would give another token once in a thousand draws.  Each warp has the sum of a contiguous part; that in which the
 //           token lies goes to all warps of its CTA once more, and a part of that is scanned.
+//
+// Bound.  rows: memory where there are many.  draw: 64-bit instructions (a weight is a root of 16 from a table and a polynomial of degree 5) and, for few sequences, the chain of launch, row sums,
+// cluster barriers and parts.  us: 64 sequences, 3.6 drafts each on the average, rows of 128 256 in 32 bits, 115 (47 of them the rows, 5 TB/s); 24 with drafts from elsewhere, 151 937 in bf16, 37; one
+// sequence, 3 drafts, 32 000, 17 to 19.  exp in 64 bits instead of the table 248, 69 and 23.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
