@@ -363,6 +363,22 @@ def test_weights(pkg, lib, cuda, type_, dim, case):
     check_weights(b, np.full((len(q), width), 5.0), sums.double().cpu().numpy(), 0.75, old.double().cpu().numpy())
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("case", [(12, 9, 3000, 4, 1), (6, 9, 3000, 4, 1), (1, 9, 200, 4, 1), (6, 9, 3000, 8, 2), (40, 9, 200, 8, 2), (1, 9, 200, 8, 2), (40, 9, 200, 12, 3), (8, 9, 500, 12, 3), (1, 9, 200, 12, 3),
+                                  (4, 20, 900, 12, 3), (8, 20, 200, 12, 3), (1, 20, 200, 12, 3)], ids=lambda c: "%dx%dof%d_h%dover%d" % c)
+@pytest.mark.parametrize("window", [0, 90])
+def test_weights_of_many_rows_however_items_are_cut(pkg, lib, cuda, type_, case, window):
+    """sizes for which one, two, four or eight CTAs have an item, and one, two or four warps the same cells"""
+    n, q, kv, heads, kv_heads = case
+    kv = [max(0, kv - 41 * i % kv) if i else kv for i in range(n)]
+    b = Batch(pkg, lib, 27, type_, heads, kv_heads, 64 if window else 128, [q] * n, kv, window=window, first=5 if window else 0)
+    lse = dev(np.nan_to_num(b.want()[2], nan=7.0, neginf=-np.inf), np.float32)
+    width = max(kv) + 3
+    sums = torch.full((n, width), 5.0, device="cuda")
+    weigh(b, lse, 0.0, None, sums)
+    check_weights(b, np.full((n, width), 5.0), sums.double().cpu().numpy(), 0.0, None)
+
+
 def test_weights_behind_attention_sum_up_to_the_queries(pkg, lib, cuda):
     """attn_lse, then weigh in place twice: all weights of a row are 1, whatever kernel its logarithm came from."""
     b = Batch(pkg, lib, 21, "bf16", 16, 2, 128, [1, 80, 5], [900, 333, 64])
