@@ -9,7 +9,7 @@
 // CTAs' order (equal calls give equal bits).
 //
 // Bound: instructions.  Few rows: a key's numbers are taken apart once for up to 16 rows (32 sequences of up to 8192 cells 33 us; their keys' bytes take 12).  Many rows: of a block of 64 rows 1.2 us go into
-// loading and converting, 2 into the products' chains and exponentials (64 queries of 32 heads behind 16 000 cells 45 us, 0.07 of the tensor cores' rate; 2048 of a prompt, on 128 CTAs, 293).
+// loading and converting, 2 into the products' chains and exponentials (64 queries of 32 heads behind 16 000 cells 41 us, 0.12 of the tensor cores' rate; 2048 of a prompt, on 128 CTAs, 259).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -217,6 +217,8 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
         uint32_t kf[2][NB][2][4];                           // eights of cells 16 m + g (+ 8): block, half of the eight numbers
         float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
         int held = -1;
+        constexpr bool WIDE = !F32 && D == 128;             // rows by 16 bytes where they lie so (bf16, 2048 x 2048 293 -> 259 us, 64 x 16 000 45 -> 41; heads of 64 2 % slower)
+        const bool wide = (((uintptr_t) A.q | (uintptr_t) (A.ldq * sizeof(T))) & 15) == 0;
         for (int u = u0; u < u1; u++) {
             const int hk = u / blocks, row0 = r_lo + (u - hk * blocks) * KW_ROWS, n = min(KW_ROWS, r_lo + rows - row0);
             if (held != hk && page >= 0) {
@@ -239,9 +241,14 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
                 float x[EACH], top = 0.f;
                 const T * src = (const T *) A.q + (q0 + t) * A.ldq + (int64_t) head * D + 8 * quarter;
 #pragma unroll
-                for (int i = 0; i < EACH; i += 4) {
-                    const float4 v = have ? load4(src + (i & ~7) * 4 + (i & 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+                for (int i = 0; i < EACH; i += 8) {
+                    __align__(16) T w[8];
+                    if (WIDE && wide) *reinterpret_cast<uint4 *>(w) = have ? *reinterpret_cast<const uint4 *>(src + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                    for (int k = 0; k < 8; k += 4) {
+                        const float4 v = WIDE && wide ? load4(w + k) : have ? load4(src + 4 * i + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[i + k] = v.x; x[i + k + 1] = v.y; x[i + k + 2] = v.z; x[i + k + 3] = v.w;
+                    }
                 }
                 const float lse = have ? W.lse[(q0 + t) * W.ld_lse + head] : -INFINITY;
                 const float up = row_power<EACH>(x, top) * (A.scale < 0.f ? -1.f : 1.f);
@@ -690,7 +697,7 @@ int weigh_launch(const Kv4Weigh & w, cudaStream_t st) {
     if (e != cudaSuccess) return (int) e;
     const int64_t units = hks * ((rows + KW_ROWS - 1) / KW_ROWS);
     // How items are cut, by what a launch takes, in us: an item 6, a unit 1.2 to load and convert and 2 for its products, where two CTAs share an SM 0.8 + 2 for each; items behind those at once wait.
-    // Measured, bf16, 32 query heads of 8, D = 128: 64 queries x 16 000 cells 1 CTA 112, 4 CTAs 45, 8 62, 4 with warps in pairs 62; 100 x 1000 8 CTAs 29, in pairs 23; 2048 x 2048 411 and 293.
+    // Measured (rows by 8 bytes), bf16, 32 query heads of 8, D = 128: 64 queries x 16 000 cells 1 CTA 112, 4 CTAs 45, 8 62, 4 with warps in pairs 62; 100 x 1000 8 CTAs 29, in pairs 23; 2048 x 2048 411 and 293.
     const int64_t cells = std::min<int64_t>(w.ld_sums, (int64_t) w.attn.table_ld * KV4_CELLS);
     int ctas = 1, cuts = 1;
     double best = INFINITY;

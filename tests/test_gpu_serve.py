@@ -379,6 +379,17 @@ def test_weights_of_many_rows_however_items_are_cut(pkg, lib, cuda, type_, case,
     check_weights(b, np.full((n, width), 5.0), sums.double().cpu().numpy(), 0.0, None)
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_of_many_rows_eight_bytes_apart(pkg, lib, cuda, type_, dim):
+    """rows that lie on 8 bytes, but not on 16, in 16 bits; rows in front and behind that are nobody's"""
+    b = Batch(pkg, lib, 28, type_, 16, 2, dim, [40, 9], [300, 170], pad=4, front=3, behind=2)
+    lse = dev(np.nan_to_num(b.want()[2], nan=7.0, neginf=-np.inf), np.float32)
+    sums = torch.full((2, 301), 5.0, device="cuda")
+    weigh(b, lse, 0.0, None, sums)
+    check_weights(b, np.full((2, 301), 5.0), sums.double().cpu().numpy(), 0.0, None)
+
+
 def test_weights_behind_attention_sum_up_to_the_queries(pkg, lib, cuda):
     """attn_lse, then weigh in place twice: all weights of a row are 1, whatever kernel its logarithm came from."""
     b = Batch(pkg, lib, 21, "bf16", 16, 2, 128, [1, 80, 5], [900, 333, 64])

@@ -90,6 +90,7 @@ def test_sizes_beyond_the_kernels_counts(lib, cache, pkg):
     many = pkg.Kv4Cache(BASE, 1 << 30, 1, 8, 128)
     big = dict(ldq=1024, ldo=1024, n_head=8, out=1 << 50, n_tokens=1 << 20, max_q=1, n_seq=1, ld_lse=8, ws_bytes=1 << 50)
     assert c.pb200_kv4_attn_shared(*args(many, SHARED, **dict(big, n_seq=1 << 16, n_group=1 << 16, prefix_ld=1 << 12))) == -3
+    assert c.pb200_kv4_attn_shared(*args(cache, SHARED, n_group=(1 << 24) + 1)) == -3
 
 
 def test_reference_of_verification_keeps_the_targets_distribution():
