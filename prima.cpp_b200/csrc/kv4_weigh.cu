@@ -2,7 +2,7 @@
 //
 // Mathematics.  sums[j] = decay * old[j] + sum over queries t and heads h that see cell j of 2^(c q_th . k_j - L_th): L is the logarithm of the row's sum, which attention left, so that no row
 // has to be looked at as a whole: a cell's sum is that of its own column.  Scores are m16n8k16 products, cells x rows: a thread holds two rows' scores of a cell next to each other, and adds
-// them up without asking others.  Keys are f16 numbers exactly and go to registers once for all rows; a query row is f16 times a power of two (F32: two of them, 22 bits, low parts first).
+// them up without asking others.  Keys are f16 numbers exactly and go to registers once for all rows; a query row is f16 times a power of two (F32: two of them, 22 bits, low parts first; many rows of F16 are as they are).
 //
 // Work.  Two kernels.  Few rows (tokens that decode): keys stream through shared memory, rows stay there.  Many rows: an item is 256, 128 or 64 cells of a sequence, 32 to each of a CTA's warps (128 and
 // 64: two or four warps have the same cells, and each a part of the rows).  A cluster has an item; its CTAs share the kv heads, and the rows in blocks of 64; their sums meet in shared memory, in the
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
         uint32_t kf[2][NB][2][4];                           // eights of cells 16 m + g (+ 8): block, half of the eight numbers
         float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
         int held = -1;
-        constexpr bool WIDE = !F32 && D == 128;             // rows by 16 bytes where they lie so (bf16, 2048 x 2048 293 -> 259 us, 64 x 16 000 45 -> 41; heads of 64 2 % slower)
+        constexpr bool WIDE = std::is_same<T, __nv_bfloat16>::value && D == 128;             // rows by 16 bytes where they lie so (bf16, 2048 x 2048 293 -> 259 us, 64 x 16 000 45 -> 41; heads of 64 2 % slower).  F16 always
         const bool wide = (((uintptr_t) A.q | (uintptr_t) (A.ldq * sizeof(T))) & 15) == 0;
         for (int u = u0; u < u1; u++) {
             const int hk = u / blocks, row0 = r_lo + (u - hk * blocks) * KW_ROWS, n = min(KW_ROWS, r_lo + rows - row0);
@@ -238,22 +238,39 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
                 const int r = tid >> 2, quarter = tid & 3, row = row0 + r, t = row / A.group, head = hk * A.group + row - t * A.group;
                 const bool have = r < n;
                 constexpr int EACH = D / 4;
-                float x[EACH], top = 0.f;
                 const T * src = (const T *) A.q + (q0 + t) * A.ldq + (int64_t) head * D + 8 * quarter;
-#pragma unroll
-                for (int i = 0; i < EACH; i += 8) {
-                    __align__(16) T w[8];
-                    if (WIDE && wide) *reinterpret_cast<uint4 *>(w) = have ? *reinterpret_cast<const uint4 *>(src + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                    for (int k = 0; k < 8; k += 4) {
-                        const float4 v = WIDE && wide ? load4(w + k) : have ? load4(src + 4 * i + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[i + k] = v.x; x[i + k + 1] = v.y; x[i + k + 2] = v.z; x[i + k + 3] = v.w;
-                    }
-                }
                 const float lse = have ? W.lse[(q0 + t) * W.ld_lse + head] : -INFINITY;
-                const float up = row_power<EACH>(x, top) * (A.scale < 0.f ? -1.f : 1.f);
+                float up = 1.f;
+                if constexpr (std::is_same<T, __half>::value) {            // as they are
+                    const uint32_t turned = A.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-                for (int i = 0; i < EACH; i += 8) row_store<T, 8>(reinterpret_cast<float(&)[8]>(x[i]), up, &S.q[0][r][16 * quarter + 8 * i], &S.q[LO - 1][r][16 * quarter + 8 * i]);
+                    for (int i = 0; i < EACH; i += 8) {
+                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                        if (have) {
+                            if (wide) w = *reinterpret_cast<const uint4 *>(src + 4 * i);
+                            else {
+                                const uint2 x = *reinterpret_cast<const uint2 *>(src + 4 * i), y = *reinterpret_cast<const uint2 *>(src + 4 * i + 4);
+                                w = make_uint4(x.x, x.y, y.x, y.y);
+                            }
+                        }
+                        *reinterpret_cast<uint4 *>(&S.q[0][r][16 * quarter + 8 * i]) = make_uint4(w.x ^ turned, w.y ^ turned, w.z ^ turned, w.w ^ turned);
+                    }
+                } else {
+                    float x[EACH];
+#pragma unroll
+                    for (int i = 0; i < EACH; i += 8) {
+                        __align__(16) T w[8];
+                        if (WIDE && wide) *reinterpret_cast<uint4 *>(w) = have ? *reinterpret_cast<const uint4 *>(src + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                        for (int k = 0; k < 8; k += 4) {
+                            const float4 v = WIDE && wide ? load4(w + k) : have ? load4(src + 4 * i + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            x[i + k] = v.x; x[i + k + 1] = v.y; x[i + k + 2] = v.z; x[i + k + 3] = v.w;
+                        }
+                    }
+                    up = row_power<EACH>(x, 0.f) * (A.scale < 0.f ? -1.f : 1.f);
+#pragma unroll
+                    for (int i = 0; i < EACH; i += 8) row_store<T, 8>(reinterpret_cast<float(&)[8]>(x[i]), up, &S.q[0][r][16 * quarter + 8 * i], &S.q[LO - 1][r][16 * quarter + 8 * i]);
+                }
                 if (quarter == 0) {
                     S.row[r] = row_factors(A.scale, up, lse);
                     S.pos[r] = have ? max(p0 + t, -1) : -1;
