@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) k_verify_draw(const __
         for (int k = 1; k < ONCE; k++) x += w[k];
         return x;
     };
-    double z[2] = {1.0, 0.0};
+    double part_p = 0.0, part_q = 0.0;                      // of a weight its part of the row's
     if (minus_q) {
         double x = 0.0, y = 0.0;
         walk(from, to, [&](int, const float (&lp)[ONCE], const float (&lq)[ONCE]) {
@@ -422,8 +422,8 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) k_verify_draw(const __
             if (lane == 0) { S.z[0] = x; S.z[1] = y; }
         }
         cluster_sync();
-        z[0] = warp_sum_d(lane < ctas ? remote(&S.z[0], lane % ctas) : 0.0);
-        z[1] = warp_sum_d(lane < ctas ? remote(&S.z[1], lane % ctas) : 0.0);
+        part_p = 1.0 / warp_sum_d(lane < ctas ? remote(&S.z[0], lane % ctas) : 0.0);
+        part_q = 1.0 / warp_sum_d(lane < ctas ? remote(&S.z[1], lane % ctas) : 0.0);
     }
     bool rest = minus_q || out_of >= 0;                     // max(p - q, 0), or p
     auto weights = [&](int i0, int step, const float (&lp)[ONCE], const float (&lq)[ONCE], double (&w)[ONCE]) {
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) k_verify_draw(const __
             double q[ONCE];
             wq(lq, q);
 #pragma unroll
-            for (int k = 0; k < ONCE; k++) w[k] = fmax(fma(w[k], z[1], -q[k] * z[0]), 0.0);
+            for (int k = 0; k < ONCE; k++) w[k] = fmax(__dmul_rn(w[k], part_p) - __dmul_rn(q[k], part_q), 0.0);      // either rounded by itself: of equal rows nothing is left
         } else if (rest)
 #pragma unroll
             for (int k = 0; k < ONCE; k++) w[k] = i0 + step * k == out_of ? 0.0 : w[k];
