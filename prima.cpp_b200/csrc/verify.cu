@@ -286,7 +286,8 @@ struct Chunks {
         for (int k = 0; k < VERIFY_CHUNKS / 32; k++)
             if (p[k].x > -INFINITY) l += p[k].y * w(p[k].x);
         l = warp_sum_d(l);
-        return lx > -INFINITY ? w(lx) / l : 0.0;
+        const double of_x = w(lx);
+        return of_x > NOTHING ? of_x / l : 0.0;
     }
 };
 

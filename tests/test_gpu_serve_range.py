@@ -3,9 +3,37 @@
 import numpy as np
 import pytest
 
+import ref_serve as V
 from test_gpu_serve import TYPES, drafted, verify
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def weights_that_count_as_nothing(monkeypatch):
+    """Weights below 2^-960 of a row's largest count as 0, where numbers of 64 bits go on to 2^-1074: at temperatures as small as here's that is what all others of a row have."""
+    full = V.softmax
+
+    def softmax(x, t):
+        w = full(x, t)
+        if w is None:
+            return None
+        w = np.where(w < 2.0 ** -960 * w.max(), 0.0, w)
+        return w / w.sum()
+
+    monkeypatch.setattr(V, "softmax", softmax)
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_tokens_without_weight_are_not_accepted(lib, cuda, with_draft):
+    """A drafted token so far below the largest logit of both models that it has no weight in either: 0 < 0 is false, whatever u."""
+    rng = np.random.default_rng(72)
+    drafts, vocab = [1] * 24, 4001
+    target, draft, _, u, v = drafted(rng, "f32", vocab, drafts)
+    tokens = rng.integers(0, vocab, 24).astype(np.int32)
+    target[2 * np.arange(24), tokens], draft[np.arange(24), tokens] = -30.0, -30.0
+    u[::4] = 0.0
+    verify(lib, "f32", target, draft if with_draft else None, drafts, tokens, np.float32([40.0, 1e3, 1e4] * 8), u, v)
 
 
 @pytest.mark.parametrize("type_", TYPES)
