@@ -67,11 +67,7 @@ __device__ __forceinline__ void get_vec(const T * row, int n, int skew, int v, u
 }
 template <typename T> __device__ __forceinline__ int skew_of(const T * row) { return (int) (((uintptr_t) row & 15) / sizeof(T)); }
 
-// 1 / temperature of a sequence: of 0 the smallest number, so that times -inf it is no NaN; none where it is below 0 or no number
-__device__ __forceinline__ float inv_temp_of(const Verify & A, int s) {
-    const float t = A.inv_temp ? A.inv_temp[s] : 1.f;
-    return t == 0.f ? 1.4e-45f : t;
-}
+__device__ __forceinline__ float inv_temp_of(const Verify & A, int s) { return A.inv_temp ? A.inv_temp[s] : 1.f; }      // none where it is below 0 or no number
 
 // which sequence draft i belongs to (-1: none), by all threads of a CTA
 template <int THREADS>
@@ -89,13 +85,17 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// weight of a logit relative to one that is larger, by half their difference (the whole one may be more than the largest number); c: of such a half to the power of two
+__device__ __forceinline__ float weight(float l, float top, float c) { return ex2(fmaf(l, 0.5f, -0.5f * top) * c); }
+// of 1 / temperature 0 the smallest number, so that times -inf it is no NaN; above 1e38 the largest, which leaves nothing of logits that are 1e-36 apart
+__device__ __forceinline__ float half_to_power(float t) { return t == 0.f ? 1.4e-45f : fminf(t * 2.8853900817779268f, FLT_MAX); }
 // sums of weights relative to the largest logit
 struct Sum {
     float m = -INFINITY, l = 0.f;
-    __device__ __forceinline__ void add(float m2, float l2, float c) {       // c: of a logit to the power of two
+    __device__ __forceinline__ void add(float m2, float l2, float c) {
         const float top = fmaxf(m, m2);
         if (top == INFINITY) l = (m == INFINITY ? l : 0.f) + (m2 == INFINITY ? l2 : 0.f);
-        else if (top > -INFINITY) l = l * ex2((m - top) * c) + l2 * ex2((m2 - top) * c);
+        else if (top > -INFINITY) l = l * weight(m, top, c) + l2 * weight(m2, top, c);
         m = top;
     }
 };
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(VR_THREADS, VR_CTAS) k_verify_rows(const __gri
     const T * src = of_draft ? (const T *) A.draft + i * A.ld_draft : (const T *) A.target + (i + s) * A.ld_target;
     const int skew = skew_of(src), vecs = (A.vocab + skew + VEC - 1) / VEC;
     const int from = (int) ((int64_t) vecs * chunk / A.chunks), to = (int) ((int64_t) vecs * (chunk + 1) / A.chunks);
-    const float t = inv_temp_of(A, s), c = t * 1.4426950408889634f;
+    const float t = inv_temp_of(A, s), c = half_to_power(t);
     Sum sum;
     int arg = INT_MAX;
     const bool greedy = t == INFINITY;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(VR_THREADS, VR_CTAS) k_verify_rows(const __gri
 #pragma unroll
                 for (int k = 0; k < ONCE; k++)
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) l += ex2((entry(k, e) - top) * c);
+                    for (int e = 0; e < VEC; e++) l += weight(entry(k, e), top, c);
             }
             sum.add(top, l, c);
         }
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(VR_THREADS, VR_CTAS) k_verify_rows(const __gri
     }
 }
 
-// 2^(y / 16) in 64 bits for y from -16 * 1001 to about 0: the whole part of y goes to the exponent and to one of 16 roots, 2^(r / 16) of the rest (up to a half) is the polynomial that agrees
+// 2^(y / 16) in 64 bits for y from -16 * 1000 to 0: the whole part of y goes to the exponent and to one of 16 roots, 2^(r / 16) of the rest (up to a half) is the polynomial that agrees
 // with it at the six Chebyshev nodes: within 2^-47 of it.  (Without roots nine products instead of five: 64 sequences of 128 256 logits 70 us where this takes 66.)
 __device__ __forceinline__ double power_of_two(double y, const double * roots) {
     constexpr double ROUND = 6755399441055744.0;          // 1.5 * 2^52: a sum with it has the whole number in its last bits
@@ -205,24 +205,26 @@ __device__ __forceinline__ double power_of_two(double y, const double * roots) {
     p = fma(p, r, 1.0000000000000044) * roots[k & 15];
     return __hiloint2double(__double2hiint(p) + ((k & ~15) << 16), __double2loint(p));
 }
-// The weights of a row's logits, the largest of them m; none is taken for less than 2^-1000, masked entries and what is no number among them: NOTHING is less than that, and a sum of them
-constexpr double NOTHING = 1e-290;
+// The weights of a row's logits, the largest of them m; none is taken for less than 2^-1000, masked entries and what is no number among them: NOTHING is less than that, and a sum of them.
+// The difference comes first, in 64 bits, then the temperature, then the floor: a floor under the logits themselves would be off by half a step of m times 1 / temperature, which has no bound.
+// The floor by the high word, as a whole number (y is 0 or less, and -inf above all others): 64 sequences of 128 256 logits 117 us, by a comparison of 64-bit numbers 121
+constexpr double NOTHING = 1e-290, FLOOR = -16000.0;
+constexpr uint32_t FLOOR_HIGH = 0xc0cf4000u;       // the high word of FLOOR, whose low one is 0
 struct Weights {
-    double c, mc;
-    float least;
-    bool step;                 // the same weight for all from `least` on: a largest logit of +inf, or an infinite temperature
+    double c, m;               // c: never 0: times -inf it is no NaN
+    bool step;                 // a largest logit of +inf: the same weight for all of these, none for others
     const double * roots;      // 2^(i / 16)
-    __device__ __forceinline__ Weights(float m, float t, const double * roots) : c((double) t * (16 * 1.4426950408889634)), mc((double) m * c), roots(roots) {
-        step = m == INFINITY || t < 1e-30f;
-        least = m == INFINITY ? INFINITY : t < 1e-30f ? -FLT_MAX : fmaxf((float) ((double) m - 16000.0 / c), -FLT_MAX);
-    }
+    __device__ __forceinline__ Weights(float m, float t, const double * roots) : c(fmax((double) t * (16 * 1.4426950408889634), 1e-300)), m(m), step(m == INFINITY), roots(roots) {}
     template <int N> __device__ __forceinline__ void operator()(const float (&l)[N], double (&w)[N]) const {
         if (step) {
 #pragma unroll
-            for (int i = 0; i < N; i++) w[i] = l[i] >= least ? 1.0 : 0.0;
+            for (int i = 0; i < N; i++) w[i] = l[i] == INFINITY ? 1.0 : 0.0;
         } else {
 #pragma unroll
-            for (int i = 0; i < N; i++) w[i] = power_of_two(fma((double) fmaxf(l[i], least), c, -mc), roots);
+            for (int i = 0; i < N; i++) {
+                const double y = ((double) number(l[i]) - m) * c;
+                w[i] = power_of_two((uint32_t) __double2hiint(y) <= FLOOR_HIGH ? y : FLOOR, roots);
+            }
         }
     }
     __device__ __forceinline__ double operator()(float l) const {

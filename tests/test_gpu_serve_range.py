@@ -2,11 +2,13 @@
 
 import numpy as np
 import pytest
+import torch
 
 import ref_serve as V
 from test_gpu_serve import TYPES, drafted, verify
 
 pytestmark = pytest.mark.gpu
+LOWEST = np.finfo(np.float32).min
 
 
 @pytest.fixture(autouse=True)
@@ -22,6 +24,41 @@ def weights_that_count_as_nothing(monkeypatch):
         return w / w.sum()
 
     monkeypatch.setattr(V, "softmax", softmax)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("with_draft", [True, False])
+@pytest.mark.parametrize("masked", [False, True])
+def test_verification_at_any_temperature(lib, cuda, type_, with_draft, masked):
+    """Every 1 / temperature from the smallest number to the largest, at largest logits of 1 to 60 000: a first draft that is the target's largest, and one that is drawn."""
+    rng = np.random.default_rng(70)
+    pairs = [(t, top) for t in (0.0, 1e-45, 1e-38, 1e-31, 1e-20, 1e-3, 20.0, 1e3, 1e5, 1e6, 1e7, 5e7, 1e8, 1e9, 1e10, 1e12, 1e18, 1e20, 1e30, np.finfo(np.float32).max) for top in (1.0, 24.3, 130.0, 900.0, 6e4)]
+    drafts, vocab = [2] * len(pairs), 3001
+    target, draft, _, u, v = drafted(rng, "f32", vocab, drafts, spread=2.5, apart=0.7)
+    row = np.arange(len(u)) + np.repeat(np.arange(len(pairs)), drafts)
+    tops = np.array([top for _, top in pairs])
+    hold = lambda x: torch.from_numpy(x.astype(np.float32)).to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[type_]).float().numpy()
+    target = hold(target + (np.repeat(tops, 3) - target.max(-1))[:, None])
+    draft = hold(draft + (np.repeat(tops, 2) - draft.max(-1))[:, None])
+    if masked:
+        target[:, 2000:2500], draft[:, 100:600] = -np.inf, -np.inf
+        target[::2, 700:900], draft[::2, 800:900] = hold(np.float32([LOWEST if type_ != "f16" else -65504.0])), hold(np.float32([LOWEST if type_ != "f16" else -65504.0]))
+    tokens = np.array([int(np.argmax(target[r])) if i % 2 == 0 else int(rng.integers(0, vocab)) for i, r in enumerate(row)], dtype=np.int32)
+    verify(lib, type_, target, draft if with_draft else None, drafts, tokens, np.array([t for t, _ in pairs], np.float32), u, v)
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_verification_of_the_largest_and_the_lowest_logits(lib, cuda, with_draft):
+    """Rows whose largest logit is the type's lowest number, beside -inf; rows with both ends of the type, at temperatures that leave something of either."""
+    rng = np.random.default_rng(71)
+    drafts, vocab = [2] * 12, 2500
+    target, draft, _, u, v = drafted(rng, "f32", vocab, drafts)
+    for x in (target, draft):
+        x[:18] = np.where(rng.random((len(x[:18]), vocab)) < 0.5, LOWEST, -np.inf)
+        x[18:] = np.where(rng.random((len(x[18:]), vocab)) < 0.5, LOWEST, -LOWEST)
+    tokens = np.array([int(rng.choice(np.nonzero(np.isfinite(target[i + i // 2]))[0])) for i in range(24)], dtype=np.int32)
+    t = np.array([1.0, 0.7, 1e9, 1e-40, 0.0, 3e38, 1.0, 0.0, 1e-38, 3e-39, 1e9, 1e-45], np.float32)
+    verify(lib, "f32", target, draft if with_draft else None, drafts, tokens, t, u * np.float32(0.9), v)
 
 
 @pytest.mark.parametrize("with_draft", [True, False])
