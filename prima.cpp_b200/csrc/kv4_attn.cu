@@ -56,6 +56,7 @@ int launch_kv4_attn_shared(const Kv4Attn & a, const Kv4Groups & g, int D, int ty
     b.x.prefix_ld = g.table_ld;
     b.x.n_group = g.n;
     b.x.n_own = a.n_seq;
+    b.x.room = (int) std::min<int64_t>(1 << 30, std::min<int64_t>(g.table_ld, 1 << 24) * KV4_CELLS);
     const int few = few_rows(type);
     const int64_t rows = std::min<int64_t>(a.max_q, a.n_tokens) * a.group;
     b.x.mode = KV4_SHARED;

@@ -45,10 +45,10 @@ __device__ __forceinline__ void kv4_span(const Kv4Attn & A, int lo, int hi, Kv4S
         q.from = from;
     } else kv4_pages(A, X && A.x.mode == KV4_FRONT ? A.x.prefix_ld : A.table_ld, lo, hi, q);
 }
-// cells of group g's prefix (30 bits), and whether it is by itself: what counts are all groups' pages, up to KV4_FEW_GROUPS of them; of more, the group's times their number
+// cells of group g's prefix (as many as its table has room for: pages are counted in 31 bits by what tables have), and whether it is by itself: what counts are all groups' pages, up to KV4_FEW_GROUPS of them; of more, the group's times their number
 constexpr int KV4_FEW_GROUPS = 8;
 __device__ __forceinline__ int kv4_prefix(const Kv4Attn & A, int g, bool & apart) {
-    auto cells = [&](int i) { return min(max(A.x.prefix_len[i], 0), 1 << 30); };
+    auto cells = [&](int i) { return min(max(A.x.prefix_len[i], 0), A.x.room); };
     auto pages = [&](int i) { return (int64_t) (A.x.group_start[i + 1] - A.x.group_start[i]) * ((cells(i) + KV4_CELLS - 1) / KV4_CELLS); };
     int64_t all = 0;
     if (A.x.n_group <= KV4_FEW_GROUPS)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ref_serve as V
-from test_gpu_serve import TYPES, drafted, verify
+from test_gpu_serve import TYPES, Batch, drafted, verify
 
 pytestmark = pytest.mark.gpu
 LOWEST = np.finfo(np.float32).min
@@ -84,3 +84,16 @@ def test_rows_that_are_alike_leave_the_targets_weights(lib, cuda, type_, vocab):
     draft = target[::2].copy()
     tokens = np.array([1 if i % 3 == 0 else -1 if i % 3 == 1 else vocab + i for i in range(48)], dtype=np.int32)
     verify(lib, type_, target, draft, drafts, tokens, rng.choice([1.0, 0.7, 1.4], 48), u, v)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("case", [([2, 1], [300, 64], [1, 2, 1], [5, 70, 0], 8, 2), ([64], [4000], [1] * 64, [1 + 3 * i for i in range(64)], 8, 8), ([3, 40], [600, 3000], [70, 200, 1] + [1] * 40, [70, 300, 1] + [9] * 40, 16, 8)],
+                         ids=["few", "apart", "prompts"])
+def test_a_prefix_ends_with_its_table(pkg, lib, cuda, type_, case):
+    """Lengths of prefixes far beyond what their tables have room for: cells are those of the pages that are there, and no more pages are walked or counted."""
+    groups, prefix, q, kv, heads, kv_heads = case
+    b = Batch(pkg, lib, 80, type_, heads, kv_heads, 128, q, kv, groups, prefix)
+    b.prefix_np[:] = [1 << 30, (1 << 31) - 1][:len(prefix)]
+    b.upload()
+    b.attend()
+    b.check()
