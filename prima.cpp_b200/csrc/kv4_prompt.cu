@@ -797,8 +797,10 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     cudaError_t e = ensure_dyn_smem(cache, (const void *) k_kv4_attn_prompt<T, D, X>, smem, true);
     if (e != cudaSuccess) return (int) e;
     const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
-    // (a plan adds up key tiles of all items: in 30 bits)
-    const int64_t items = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv, pages = a.table_ld < INT_MAX / KV4_CELLS ? a.table_ld : INT_MAX / KV4_CELLS;
+    // (a plan adds up key tiles of all items: in 30 bits.  An item's pages are those that the tables it walks have room for)
+    const auto room = [](int64_t ld) { return ld < INT_MAX / KV4_CELLS ? ld : (int64_t) INT_MAX / KV4_CELLS; };
+    const int64_t items = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv;
+    const int64_t pages = (a.x.mode != KV4_FRONT ? room(a.table_ld) : 0) + (a.x.mode != KV4_PLAIN ? room(a.x.prefix_ld) : 0);
     w.cut = a.n_seq <= KP_CUT_SEQ && items < ctas && KP_CUT_TILES * (pages / 2 + 1) * a.cache.n_head_kv < 1 << 30;
     launches += w.cut ? 2 : 1;
     // Behind the kernel of few rows (most_rows > 0), CTAs start where that has none at work: it has nothing that they read, and all in front of it has ended when it starts

@@ -1,11 +1,14 @@
 """The operators around the 4-bit cache at the ends of their ranges, against their definitions in 64 bits (ref_serve.py): temperatures, rows that are alike, tables and groups that end early."""
+import ctypes as C
 
 import numpy as np
 import pytest
 import torch
 
+import ref_kv4 as R
 import ref_serve as V
-from test_gpu_serve import TYPES, Batch, drafted, verify
+from gpu_util import ptr
+from test_gpu_serve import TYPES, Batch, drafted, stream, verify
 
 pytestmark = pytest.mark.gpu
 LOWEST = np.finfo(np.float32).min
@@ -97,3 +100,19 @@ def test_a_prefix_ends_with_its_table(pkg, lib, cuda, type_, case):
     b.upload()
     b.attend()
     b.check()
+
+
+@pytest.mark.parametrize("q,kv,groups,prefix", [([70, 200, 1], [70, 300, 1], [3], [600]), ([1] * 24, [9 + i for i in range(24)], [24], [6000])], ids=["prompts", "apart"])
+def test_items_are_cut_by_the_pages_of_both_tables(pkg, lib, cuda, q, kv, groups, prefix):
+    """A plan of cut items adds up their key tiles in 30 bits: with a table of prefixes whose rows have room for more, items stay whole, and the launch that joins pieces is not made."""
+    b = Batch(pkg, lib, 81, "bf16", 16, 8, 128, q, kv, groups, prefix)
+    counts = []
+    for ld in (b.prefix_table_np.shape[1], 2 * (2 ** 30 // (184 * 8)), 2 ** 23):      # (the one row of the table is read as far as the prefix goes, whatever the rows' stride)
+        b.out.fill_(7.0)
+        b.lse.fill_(7.0)
+        before = lib.c.pb200_kernel_launches()
+        lib.check(lib.c.pb200_kv4_attn_shared(C.byref(b.cache), 0, R.CODE["bf16"], ptr(b.q), b.ldq, ptr(b.out), b.ldo, b.heads, len(kv), ptr(b.q_start), ptr(b.kv), ptr(b.table), b.table_np.shape[1], 1,
+                                              ptr(b.group), ptr(b.prefix), ptr(b.prefix_table), ld, b.tokens, b.max_q, b.scale, ptr(b.lse), b.ldl, ptr(b.ws), b.ws.numel(), stream()))
+        counts.append(lib.c.pb200_kernel_launches() - before)
+        b.check()
+    assert counts == [3, 2, 2]
