@@ -85,13 +85,17 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_row
     const bool front = X && A.x.mode == KV4_FRONT;
     int s0 = s, s1 = s + 1, prefix = 0;
     if (front) {
-        s0 = A.x.group_start[s];
-        s1 = A.x.group_start[s + 1];
+        s0 = max(A.x.group_start[s], 0);
+        s1 = min(A.x.group_start[s + 1], A.x.n_own);
         bool apart;
         prefix = kv4_prefix(A, s, apart);
-        if (!apart || s0 < 0 || s1 <= s0 || s1 > A.x.n_own) return q;
+        if (!apart || s1 <= s0) return q;
     }
-    const long long a = A.q_start[s0], b = A.q_start[s1], cells = front ? prefix : A.kv_len[s];     // (all on their way)
+    long long a = A.q_start[s0], b = A.q_start[s1], cells = front ? prefix : A.kv_len[s];           // (all on their way)
+    if (front) {                               // rows of sequences that are none have no marks: what counts is that those of the others are among these
+        a = max(a, 0ll);
+        b = min(b, (long long) A.n_tokens);
+    }
     if (a < 0 || b <= a || b > A.n_tokens) return q;
     const int all = (int) (b - a), n = front ? all : min(all, A.max_q);
     if (((long long) n * A.group > most_rows) != many) return q;

@@ -6,27 +6,11 @@ import pytest
 import torch
 
 import ref_kv4 as R
-import ref_serve as V
 from gpu_util import ptr
 from test_gpu_serve import TYPES, Batch, drafted, stream, verify
 
 pytestmark = pytest.mark.gpu
 LOWEST = np.finfo(np.float32).min
-
-
-@pytest.fixture(autouse=True)
-def weights_that_count_as_nothing(monkeypatch):
-    """Weights below 2^-960 of a row's largest count as 0, where numbers of 64 bits go on to 2^-1074: at temperatures as small as here's that is what all others of a row have."""
-    full = V.softmax
-
-    def softmax(x, t):
-        w = full(x, t)
-        if w is None:
-            return None
-        w = np.where(w < 2.0 ** -960 * w.max(), 0.0, w)
-        return w / w.sum()
-
-    monkeypatch.setattr(V, "softmax", softmax)
 
 
 @pytest.mark.parametrize("type_", TYPES)
@@ -116,3 +100,21 @@ def test_items_are_cut_by_the_pages_of_both_tables(pkg, lib, cuda, q, kv, groups
         counts.append(lib.c.pb200_kernel_launches() - before)
         b.check()
     assert counts == [3, 2, 2]
+
+
+@pytest.mark.parametrize("case", ["groups", "rows"])
+def test_groups_that_end_behind_the_batch(pkg, lib, cuda, case):
+    """Prefixes by themselves: groups from in front of the first sequence to behind the last one; a last sequence whose rows lie behind the arrays.  The sequences that are there have their results."""
+    n = 64
+    b = Batch(pkg, lib, 82, "bf16", 16, 8, 128, [1] * n, [40 + i for i in range(n)], [20, n - 20], [3000, 3500])
+    b.group_np = np.array([-2, 20, n + 5], np.int32) if case == "groups" else np.array([0, 20, n + 1], np.int32)
+    b.upload()
+    extra = case == "rows"
+    q_start, kv = (torch.from_numpy(np.append(x, y).astype(np.int32)).cuda() for x, y in ((b.q_start_np, b.tokens + 7), (b.kv_np, 30)))
+    table = torch.from_numpy(np.concatenate((b.table_np, b.table_np[:1]))).cuda()
+    before = lib.c.pb200_kernel_launches()
+    lib.check(lib.c.pb200_kv4_attn_shared(C.byref(b.cache), 0, R.CODE["bf16"], ptr(b.q), b.ldq, ptr(b.out), b.ldo, b.heads, n + extra, ptr(q_start), ptr(kv), ptr(table), b.table_np.shape[1], 2,
+                                          ptr(b.group), ptr(b.prefix), ptr(b.prefix_table), b.prefix_table_np.shape[1], b.tokens, 1, b.scale, ptr(b.lse), b.ldl, ptr(b.ws), b.ws.numel(), stream()))
+    assert lib.c.pb200_kernel_launches() - before >= 2, "the prefix has no kernel of its own"
+    b.group_np = np.array([0, 20, n], np.int32)
+    b.check()
