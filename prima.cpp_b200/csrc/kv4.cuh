@@ -110,7 +110,8 @@ struct Kv4Ext {
     const int32_t * prefix_len, * prefix_table;
     int64_t prefix_ld;
     int n_group, n_own, room;             // groups, sequences; cells that a prefix has at most: what its table has room for, in 30 bits
-    int64_t least, of_page;               // where sequences would walk as many pages in front of their own, prefixes are by themselves; what a page of a prefix counts for a sequence: tiles x kv heads
+    int64_t least;                        // what has to be saved for prefixes to be by themselves: pages x kv heads x tiles of eight rows, times 16
+    int of_seq, of_tile, rows, log_tile;  // of that, a page of a prefix costs a sequence that walks it, with so many rows, and a tile of 2^log_tile rows in the prompts' kernel
     float * o; float4 * ml;               // parts of rows [token][head]: sums [D]; reference, sum of weights, and the mark of the call
     int * sync;                           // calls that have ended, CTAs of a call's last kernel that have
 };

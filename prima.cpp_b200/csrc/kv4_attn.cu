@@ -37,12 +37,14 @@ static size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 size_t kv4_attn_shared_workspace(int64_t rows, int D) { return round_up(kv4_attn_workspace(D)) + round_up((size_t) rows * D * sizeof(float)) + (size_t) rows * sizeof(float4); }
 
 // A prefix is read once for the rows of all its sequences, by the prompts' kernel, where each sequence has few and these would walk many pages in front of their own; otherwise they do: nothing
-// has to be added up, and there is one launch.  How many pages (times kv heads and tiles of eight rows) is decided twice: the prompts' kernel is launched where tables have room for that many; it has
-// work where there are half as many, as lengths, on the device, say: by then its launch, and the join's, have to be paid for anyway (8 us).
-// us, pages in front of the own ones / by themselves, n sequences of one token, 32 heads over 8, bf16: 1000 cells, 64 39 / 45, 128 55 / 46; 4000, 16 33 / 36, 24 41 / 40, 32 47 / 41, 128 123 / 63;
+// has to be added up, and there is one launch.  What counts is what is saved: pages (times kv heads and tiles of eight rows) that sequences would walk, less those that the prompts' kernel does, whose tile takes
+// KV4_TILE times as long for a page whatever rows it has.  This is decided twice: the prompts' kernel is launched where tables have room for so many pages, all of one group's; it has
+// work where there are half as many, as lengths, on the device: by then its launch, and the join's, have to be paid for anyway (8 us).
+// us, pages in front of the own ones / by themselves, n sequences of one token in one group, 32 heads over 8, bf16: 1000 cells, 64 39 / 45, 128 55 / 46; 4000, 16 33 / 36, 24 41 / 40, 32 47 / 41, 128 123 / 63;
 // 16 000, 8 46 / 49, 12 56 / 49, 32 117 / 51, 128 405 / 90; 16 heads over 2: 4000, 64 34 / 39, 128 47 / 46; F32, 32 over 8: 1000, 32 37 / 43, 64 56 / 46; 4000, 8 36 / 37, 12 39 / 38, 16 45 / 38;
-// 16 000, 4 43 / 49, 8 67 / 54.  128 requests behind 16 009 cells, 5 to 900 of their own: 119 us, about 52 for the own cells, 55 for the prefix (0.4 of the tensor cores' rate) and 12 for the join
-constexpr int KV4_APART = 14000, KV4_APART_F32 = 8500;
+// 16 000, 4 43 / 49, 8 67 / 54.  Groups of their own prefixes of 4000, bf16: 16 of 4 76 / 111, of 6 104 / 115, of 8 131 / 120, 4 of 12 66 / 55, 8 of 6 with a row each 67 / 73; F32: 16 of 3 99 / 141, of 4
+// 119 / 144, of 6 168 / 149; 64 prefixes of one sequence each 75 / 339 (87 with the launch that has no work).  128 requests behind 16 009 cells, 5 to 900 of their own: 119 us, about 52 for the own cells, 55 for the prefix (0.4 of the tensor cores' rate) and 12 for the join
+constexpr int KV4_APART = 8600, KV4_APART_F32 = 5000, KV4_TILE = 7, KV4_TILE_F32 = 5;
 int launch_kv4_attn_shared(const Kv4Attn & a, const Kv4Groups & g, int D, int type, void * ws, cudaStream_t st, int & launches) {
     Kv4Attn b = a;
     int * words = (int *) ws;
@@ -57,13 +59,16 @@ int launch_kv4_attn_shared(const Kv4Attn & a, const Kv4Groups & g, int D, int ty
     b.x.n_group = g.n;
     b.x.n_own = a.n_seq;
     b.x.room = (int) std::min<int64_t>(1 << 30, std::min<int64_t>(g.table_ld, 1 << 24) * KV4_CELLS);
-    const int few = few_rows(type);
-    const int64_t rows = std::min<int64_t>(a.max_q, a.n_tokens) * a.group;
+    const bool f32 = type == PB200_TYPE_F32;
+    const int64_t most = std::min<int64_t>(a.max_q, a.n_tokens) * a.group, rows = std::min<int64_t>(most, few_rows(type)), least = 16 * (f32 ? KV4_APART_F32 : KV4_APART);
     b.x.mode = KV4_SHARED;
-    b.x.of_page = (rows + 7) / 8 * a.cache.n_head_kv;
-    const int least = type == PB200_TYPE_F32 ? KV4_APART_F32 : KV4_APART;
+    // tiles of a sequence: those of the longest, but no more than all tokens make on the average
+    b.x.of_seq = (int) (16 * a.cache.n_head_kv * std::min<double>((rows + 7) / 8, 1 + (double) a.n_tokens * a.group / 8 / a.n_seq));
+    b.x.of_tile = 16 * a.cache.n_head_kv * (f32 ? KV4_TILE_F32 : KV4_TILE);
+    b.x.rows = (int) rows;
+    b.x.log_tile = f32 ? 7 : 8;                  // rows of an item: kp_rows
     b.x.least = least / 2;
-    const bool apart = rows <= few && (double) a.n_seq * g.table_ld * b.x.of_page >= (double) least;
+    const bool apart = most == rows && (double) kv4_saved(b.x, a.n_seq) * g.table_ld >= (double) least;
     if (!apart) b.x.least = INT64_MAX;
     const int e = launch_kv4_attn(b, D, type, ws, st, launches);
     if (e || !apart) return e;

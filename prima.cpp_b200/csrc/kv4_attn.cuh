@@ -45,17 +45,24 @@ __device__ __forceinline__ void kv4_span(const Kv4Attn & A, int lo, int hi, Kv4S
         q.from = from;
     } else kv4_pages(A, X && A.x.mode == KV4_FRONT ? A.x.prefix_ld : A.table_ld, lo, hi, q);
 }
-// cells of group g's prefix (as many as its table has room for: pages are counted in 31 bits by what tables have), and whether it is by itself: what counts are all groups' pages, up to KV4_FEW_GROUPS of them; of more, the group's times their number
+// what n sequences save of a page if their prefix is by itself
+__host__ __device__ __forceinline__ int64_t kv4_saved(const Kv4Ext & x, int64_t n) { return n * x.of_seq - ((n * x.rows - 1 >> x.log_tile) + 1) * x.of_tile; }
+// cells of group g's prefix (as many as its table has room for: pages are counted in 31 bits by what tables have), and whether it is by itself: where that saves the group something, and all groups
+// enough for the launch, up to KV4_FEW_GROUPS of them; of more, the group's times their number
 constexpr int KV4_FEW_GROUPS = 8;
 __device__ __forceinline__ int kv4_prefix(const Kv4Attn & A, int g, bool & apart) {
     auto cells = [&](int i) { return min(max(A.x.prefix_len[i], 0), A.x.room); };
-    auto pages = [&](int i) { return (int64_t) (A.x.group_start[i + 1] - A.x.group_start[i]) * ((cells(i) + KV4_CELLS - 1) / KV4_CELLS); };
+    auto saved = [&](int i) {
+        const int64_t of_page = kv4_saved(A.x, min(max(A.x.group_start[i + 1], 0), A.x.n_own) - min(max(A.x.group_start[i], 0), A.x.n_own));
+        return of_page > 0 ? of_page * ((cells(i) + KV4_CELLS - 1) / KV4_CELLS) : 0;
+    };
+    const int64_t own = saved(g);
     int64_t all = 0;
     if (A.x.n_group <= KV4_FEW_GROUPS)
 #pragma unroll 1
-        for (int i = 0; i < A.x.n_group; i++) all += pages(i);
-    else all = pages(g) * A.x.n_group;
-    apart = all * A.x.of_page >= A.x.least;
+        for (int i = 0; i < A.x.n_group; i++) all += saved(i);
+    else all = own * A.x.n_group;
+    apart = own > 0 && all >= A.x.least;
     return cells(g);
 }
 // KV4_SHARED: a sequence's `keep` and `from`.  A call, not code in its place: kernels have it in many, and what they are short of is the time to fetch code (a token behind 1000 cells 16 -> 14 us)

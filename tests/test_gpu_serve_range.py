@@ -118,3 +118,30 @@ def test_groups_that_end_behind_the_batch(pkg, lib, cuda, case):
     assert lib.c.pb200_kernel_launches() - before >= 2, "the prefix has no kernel of its own"
     b.group_np = np.array([0, 20, n], np.int32)
     b.check()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("groups", [[1] * 64, [1] * 8, [2, 1, 1, 2, 1, 1], [1, 3] * 10], ids=lambda g: f"{len(g)}of{max(g)}")
+def test_prefixes_of_few_sequences_are_walked(pkg, lib, cuda, type_, groups):
+    """Long prefixes of a sequence or three each: by themselves they would save nothing.  What is walked has the bits of sequences with all pages in one table."""
+    n, front = sum(groups), 16128 if len(groups) <= 8 else 4032
+    b = Batch(pkg, lib, 83, type_, 16, 8, 128, [1] * n, [1 + 11 * i for i in range(n)], groups, [front] * len(groups))
+    got = b.attend().clone()
+    row = np.repeat(np.arange(len(groups)), groups)
+    b.table_np = np.concatenate((b.prefix_table_np[row, :front // 64], b.table_np), 1)
+    b.kv_np, b.group_np = b.kv_np + front, None
+    b.upload()
+    b.out.fill_(7.0)
+    assert torch.equal(b.attend(), got)
+
+
+@pytest.mark.parametrize("max_q", [1, 6])
+def test_more_queries_than_there_are_do_not_change_the_way(pkg, lib, cuda, max_q):
+    """Tokens behind a prefix that they walk: with a max_q beyond what there is, too."""
+    b = Batch(pkg, lib, 84, "bf16", 32, 8, 128, [1] * 16, [30 + i for i in range(16)], [16], [4032])
+    got = b.attend(max_q=max_q).clone()
+    b.check()
+    b.table_np = np.concatenate((np.repeat(b.prefix_table_np[:, :63], 16, 0), b.table_np), 1)
+    b.kv_np, b.group_np = b.kv_np + 4032, None
+    b.upload()
+    assert torch.equal(b.attend(max_q=max_q), got)
