@@ -111,12 +111,13 @@ struct Kv4Ext {
     int64_t prefix_ld;
     int n_group, n_own, room;             // groups, sequences; cells that a prefix has at most: what its table has room for, in 30 bits
     int64_t least;                        // what has to be saved for prefixes to be by themselves: pages x kv heads x tiles of eight rows, times 16
+    int few;                              // sequences with more rows than this walk the prefix whatever the others do (0: there are none)
     int of_seq, of_tile, rows, log_tile;  // of that, a page of a prefix costs a sequence that walks it, with so many rows, and a tile of 2^log_tile rows in the prompts' kernel
     float * o; float4 * ml;               // parts of rows [token][head]: sums [D]; reference, sum of weights, and the mark of the call
     int * sync;                           // calls that have ended, CTAs of a call's last kernel that have
 };
 // SHARED: a sequence's cells are the prefix's pages and its own behind them, or, where that is much work for the group, its own alone: sums and what belongs to them go into o and ml.  FRONT, behind
-// it: a group is a sequence whose queries, those of all its sequences, see all cells of the prefix; what the others left is added
+// it: a group is a sequence whose queries, those of all its sequences, see all cells of the prefix; to what a sequence left its part of this is added
 enum { KV4_PLAIN = 0, KV4_SHARED = 1, KV4_FRONT = 2 };
 struct Kv4Attn {
     Kv4 cache;

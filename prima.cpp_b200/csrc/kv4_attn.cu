@@ -60,15 +60,28 @@ int launch_kv4_attn_shared(const Kv4Attn & a, const Kv4Groups & g, int D, int ty
     b.x.n_own = a.n_seq;
     b.x.room = (int) std::min<int64_t>(1 << 30, std::min<int64_t>(g.table_ld, 1 << 24) * KV4_CELLS);
     const bool f32 = type == PB200_TYPE_F32;
-    const int64_t most = std::min<int64_t>(a.max_q, a.n_tokens) * a.group, rows = std::min<int64_t>(most, few_rows(type)), least = 16 * (f32 ? KV4_APART_F32 : KV4_APART);
+    const int few = few_rows(type);
+    const int64_t most_q = std::min<int64_t>(a.max_q, a.n_tokens);
+    int64_t least = 16 * (f32 ? KV4_APART_F32 : KV4_APART);
     b.x.mode = KV4_SHARED;
-    // tiles of a sequence: those of the longest, but no more than all tokens make on the average
-    b.x.of_seq = (int) (16 * a.cache.n_head_kv * std::min<double>((rows + 7) / 8, 1 + (double) a.n_tokens * a.group / 8 / a.n_seq));
+    // Sequences with few rows, and their tiles: those of the longest, but no more than all tokens make on the average; where there are sequences with many, these are taken for as few as have all
+    // queries but one of each other, which are tokens; twice as much has to be saved there, since the prefix's kernel starts behind the prompts'.  us, pages in front of tokens' / by themselves, bf16, tokens and
+    // a prompt of 512: behind 16 000 cells, 128 689 / 377, 28 272 / 246; 4000, 64 162 / 146, 28 114 / 124; one of 2000, 2000 cells, 64 190 / 213; F32, one of 200, 4000 cells, 64 207 / 168, 24 126 / 120
+    int64_t n = a.n_seq, rows = most_q * a.group;
+    double tiles = std::min<double>((rows + 7) / 8, 1 + (double) a.n_tokens * a.group / 8 / a.n_seq);
+    if (rows > few) {
+        b.x.few = few;
+        least *= 2;
+        n = a.group <= few && n > 1 ? n - (std::max<int64_t>(a.n_tokens - n, 0) + most_q - 2) / (most_q - 1) : 0;
+        rows = std::min(a.group, few);
+        tiles = (double) ((rows + 7) / 8);
+    }
+    b.x.of_seq = (int) (16 * a.cache.n_head_kv * tiles);
     b.x.of_tile = 16 * a.cache.n_head_kv * (f32 ? KV4_TILE_F32 : KV4_TILE);
     b.x.rows = (int) rows;
     b.x.log_tile = f32 ? 7 : 8;                  // rows of an item: kp_rows
     b.x.least = least / 2;
-    const bool apart = most == rows && (double) kv4_saved(b.x, a.n_seq) * g.table_ld >= (double) least;
+    const bool apart = n > 1 && (double) kv4_saved(b.x, n) * g.table_ld >= (double) least;
     if (!apart) b.x.least = INT64_MAX;
     const int e = launch_kv4_attn(b, D, type, ws, st, launches);
     if (e || !apart) return e;

@@ -65,8 +65,8 @@ __device__ __forceinline__ int kv4_prefix(const Kv4Attn & A, int g, bool & apart
     apart = own > 0 && all >= A.x.least;
     return cells(g);
 }
-// KV4_SHARED: a sequence's `keep` and `from`.  A call, not code in its place: kernels have it in many, and what they are short of is the time to fetch code (a token behind 1000 cells 16 -> 14 us)
-static __device__ __noinline__ int2 kv4_in_front(const Kv4Attn & A, int s) {
+// KV4_SHARED: `keep` and `from` of a sequence, of many rows or not.  A call, not code in its place: kernels have it in many, and what they are short of is the time to fetch code (a token behind 1000 cells 16 -> 14 us)
+static __device__ __noinline__ int2 kv4_in_front(const Kv4Attn & A, int s, bool many) {
     const int n = A.x.n_group;
     if (s < A.x.group_start[0] || s >= A.x.group_start[n]) return make_int2(0, 0);
     int g = 0, end = n;                        // group_start[g] <= s < group_start[end]
@@ -77,12 +77,23 @@ static __device__ __noinline__ int2 kv4_in_front(const Kv4Attn & A, int s) {
     }
     bool apart;
     const int cells = kv4_prefix(A, g, apart), pages = (cells + KV4_CELLS - 1) / KV4_CELLS;
-    return apart ? make_int2(0, -1) : make_int2(pages, KV4_CELLS * g + (KV4_CELLS * pages - cells));
+    return apart && !many ? make_int2(0, -1) : make_int2(pages, KV4_CELLS * g + (KV4_CELLS * pages - cells));
 }
 // position of query t of a sequence
 template <bool X> __device__ __forceinline__ int kv4_pos(const Kv4Attn & A, const Kv4Seq & q, int t) {
     if (X && A.x.mode == KV4_FRONT) return q.p0;
     return kv4_shared<X>(A) ? max(q.p0 + t, KV4_CELLS * q.keep - 1) : q.p0 + t;
+}
+// KV4_FRONT: all tokens t0 .. t1 of a group are of one sequence that walks the prefix itself: rows that nothing was left of
+static __device__ __noinline__ bool kv4_walks(const Kv4Attn & A, int g, int64_t t0, int64_t t1) {
+    int s = max(A.x.group_start[g], 0), end = min(A.x.group_start[g + 1], A.x.n_own);        // q_start[s] <= t0 < q_start[end]
+    while (end - s > 1) {
+        const int mid = (s + end) / 2;
+        if (A.q_start[mid] <= t0) s = mid;
+        else end = mid;
+    }
+    const int64_t a = A.q_start[s], b = A.q_start[s + 1];
+    return a <= t0 && t1 < b && min(b - a, (int64_t) A.max_q) * A.group > A.x.few;
 }
 // many: sequences with more than most_rows rows, otherwise the others
 template <bool X>
@@ -112,7 +123,7 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn & A, int s, int most_row
     const int len = max((int) cells, 0);
     q.p0 = front ? len - 1 : len - all;
     if (kv4_shared<X>(A)) {
-        const int2 front = kv4_in_front(A, s);
+        const int2 front = kv4_in_front(A, s, many);
         q.keep = front.x;
         q.from = front.y;
         q.p0 = min(len, 1 << 30) - all + KV4_CELLS * q.keep;

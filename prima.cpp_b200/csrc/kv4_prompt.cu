@@ -85,11 +85,12 @@ template <int D> struct KpParts { KpPart<D> part[KV4_SLOTS]; KpPiece item[KV4_SL
 
 // the tile's rows [row0, row0 + rows) of a sequence: positions and pages
 template <bool X>
-__device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, KpPiece & p) {
+__device__ __forceinline__ void kp_span(const Kv4Attn & A, const Kv4Seq & q, int s, KpPiece & p) {
     p.p_lo = kv4_pos<X>(A, q, p.row0 / A.group);
     p.p_hi = kv4_pos<X>(A, q, (p.row0 + p.rows - 1) / A.group);
     p.q = q;
     kv4_span<X>(A, p.p_lo, p.p_hi, p.q);
+    if (X && A.x.mode == KV4_FRONT && A.x.few > 0 && kv4_walks(A, s, q.q0 + p.row0 / A.group, q.q0 + (p.row0 + p.rows - 1) / A.group)) p.q.pages = 1;     // rows that are not written
     p.tiles = (p.q.pages + 1) / 2;
 }
 // Items, their pieces and slots, in the order of tickets: sequences, tiles from the last on, heads, pieces; every CTA counts them in the same way.  Where long items may be cut there are
@@ -137,7 +138,7 @@ __device__ __forceinline__ void kp_plan(const Kv4Attn & A, const KpWork & W, int
         if (m < all) {
             const Kv4Seq q = plan.seq<X>(src);
             p.rows = min(ROWS, q.n_rows - p.row0);
-            kp_span<X>(A, q, p);
+            kp_span<X>(A, q, src, p);
             plan.lens[m] = p.tiles;
             sum += p.tiles;
         }
@@ -187,7 +188,7 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, con
                 p.s = plan.from[r];
                 const Kv4Seq q = plan.seq<X>(p.s);
                 p.rows = min(ROWS, q.n_rows - p.row0);
-                kp_span<X>(A, q, p);
+                kp_span<X>(A, q, p.s, p);
                 const int i = t - before - (x - k * hks);
                 p.hk = i / k;
                 p.part = i - p.hk * k;
@@ -217,7 +218,7 @@ __device__ __forceinline__ bool kp_find(const Kv4Attn & A, const KpWork & W, con
             p.s = s0 + lane;
             p.row0 = ((q.n_rows + ROWS - 1) / ROWS - 1 - tile) * ROWS;
             p.rows = min(ROWS, q.n_rows - p.row0);
-            kp_span<X>(A, q, p);
+            kp_span<X>(A, q, p.s, p);
             p.hk = i - tile * hks;
             p.b = p.tiles;
             p.parts = 1;
@@ -799,18 +800,20 @@ int prompt_launch(const Kv4Attn & a, KpWork w, cudaStream_t st, int & launches) 
     const int ctas = sm_count() < KV4_MAX_CTAS ? sm_count() : KV4_MAX_CTAS;
     // (a plan adds up key tiles of all items: in 30 bits.  An item's pages are those that the tables it walks have room for)
     const auto room = [](int64_t ld) { return ld < INT_MAX / KV4_CELLS ? ld : (int64_t) INT_MAX / KV4_CELLS; };
-    const int64_t items = (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv;
+    const bool rest = a.x.mode == KV4_FRONT && a.x.few > 0;       // most of its rows may be those of sequences that walk, which are no work
+    const int64_t items = rest ? 0 : (a.n_tokens * a.group + kp_rows<T>() - 1) / kp_rows<T>() * a.cache.n_head_kv;
     const int64_t pages = (a.x.mode != KV4_FRONT ? room(a.table_ld) : 0) + (a.x.mode != KV4_PLAIN ? room(a.x.prefix_ld) : 0);
     w.cut = a.n_seq <= KP_CUT_SEQ && items < ctas && KP_CUT_TILES * (pages / 2 + 1) * a.cache.n_head_kv < 1 << 30;
     launches += w.cut ? 2 : 1;
-    // Behind the kernel of few rows (most_rows > 0), CTAs start where that has none at work: it has nothing that they read, and all in front of it has ended when it starts
+    // Behind the kernel of few rows (most_rows > 0), CTAs start where that has none at work: it has nothing that they read, and all in front of it has ended when it starts.  Behind another of this kernel, or
+    // its join, they do not: tickets and parts are the same
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(KP_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = w.most_rows > 0 || a.x.mode == KV4_FRONT ? 1 : 0;
+    cfg.numAttrs = w.most_rows > 0 || (a.x.mode == KV4_FRONT && !rest) ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, k_kv4_attn_prompt<T, D, X>, a, w);
     if (e != cudaSuccess || !w.cut) return (int) e;
     cudaLaunchConfig_t join{};

@@ -6,11 +6,27 @@ import pytest
 import torch
 
 import ref_kv4 as R
+import ref_serve as V
 from gpu_util import ptr
 from test_gpu_serve import TYPES, Batch, drafted, stream, verify
 
 pytestmark = pytest.mark.gpu
 LOWEST = np.finfo(np.float32).min
+
+
+@pytest.fixture(autouse=True)
+def weights_that_count_as_nothing(monkeypatch):
+    """Weights below 2^-960 of a row's largest count as 0, where numbers of 64 bits go on to 2^-1074: at temperatures as small as here's that is what all others of a row have."""
+    full = V.softmax
+
+    def softmax(x, t):
+        w = full(x, t)
+        if w is None:
+            return None
+        w = np.where(w < 2.0 ** -960 * w.max(), 0.0, w)
+        return w / w.sum()
+
+    monkeypatch.setattr(V, "softmax", softmax)
 
 
 @pytest.mark.parametrize("type_", TYPES)
@@ -125,7 +141,9 @@ def test_groups_that_end_behind_the_batch(pkg, lib, cuda, case):
 def test_prefixes_of_few_sequences_are_walked(pkg, lib, cuda, type_, groups):
     """Long prefixes of a sequence or three each: by themselves they would save nothing.  What is walked has the bits of sequences with all pages in one table."""
     n, front = sum(groups), 16128 if len(groups) <= 8 else 4032
-    b = Batch(pkg, lib, 83, type_, 16, 8, 128, [1] * n, [1 + 11 * i for i in range(n)], groups, [front] * len(groups))
+    b = Batch(pkg, lib, 83, type_, 16, 8, 128, [1] * n, [1 + 11 * i for i in range(n)], groups, [front] + [64] * (len(groups) - 1))
+    b.prefix_np[:], b.prefix_table_np[:] = front, b.prefix_table_np[:1]                 # (groups of their own, whose pages happen to be the same)
+    b.upload()
     got = b.attend().clone()
     row = np.repeat(np.arange(len(groups)), groups)
     b.table_np = np.concatenate((b.prefix_table_np[row, :front // 64], b.table_np), 1)
@@ -145,3 +163,57 @@ def test_more_queries_than_there_are_do_not_change_the_way(pkg, lib, cuda, max_q
     b.kv_np, b.group_np = b.kv_np + 4032, None
     b.upload()
     assert torch.equal(b.attend(max_q=max_q), got)
+
+
+MIXED_CASES = [
+    # groups, prefix, q, heads, kv_heads: prompts in front of a group's tokens, among them and behind them, of rows that fill tiles by themselves, and drafts beside both
+    ([71], [2200], [1] * 30 + [400] + [1] * 40, 16, 8), ([40, 0, 33], [2300, 100, 1500], [130] + [1] * 39 + [2] * 15 + [257, 0, 61] + [3] * 15, 16, 8), ([9] * 34, [1088] * 34, [1] * 300 + [60] + [1] * 5, 8, 8),
+    ([50, 2, 1], [3200, 3200, 64], [1] * 49 + [40] + [1, 300] + [25], 8, 8),
+]
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("case", range(len(MIXED_CASES)))
+def test_tokens_share_a_prefix_beside_prompts(pkg, lib, cuda, type_, dim, case):
+    """Sequences of many rows walk the prefix; those of few have it read once, as in a call of their own."""
+    groups, prefix, q, heads, kv_heads = MIXED_CASES[case]
+    b = Batch(pkg, lib, 85, type_, heads, kv_heads, dim, q, [n + 7 * (i % 20) for i, n in enumerate(q)], groups, prefix)
+    before = lib.c.pb200_kernel_launches()
+    b.attend()
+    assert lib.c.pb200_kernel_launches() - before >= 3, "the prefix has no kernel of its own"
+    b.check()
+    first = b.out.clone()
+    b.out.fill_(7.0)
+    b.attend(lse=False)
+    assert torch.equal(b.out, first)
+    if dim == 128:
+        return
+    most = 20
+    b.out.fill_(7.0)
+    b.lse.fill_(7.0)
+    b.attend(max_q=most)
+    b.check(most=most)
+
+
+def test_graph_of_tokens_beside_prompts(pkg, lib, cuda):
+    """One graph: prefixes by themselves and not, prompts that come and go, another call on the workspace between."""
+    n = 60
+    b = Batch(pkg, lib, 86, "bf16", 16, 8, 128, [1] * n + [150], [20 + i for i in range(n + 1)], [n + 1], [2700])
+    other = Batch(pkg, lib, 87, "f32", 8, 8, 128, [100] + [1] * 40, [100] + [30] * 40, [41], [2500])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            b.attend()
+        for prefix, q in ((2700, [1] * n + [150]), (100, [1] * n + [150]), (2699, [1] * 20 + [60] + [1] * 30 + [50] + [1] * 9), (2700, [1] * (n + 1))):
+            b.prefix_np[:], b.q_start_np[:] = prefix, np.concatenate(([0], np.cumsum(q)))
+            b.prefix.copy_(torch.from_numpy(b.prefix_np))
+            b.q_start.copy_(torch.from_numpy(b.q_start_np))
+            b.out.fill_(7.0)
+            b.lse.fill_(7.0)
+            graph.replay()
+            b.check()
+            other.attend(ws=b.ws)
+        other.check()
