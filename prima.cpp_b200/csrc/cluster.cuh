@@ -41,11 +41,6 @@ __device__ __forceinline__ int remote(const int * at, uint32_t cta) {
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote_addr(at, cta)) : "memory");
     return v;
 }
-__device__ __forceinline__ uint2 remote(const uint2 * at, uint32_t cta) {
-    uint2 v;
-    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(remote_addr(at, cta)) : "memory");
-    return v;
-}
 
 // clusters of 1, 2, 4 or 8 CTAs that run at the same time where a CTA takes an SM: a cluster stays within a group of SMs.  What cudaOccupancyMaxActiveClusters says on a B200 with 148 SMs, 8 from
 // below; persistent kernels launch no more, since the rest of a grid would start where these have ended

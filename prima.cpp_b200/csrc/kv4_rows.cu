@@ -699,8 +699,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const __grid_co
             KrSum sum;
             sum.add<16, true>(c1 - c0 + 1, r, d4, [&](int i) { return &parts.cta[c0 + i][i == 0 ? 1 : 0]; });
             if (r >= rows) return;
-                if constexpr (X) sum.write(kr_row<T, D>(A, at, r) + d4, kr_ext<D>(A, at, r, sum.top, sum.l, d4 == 0), d4);
-                else sum.write(kr_row<T, D>(A, at, r) + d4);
+            if constexpr (X) sum.write(kr_row<T, D>(A, at, r) + d4, kr_ext<D>(A, at, r, sum.top, sum.l, d4 == 0), d4);
+            else sum.write(kr_row<T, D>(A, at, r) + d4);
         });
     }
 }

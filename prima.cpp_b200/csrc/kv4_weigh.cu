@@ -52,7 +52,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // ---- a query row in shared memory, a part of it to each of four threads next to each other ----
 // its power of two: the largest number comes to 2^13 .. 2^14
 template <int EACH>
-__device__ __forceinline__ float row_power(const float (&x)[EACH], float top) {
+__device__ __forceinline__ float row_power(const float (&x)[EACH]) {
+    float top = 0.f;
 #pragma unroll
     for (int i = 0; i < EACH; i++) top = fmaxf(top, fabsf(x[i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(KW_THREADS, 2) k_kv4_weigh(const __grid_consta
                             x[i + k] = v.x; x[i + k + 1] = v.y; x[i + k + 2] = v.z; x[i + k + 3] = v.w;
                         }
                     }
-                    up = row_power<EACH>(x, 0.f) * (A.scale < 0.f ? -1.f : 1.f);
+                    up = row_power<EACH>(x) * (A.scale < 0.f ? -1.f : 1.f);
 #pragma unroll
                     for (int i = 0; i < EACH; i += 8) row_store<T, 8>(reinterpret_cast<float(&)[8]>(x[i]), up, &S.q[0][r][16 * quarter + 8 * i], &S.q[LO - 1][r][16 * quarter + 8 * i]);
                 }
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) k_kv4_weigh_few(const __grid_co
                 const float lse = have ? W.lse[(q.q0 + t) * W.ld_lse + head] : -INFINITY;
                 if (f_n == 0)                               // the first keys, behind the first queries
                     for (int k = 0; k < STAGES; k++) fetch();
-                const float up = row_power<EACH>(x, 0.f) * (A.scale < 0.f ? -1.f : 1.f);
+                const float up = row_power<EACH>(x) * (A.scale < 0.f ? -1.f : 1.f);
                 float block = 0.f;                          // sum of the block's numbers
                 if (RAW) {
 #pragma unroll

@@ -354,16 +354,14 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) k_verify_draw(const __
         arg = p.first(m[0]);
     } else {
         constexpr int ONCE = 8;
-            for (int i0 = from + lane; i0 < to; i0 += 32 * ONCE) {
-                float x[ONCE];
+        for (int i0 = from + lane; i0 < to; i0 += 32 * ONCE) {
+            float x[ONCE];
 #pragma unroll
-                for (int k = 0; k < ONCE; k++) x[k] = i0 + 32 * k < to ? raw(row_p + i0 + 32 * k) : -INFINITY;
+            for (int k = 0; k < ONCE; k++) x[k] = i0 + 32 * k < to ? raw(row_p + i0 + 32 * k) : -INFINITY;
 #pragma unroll
-                for (int k = 0; k < ONCE; k++)
-                    if (x[k] > m[0]) { m[0] = x[k]; arg = i0 + 32 * k; }
-            }
-    }
-    if (!rejected) {
+            for (int k = 0; k < ONCE; k++)
+                if (x[k] > m[0]) { m[0] = x[k]; arg = i0 + 32 * k; }
+        }
         const float own = m[0];
         m[0] = warp_max(m[0]);
         arg = __reduce_min_sync(0xffffffffu, own == m[0] && own > -INFINITY ? arg : INT_MAX);
