@@ -175,11 +175,14 @@ PB200_API int pb200_kv4_attn(const pb200_kv4_cache * cache, int layer, int type,
 PB200_API int pb200_kv4_attn_lse(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
                                  const int32_t * kv_len, const int32_t * table, int64_t table_ld, int64_t n_tokens, int max_q, float scale, int window, int keep_first, float * lse,
                                  int64_t ld_lse, void * ws, size_t ws_bytes, void * stream);
-/* Attention of a batch whose sequences come in groups with a prefix in common, whose pages are read once for the group.  Group g has the sequences group_start[g] .. group_start[g+1]-1 (device
+/* Attention of a batch whose sequences come in groups with a prefix in common, whose pages are kept once.  Group g has the sequences group_start[g] .. group_start[g+1]-1 (device
  * [n_group + 1], rising; sequences outside of group_start[0] .. group_start[n_group]-1 have no prefix), whose queries all see the prefix_len[g] cells of row g of prefix_table (as table's,
  * prefix_ld pages a row) in front of their own, which are those of pb200_kv4_attn without a window: kv_len counts them alone, and rotations count from the prefix's start.  A prefix may end
- * inside a page.  lse: as in pb200_kv4_attn_lse, or NULL.  Precision: as in pb200_kv4_attn, of one sequence with all the cells; a prefix
- * that is read once for many rows has a prompt's.  A prefix and the cells behind it lie within 2^30, groups within 2^24.
+ * inside a page, and ends with its row of the table at the latest.  Sequences with few rows (up to 48 queries x heads of a group, 32 in F32) have the prefix's pages read once for all of the group,
+ * by a kernel of its own, where that saves enough pages; where it does not (a few sequences, a short prefix), and for sequences with many rows, each reads them in front of its own.  Which, goes by lengths and
+ * groups on the device, so that a graph follows them; max_q and n_tokens, if they are more than there is, may cost time.
+ * lse: as in pb200_kv4_attn_lse, or NULL.  Precision: as in pb200_kv4_attn, of one sequence with all the cells; a prefix that is read once has a prompt's: in F16 and BF16 weights of 11 bits and
+ * sums of the tensor core's (F16: 2.8e-4 of the output's norm where 32-bit operations have 2.1e-4).  A prefix and the cells behind it lie within 2^30, groups within 2^24.
  * ws: pb200_kv4_attn_shared_workspace_bytes, zeroed once, as pb200_kv4_attn's, for which it serves, too. */
 PB200_API size_t pb200_kv4_attn_shared_workspace_bytes(int n_head, int n_head_kv, int head_dim, int64_t n_tokens);
 PB200_API int pb200_kv4_attn_shared(const pb200_kv4_cache * cache, int layer, int type, const void * q, int64_t ldq, void * out, int64_t ldo, int n_head, int n_seq, const int32_t * q_start,
@@ -211,7 +214,7 @@ PB200_API int pb200_kv4_compact(const pb200_kv4_cache * cache, int n_seq, const 
  * Sequence s has the drafts start[s] .. start[s+1]-1 (device [n_seq + 1], rising from 0 to n_drafts): tokens and, in rows of n_vocab logits of a type (PB200_TYPE_F32, F16 or BF16; any stride), what
  * the draft model had: row i of `draft` for draft i, or draft NULL: the tokens come from elsewhere, as if with probability 1.  target: for each of its drafts and for the token behind the last one
  * a row: start[s] + s .. start[s+1] + s.  p and q: softmax of logits times inv_temp[s] (NULL: 1; infinite: all on the largest, of several the lowest; 0: even over all finite logits).
- * Draft x with its number u = u_accept[i] is accepted where u q(x) < p(x); n_accepted[s]: how many are, up to the first that is not.  Behind them comes a token drawn by u_draw[s]: with weights
+ * Draft x with its number u = u_accept[i] is accepted where u q(x) < p(x), p and q by sums in 32 bits: to 1e-6 as a rule, 1e-5 at most (vocabularies of up to 200 000); n_accepted[s]: how many are, up to the first that is not.  Behind them comes a token drawn by u_draw[s]: with weights
  * w = max(p - q, 0) of the first that is not accepted (p, where these are all 0), with p behind the last: the lowest i with w_0 + .. + w_i > u_draw[s] * (sum of w), in 64 bits.
  * out[s * ld_out + ..]: the accepted tokens and that one (as far as ld_out goes; what lies behind stays as it was).  kv_len_out[s] = kv_len[s] less the drafts that were not accepted (both NULL:
  * not wanted; may be the same): the cells of these are free.  Logits that are no number count as -inf, +inf takes all weight; tokens outside the vocabulary are not accepted; weights below 2^-960

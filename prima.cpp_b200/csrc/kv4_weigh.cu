@@ -8,7 +8,8 @@
 // 64: two or four warps have the same cells, and each a part of the rows).  A cluster has an item; its CTAs share the kv heads, and the rows in blocks of 64; their sums meet in shared memory, in the
 // CTAs' order (equal calls give equal bits).
 //
-// Bound: instructions.  Few rows: a key's numbers are taken apart once for up to 16 rows (32 sequences of up to 8192 cells 33 us; their keys' bytes take 12).  Many rows: of a block of 64 rows 1.2 us go into
+// Bound: latency, no pipe is full.  Few rows: a key's numbers are taken apart once for up to 16 rows, by the 16 warps that an SM has room for (32 sequences of up to 8192 cells 33 us; their keys' bytes take 12: issue
+// slots 40 %, DRAM 28 %).  Many rows (tensor pipe 19 %, XU 29 %, issue slots 26 %): of a block of 64 rows 1.2 us go into
 // loading and converting, 2 into the products' chains and exponentials (64 queries of 32 heads behind 16 000 cells 41 us, 0.12 of the tensor cores' rate; 2048 of a prompt, on 128 CTAs, 259).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -3,14 +3,15 @@
 // Mathematics.  With p and q the softmax of the target's and the draft's logits times t = 1 / temperature, drafted token x is accepted where u q(x) < p(x).  Behind the accepted ones comes a
 // token from max(p - q, 0) at the place of the rejection, from p behind the last draft: by the inverse of the cumulative sum at v times the whole.  What is emitted then has the target's
 // distribution, whatever the draft's.
-//   rows    a CTA has a chunk of a row: its largest logit m and the sum of 2^((l - m) t log2 e), in 32 bits: a decision u q < p changes where they are within 1e-7 of each other
+//   rows    a CTA has a chunk of a row: its largest logit m and the sum of 2^((l - m) t log2 e), in 32 bits: a decision u q < p may change
+//           where they are within 1e-5 of each other (additions one behind the other, up to 60 of a thread's, and exponents that are rounded three times; 1e-6 as a rule)
 //   draw    a cluster has a sequence.  It joins its rows' chunks, decides, and adds up the weights that the token is drawn with, of one row, or of two with draft logits.  Weights and sums are in
 //           64 bits: a cumulative sum of 100 000 weights with errors of 1e-8 each would give another token once in a thousand draws.  Each warp has the sum of a contiguous part; that in which the
 //           token lies goes to all warps of its CTA once more, and a part of that is scanned.
 //
-// Bound.  rows: memory where there are many.  draw: 64-bit instructions (a weight is a root of 16 from a table and a polynomial of degree 5) and, for few sequences, the chain of launch, row sums,
-// cluster barriers and parts.  us: 64 sequences, 3.6 drafts each on the average, rows of 128 256 in 32 bits, 115 (47 of them the rows, 5 TB/s); 24 with drafts from elsewhere, 151 937 in bf16, 37; one
-// sequence, 3 drafts, 32 000, 17 to 19.  exp in 64 bits instead of the table 248, 69 and 23.
+// Bound.  rows: memory where there are many.  draw: no pipe is full (64 sequences: fp64 35 %, issue slots 39 %, 36 % of the warps): chains of loads and 64-bit instructions (a weight is a root of 16 from a
+// table and a polynomial of degree 5), twice over two rows, and, for few sequences, of launch, row sums, cluster barriers and parts.  us: 64 sequences, 3.6 drafts each on the average, rows of 128 256
+// in 32 bits, 117 (47 of them the rows, 5 TB/s); 24 with drafts from elsewhere, 151 937 in bf16, 33; one sequence, 3 drafts, 32 000, 17 to 19.  exp in 64 bits instead of the table 248, 69 and 23.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(VR_THREADS, VR_CTAS) k_verify_rows(const __gri
 }
 
 // 2^(y / 16) in 64 bits for y from -16 * 1000 to 0: the whole part of y goes to the exponent and to one of 16 roots, 2^(r / 16) of the rest (up to a half) is the polynomial that agrees
-// with it at the six Chebyshev nodes: within 2^-47 of it.  (Without roots nine products instead of five: 64 sequences of 128 256 logits 70 us where this takes 66.)
+// with it at the six Chebyshev nodes: within 2^-47 of it.  (Without roots nine products instead of five: 64 sequences of 128 256 logits 4 us more.)
 __device__ __forceinline__ double power_of_two(double y, const double * roots) {
     constexpr double ROUND = 6755399441055744.0;          // 1.5 * 2^52: a sum with it has the whole number in its last bits
     const double z = y + ROUND, r = y - (z - ROUND);
