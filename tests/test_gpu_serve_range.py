@@ -217,3 +217,31 @@ def test_graph_of_tokens_beside_prompts(pkg, lib, cuda):
             b.check()
             other.attend(ws=b.ws)
         other.check()
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_tokens_beside_a_prompt_of_more_tiles_than_a_plan_has(pkg, lib, cuda, type_):
+    """A prompt between tokens with more tiles of rows than items are cut by: the tokens have what they have without it."""
+    n, long = 128, 12500
+    b = Batch(pkg, lib, 88, type_, 4, 1, 128, [1] * n, [3 + i for i in range(n)], [n], [10240])
+    half, rng = n // 2, np.random.default_rng(89)
+    prompt = torch.from_numpy(rng.standard_normal((long, b.ldq)).astype(np.float32)).cuda().to(b.q.dtype)
+    q = torch.cat((b.q[:half], prompt, b.q[half:]))
+    out, lse = torch.full((n + long, b.ldo), 7.0, dtype=b.q.dtype, device="cuda"), torch.full((n + long, b.ldl), 7.0, device="cuda")
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).cuda()
+    starts = np.concatenate((np.arange(half + 1), half + long + np.arange(half + 1)))
+    kv = np.concatenate((b.kv_np[:half], [long], b.kv_np[half:]))
+    table = np.full((n + 1, -(-long // R.CELLS)), -1)
+    table[:half, :b.table_np.shape[1]], table[half + 1:, :b.table_np.shape[1]] = b.table_np[:half], b.table_np[half:]
+    table[half] = np.arange(table.shape[1]) % len(b.pages_np)
+    d = [dev(starts), dev(kv), dev(table), dev([0, n + 1])]
+    ws = torch.zeros(lib.c.pb200_kv4_attn_shared_workspace_bytes(4, 1, 128, n + long), dtype=torch.uint8, device="cuda")
+    before = lib.c.pb200_kernel_launches()
+    lib.check(lib.c.pb200_kv4_attn_shared(C.byref(b.cache), 0, R.CODE[type_], ptr(q), b.ldq, ptr(out), b.ldo, 4, n + 1, ptr(d[0]), ptr(d[1]), ptr(d[2]), table.shape[1], 1, ptr(d[3]), ptr(b.prefix),
+                                          ptr(b.prefix_table), b.prefix_table_np.shape[1], n + long, long, b.scale, ptr(lse), b.ldl, ptr(ws), ws.numel(), stream()))
+    assert lib.c.pb200_kernel_launches() - before == 4, "the prefix has no kernel of its own"
+    torch.cuda.synchronize()
+    assert not torch.any(torch.all(out == 7.0, 1))
+    b.out.copy_(torch.cat((out[:half], out[half + long:])))
+    b.lse.copy_(torch.cat((lse[:half], lse[half + long:])))
+    b.check()
